@@ -613,6 +613,122 @@ enum { KVIP_TIME_START = 0, KVIP_TIME_LI, KVIP_TIME_TOPK, KVIP_TIME_RESOLVE, KVI
        KVIP_TIME_FETCH, KVIP_TIME_GATHER, KVIP_TIME_STAMPS };
 uint32_t kvip_prepare_shape(KvipRuntimeShape* shape);    /* include/api.h:9 */
 
+/* ---- the rest of a decode step: slot maps, rotary positions, attention, draft verification ----------
+ * What stands round the selection path in a step with drafted tokens. The reference leaves these to the
+ * serving framework above it; none of them has a counterpart there. Every index that comes from device memory
+ * is range-checked in the kernel: a bad one is skipped and reported in the status word. */
+
+/* Block tables and slot maps of a step from the requests' lengths, in one launch. Request b has lengths[b] cached
+ * tokens, owns the first held[b] entries of its table row and adds counts[b] tokens; with
+ *   need = ceil((lengths + counts) / block), new = max(0, need - held), off = exclusive prefix sum of new
+ * entry held + j of its row becomes free_blocks[head + off + j], and its token i (packed token starts[b] + i) gets
+ * position lengths + i and slot row[position / block] * block + position % block. Rows t >= starts[batch] of the token
+ * outputs are -1. A request whose range does not fit its row (or is negative) adds no token and sets
+ * KVIP_ERR_TOKEN_RANGE; one that the free list cannot serve keeps its packed tokens, with position and slot -1, and
+ * takes no block (KVIP_ERR_NO_SLOT); a packed token behind the last output row is dropped (KVIP_ERR_TOKEN_RANGE).
+ * lengths, held, counts and head are not written: the call can be repeated. */
+typedef struct KvipSlotMapsArgs {
+  const int32_t* lengths;      /* [batch] */
+  const int32_t* counts;       /* [batch] */
+  const int32_t* held;         /* [batch] */
+  const int32_t* free_blocks;  /* [blocks] */
+  const int32_t* head;         /* [1] first free entry of free_blocks */
+  int32_t* table;              /* [batch, pages] */
+  int64_t* positions;          /* [tokens] */
+  int64_t* slot_mapping;       /* [tokens] */
+  int32_t* requests;           /* [tokens] request of the packed token */
+  int32_t* starts;             /* [batch + 1] */
+  int32_t* ends;               /* [batch] lengths + counts, or lengths where the request got nothing */
+  int32_t* held_after;         /* [batch] */
+  int32_t* taken;              /* [1] entries of free_blocks used */
+  int32_t* status;             /* [1] OR-ed KVIP_ERR_* */
+  int64_t* layout;             /* [4, batch * queries] the QueryInputs rows GATHER, QUERY_VALID, UNPACK, OUTPUT_VALID, or NULL;
+                                  with it a count above `queries` is a KVIP_ERR_TOKEN_RANGE */
+  uint32_t batch, pages, blocks, tokens, block, queries;
+} KvipSlotMapsArgs;
+uint32_t kvip_b200_slot_maps(const KvipSlotMapsArgs* args, void* stream);
+
+/* Rotary positions. Pair i of a rotated row (elements i and i + width/2 in the half layout, 2i and 2i + 1 in the
+ * interleaved one) turns by the angle position * frequency_i; turns[i] = frequency_i / 2 pi. Rows of tokens with a
+ * negative position are not written. `x[s]`: two sets of rows [tokens, heads[s], width] with their own strides (in
+ * elements, innermost stride 1); y may be x. */
+enum { KVIP_ROTARY_HALF = 0, KVIP_ROTARY_INTERLEAVED = 1 };
+enum { KVIP_FLOAT_BF16 = 0, KVIP_FLOAT_FP16 = 1, KVIP_FLOAT_FP32 = 2 };
+typedef struct KvipRotaryArgs {
+  const int64_t* positions;    /* [tokens] */
+  const double* turns;         /* [width / 2] */
+  const void* x[2];            /* the second may be NULL */
+  void* y[2];                  /* rows of the same type; with codes NULL */
+  uint8_t* codes;              /* [tokens, heads[0], dim] FP8 e4m3: rotate the first `width` of `dim` elements of x[0] and */
+  float* scales;               /* [tokens, heads[0]] quantise the row with scale = amax / 448 (1 for a row of zeros) */
+  int64_t x_token[2], x_head[2], y_token[2], y_head[2];
+  uint32_t heads[2];
+  uint32_t tokens, width, dim, layout, dtype;
+  float factor;                /* multiplies the rotated elements (cos and sin) */
+} KvipRotaryArgs;
+uint32_t kvip_b200_rotary(const KvipRotaryArgs* args, void* stream);
+
+/* Attention of packed query tokens over selected rows of the resident pool and, for a tree of drafted tokens, over
+ * the drafted rows of their own request. Token t of request r = requests[t] sees the pool rows
+ *   owner(r) * output_stride + slots[t, k]   for every slots[t, k] >= 0, and
+ *   drafted row starts[r] + j                for every set bit j of ancestors[t] (j < starts[r+1] - starts[r], j < 64).
+ * A row has 576 elements, its first 512 are also the value:
+ *   out[t,h] = sum p v, p = softmax(scale * query[t,h] . row); lse[t,h] = log of the sum of exp(scale * query . row).
+ * A token that sees no row gets zeros and lse = -inf; a token with requests[t] < 0 is padding, its outputs are left as they are. */
+#define KVIP_ATTENTION_WIDTH 576u
+#define KVIP_ATTENTION_VALUE 512u
+typedef struct KvipAttentionArgs {
+  const void* query;           /* [tokens, heads, 576] bf16 or fp16, innermost stride 1 */
+  const void* pool;            /* [pool_rows, 576] same type */
+  const int32_t* slots;        /* [tokens, entries] */
+  const int32_t* requests;     /* [tokens], or NULL: token t is request t / queries */
+  const int32_t* row_owners;   /* [batch], or NULL: owner = request */
+  const int32_t* starts;       /* [batch + 1], or NULL: no drafted rows */
+  const void* draft;           /* [tokens, 576] same type, or NULL */
+  const int64_t* ancestors;    /* [tokens], or NULL: every drafted row up to the token's own (a chain) */
+  void* out;                   /* [tokens, heads, 512] same type as the query */
+  float* lse;                  /* [tokens, heads] */
+  float* partial;              /* [partial_rows, 512] workspace of the shares, or NULL: every token in one piece */
+  float* partial_stats;        /* [partial_rows, 2] */
+  int32_t* status;             /* [1] OR-ed KVIP_ERR_* */
+  int64_t query_token, query_head;   /* strides of query in elements, multiples of 8 */
+  int64_t draft_token;               /* stride of draft in elements, a multiple of 8 */
+  uint64_t pool_rows;
+  uint32_t tokens, heads, entries, batch, queries, output_stride, dtype;
+  uint32_t splits;             /* shares of a token's rows that are computed apart and joined (splits * tokens * heads <= */
+  uint32_t partial_rows;       /* partial_rows); 0 = by the sizes */
+  uint32_t wait_kilocycles;    /* limit of every barrier wait, in units of 1024 SM clock cycles; 0 = about one second */
+  float scale;
+  uint32_t reserved0;
+} KvipAttentionArgs;
+uint32_t kvip_b200_slot_attention(const KvipAttentionArgs* args, void* stream);
+
+/* Verification of drafted tokens against the target's probabilities, from given random numbers. Request b owns the
+ * packed rows starts[b] .. starts[b + 1]: row 0 is its last committed token, every other row a drafted token whose parent
+ * (a smaller local index) precedes it; at most 64 rows. target row j: the target's distribution behind node j; draft row j:
+ * the distribution that the children of node j were drawn from (NULL: the draft was certain of its tokens). Walk: at
+ * node c, r = target[c], Z = 1; its children in order: child x with token t is accepted if
+ * accept[x] * draft[c][t] * Z < r[t], and the walk goes on from it; else r = max(r - Z * draft[c], 0), Z = sum r (with no
+ * draft rows: r[t] = 0). Where no child is left the token drawn is the smallest v with sum_{w <= v} r[w] > sample[b] * sum r.
+ * All of it in 64-bit floating point. Where nothing is left of r the walk ends and the token comes from target[c] itself.
+ * Probabilities that are negative or NaN count as 0. A node with a token outside the vocabulary is never tested. */
+typedef struct KvipVerifyArgs {
+  const void* target;          /* [rows, vocabulary] fp32, bf16 or fp16 */
+  const void* draft;           /* same type, or NULL */
+  const int64_t* tokens;       /* [rows] */
+  const int32_t* parents;      /* [rows] local index of the parent; ignored for row 0 of a request */
+  const int32_t* starts;       /* [batch + 1] */
+  const float* accept;         /* [rows] in [0, 1) */
+  const float* sample;         /* [batch] in [0, 1) */
+  int64_t* out_tokens;         /* [batch, depth + 1] accepted tokens, then the drawn one, then -1 */
+  int32_t* out_nodes;          /* [batch, depth + 1] local indices 0 and the accepted nodes, then -1 */
+  int32_t* out_counts;         /* [batch] accepted + 1; 0 for a request without rows */
+  int32_t* status;             /* [1] OR-ed KVIP_ERR_TOKEN_RANGE */
+  int64_t target_row, draft_row;  /* row strides in elements */
+  uint32_t rows, vocabulary, batch, depth, dtype, reserved0;
+} KvipVerifyArgs;
+uint32_t kvip_b200_verify_drafts(const KvipVerifyArgs* args, void* stream);
+
 /* ---- host-DDR KV pool ---------------------------------------------------------------
  * Pins `bytes` of host memory at `host` (page-aligned, owned by the caller) and maps it into the
  * device address space; *device_alias receives the pointer kernels read it through. The pool

@@ -24,6 +24,10 @@ _EXPORTS = {
     "PagedIndexer": ("adapters", "PagedIndexer"),
     "RequestPlan": ("adapters", "RequestPlan"),
     "PageUpdates": ("cache.page_updates", "PageUpdates"),  # reference: kvip.cache.page_updates.PageUpdates
+    "BlockTables": ("cache.block_tables", "BlockTables"),
+    "Rotary": ("rotary", "Rotary"),
+    "SlotAttention": ("operators.attention", "SlotAttention"),
+    "DraftVerifier": ("operators.verify", "DraftVerifier"),
     "FusedQueryInputs": ("inputs", "QueryInputs"),
     "FusedWorkspace": ("operators.lifetch", "LIFetchWorkspace"),
 }

@@ -22,6 +22,8 @@ BAD_ARGUMENT = 100000
 KEY_FP8, KEY_BF16 = 0, 1
 WEIGHT_BF16, WEIGHT_FP32 = 0, 1
 SCORE_FP32, SCORE_BF16_AWAY = 0, 1
+FLOAT_BF16, FLOAT_FP16, FLOAT_FP32 = 0, 1, 2
+ATTENTION_WIDTH, ATTENTION_VALUE, MAX_NODES = 576, 512, 64
 
 
 def _struct(name, pointer_fields, scalar_fields):
@@ -138,6 +140,30 @@ SpeculateArgs = _struct("SpeculateArgs", (
         "reserved0")])
 
 
+SlotMapsArgs = _struct("SlotMapsArgs", (
+    "lengths", "counts", "held", "free_blocks", "head", "table", "positions", "slot_mapping", "requests", "starts", "ends",
+    "held_after", "taken", "status", "layout"), [(n, u32) for n in ("batch", "pages", "blocks", "tokens", "block", "queries")])
+
+
+class RotaryArgs(ctypes.Structure):
+    """KvipRotaryArgs: up to two sets of rows (queries, keys) with strides of their own."""
+
+    _fields_ = [("positions", vp), ("turns", vp)] + [(n, vp) for n in ("x0", "x1", "y0", "y1", "codes", "scales")] + [
+        (n, i64) for n in ("x_token0", "x_token1", "x_head0", "x_head1", "y_token0", "y_token1", "y_head0", "y_head1")] + [
+        (n, u32) for n in ("heads0", "heads1", "tokens", "width", "dim", "layout", "dtype")] + [("factor", f32)]
+
+
+AttentionArgs = _struct("AttentionArgs", (
+    "query", "pool", "slots", "requests", "row_owners", "starts", "draft", "ancestors", "out", "lse", "partial",
+    "partial_stats", "status"), [(n, i64) for n in ("query_token", "query_head", "draft_token")] + [("pool_rows", u64)] + [
+        (n, u32) for n in ("tokens", "heads", "entries", "batch", "queries", "output_stride", "dtype", "splits", "partial_rows",
+                           "wait_kilocycles")] + [("scale", f32), ("reserved0", u32)])
+
+VerifyArgs = _struct("VerifyArgs", (
+    "target", "draft", "tokens", "parents", "starts", "accept", "sample", "out_tokens", "out_nodes", "out_counts", "status"),
+    [("target_row", i64), ("draft_row", i64)] + [(n, u32) for n in ("rows", "vocabulary", "batch", "depth", "dtype", "reserved0")])
+
+
 class Context(ctypes.Structure):
     """KvipContext; reference: rotating::Context (include/context.h:36-52)."""
 
@@ -169,7 +195,8 @@ _STAGES = {
     "kvip_b200_ingest_spans": IngestSpanArgs, "kvip_b200_peer_exchange": PeerExchangeArgs,
     "kvip_b200_lru_commit": LruArgs, "kvip_b200_lidu": LiduArgs, "kvip_b200_publish_pages": PagesArgs,
     "kvip_b200_window_bounds": WindowArgs, "kvip_b200_resident_threshold": ThresholdArgs,
-    "kvip_b200_speculate_window": SpeculateArgs,
+    "kvip_b200_speculate_window": SpeculateArgs, "kvip_b200_slot_maps": SlotMapsArgs, "kvip_b200_rotary": RotaryArgs,
+    "kvip_b200_slot_attention": AttentionArgs, "kvip_b200_verify_drafts": VerifyArgs,
 }
 # every symbol include/kvip_b200.h declares
 EXPORTS = tuple(_STAGES) + (
@@ -223,6 +250,20 @@ def load_library(path=None):
 def last_error(library=None):
     lib = library or load_library()
     return lib.kvip_b200_last_error().decode(errors="replace")
+
+
+def enqueue(function, args, device, what):
+    """One entry point on the current stream of `device` (an index), which need not be the current device."""
+    import torch
+
+    stream = torch.cuda.current_stream(device).cuda_stream
+    if torch.cuda.current_device() == device:
+        code = function(ctypes.byref(args), stream)
+    else:
+        with torch.cuda.device(device):
+            code = function(ctypes.byref(args), stream)
+    if code:
+        check(code, what)
 
 
 def check(code, what, library=None):

@@ -1,0 +1,111 @@
+"""Block tables of the paged caches, kept on the GPU, and the slot maps of a step made from the requests' lengths there.
+
+The reference receives `metadata.slot_mapping`, positions and block tables from the serving framework's host code. A step
+that follows a verification of drafted tokens knows its lengths only on the GPU; `BlockTables` makes the maps from
+them in one launch, with no copy to the host and none from it: blocks from a free list, packed positions, slots and
+requests, and (for `QueryInputs.prepare_device`) the layout of the query slots."""
+from .. import _lib
+
+
+class BlockTables:
+    """State of `batch` requests over a pool of `blocks` blocks of `block` tokens: `table` [batch, pages] int32,
+    `lengths` [batch] cached tokens, `held` [batch] blocks in the row, `free` [blocks] and `head` [1], the first entry of
+    the free list that is still free. A step is
+
+        tables.plan(counts)       # one launch: appends blocks, fills positions, slot_mapping, requests, starts, ends
+        ...                       # the forward reads them
+        tables.commit(kept)       # lengths += kept (the tokens that stay), the blocks of the plan become the request's
+
+    `plan` changes nothing but the table entries behind `held`, so a step that is planned again plans the same. Outputs are
+    persistent buffers of this object, sized by `tokens` (packed tokens per step at most): the captured graph of a
+    step finds them at the same place. `status` collects KVIP_ERR_* bits (include/kvip_b200.h: KvipSlotMapsArgs)."""
+
+    def __init__(self, torch, device, *, batch, pages, blocks, tokens, block=_lib.BLOCK_TOKENS, queries=0):
+        self.torch = torch
+        device = torch.device(device)
+        if device.type != "cuda":
+            raise ValueError("BlockTables live on a CUDA device (kvip_b200 has no CPU path)")
+        if not 1 <= batch <= 1024 or pages < 1 or tokens < 1 or block < 1 or blocks < 0:
+            raise ValueError("BlockTables: 1..1024 requests, at least one page, one token and one token per block")
+        if pages * block > 0x7fffffff or batch * pages * block > 0xffffffff:
+            raise ValueError("BlockTables: pages * block must fit int32, batch * pages * block 32 bits")
+        if not 0 <= queries <= _lib.MAX_QUERIES:
+            raise ValueError("BlockTables: zero to four query slots per request")
+        self.batch, self.pages, self.blocks, self.tokens, self.block, self.queries = batch, pages, blocks, tokens, block, queries
+        i32, i64 = dict(dtype=torch.int32, device=device), dict(dtype=torch.int64, device=device)
+        self.lengths, self.held = torch.zeros(batch, **i32), torch.zeros(batch, **i32)
+        self.table = torch.full((batch, pages), -1, **i32)
+        self.free, self.head = torch.arange(max(1, blocks), **i32), torch.zeros(1, **i32)
+        self.positions, self.slot_mapping = torch.full((tokens,), -1, **i64), torch.full((tokens,), -1, **i64)
+        self.requests, self.starts = torch.full((tokens,), -1, **i32), torch.zeros(batch + 1, **i32)
+        self.ends, self.held_after = torch.zeros(batch, **i32), torch.zeros(batch, **i32)
+        self.taken, self.status = torch.zeros(1, **i32), torch.zeros(1, **i32)
+        self.layout = torch.zeros((4, batch * queries), **i64) if queries else None
+        self.device, self.index = self.table.device, self.table.get_device()
+        self.function = _lib.load_library().kvip_b200_slot_maps
+        outputs = (self.table, self.positions, self.slot_mapping, self.requests, self.starts, self.ends, self.held_after, self.taken,
+                   self.status)
+        self._outputs = tuple(t.data_ptr() for t in outputs) + (self.layout.data_ptr() if queries else None,)
+        self._state = (self.held.data_ptr(), self.free.data_ptr(), self.head.data_ptr())
+        self._sizes = (batch, pages, blocks, tokens, block, queries)
+
+    @property
+    def nbytes(self):
+        tensors = [self.lengths, self.held, self.table, self.free, self.head, self.positions, self.slot_mapping, self.requests,
+                   self.starts, self.ends, self.held_after, self.taken, self.status]
+        return sum(t.numel() * t.element_size() for t in tensors + ([self.layout] if self.queries else []))
+
+    def load(self, *, lengths, held, table, free, head=0):
+        """Take over a state made elsewhere (copies; the free list may be shorter than `blocks`)."""
+        if free.numel() > self.blocks or not 0 <= head <= free.numel():
+            raise ValueError("BlockTables.load: the free list does not fit")
+        if tuple(table.shape) != (self.batch, self.pages) or lengths.numel() != self.batch or held.numel() != self.batch:
+            raise ValueError("BlockTables.load: lengths, held and table must match the batch and its pages")
+        self.lengths.copy_(lengths)
+        self.held.copy_(held)
+        self.table.copy_(table)
+        gap = self.blocks - free.numel()          # the list ends where the storage ends
+        self.free[gap:self.blocks].copy_(free)
+        self.head.fill_(gap + head)
+
+    def plan(self, counts):
+        """Maps of a step that adds counts[b] tokens to request b (int32 [batch] on the device): one launch, no host
+        copy, capturable. Returns self."""
+        if (counts.dtype != self.torch.int32 or counts.ndim != 1 or counts.numel() != self.batch or counts.get_device() != self.index
+                or not counts.is_contiguous()):
+            raise ValueError("BlockTables counts must be contiguous int32 [batch] on the tables' device")
+        args = _lib.SlotMapsArgs(self.lengths.data_ptr(), counts.data_ptr(), *self._state, *self._outputs, *self._sizes)
+        _lib.enqueue(self.function, args, self.index, "slot_maps")
+        return self
+
+    def commit(self, kept):
+        """The planned blocks become the requests' own and `kept` [batch] int32 of the planned tokens stay (all of them, or
+        what a verification accepted). A request that keeps fewer holds its blocks for the tokens to come."""
+        self.lengths.add_(kept)
+        self.held.copy_(self.held_after)
+        self.head.add_(self.taken)
+
+    def release(self, rows):
+        """Requests that have ended (host list of row numbers): their blocks return to the free list, their rows are
+        empty. Fixed shapes, no device read on the host."""
+        rows = sorted(set(int(r) for r in rows))
+        if not rows:
+            return
+        if rows[0] < 0 or rows[-1] >= self.batch:
+            raise IndexError("BlockTables.release: row out of range")
+        torch = self.torch
+        index = torch.tensor(rows, dtype=torch.int64, device=self.device)
+        table, held = self.table[index], self.held[index]
+        page = torch.arange(self.pages, dtype=torch.int32, device=self.device)
+        mine = (page[None, :] < held[:, None]).reshape(-1)
+        order = mine.cumsum(0)
+        total = order[-1:]
+        # the list grows downwards from head; entries that are no block go to a place that is written back as it was
+        place = torch.where(mine, self.head.long() - total + order - 1, self.blocks)
+        longer = torch.cat((self.free[:self.blocks], self.free[:1]))
+        longer.scatter_(0, place, torch.where(mine, table.reshape(-1), longer[-1]))
+        self.free[:self.blocks].copy_(longer[:-1])
+        self.head.sub_(total.to(torch.int32))
+        self.table[index] = -1
+        self.held[index] = 0
+        self.lengths[index] = 0

@@ -1,0 +1,186 @@
+// Block tables and slot maps of a step from the requests' lengths (include/kvip_b200.h: KvipSlotMapsArgs).
+//
+// Two prefix sums over the requests (packed tokens, new blocks) decide everything, and they are small: every CTA makes
+// both in shared memory, then writes its own share of the packed tokens, of the table rows and of the layout. No CTA
+// needs another's result: a token on a page that this very launch appends takes the block from the free list, not from
+// the table. Bound by latency: the lengths, one page entry, the stores.
+#include "common.cuh"
+
+namespace kvip {
+namespace {
+
+constexpr uint32_t kMapThreads = 256;
+constexpr uint32_t kMapBatch = 1024;              // requests per launch
+constexpr uint32_t kPerThread = kMapBatch / kMapThreads;
+constexpr uint32_t kTokensPerThread = 4;
+
+struct Request {
+  int32_t length, count, held, fresh;   // count: tokens that are numbered; fresh: new blocks
+  bool placed;                          // false: its tokens get no slot
+};
+
+__global__ void __launch_bounds__(kMapThreads) slot_map_rows(const KvipSlotMapsArgs a) {
+  __shared__ uint32_t s_start[kMapBatch + 1], s_off[kMapBatch];
+  __shared__ int32_t s_length[kMapBatch], s_held[kMapBatch];
+  __shared__ uint8_t s_placed[kMapBatch];
+  __shared__ uint32_t scratch[33];
+  const uint32_t tid = threadIdx.x;
+  const int32_t head = a.head[0];
+  const int64_t available = head < 0 ? 0 : static_cast<int64_t>(a.blocks) - head;
+  const int64_t room = static_cast<int64_t>(a.pages) * a.block;
+  int32_t bad = 0;
+
+  // requests tid * kPerThread + i: consecutive per thread, so one block scan of the threads' sums orders them all
+  int32_t length[kPerThread], count[kPerThread], held[kPerThread];
+  uint32_t fresh[kPerThread], tokens_here = 0, fresh_here = 0;
+#pragma unroll
+  for (uint32_t i = 0; i < kPerThread; ++i) {
+    const uint32_t b = tid * kPerThread + i;
+    const bool live = b < a.batch;
+    length[i] = live ? a.lengths[b] : 0;
+    count[i] = live ? a.counts[b] : 0;
+    held[i] = live ? a.held[b] : 0;
+  }
+#pragma unroll
+  for (uint32_t i = 0; i < kPerThread; ++i) {
+    fresh[i] = 0;
+    const int64_t end = static_cast<int64_t>(length[i]) + count[i];
+    if (length[i] < 0 || count[i] < 0 || held[i] < 0 || held[i] > static_cast<int64_t>(a.pages) || end > room ||
+        (a.layout && count[i] > static_cast<int32_t>(a.queries))) {
+      bad |= static_cast<int32_t>(KVIP_ERR_TOKEN_RANGE);
+      count[i] = 0;
+    } else if (count[i] > 0) {
+      const int64_t need = (end + a.block - 1) / a.block;
+      if (need > held[i]) fresh[i] = static_cast<uint32_t>(need - held[i]);
+    }
+    tokens_here += static_cast<uint32_t>(count[i]);
+    fresh_here += fresh[i];
+  }
+  uint32_t total_tokens = 0;
+  uint32_t start = block_exclusive_scan(tokens_here, scratch, &total_tokens);
+  uint32_t off = block_exclusive_scan(fresh_here, scratch, nullptr);
+  // entries used: the requests up to the first one that the list cannot serve
+  uint32_t served = 0;
+#pragma unroll
+  for (uint32_t i = 0; i < kPerThread; ++i) {
+    const uint32_t b = tid * kPerThread + i;
+    const bool placed = fresh[i] == 0u || static_cast<int64_t>(off) + fresh[i] <= available;
+    if (!placed) bad |= static_cast<int32_t>(KVIP_ERR_NO_SLOT);
+    else if (fresh[i]) served = off + fresh[i];
+    if (b < a.batch) {
+      s_start[b] = start; s_off[b] = off; s_length[b] = length[i]; s_held[b] = held[i];
+      s_placed[b] = placed ? 1u : 0u;
+      if (blockIdx.x == 0) {
+        a.starts[b] = static_cast<int32_t>(min(start, a.tokens));
+        a.ends[b] = length[i] + (placed ? count[i] : 0);
+        a.held_after[b] = held[i] + (placed ? static_cast<int32_t>(fresh[i]) : 0);
+      }
+      if (b + 1 == a.batch) s_start[a.batch] = start + static_cast<uint32_t>(count[i]);
+    }
+    start += static_cast<uint32_t>(count[i]);
+    off += fresh[i];
+  }
+  if (total_tokens > a.tokens) bad |= static_cast<int32_t>(KVIP_ERR_TOKEN_RANGE);
+  const int any_bad = __syncthreads_or(bad);   // also publishes the shared tables
+  if (blockIdx.x == 0) {
+    // max over the block of `served`
+    const uint32_t most = __reduce_max_sync(0xffffffffu, served);
+    if ((tid & 31u) == 0) scratch[tid >> 5] = most;
+    __syncthreads();
+    if (tid == 0) {
+      uint32_t taken = 0;
+      for (uint32_t w = 0; w < kMapThreads / 32u; ++w) taken = max(taken, scratch[w]);
+      a.taken[0] = static_cast<int32_t>(taken);
+      a.starts[a.batch] = static_cast<int32_t>(min(total_tokens, a.tokens));
+    }
+    if (any_bad && bad) atomicOr(a.status, bad);
+  }
+
+  // the appended entries of the table rows: a warp per request
+  for (uint32_t b = blockIdx.x * (kMapThreads / 32u) + (tid >> 5); b < a.batch; b += gridDim.x * (kMapThreads / 32u)) {
+    if (!s_placed[b]) continue;
+    const int64_t end = static_cast<int64_t>(s_length[b]) + (s_start[b + 1] - s_start[b]);
+    const int32_t need = s_start[b + 1] == s_start[b] ? 0 : static_cast<int32_t>((end + a.block - 1) / a.block);
+    for (int32_t p = s_held[b] + static_cast<int32_t>(tid & 31u); p < need; p += 32)
+      a.table[static_cast<uint64_t>(b) * a.pages + p] = a.free_blocks[head + s_off[b] + (p - s_held[b])];
+  }
+
+  // packed tokens: four consecutive ones per thread, one search for the first
+  for (uint32_t t0 = (blockIdx.x * kMapThreads + tid) * kTokensPerThread; t0 < a.tokens;
+       t0 += gridDim.x * kMapThreads * kTokensPerThread) {
+    uint32_t lo = 0, hi = a.batch;   // largest b with s_start[b] <= t0
+    while (hi - lo > 1u) {
+      const uint32_t mid = (lo + hi) >> 1;
+      if (s_start[mid] <= t0) lo = mid; else hi = mid;
+    }
+    uint32_t b = lo;
+#pragma unroll
+    for (uint32_t i = 0; i < kTokensPerThread; ++i) {
+      const uint32_t t = t0 + i;
+      if (t >= a.tokens) break;
+      int64_t position = -1, slot = -1;
+      int32_t request = -1;
+      if (t < total_tokens) {
+        while (s_start[b + 1] <= t) ++b;
+        request = static_cast<int32_t>(b);
+        if (s_placed[b]) {
+          const uint32_t p = static_cast<uint32_t>(s_length[b]) + (t - s_start[b]);   // below pages * block
+          const uint32_t page = p / a.block, held_b = static_cast<uint32_t>(s_held[b]);
+          const int32_t block = page < held_b ? a.table[static_cast<uint64_t>(b) * a.pages + page]
+                                              : a.free_blocks[head + s_off[b] + (page - held_b)];
+          position = p;
+          if (block >= 0) slot = static_cast<int64_t>(block) * a.block + (p - page * a.block);
+        }
+      }
+      a.positions[t] = position;
+      a.slot_mapping[t] = slot;
+      a.requests[t] = request;
+    }
+  }
+
+  if (a.layout) {   // rows GATHER, QUERY_VALID, UNPACK, OUTPUT_VALID of the query slots
+    const uint32_t slots = a.batch * a.queries;
+    for (uint32_t s = blockIdx.x * kMapThreads + tid; s < slots; s += gridDim.x * kMapThreads) {
+      const uint32_t b = s / a.queries, q = s - b * a.queries;
+      const bool live = q < s_start[b + 1] - s_start[b];
+      a.layout[s] = live ? static_cast<int64_t>(s_start[b] + q) : 0;
+      a.layout[slots + s] = live ? 1 : 0;
+      int64_t from = 0;
+      if (s < total_tokens) {
+        uint32_t lo = 0, hi = a.batch;
+        while (hi - lo > 1u) {
+          const uint32_t mid = (lo + hi) >> 1;
+          if (s_start[mid] <= s) lo = mid; else hi = mid;
+        }
+        while (s_start[lo + 1] <= s) ++lo;
+        from = static_cast<int64_t>(lo) * a.queries + (s - s_start[lo]);
+      }
+      a.layout[2 * slots + s] = from;
+      a.layout[3 * slots + s] = s < total_tokens ? 1 : 0;
+    }
+  }
+}
+
+}  // namespace
+}  // namespace kvip
+
+extern "C" uint32_t kvip_b200_slot_maps(const KvipSlotMapsArgs* a, void* stream) {
+  using namespace kvip;
+  KVIP_REQUIRE(a && a->lengths && a->counts && a->held && a->free_blocks && a->head && a->table && a->positions &&
+                   a->slot_mapping && a->requests && a->starts && a->ends && a->held_after && a->taken && a->status,
+               "slot_maps: null pointer");
+  KVIP_REQUIRE(a->batch >= 1 && a->batch <= kMapBatch, "slot_maps: batch must be in 1..1024");
+  KVIP_REQUIRE(a->block >= 1 && a->pages >= 1 && static_cast<uint64_t>(a->pages) * a->block <= 0x7fffffffull,
+               "slot_maps: pages * block must fit int32");
+  // the packed numbering is kept in 32 bits
+  KVIP_REQUIRE(static_cast<uint64_t>(a->batch) * a->pages * a->block <= 0xffffffffull && a->tokens >= 1 && a->tokens <= 0x7fffffffu,
+               "slot_maps: batch * pages * block must fit 32 bits, tokens 31");
+  KVIP_REQUIRE(a->blocks <= 0x7fffffffu, "slot_maps: too many blocks");
+  KVIP_REQUIRE(!a->layout || (a->queries >= 1 && a->queries <= KVIP_MAX_QUERIES), "slot_maps: 1..4 query slots per request");
+  const uint32_t share = kMapThreads * kTokensPerThread;
+  uint32_t grid = (a->tokens + share - 1) / share;
+  if (grid > device_sm_count()) grid = device_sm_count();
+  slot_map_rows<<<grid, kMapThreads, 0, static_cast<cudaStream_t>(stream)>>>(*a);
+  count_launch();
+  return check_launch("slot_map_rows");
+}
