@@ -122,6 +122,9 @@ extern "C" uint32_t kvip_b200_slot_attention(const KvipAttentionArgs* a, void* s
   KVIP_REQUIRE(((reinterpret_cast<uintptr_t>(a->query) | reinterpret_cast<uintptr_t>(a->pool) | reinterpret_cast<uintptr_t>(a->out) |
                  reinterpret_cast<uintptr_t>(a->draft)) & 15u) == 0 && ((a->query_token | a->query_head | a->draft_token) & 7) == 0,
                "slot_attention: 16-byte aligned rows");
+  KVIP_REQUIRE(a->splits <= 1 || (a->partial && a->partial_stats &&
+                                  static_cast<uint64_t>(a->splits) * a->tokens * a->heads <= a->partial_rows),
+               "slot_attention: the workspace does not hold the shares");
   const dim3 grid(a->tokens, (a->heads + 3u) / 4u);
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (a->dtype == KVIP_FLOAT_BF16) attend_rows<__nv_bfloat16><<<grid, 128, 0, s>>>(*a);
