@@ -21,7 +21,9 @@ void set_error(const char* message);
 // count belong to ONE device: a process that drives several GPUs configures every kernel once per device.
 enum KernelSlot : uint32_t {
   kSlotLiFp8, kSlotLiBf16, kSlotTopkSelect, kSlotTopkMerge, kSlotTopkMergeCluster, kSlotTopkPivot, kSlotSplitEmit, kSlotSplitFallback,
-  kSlotResolve, kSlotLidu, kSlotCount
+  kSlotResolve, kSlotLidu,
+  kSlotAttentionBf16, kSlotAttentionFp16 = kSlotAttentionBf16 + 4,   // a slot per width of the head group
+  kSlotCount = kSlotAttentionFp16 + 4
 };
 // Raises the dynamic shared-memory limit of `kernel` on the current device the first time it is asked to there.
 // Returns 0, or the launch-error code with the message set.

@@ -1,7 +1,22 @@
 // Attention of packed query tokens over selected pool rows and drafted rows (include/kvip_b200.h: KvipAttentionArgs).
 //
-// One warp per (token, head), one pass over the token's rows with the running maximum and sum of the softmax. A lane
-// holds 18 query elements (16 of the value part, 2 of the rest) and 16 accumulators.
+//   out[t,h] = sum_j p_j v_j / sum_j p_j,   p_j = 2^(scale' q.k_j - ref),   v_j = the first 512 elements of k_j
+//
+// A CTA takes one share of the rows of one (token, group of at most 64 heads) and turns the products round so that the
+// gathered rows are always the M operand and the heads the N operand:
+//
+//   S^T [64 rows x heads]   = K [64 x 576] . Q^T            (one accumulator lane per row, one column per head)
+//   O^T [512 x heads]      += V^T [512 x 64] . P^T [64 x heads]   (four accumulators of 128 value elements)
+//
+// Both read the same tile in shared memory: a row is nine 128-byte pieces, each piece a column of the 128-byte swizzle
+// atom, K-major for the first product (elements along K) and M-major for the second (elements along M, rows along K).
+// So every row is fetched once, 512 accumulator columns of a [heads x 512] output become 4 x heads <= 256, and small head
+// counts cost small N. Rows as lanes also make the softmax cheap: p is scaled by a reference `ref` per head that only has
+// to be near the running maximum, so a tile needs no reduction over rows unless some score leaves ref + 8 (then the
+// maximum is taken, and the accumulators and sums are rescaled); sums of p stay per thread until the end.
+//
+// p is rounded to the rows' type for the second product (half a step, as the output is); its sum is taken before the
+// rounding, in fp32, because the log-sum is an output too.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include "common.cuh"
@@ -10,101 +25,595 @@ namespace kvip {
 namespace {
 
 constexpr uint32_t kWidth = KVIP_ATTENTION_WIDTH, kValue = KVIP_ATTENTION_VALUE;
+constexpr uint32_t kTile = 64;                          // rows per tile
+constexpr uint32_t kPieces = kWidth / 64;               // 128-byte pieces per row
+constexpr uint32_t kPieceBytes = kTile * 128;           // one piece of every row of a tile
+constexpr uint32_t kStageBytes = kPieces * kPieceBytes; // 73,728
+constexpr uint32_t kStages = 2;
+constexpr uint32_t kGroupHeads = 64;
+constexpr uint32_t kLoaders = 128;                      // threads that fill one stage; a group of them per stage
+// Warpgroups: softmax (warps 0-3), MMA issuer (warp 4; 5-7 idle), two loader groups. 512 threads start with 128 registers;
+// 184 + 72 + 2 x 112 is within that total, and the softmax keeps two rows of 64 heads in registers without spilling.
+constexpr uint32_t kSoftmaxWarps = 4, kMmaWarp = 4, kFirstLoaderWarp = 8;
+constexpr uint32_t kSoftmaxRegisters = 184, kMmaRegisters = 72, kLoaderRegisters = 112;
+constexpr uint32_t kAttentionThreads = 32 * kFirstLoaderWarp + kStages * kLoaders;
+constexpr float kSlack = 8.f;                           // log2: p may reach 2^8 before the reference moves
+constexpr uint32_t kDefaultWaitKilocycles = 2000000u;   // about one second of SM clock
 
-__device__ __forceinline__ float2 pair_to_float(uint32_t w, __nv_bfloat16) {
-  return __bfloat1622float2(*reinterpret_cast<__nv_bfloat162*>(&w));
+struct Control {                                        // behind the tiles in shared memory
+  uint64_t full[kStages], empty[kStages], scored[2], weighted, query_full;
+  uint64_t source[kStages][kTile];                      // address of every row of the stage's tile, 0 = no row
+  uint32_t valid[kStages][2];                           // bit per row
+  float reduce[kSoftmaxWarps][kGroupHeads];
+  float factor[kGroupHeads];
+  uint32_t tmem, abort_flag, last;
+};
+
+template <uint32_t kN> struct Layout {
+  static constexpr uint32_t kQuery = kStages * kStageBytes;
+  static constexpr uint32_t kWeights = kQuery + kPieces * kN * 128;
+  static constexpr uint32_t kControl = kWeights + kTile * 128;
+  static constexpr uint32_t kBytes = kControl + sizeof(Control);
+};
+static_assert(Layout<kGroupHeads>::kBytes <= 227 * 1024, "shared memory");
+
+__device__ __forceinline__ uint32_t smem_u32(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
+__device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
+  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
 }
-__device__ __forceinline__ float2 pair_to_float(uint32_t w, __half) { return __half22float2(*reinterpret_cast<__half2*>(&w)); }
-__device__ __forceinline__ uint32_t pair_from_float(float x, float y, __nv_bfloat16) {
+__device__ __forceinline__ void mbar_arrive(uint32_t bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ bool mbar_test(uint32_t bar, uint32_t parity) {
+  uint32_t done;
+  asm volatile("{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+               : "=r"(done) : "r"(bar), "r"(parity) : "memory");
+  return done != 0u;
+}
+__device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
+  uint32_t done;
+  asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+               : "=r"(done) : "r"(bar), "r"(parity) : "memory");
+  return done != 0u;
+}
+struct Waits {
+  volatile uint32_t* abort_flag;   // set by the first wait of the CTA that gives up; read by all the others
+  long long limit;                 // SM clock cycles a wait may take
+};
+__device__ __forceinline__ bool mbar_wait_slow(uint32_t bar, uint32_t parity, const Waits& w) {
+  const long long start = clock64();
+  for (;;) {
+    for (int i = 0; i < 32; ++i)
+      if (mbar_try(bar, parity)) return true;
+    if (*w.abort_flag) return false;
+    if (clock64() - start > w.limit) break;
+  }
+  *w.abort_flag = 1u;
+  return false;
+}
+__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, const Waits& w) {
+  return mbar_try(bar, parity) || mbar_wait_slow(bar, parity, w);
+}
+// Barrier of one role's 128 threads that also tells all of them whether any has `flag`.
+__device__ __forceinline__ bool role_any(uint32_t id, bool flag) {
+  uint32_t any;
+  asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbarrier.cta.red.or.pred q, %2, 128, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+               : "=r"(any) : "r"(flag ? 1u : 0u), "r"(id) : "memory");
+  return any != 0u;
+}
+__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+__device__ __forceinline__ void commit(uint32_t bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool accumulate) {
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+               ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate ? 1u : 0u) : "memory");
+}
+// Shared-memory operand in 128-byte swizzle, 8-row groups 1024 bytes apart; `pieces` is the distance between 64-element
+// columns of an M-major operand (unused by K-major ones).
+__device__ __forceinline__ uint64_t operand(uint32_t address, uint32_t pieces) {
+  return static_cast<uint64_t>((address & 0x3ffffu) >> 4) | (static_cast<uint64_t>(pieces >> 4) << 16) |
+         (static_cast<uint64_t>(1024u >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+// 16 lanes x 16 fp32 columns: a thread holds rows lane/4 (v[0], v[1], v[4], v[5]) and lane/4 + 8, columns 2 (lane%4) + {0, 1}
+// of each 8.
+__device__ __forceinline__ void tmem_ld_scores(uint32_t address, uint32_t* v) {
+  asm volatile("tcgen05.ld.sync.aligned.16x256b.x2.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]) : "r"(address) : "memory");
+}
+// 32 lanes x 16 fp32 columns: a thread holds its lane's row.
+__device__ __forceinline__ void tmem_ld_rows(uint32_t address, uint32_t (&v)[16]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+               : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
+                 "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+               : "r"(address) : "memory");
+}
+__device__ __forceinline__ void tmem_st_rows(uint32_t address, const uint32_t (&v)[16]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
+               ::"r"(address), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]),
+                 "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+               : "memory");
+}
+__device__ __forceinline__ void tmem_ld_done() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_st_done() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// 16 bytes of a row into shared memory, zeros where `present` is false.
+__device__ __forceinline__ void copy16(uint32_t to, const void* from, bool present) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(present ? 16u : 0u) : "memory");
+}
+template <typename T> __device__ __forceinline__ uint32_t pack_pair(float x, float y);
+template <> __device__ __forceinline__ uint32_t pack_pair<__nv_bfloat16>(float x, float y) {
   __nv_bfloat162 v = __floats2bfloat162_rn(x, y);
   return *reinterpret_cast<uint32_t*>(&v);
 }
-__device__ __forceinline__ uint32_t pair_from_float(float x, float y, __half) {
+template <> __device__ __forceinline__ uint32_t pack_pair<__half>(float x, float y) {
   __half2 v = __floats2half2_rn(x, y);
   return *reinterpret_cast<uint32_t*>(&v);
 }
+template <typename T> __device__ __forceinline__ T round_to(float x);
+template <> __device__ __forceinline__ __nv_bfloat16 round_to(float x) { return __float2bfloat16_rn(x); }
+template <> __device__ __forceinline__ __half round_to(float x) { return __float2half_rn(x); }
 
-template <typename T>
-__global__ void __launch_bounds__(128) attend_rows(const KvipAttentionArgs a) {
-  const uint32_t lane = threadIdx.x & 31u, t = blockIdx.x, h = blockIdx.y * 4u + (threadIdx.x >> 5);
-  if (h >= a.heads) return;
+// What token t may read.
+struct Rows {
+  const uint8_t* pool;        // first row of the owner
+  const uint8_t* draft;       // first drafted row of the request
+  uint64_t draft_bytes, seen; // distance of drafted rows; the ones the token sees
+  uint32_t limit, drafted;    // rows of the owner (0: none may be read), drafted rows of the request
+  int32_t bad;
+};
+__device__ __forceinline__ Rows rows_of(const KvipAttentionArgs& a, uint32_t t, int32_t request) {
+  Rows r{static_cast<const uint8_t*>(a.pool), nullptr, static_cast<uint64_t>(a.draft_token) * 2u, 0ull, a.output_stride, 0u, 0};
+  if (static_cast<uint32_t>(request) >= a.batch) {
+    r.limit = 0;
+    r.bad = static_cast<int32_t>(KVIP_ERR_TOKEN_RANGE);
+    return r;
+  }
+  const int32_t owner = a.row_owners ? a.row_owners[request] : request;
+  const uint64_t base = static_cast<uint64_t>(static_cast<uint32_t>(owner)) * a.output_stride;
+  if (owner < 0 || base + a.output_stride > a.pool_rows) {
+    r.limit = 0;
+    r.bad = static_cast<int32_t>(KVIP_ERR_SOURCE);
+  } else {
+    r.pool += base * (kWidth * 2u);
+  }
+  if (a.draft) {
+    const int64_t first = a.starts[request], behind = a.starts[request + 1], own = static_cast<int64_t>(t) - first;
+    if (first < 0 || behind < first || behind > static_cast<int64_t>(a.tokens)) {
+      r.bad |= static_cast<int32_t>(KVIP_ERR_TOKEN_RANGE);
+    } else {
+      r.drafted = static_cast<uint32_t>(min(static_cast<int64_t>(64), behind - first));
+      r.draft = static_cast<const uint8_t*>(a.draft) + static_cast<uint64_t>(first) * r.draft_bytes;
+      r.seen = a.ancestors ? static_cast<uint64_t>(a.ancestors[t]) : (own < 0 ? 0ull : own >= 63 ? ~0ull : (2ull << own) - 1ull);
+      if (r.drafted < 64u) r.seen &= (1ull << r.drafted) - 1ull;
+      r.drafted = r.seen ? 64u - static_cast<uint32_t>(__clzll(static_cast<long long>(r.seen))) : 0u;
+    }
+  }
+  return r;
+}
+
+template <typename T, uint32_t kN>
+__global__ void __launch_bounds__(kAttentionThreads, 1)
+attend_tiles(const __grid_constant__ KvipAttentionArgs a, const uint32_t groups, const uint32_t group_heads, const uint32_t splits) {
+  extern __shared__ __align__(1024) uint8_t smem[];
+  const uint32_t base = smem_u32(smem);
+  Control& c = *reinterpret_cast<Control*>(smem + Layout<kN>::kControl);
+  const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u;
+  const uint32_t split = blockIdx.x % splits, unit = blockIdx.x / splits, group = unit % groups, t = unit / groups;
+  const uint32_t head0 = group * group_heads, heads = min(group_heads, a.heads - head0);
   const int32_t request = a.requests ? a.requests[t] : static_cast<int32_t>(t / a.queries);
   if (request < 0) return;
-  int32_t bad = 0;
-  uint64_t base = 0;
-  uint32_t drafted = 0, limit = a.output_stride;
-  int64_t first = 0;
-  uint64_t seen = 0;
-  if (static_cast<uint32_t>(request) >= a.batch) {
-    bad = static_cast<int32_t>(KVIP_ERR_TOKEN_RANGE);
-    limit = 0;
-  } else {
-    const int32_t owner = a.row_owners ? a.row_owners[request] : request;
-    base = static_cast<uint64_t>(static_cast<uint32_t>(owner)) * a.output_stride;
-    if (owner < 0 || base + a.output_stride > a.pool_rows) { bad = static_cast<int32_t>(KVIP_ERR_SOURCE); limit = 0; }
-    if (a.draft) {
-      first = a.starts[request];
-      const int64_t behind = a.starts[request + 1];
-      if (first < 0 || behind < first || behind > static_cast<int64_t>(a.tokens)) bad |= static_cast<int32_t>(KVIP_ERR_TOKEN_RANGE);
-      else drafted = static_cast<uint32_t>(min(static_cast<int64_t>(64), behind - first));
-      const int64_t own = static_cast<int64_t>(t) - first;
-      seen = a.ancestors ? static_cast<uint64_t>(a.ancestors[t])
-                         : (own < 0 ? 0ull : own >= 63 ? ~0ull : (2ull << own) - 1ull);
-    }
-  }
-  const uint32_t* q = reinterpret_cast<const uint32_t*>(static_cast<const T*>(a.query) + t * a.query_token + h * a.query_head);
-  float2 qv[9], acc[8];
-#pragma unroll
-  for (uint32_t i = 0; i < 9; ++i) {
-    qv[i] = pair_to_float(q[i * 32u + lane], T());
-    qv[i].x *= a.scale; qv[i].y *= a.scale;
-  }
-#pragma unroll
-  for (uint32_t i = 0; i < 8; ++i) acc[i] = make_float2(0.f, 0.f);
-  float top = -INFINITY, total = 0.f;
+  const Rows rows = rows_of(a, t, request);
   const int32_t* list = a.slots + static_cast<uint64_t>(t) * a.entries;
-  for (uint32_t k = 0; k < a.entries + drafted; ++k) {
-    const T* row;
-    if (k < a.entries) {
-      const int32_t slot = list[k];
-      if (slot < 0) continue;
-      if (static_cast<uint32_t>(slot) >= limit) { bad |= static_cast<int32_t>(KVIP_ERR_SOURCE); continue; }
-      row = static_cast<const T*>(a.pool) + (base + static_cast<uint32_t>(slot)) * kWidth;
-    } else {
-      const uint32_t j = k - a.entries;
-      if (!((seen >> j) & 1ull)) continue;
-      row = static_cast<const T*>(a.draft) + (first + j) * a.draft_token;
+
+  auto bar = [&](const uint64_t& b) { return smem_u32(&b); };
+  if (tid == 0) {
+    for (uint32_t s = 0; s < kStages; ++s) { mbar_init(bar(c.full[s]), kLoaders); mbar_init(bar(c.empty[s]), 1); }
+    mbar_init(bar(c.scored[0]), 1); mbar_init(bar(c.scored[1]), 1);
+    mbar_init(bar(c.weighted), 128); mbar_init(bar(c.query_full), kStages * kLoaders);
+    c.abort_flag = 0;
+    c.last = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    fence_async();
+  }
+  if (warp == kMmaWarp) {  // all of tensor memory: one CTA per SM
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&c.tmem)) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  // lists end in -1 where a context is short: the last entry in use bounds the tiles
+  uint32_t last = 0;
+  if (rows.limit)
+    for (uint32_t k = tid; k < a.entries; k += kAttentionThreads)
+      if (list[k] >= 0) last = k + 1u;
+  last = __reduce_max_sync(0xffffffffu, last);
+  fence_before();
+  __syncthreads();
+  fence_after();
+  if (lane == 0 && last) atomicMax(&c.last, last);
+  __syncthreads();
+  const uint32_t tmem = c.tmem;
+  const uint32_t listed = c.last, total = listed + rows.drafted;
+  const uint32_t tiles = (total + kTile - 1) / kTile;
+  const uint32_t first = static_cast<uint32_t>(static_cast<uint64_t>(tiles) * split / splits);
+  const uint32_t behind = static_cast<uint32_t>(static_cast<uint64_t>(tiles) * (split + 1) / splits);
+  const uint32_t count = behind - first;
+  const Waits waits{&c.abort_flag, static_cast<long long>(a.wait_kilocycles ? a.wait_kilocycles : kDefaultWaitKilocycles) << 10};
+  constexpr uint32_t kScores = 0, kOut = 2 * kN;   // tensor-memory columns: two score tiles, four value blocks
+
+  if (warp >= kFirstLoaderWarp) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kLoaderRegisters));
+    // ================= loaders: group g fills stage g with the tiles g, g + 2, ... =================
+    const uint32_t g = (warp - kFirstLoaderWarp) >> 2, i = tid - 32u * kFirstLoaderWarp - g * kLoaders;
+    if (count) {
+      const uint8_t* query = reinterpret_cast<const uint8_t*>(static_cast<const T*>(a.query) + t * a.query_token + head0 * a.query_head);
+      for (uint32_t x = g * kLoaders + i; x < kN * 72u; x += kStages * kLoaders) {
+        const uint32_t h = x / 72u, u = x - h * 72u;
+        copy16(base + Layout<kN>::kQuery + (u >> 3) * (kN * 128u) + h * 128u + (((u & 7u) ^ (h & 7u)) << 4),
+               query + (h < heads ? static_cast<uint64_t>(h) * a.query_head * 2u : 0ull) + u * 16u, h < heads);
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+      int32_t bad = 0;
+      bool query_sent = false, stop = false;
+      auto entry_of = [&](uint32_t n) -> int32_t {   // list entry of row i of tile n, -1 behind the list
+        const uint32_t k = (first + n) * kTile + i;
+        return i < kTile && n < count && k < listed ? list[k] : -1;
+      };
+      int32_t slot = entry_of(g);
+      for (uint32_t n = g; n < count; n += kStages) {
+        const bool ok = mbar_wait(bar(c.empty[g]), ((n >> 1) & 1u) ^ 1u, waits);
+        if (i < kTile) {
+          const uint32_t k = (first + n) * kTile + i;
+          uint64_t source = 0;
+          if (k < listed) {
+            if (slot >= 0) {
+              if (static_cast<uint32_t>(slot) < rows.limit) source = reinterpret_cast<uint64_t>(rows.pool) + static_cast<uint64_t>(slot) * (kWidth * 2u);
+              else bad |= static_cast<int32_t>(KVIP_ERR_SOURCE);
+            }
+          } else if (k < total && ((rows.seen >> (k - listed)) & 1ull)) {
+            source = reinterpret_cast<uint64_t>(rows.draft) + (k - listed) * rows.draft_bytes;
+          }
+          c.source[g][i] = source;
+          const uint32_t present = __ballot_sync(0xffffffffu, source != 0);
+          if (lane == 0) c.valid[g][i >> 5] = present;
+        }
+        slot = entry_of(n + kStages);      // lands while this tile is fetched
+        if (role_any(2u + g, !ok)) { stop = true; break; }
+        const bool any = (c.valid[g][0] | c.valid[g][1]) != 0u;
+        if (any) {
+          uint32_t row = i / 72u, u = i - row * 72u;
+#pragma unroll 9
+          for (uint32_t x = 0; x < kTile * 72u / kLoaders; ++x) {
+            const uint64_t source = c.source[g][row];
+            copy16(base + g * kStageBytes + (u >> 3) * kPieceBytes + row * 128u + (((u & 7u) ^ (row & 7u)) << 4),
+                   reinterpret_cast<const void*>((source ? source : reinterpret_cast<uint64_t>(a.pool)) + u * 16u), source != 0);
+            u += kLoaders - 72u; ++row;
+            if (u >= 72u) { u -= 72u; ++row; }
+          }
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        if (!query_sent) {
+          asm volatile("cp.async.wait_group 1;" ::: "memory");
+          fence_async();
+          mbar_arrive(bar(c.query_full));
+          query_sent = true;
+        }
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+        fence_async();
+        mbar_arrive(bar(c.full[g]));
+      }
+      if (!query_sent) {
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+        fence_async();
+        if (!stop) mbar_arrive(bar(c.query_full));
+      }
+      asm volatile("cp.async.wait_all;" ::: "memory");
+      if (i == 0 && g == 0) bad |= rows.bad;
+      if (bad) atomicOr(a.status, bad);
+    } else if (rows.bad && i == 0 && g == 0) {
+      atomicOr(a.status, rows.bad);
     }
-    const uint32_t* w = reinterpret_cast<const uint32_t*>(row);
-    float2 v[9];
-    float dot = 0.f;
+  } else if (warp >= kMmaWarp) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kMmaRegisters));
+    // ================= MMA issuer: one thread =================
+    if (warp == kMmaWarp && lane == 0 && count) {
+      constexpr uint32_t kFormat = sizeof(T) == 2 && __is_same(T, __nv_bfloat16) ? 1u : 0u;
+      constexpr uint32_t kBase = (1u << 4) | (kFormat << 7) | (kFormat << 10) | ((kN >> 3) << 17);
+      constexpr uint32_t kScoreDesc = kBase | ((64u >> 4) << 24);
+      constexpr uint32_t kValueDesc = kBase | (1u << 15) | (1u << 16) | ((128u >> 4) << 24);   // both operands M/N-major
+      bool written = false, alive = mbar_wait(bar(c.query_full), 0, waits);
+      auto score = [&](uint32_t n) {         // S^T of tile n, whose rows are in place
+        const uint32_t s = n & 1u;
+        if (!(c.valid[s][0] | c.valid[s][1])) { mbar_arrive(bar(c.scored[s])); return; }
+        fence_after();
+        const uint32_t d = tmem + kScores + s * kN;
+        uint64_t da = operand(base + s * kStageBytes, 16u), db = operand(base + Layout<kN>::kQuery, 16u);
+        asm volatile("" : "+l"(da), "+l"(db));   // offsets are added at each use, not kept in registers over the tiles
 #pragma unroll
-    for (uint32_t i = 0; i < 9; ++i) {
-      v[i] = pair_to_float(w[i * 32u + lane], T());
-      dot = fmaf(qv[i].x, v[i].x, dot);
-      dot = fmaf(qv[i].y, v[i].y, dot);
+        for (uint32_t piece = 0; piece < kPieces; ++piece) {
+#pragma unroll
+          for (uint32_t k = 0; k < 4; ++k)
+            mma(d, da + (piece * (kPieceBytes >> 4) + 2u * k), db + (piece * (kN * 8u) + 2u * k), kScoreDesc, (piece | k) != 0u);
+        }
+        commit(bar(c.scored[s]));
+      };
+      uint32_t scored = 0;                   // tiles whose scores have been issued
+      for (uint32_t n = 0; alive && n < count; ++n) {
+        const uint32_t s = n & 1u, phase = (n >> 1) & 1u;
+        if (scored == n) {
+          if (!mbar_wait(bar(c.full[s]), phase, waits)) break;
+          score(n);
+          ++scored;
+        }
+        // while the weights of tile n are made: the scores of the next tile, if its rows have come
+        if (scored == n + 1 && n + 1 < count) {
+          const uint32_t s1 = s ^ 1u, phase1 = ((n + 1) >> 1) & 1u;
+          while (!mbar_test(bar(c.weighted), n & 1u)) {
+            if (mbar_test(bar(c.full[s1]), phase1)) {
+              score(n + 1);
+              ++scored;
+              break;
+            }
+            if (c.abort_flag) break;
+          }
+        }
+        if (!mbar_wait(bar(c.weighted), n & 1u, waits)) break;
+        if (!(c.valid[s][0] | c.valid[s][1])) { commit(bar(c.empty[s])); continue; }   // in order behind the products before
+        fence_after();
+        uint64_t da = operand(base + s * kStageBytes, kPieceBytes), db = operand(base + Layout<kN>::kWeights, 16u);
+        asm volatile("" : "+l"(da), "+l"(db));
+#pragma unroll
+        for (uint32_t m = 0; m < 4; ++m) {
+#pragma unroll
+          for (uint32_t k = 0; k < kTile / 16u; ++k)
+            mma(tmem + kOut + m * kN, da + (2u * m * (kPieceBytes >> 4) + k * 128u), db + k * 128u, kValueDesc, written || k != 0u);
+        }
+        written = true;
+        commit(bar(c.empty[s]));
+      }
     }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegisters));
+    // ================= softmax: rows 16 w + lane / 4 and + 8 of every tile =================
+    constexpr uint32_t kBlocks = kN / 8;     // blocks of eight heads; a thread holds two of each
+    float ref[2 * kBlocks], sum[2 * kBlocks];
 #pragma unroll
-    for (uint32_t o = 16; o > 0; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
-    const float next = fmaxf(top, dot);
-    const float shrink = expf(top - next), p = expf(dot - next);
-    top = next;
-    total = total * shrink + p;
+    for (uint32_t j = 0; j < 2 * kBlocks; ++j) { ref[j] = -INFINITY; sum[j] = 0.f; }
+    const float scale = a.scale * 1.4426950408889634f;
+    const uint32_t quad = (warp * 32u) << 16;
+    const uint32_t row0 = warp * 16u + (lane >> 2);
+    bool dead = false, written = false;
+    for (uint32_t n = 0; n < count; ++n) {
+      const uint32_t s = n & 1u, phase = (n >> 1) & 1u;
+      bool ok = !dead && mbar_wait(bar(c.scored[s]), phase, waits) && mbar_wait(bar(c.full[s]), phase, waits);
+      ok = __all_sync(0xffffffffu, ok);
+      const uint32_t present = c.valid[s][warp >> 1] >> ((warp & 1u) * 16u);
+      const bool empty = ok && !(c.valid[s][0] | c.valid[s][1]);
+      if (empty) { mbar_arrive(bar(c.weighted)); continue; }   // the same for all: the mask belongs to the tile
+      const bool has0 = (present >> (lane >> 2)) & 1u, has1 = (present >> ((lane >> 2) + 8u)) & 1u;
+      uint32_t v[4 * kBlocks];
+      if (ok) {
+        fence_after();
 #pragma unroll
-    for (uint32_t i = 0; i < 8; ++i) {
-      acc[i].x = acc[i].x * shrink + p * v[i].x;
-      acc[i].y = acc[i].y * shrink + p * v[i].y;
+        for (uint32_t j = 0; j < kBlocks; j += 2) tmem_ld_scores(tmem + quad + kScores + s * kN + j * 8u, v + 4 * j);
+        tmem_ld_done();
+      }
+      // d = scale' s - ref; one score more than 2^8 above its reference makes the whole role take the maximum
+      bool above = false;
+#pragma unroll
+      for (uint32_t j = 0; j < 2 * kBlocks; ++j) {
+        const uint32_t at = (j >> 1) * 4u + (j & 1u);
+        const float x0 = __uint_as_float(v[at]), x1 = __uint_as_float(v[at + 2]);
+        above |= (has0 && fmaf(x0, scale, -ref[j]) > kSlack) || (has1 && fmaf(x1, scale, -ref[j]) > kSlack);
+      }
+      if (role_any(1u, above || !ok)) {
+        if (role_any(1u, !ok)) { dead = true; break; }
+#pragma unroll
+        for (uint32_t j = 0; j < 2 * kBlocks; ++j) {
+          const uint32_t at = (j >> 1) * 4u + (j & 1u);
+          float top = fmaxf(has0 ? __uint_as_float(v[at]) * scale : -INFINITY, has1 ? __uint_as_float(v[at + 2]) * scale : -INFINITY);
+#pragma unroll
+          for (uint32_t o = 4; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+          if (lane < 4) c.reduce[warp][(j >> 1) * 8u + lane * 2u + (j & 1u)] = top;
+        }
+        role_any(1u, false);
+#pragma unroll
+        for (uint32_t j = 0; j < 2 * kBlocks; ++j) {
+          const uint32_t h = (j >> 1) * 8u + (lane & 3u) * 2u + (j & 1u);
+          const float top = fmaxf(fmaxf(c.reduce[0][h], c.reduce[1][h]), fmaxf(c.reduce[2][h], c.reduce[3][h]));
+          const float next = fmaxf(ref[j], top);
+          const float factor = next == ref[j] ? 1.f : exp2_fast(ref[j] - next);   // 0 the first time
+          ref[j] = next;
+          sum[j] *= factor;
+          if (warp == 0 && lane < 4) c.factor[h] = factor;
+        }
+        role_any(1u, false);
+        if (written) {                         // the accumulators hold the tiles before this one, which must be in
+          const uint32_t before = n - 1u;      // stages are released in order, an empty tile's too
+          ok = mbar_wait(bar(c.empty[before & 1u]), (before >> 1) & 1u, waits);
+          if (__all_sync(0xffffffffu, ok)) {
+            fence_after();
+            for (uint32_t m = 0; m < 4; ++m) {
+#pragma unroll
+              for (uint32_t h = 0; h < kN; h += 16) {
+                uint32_t o[16];
+                tmem_ld_rows(tmem + quad + kOut + m * kN + h, o);
+                tmem_ld_done();
+#pragma unroll
+                for (uint32_t x = 0; x < 16; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * c.factor[h + x]);
+                tmem_st_rows(tmem + quad + kOut + m * kN + h, o);
+              }
+            }
+            tmem_st_done();
+          } else {
+            dead = true;
+          }
+        }
+      }
+      uint32_t p[2 * kBlocks];                 // weights of a row, two heads in a word: row 0 then row 1
+#pragma unroll
+      for (uint32_t j = 0; j < kBlocks; ++j) {
+        const float x0 = has0 ? exp2_fast(fmaf(__uint_as_float(v[4 * j]), scale, -ref[2 * j])) : 0.f;
+        const float y0 = has0 ? exp2_fast(fmaf(__uint_as_float(v[4 * j + 1]), scale, -ref[2 * j + 1])) : 0.f;
+        const float x1 = has1 ? exp2_fast(fmaf(__uint_as_float(v[4 * j + 2]), scale, -ref[2 * j])) : 0.f;
+        const float y1 = has1 ? exp2_fast(fmaf(__uint_as_float(v[4 * j + 3]), scale, -ref[2 * j + 1])) : 0.f;
+        sum[2 * j] += x0 + x1;
+        sum[2 * j + 1] += y0 + y1;
+        p[2 * j] = pack_pair<T>(x0, y0);
+        p[2 * j + 1] = pack_pair<T>(x1, y1);
+      }
+      // the product of the tile before has read its weights
+      if (n && !dead && !mbar_wait(bar(c.empty[(n - 1u) & 1u]), ((n - 1u) >> 1) & 1u, waits)) dead = true;
+      if (!dead) {
+        const uint32_t to = base + Layout<kN>::kWeights + row0 * 128u + (lane & 3u) * 4u;
+#pragma unroll
+        for (uint32_t j = 0; j < kBlocks; ++j) {
+          const uint32_t at = to + ((j ^ (row0 & 7u)) << 4);   // row0 + 8 has the same swizzle
+          asm volatile("st.shared.b32 [%0], %1;" ::"r"(at), "r"(p[2 * j]) : "memory");
+          asm volatile("st.shared.b32 [%0], %1;" ::"r"(at + 1024u), "r"(p[2 * j + 1]) : "memory");
+        }
+        fence_async();
+        fence_before();
+        mbar_arrive(bar(c.weighted));
+      }
+      written = true;
+    }
+    if (count && !dead && !mbar_wait(bar(c.empty[(count - 1u) & 1u]), ((count - 1u) >> 1) & 1u, waits)) dead = true;
+    if (!role_any(1u, dead)) {
+      fence_after();
+      // sums over the rows of all tiles; then one value element per lane and block, heads along the columns
+      float* top = reinterpret_cast<float*>(smem + Layout<kN>::kWeights);   // the weights have been read
+      auto over_rows = [&](float x) {
+#pragma unroll
+        for (uint32_t o = 4; o < 32; o <<= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+        return x;
+      };
+#pragma unroll
+      for (uint32_t j = 0; j < 2 * kBlocks; ++j) {
+        const uint32_t h = (j >> 1) * 8u + (lane & 3u) * 2u + (j & 1u);
+        const float x = over_rows(sum[j]);
+        if (lane < 4) {
+          c.reduce[warp][h] = x;
+          if (warp == 0) top[h] = ref[j];
+        }
+      }
+      role_any(1u, false);
+      const uint64_t out_row = static_cast<uint64_t>(t) * a.heads + head0;
+      const uint64_t part_row = (static_cast<uint64_t>(split) * a.tokens + t) * a.heads + head0;
+      if (tid < heads) {
+        const float whole = (c.reduce[0][tid] + c.reduce[1][tid]) + (c.reduce[2][tid] + c.reduce[3][tid]);
+        if (splits == 1) {
+          a.lse[out_row + tid] = written ? (top[tid] + log2f(whole)) * 0.6931471805599453f : -INFINITY;
+        } else {
+          a.partial_stats[2 * (part_row + tid)] = written ? top[tid] : -INFINITY;
+          a.partial_stats[2 * (part_row + tid) + 1] = whole;
+        }
+        c.factor[tid] = written ? 1.f / whole : 0.f;
+      }
+      role_any(1u, false);
+      for (uint32_t m = 0; m < 4; ++m) {
+        const uint32_t element = m * 128u + warp * 32u + lane;
+#pragma unroll
+        for (uint32_t h0 = 0; h0 < kN; h0 += 16) {
+          uint32_t o[16];
+          if (written) {
+            tmem_ld_rows(tmem + quad + kOut + m * kN + h0, o);
+            tmem_ld_done();
+          }
+#pragma unroll
+          for (uint32_t x = 0; x < 16; ++x) {
+            const uint32_t h = h0 + x;
+            if (h >= heads) break;
+            const float y = written ? __uint_as_float(o[x]) * c.factor[h] : 0.f;
+            if (splits == 1) static_cast<T*>(a.out)[(out_row + h) * kValue + element] = round_to<T>(y);
+            else a.partial[(part_row + h) * kValue + element] = y;
+          }
+        }
+      }
+      fence_before();
     }
   }
-  const uint64_t out_row = static_cast<uint64_t>(t) * a.heads + h;
-  uint32_t* out = reinterpret_cast<uint32_t*>(static_cast<T*>(a.out) + out_row * kValue);
-  const float inverse = total > 0.f ? 1.f / total : (total == 0.f ? 0.f : total);
-#pragma unroll
-  for (uint32_t i = 0; i < 8; ++i) out[i * 32u + lane] = pair_from_float(acc[i].x * inverse, acc[i].y * inverse, T());
-  if (lane == 0) {
-    a.lse[out_row] = total == 0.f ? -INFINITY : top + logf(total);
-    if (bad) atomicOr(a.status, bad);
+
+  // ---- teardown ----------------------------------------------------------------------------
+  __syncthreads();
+  if (c.abort_flag) {
+    if (tid == 0) atomicOr(a.status, static_cast<int32_t>(KVIP_ERR_PIPELINE));
+    for (int i = 0; i < 64; ++i) __nanosleep(2000);   // products in flight end before their memory is released
+    __syncthreads();
   }
+  if (warp == kMmaWarp) {
+    fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+  }
+}
+
+// Joins the shares of one (token, head): out = sum_s w_s o_s / sum_s w_s, w_s = sum of the share * 2^(its reference).
+template <typename T>
+__global__ void __launch_bounds__(128) join_shares(const __grid_constant__ KvipAttentionArgs a, const uint32_t splits) {
+  const uint32_t row = blockIdx.x, t = row / a.heads;
+  if (a.requests && a.requests[t] < 0) return;
+  const uint64_t rows = static_cast<uint64_t>(a.tokens) * a.heads;
+  float top = -INFINITY;
+  for (uint32_t s = 0; s < splits; ++s) top = fmaxf(top, a.partial_stats[2 * (s * rows + row)]);
+  float total = 0.f;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (uint32_t s = 0; s < splits; ++s) {
+    const float2 stat = reinterpret_cast<const float2*>(a.partial_stats)[s * rows + row];
+    const float weight = stat.x == -INFINITY ? 0.f : stat.y * exp2_fast(stat.x - top);
+    const float4 o = reinterpret_cast<const float4*>(a.partial + (s * rows + row) * kValue)[threadIdx.x];
+    total += weight;
+    if (weight != 0.f) {
+      acc.x = fmaf(weight, o.x, acc.x); acc.y = fmaf(weight, o.y, acc.y);
+      acc.z = fmaf(weight, o.z, acc.z); acc.w = fmaf(weight, o.w, acc.w);
+    }
+  }
+  const float inverse = total == 0.f ? 0.f : 1.f / total;
+  uint2 packed = make_uint2(pack_pair<T>(acc.x * inverse, acc.y * inverse), pack_pair<T>(acc.z * inverse, acc.w * inverse));
+  reinterpret_cast<uint2*>(static_cast<T*>(a.out) + static_cast<uint64_t>(row) * kValue)[threadIdx.x] = packed;
+  if (threadIdx.x == 0) a.lse[row] = total == 0.f ? -INFINITY : (top + log2f(total)) * 0.6931471805599453f;
+}
+
+template <typename T, uint32_t kN>
+uint32_t launch_tiles(const KvipAttentionArgs& a, KernelSlot slot, uint32_t groups, uint32_t group_heads, uint32_t splits, cudaStream_t stream) {
+  if (uint32_t bad = raise_dynamic_smem(slot, reinterpret_cast<const void*>(attend_tiles<T, kN>), static_cast<int>(Layout<kN>::kBytes),
+                                        "slot_attention attribute"))
+    return bad;
+  attend_tiles<T, kN><<<a.tokens * groups * splits, kAttentionThreads, Layout<kN>::kBytes, stream>>>(a, groups, group_heads, splits);
+  count_launch();
+  return check_launch("attend_tiles");
+}
+
+template <typename T>
+uint32_t launch_attention(const KvipAttentionArgs& a, uint32_t first_slot, cudaStream_t stream) {
+  const uint32_t groups = (a.heads + kGroupHeads - 1) / kGroupHeads, group_heads = (a.heads + groups - 1) / groups;
+  const uint64_t units = static_cast<uint64_t>(a.tokens) * groups;
+  uint32_t splits = a.splits;
+  if (!splits) {
+    // few tokens: shares of at least two tiles, as many as the SMs take at once
+    const uint32_t tiles = (a.entries + (a.draft ? 64u : 0u) + kTile - 1) / kTile, sms = device_sm_count();
+    splits = units < sms ? static_cast<uint32_t>(sms / units) : 1u;
+    if (splits > tiles / 2u) splits = tiles / 2u;
+    if (!a.partial || !a.partial_stats) splits = 1;
+    const uint64_t room = a.partial_rows / (static_cast<uint64_t>(a.tokens) * a.heads);
+    if (splits > room) splits = static_cast<uint32_t>(room);
+    if (splits < 1) splits = 1;
+  }
+  if (units * splits > 0x7fffffffull) { set_error("slot_attention: too many tokens in one call"); return KVIP_BAD_ARGUMENT; }
+  uint32_t bad;
+  const KernelSlot slot = static_cast<KernelSlot>(first_slot + (group_heads + 15u) / 16u - 1u);
+  if (group_heads <= 16) bad = launch_tiles<T, 16>(a, slot, groups, group_heads, splits, stream);
+  else if (group_heads <= 32) bad = launch_tiles<T, 32>(a, slot, groups, group_heads, splits, stream);
+  else if (group_heads <= 48) bad = launch_tiles<T, 48>(a, slot, groups, group_heads, splits, stream);
+  else bad = launch_tiles<T, 64>(a, slot, groups, group_heads, splits, stream);
+  if (bad || splits == 1) return bad;
+  join_shares<T><<<a.tokens * a.heads, 128, 0, stream>>>(a, splits);
+  count_launch();
+  return check_launch("join_shares");
 }
 
 }  // namespace
@@ -125,10 +634,6 @@ extern "C" uint32_t kvip_b200_slot_attention(const KvipAttentionArgs* a, void* s
   KVIP_REQUIRE(a->splits <= 1 || (a->partial && a->partial_stats &&
                                   static_cast<uint64_t>(a->splits) * a->tokens * a->heads <= a->partial_rows),
                "slot_attention: the workspace does not hold the shares");
-  const dim3 grid(a->tokens, (a->heads + 3u) / 4u);
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (a->dtype == KVIP_FLOAT_BF16) attend_rows<__nv_bfloat16><<<grid, 128, 0, s>>>(*a);
-  else attend_rows<__half><<<grid, 128, 0, s>>>(*a);
-  count_launch();
-  return check_launch("attend_rows");
+  return a->dtype == KVIP_FLOAT_BF16 ? launch_attention<__nv_bfloat16>(*a, kSlotAttentionBf16, s) : launch_attention<__half>(*a, kSlotAttentionFp16, s);
 }
