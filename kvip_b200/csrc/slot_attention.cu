@@ -17,6 +17,7 @@
 //
 // p is rounded to the rows' type for the second product (half a step, as the output is); its sum is taken before the
 // rounding, in fp32, because the log-sum is an output too.
+#include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include "common.cuh"
@@ -31,21 +32,17 @@ constexpr uint32_t kPieceBytes = kTile * 128;           // one piece of every ro
 constexpr uint32_t kStageBytes = kPieces * kPieceBytes; // 73,728
 constexpr uint32_t kStages = 2;
 constexpr uint32_t kGroupHeads = 64;
-constexpr uint32_t kLoaders = 128;                      // threads that fill one stage; a group of them per stage
-// Warpgroups: softmax (warps 0-3), MMA issuer (warp 4; 5-7 idle), two loader groups. 512 threads start with 128 registers;
-// 184 + 72 + 2 x 112 is within that total, and the softmax keeps two rows of 64 heads in registers without spilling.
-constexpr uint32_t kSoftmaxWarps = 4, kMmaWarp = 4, kFirstLoaderWarp = 8;
-constexpr uint32_t kSoftmaxRegisters = 184, kMmaRegisters = 72, kLoaderRegisters = 112;
-constexpr uint32_t kAttentionThreads = 32 * kFirstLoaderWarp + kStages * kLoaders;
+// Warps 0-3 and 4-7: softmax of the lower and the upper half of the heads; 8-11: loaders, two per stage; 12: MMA issuer.
+constexpr uint32_t kFirstLoaderWarp = 8, kMmaWarp = 12, kAttentionThreads = 32 * 13;
+constexpr uint32_t kRole = 128;                         // threads of one softmax half
 constexpr float kSlack = 8.f;                           // log2: p may reach 2^8 before the reference moves
 constexpr uint32_t kDefaultWaitKilocycles = 2000000u;   // about one second of SM clock
 
 struct Control {                                        // behind the tiles in shared memory
   uint64_t full[kStages], empty[kStages], scored[2], weighted, query_full;
-  uint64_t source[kStages][kTile];                      // address of every row of the stage's tile, 0 = no row
-  uint32_t valid[kStages][2];                           // bit per row
-  float reduce[kSoftmaxWarps][kGroupHeads];
-  float factor[kGroupHeads];
+  uint32_t valid[kStages][4];                           // row 4 l + c of the tile is there: bit l of word c
+  float reduce[4][kGroupHeads];
+  float factor[kGroupHeads], top[kGroupHeads];
   uint32_t tmem, abort_flag, last;
 };
 
@@ -94,11 +91,11 @@ __device__ __forceinline__ bool mbar_wait_slow(uint32_t bar, uint32_t parity, co
 __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, const Waits& w) {
   return mbar_try(bar, parity) || mbar_wait_slow(bar, parity, w);
 }
-// Barrier of one role's 128 threads that also tells all of them whether any has `flag`.
-__device__ __forceinline__ bool role_any(uint32_t id, bool flag) {
+// Barrier of `kThreads` threads that also tells all of them whether any has `flag`.
+template <uint32_t kThreads = kRole> __device__ __forceinline__ bool role_any(uint32_t id, bool flag) {
   uint32_t any;
-  asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbarrier.cta.red.or.pred q, %2, 128, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
-               : "=r"(any) : "r"(flag ? 1u : 0u), "r"(id) : "memory");
+  asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbarrier.cta.red.or.pred q, %2, %3, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+               : "=r"(any) : "r"(flag ? 1u : 0u), "r"(id), "n"(kThreads) : "memory");
   return any != 0u;
 }
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
@@ -117,24 +114,31 @@ __device__ __forceinline__ uint64_t operand(uint32_t address, uint32_t pieces) {
   return static_cast<uint64_t>((address & 0x3ffffu) >> 4) | (static_cast<uint64_t>(pieces >> 4) << 16) |
          (static_cast<uint64_t>(1024u >> 4) << 32) | (1ull << 46) | (2ull << 61);
 }
-// 16 lanes x 16 fp32 columns: a thread holds rows lane/4 (v[0], v[1], v[4], v[5]) and lane/4 + 8, columns 2 (lane%4) + {0, 1}
-// of each 8.
-__device__ __forceinline__ void tmem_ld_scores(uint32_t address, uint32_t* v) {
-  asm volatile("tcgen05.ld.sync.aligned.16x256b.x2.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+// 16 lanes x 8 kBlocks fp32 columns: a thread holds rows lane/4 (v[4j], v[4j + 1]) and lane/4 + 8 (v[4j + 2], v[4j + 3]),
+// columns 8j + 2 (lane%4) + {0, 1}.
+template <uint32_t kBlocks> __device__ __forceinline__ void tmem_ld_scores(uint32_t address, uint32_t* v) {
+  if constexpr (kBlocks == 4) {
+    asm volatile("tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
+                   "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+                 : "r"(address) : "memory");
+  } else if constexpr (kBlocks >= 2) {
+    asm volatile("tcgen05.ld.sync.aligned.16x256b.x2.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]) : "r"(address) : "memory");
+    if constexpr (kBlocks == 3) tmem_ld_scores<1>(address + 16u, v + 8);
+  } else {
+    asm volatile("tcgen05.ld.sync.aligned.16x256b.x1.b32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(address) : "memory");
+  }
+}
+// 32 lanes x 8 fp32 columns: a thread holds its lane's row.
+__device__ __forceinline__ void tmem_ld_rows(uint32_t address, uint32_t* v) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
                : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]) : "r"(address) : "memory");
 }
-// 32 lanes x 16 fp32 columns: a thread holds its lane's row.
-__device__ __forceinline__ void tmem_ld_rows(uint32_t address, uint32_t (&v)[16]) {
-  asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
-               : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
-                 "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
-               : "r"(address) : "memory");
-}
-__device__ __forceinline__ void tmem_st_rows(uint32_t address, const uint32_t (&v)[16]) {
-  asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
-               ::"r"(address), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]),
-                 "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
-               : "memory");
+__device__ __forceinline__ void tmem_st_rows(uint32_t address, const uint32_t* v) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+               ::"r"(address), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]) : "memory");
 }
 __device__ __forceinline__ void tmem_ld_done() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_st_done() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
@@ -143,9 +147,24 @@ __device__ __forceinline__ float exp2_fast(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-// 16 bytes of a row into shared memory, zeros where `present` is false.
-__device__ __forceinline__ void copy16(uint32_t to, const void* from, bool present) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(present ? 16u : 0u) : "memory");
+// Four rows of a [rows, 576] tensor, 64 elements from `x` on, to `to` and the three 128-byte rows behind it (swizzled).
+__device__ __forceinline__ void load_rows(uint32_t to, const CUtensorMap* map, uint32_t x, int4 rows, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5, %6}], [%7];"
+      ::"r"(to), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(rows.x), "r"(rows.y), "r"(rows.z), "r"(rows.w), "r"(bar)
+      : "memory");
+}
+__device__ __forceinline__ void load_query(uint32_t to, const CUtensorMap* map, uint32_t x, uint32_t head, uint32_t token, uint32_t bar) {
+  asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+               ::"r"(to), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(head), "r"(token), "r"(bar) : "memory");
+}
+__device__ __forceinline__ void expect_bytes(uint32_t bar, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ bool elect_one() {
+  uint32_t leader;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(leader));
+  return leader != 0u;
 }
 template <typename T> __device__ __forceinline__ uint32_t pack_pair(float x, float y);
 template <> __device__ __forceinline__ uint32_t pack_pair<__nv_bfloat16>(float x, float y) {
@@ -162,14 +181,13 @@ template <> __device__ __forceinline__ __half round_to(float x) { return __float
 
 // What token t may read.
 struct Rows {
-  const uint8_t* pool;        // first row of the owner
-  const uint8_t* draft;       // first drafted row of the request
-  uint64_t draft_bytes, seen; // distance of drafted rows; the ones the token sees
-  uint32_t limit, drafted;    // rows of the owner (0: none may be read), drafted rows of the request
+  uint32_t base, limit;       // first pool row of the owner and how many it has (0: none may be read)
+  uint32_t draft, drafted;    // first drafted row of the request, and how many of them bound those the token sees
+  uint64_t seen;
   int32_t bad;
 };
 __device__ __forceinline__ Rows rows_of(const KvipAttentionArgs& a, uint32_t t, int32_t request) {
-  Rows r{static_cast<const uint8_t*>(a.pool), nullptr, static_cast<uint64_t>(a.draft_token) * 2u, 0ull, a.output_stride, 0u, 0};
+  Rows r{0u, a.output_stride, 0u, 0u, 0ull, 0};
   if (static_cast<uint32_t>(request) >= a.batch) {
     r.limit = 0;
     r.bad = static_cast<int32_t>(KVIP_ERR_TOKEN_RANGE);
@@ -181,17 +199,17 @@ __device__ __forceinline__ Rows rows_of(const KvipAttentionArgs& a, uint32_t t, 
     r.limit = 0;
     r.bad = static_cast<int32_t>(KVIP_ERR_SOURCE);
   } else {
-    r.pool += base * (kWidth * 2u);
+    r.base = static_cast<uint32_t>(base);
   }
   if (a.draft) {
     const int64_t first = a.starts[request], behind = a.starts[request + 1], own = static_cast<int64_t>(t) - first;
     if (first < 0 || behind < first || behind > static_cast<int64_t>(a.tokens)) {
       r.bad |= static_cast<int32_t>(KVIP_ERR_TOKEN_RANGE);
     } else {
-      r.drafted = static_cast<uint32_t>(min(static_cast<int64_t>(64), behind - first));
-      r.draft = static_cast<const uint8_t*>(a.draft) + static_cast<uint64_t>(first) * r.draft_bytes;
+      const uint32_t nodes = static_cast<uint32_t>(min(static_cast<int64_t>(64), behind - first));
+      r.draft = static_cast<uint32_t>(first);
       r.seen = a.ancestors ? static_cast<uint64_t>(a.ancestors[t]) : (own < 0 ? 0ull : own >= 63 ? ~0ull : (2ull << own) - 1ull);
-      if (r.drafted < 64u) r.seen &= (1ull << r.drafted) - 1ull;
+      if (nodes < 64u) r.seen &= (1ull << nodes) - 1ull;
       r.drafted = r.seen ? 64u - static_cast<uint32_t>(__clzll(static_cast<long long>(r.seen))) : 0u;
     }
   }
@@ -200,7 +218,9 @@ __device__ __forceinline__ Rows rows_of(const KvipAttentionArgs& a, uint32_t t, 
 
 template <typename T, uint32_t kN>
 __global__ void __launch_bounds__(kAttentionThreads, 1)
-attend_tiles(const __grid_constant__ KvipAttentionArgs a, const uint32_t groups, const uint32_t group_heads, const uint32_t splits) {
+attend_tiles(const __grid_constant__ CUtensorMap query_map, const __grid_constant__ CUtensorMap pool_map,
+             const __grid_constant__ CUtensorMap draft_map, const __grid_constant__ KvipAttentionArgs a, const uint32_t groups,
+             const uint32_t group_heads, const uint32_t splits) {
   extern __shared__ __align__(1024) uint8_t smem[];
   const uint32_t base = smem_u32(smem);
   Control& c = *reinterpret_cast<Control*>(smem + Layout<kN>::kControl);
@@ -209,14 +229,14 @@ attend_tiles(const __grid_constant__ KvipAttentionArgs a, const uint32_t groups,
   const uint32_t head0 = group * group_heads, heads = min(group_heads, a.heads - head0);
   const int32_t request = a.requests ? a.requests[t] : static_cast<int32_t>(t / a.queries);
   if (request < 0) return;
-  const Rows rows = rows_of(a, t, request);
   const int32_t* list = a.slots + static_cast<uint64_t>(t) * a.entries;
+  const bool vectors = (a.entries & 3u) == 0u && (reinterpret_cast<uintptr_t>(a.slots) & 15u) == 0u;
 
   auto bar = [&](const uint64_t& b) { return smem_u32(&b); };
   if (tid == 0) {
-    for (uint32_t s = 0; s < kStages; ++s) { mbar_init(bar(c.full[s]), kLoaders); mbar_init(bar(c.empty[s]), 1); }
+    for (uint32_t s = 0; s < kStages; ++s) { mbar_init(bar(c.full[s]), 2); mbar_init(bar(c.empty[s]), 1); }
     mbar_init(bar(c.scored[0]), 1); mbar_init(bar(c.scored[1]), 1);
-    mbar_init(bar(c.weighted), 128); mbar_init(bar(c.query_full), kStages * kLoaders);
+    mbar_init(bar(c.weighted), 2 * kRole); mbar_init(bar(c.query_full), 1);
     c.abort_flag = 0;
     c.last = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -226,11 +246,20 @@ attend_tiles(const __grid_constant__ KvipAttentionArgs a, const uint32_t groups,
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&c.tmem)) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
+  const Rows rows = rows_of(a, t, request);
   // lists end in -1 where a context is short: the last entry in use bounds the tiles
   uint32_t last = 0;
-  if (rows.limit)
-    for (uint32_t k = tid; k < a.entries; k += kAttentionThreads)
-      if (list[k] >= 0) last = k + 1u;
+  if (rows.limit) {
+    if (vectors) {
+      for (uint32_t k = tid; k < a.entries / 4u; k += kAttentionThreads) {
+        const int4 e = __ldg(reinterpret_cast<const int4*>(list) + k);
+        if (e.x >= 0 || e.y >= 0 || e.z >= 0 || e.w >= 0) last = 4u * k + (e.w >= 0 ? 4u : e.z >= 0 ? 3u : e.y >= 0 ? 2u : 1u);
+      }
+    } else {
+      for (uint32_t k = tid; k < a.entries; k += kAttentionThreads)
+        if (list[k] >= 0) last = k + 1u;
+    }
+  }
   last = __reduce_max_sync(0xffffffffu, last);
   fence_before();
   __syncthreads();
@@ -238,201 +267,223 @@ attend_tiles(const __grid_constant__ KvipAttentionArgs a, const uint32_t groups,
   if (lane == 0 && last) atomicMax(&c.last, last);
   __syncthreads();
   const uint32_t tmem = c.tmem;
-  const uint32_t listed = c.last, total = listed + rows.drafted;
-  const uint32_t tiles = (total + kTile - 1) / kTile;
+  // tiles of the list, then one of the drafted rows
+  const uint32_t listed = c.last, list_tiles = (listed + kTile - 1) / kTile, tiles = list_tiles + (rows.drafted ? 1u : 0u);
   const uint32_t first = static_cast<uint32_t>(static_cast<uint64_t>(tiles) * split / splits);
   const uint32_t behind = static_cast<uint32_t>(static_cast<uint64_t>(tiles) * (split + 1) / splits);
   const uint32_t count = behind - first;
   const Waits waits{&c.abort_flag, static_cast<long long>(a.wait_kilocycles ? a.wait_kilocycles : kDefaultWaitKilocycles) << 10};
   constexpr uint32_t kScores = 0, kOut = 2 * kN;   // tensor-memory columns: two score tiles, four value blocks
+  auto none = [&](uint32_t s) { return (c.valid[s][0] | c.valid[s][1] | c.valid[s][2] | c.valid[s][3]) == 0u; };
 
-  if (warp >= kFirstLoaderWarp) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kLoaderRegisters));
-    // ================= loaders: group g fills stage g with the tiles g, g + 2, ... =================
-    const uint32_t g = (warp - kFirstLoaderWarp) >> 2, i = tid - 32u * kFirstLoaderWarp - g * kLoaders;
+  if (warp >= kFirstLoaderWarp && warp < kMmaWarp) {
+    // ================= loaders: warps 8, 9 (10, 11) gather the first (last) 32 rows of the tiles 0, 2, .. and 1, 3, .. =======
+    const uint32_t g = (warp - kFirstLoaderWarp) & 1u, half = (warp - kFirstLoaderWarp) >> 1;
+    const bool leader = elect_one();
+    int32_t bad = warp == kFirstLoaderWarp ? rows.bad : 0;
     if (count) {
-      const uint8_t* query = reinterpret_cast<const uint8_t*>(static_cast<const T*>(a.query) + t * a.query_token + head0 * a.query_head);
-      for (uint32_t x = g * kLoaders + i; x < kN * 72u; x += kStages * kLoaders) {
-        const uint32_t h = x / 72u, u = x - h * 72u;
-        copy16(base + Layout<kN>::kQuery + (u >> 3) * (kN * 128u) + h * 128u + (((u & 7u) ^ (h & 7u)) << 4),
-               query + (h < heads ? static_cast<uint64_t>(h) * a.query_head * 2u : 0ull) + u * 16u, h < heads);
+      if (warp == kFirstLoaderWarp && leader) {
+        expect_bytes(bar(c.query_full), kPieces * kN * 128u);
+        for (uint32_t piece = 0; piece < kPieces; ++piece)
+          load_query(base + Layout<kN>::kQuery + piece * (kN * 128u), &query_map, piece * 64u, head0, t, bar(c.query_full));
       }
-      asm volatile("cp.async.commit_group;" ::: "memory");
-      int32_t bad = 0;
-      bool query_sent = false, stop = false;
-      auto entry_of = [&](uint32_t n) -> int32_t {   // list entry of row i of tile n, -1 behind the list
-        const uint32_t k = (first + n) * kTile + i;
-        return i < kTile && n < count && k < listed ? list[k] : -1;
+      auto entries_of = [&](uint32_t n) -> int4 {   // entries 4 lane .. + 3 of tile n (lanes 0-15), -1 behind the list
+        int4 e = make_int4(-1, -1, -1, -1);
+        const uint32_t k = (first + n) * kTile + 4u * lane;
+        if (lane < 16u && n < count && k < listed) {
+          if (vectors) {
+            e = __ldg(reinterpret_cast<const int4*>(list + k));
+          } else {
+            e.x = list[k];
+            if (k + 1u < listed) e.y = list[k + 1u];
+            if (k + 2u < listed) e.z = list[k + 2u];
+            if (k + 3u < listed) e.w = list[k + 3u];
+          }
+        }
+        return e;
       };
-      int32_t slot = entry_of(g);
+      int4 next = entries_of(g);
       for (uint32_t n = g; n < count; n += kStages) {
-        const bool ok = mbar_wait(bar(c.empty[g]), ((n >> 1) & 1u) ^ 1u, waits);
-        if (i < kTile) {
-          const uint32_t k = (first + n) * kTile + i;
-          uint64_t source = 0;
-          if (k < listed) {
-            if (slot >= 0) {
-              if (static_cast<uint32_t>(slot) < rows.limit) source = reinterpret_cast<uint64_t>(rows.pool) + static_cast<uint64_t>(slot) * (kWidth * 2u);
-              else bad |= static_cast<int32_t>(KVIP_ERR_SOURCE);
-            }
-          } else if (k < total && ((rows.seen >> (k - listed)) & 1ull)) {
-            source = reinterpret_cast<uint64_t>(rows.draft) + (k - listed) * rows.draft_bytes;
+        int4 e = next;
+        next = entries_of(n + kStages);            // lands while this tile is fetched
+        const bool from_list = first + n < list_tiles;
+        bool v0, v1, v2, v3;
+        if (from_list) {
+          auto check = [&](int32_t& slot) {
+            if (slot < 0) return false;
+            if (static_cast<uint32_t>(slot) >= rows.limit) { bad |= static_cast<int32_t>(KVIP_ERR_SOURCE); return false; }
+            slot = static_cast<int32_t>(rows.base + static_cast<uint32_t>(slot));
+            return true;
+          };
+          v0 = check(e.x); v1 = check(e.y); v2 = check(e.z); v3 = check(e.w);
+        } else {
+          const uint32_t bits = lane < 16u ? static_cast<uint32_t>(rows.seen >> (4u * lane)) & 15u : 0u;
+          const int32_t row = static_cast<int32_t>(rows.draft + 4u * lane);
+          e = make_int4(row, row + 1, row + 2, row + 3);
+          v0 = bits & 1u; v1 = bits & 2u; v2 = bits & 4u; v3 = bits & 8u;
+        }
+        const uint32_t b0 = __ballot_sync(0xffffffffu, v0), b1 = __ballot_sync(0xffffffffu, v1), b2 = __ballot_sync(0xffffffffu, v2),
+                       b3 = __ballot_sync(0xffffffffu, v3);
+        if (!__all_sync(0xffffffffu, mbar_wait(bar(c.empty[g]), ((n >> 1) & 1u) ^ 1u, waits))) break;
+        if (leader && half == 0) { c.valid[g][0] = b0; c.valid[g][1] = b1; c.valid[g][2] = b2; c.valid[g][3] = b3; }
+        const uint32_t any = b0 | b1 | b2 | b3;
+        if (!any) {
+          __syncwarp();
+          if (leader) mbar_arrive(bar(c.full[g]));
+          continue;
+        }
+        // a place without a row takes one of the tile's own: its weight is zero, and it holds nothing that the token does not read
+        const int32_t mine = v0 ? e.x : v1 ? e.y : v2 ? e.z : e.w;
+        const int32_t spare = __shfl_sync(0xffffffffu, mine, __ffs(static_cast<int>(any)) - 1);
+        if (!v0) e.x = spare;
+        if (!v1) e.y = spare;
+        if (!v2) e.z = spare;
+        if (!v3) e.w = spare;
+        const CUtensorMap* map = from_list ? &pool_map : &draft_map;
+        if (leader) expect_bytes(bar(c.full[g]), kStageBytes / 2u);
+        __syncwarp();
+#pragma unroll
+        for (uint32_t q = 0; q < 8u; ++q) {        // four rows each
+          const uint32_t from = half * 8u + q;
+          const int4 r = make_int4(__shfl_sync(0xffffffffu, e.x, from), __shfl_sync(0xffffffffu, e.y, from),
+                                   __shfl_sync(0xffffffffu, e.z, from), __shfl_sync(0xffffffffu, e.w, from));
+          if (leader) {
+#pragma unroll
+            for (uint32_t piece = 0; piece < kPieces; ++piece)
+              load_rows(base + g * kStageBytes + piece * kPieceBytes + from * 512u, map, piece * 64u, r, bar(c.full[g]));
           }
-          c.source[g][i] = source;
-          const uint32_t present = __ballot_sync(0xffffffffu, source != 0);
-          if (lane == 0) c.valid[g][i >> 5] = present;
         }
-        slot = entry_of(n + kStages);      // lands while this tile is fetched
-        if (role_any(2u + g, !ok)) { stop = true; break; }
-        const bool any = (c.valid[g][0] | c.valid[g][1]) != 0u;
-        if (any) {
-          uint32_t row = i / 72u, u = i - row * 72u;
-#pragma unroll 9
-          for (uint32_t x = 0; x < kTile * 72u / kLoaders; ++x) {
-            const uint64_t source = c.source[g][row];
-            copy16(base + g * kStageBytes + (u >> 3) * kPieceBytes + row * 128u + (((u & 7u) ^ (row & 7u)) << 4),
-                   reinterpret_cast<const void*>((source ? source : reinterpret_cast<uint64_t>(a.pool)) + u * 16u), source != 0);
-            u += kLoaders - 72u; ++row;
-            if (u >= 72u) { u -= 72u; ++row; }
-          }
-        }
-        asm volatile("cp.async.commit_group;" ::: "memory");
-        if (!query_sent) {
-          asm volatile("cp.async.wait_group 1;" ::: "memory");
-          fence_async();
-          mbar_arrive(bar(c.query_full));
-          query_sent = true;
-        }
-        asm volatile("cp.async.wait_group 0;" ::: "memory");
-        fence_async();
-        mbar_arrive(bar(c.full[g]));
       }
-      if (!query_sent) {
-        asm volatile("cp.async.wait_group 0;" ::: "memory");
-        fence_async();
-        if (!stop) mbar_arrive(bar(c.query_full));
-      }
-      asm volatile("cp.async.wait_all;" ::: "memory");
-      if (i == 0 && g == 0) bad |= rows.bad;
-      if (bad) atomicOr(a.status, bad);
-    } else if (rows.bad && i == 0 && g == 0) {
-      atomicOr(a.status, rows.bad);
     }
-  } else if (warp >= kMmaWarp) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kMmaRegisters));
-    // ================= MMA issuer: one thread =================
-    if (warp == kMmaWarp && lane == 0 && count) {
-      constexpr uint32_t kFormat = sizeof(T) == 2 && __is_same(T, __nv_bfloat16) ? 1u : 0u;
+    if (bad) atomicOr(a.status, bad);
+  } else if (warp == kMmaWarp) {
+    // ================= MMA issuer: the warp walks together, one elected thread issues =================
+    if (count) {
+      constexpr uint32_t kFormat = __is_same(T, __nv_bfloat16) ? 1u : 0u;
       constexpr uint32_t kBase = (1u << 4) | (kFormat << 7) | (kFormat << 10) | ((kN >> 3) << 17);
       constexpr uint32_t kScoreDesc = kBase | ((64u >> 4) << 24);
       constexpr uint32_t kValueDesc = kBase | (1u << 15) | (1u << 16) | ((128u >> 4) << 24);   // both operands M/N-major
-      bool written = false, alive = mbar_wait(bar(c.query_full), 0, waits);
+      const bool leader = elect_one();
+      bool written = false, alive = __all_sync(0xffffffffu, mbar_wait(bar(c.query_full), 0, waits));
       auto score = [&](uint32_t n) {         // S^T of tile n, whose rows are in place
         const uint32_t s = n & 1u;
-        if (!(c.valid[s][0] | c.valid[s][1])) { mbar_arrive(bar(c.scored[s])); return; }
+        if (none(s)) {
+          if (leader) mbar_arrive(bar(c.scored[s]));
+          return;
+        }
         fence_after();
         const uint32_t d = tmem + kScores + s * kN;
-        uint64_t da = operand(base + s * kStageBytes, 16u), db = operand(base + Layout<kN>::kQuery, 16u);
-        asm volatile("" : "+l"(da), "+l"(db));   // offsets are added at each use, not kept in registers over the tiles
+        const uint64_t da = operand(base + s * kStageBytes, 16u), db = operand(base + Layout<kN>::kQuery, 16u);
+        if (leader) {
 #pragma unroll
-        for (uint32_t piece = 0; piece < kPieces; ++piece) {
+          for (uint32_t piece = 0; piece < kPieces; ++piece) {
 #pragma unroll
-          for (uint32_t k = 0; k < 4; ++k)
-            mma(d, da + (piece * (kPieceBytes >> 4) + 2u * k), db + (piece * (kN * 8u) + 2u * k), kScoreDesc, (piece | k) != 0u);
+            for (uint32_t k = 0; k < 4; ++k)
+              mma(d, da + (piece * (kPieceBytes >> 4) + 2u * k), db + (piece * (kN * 8u) + 2u * k), kScoreDesc, (piece | k) != 0u);
+          }
+          commit(bar(c.scored[s]));
         }
-        commit(bar(c.scored[s]));
+        __syncwarp();
       };
       uint32_t scored = 0;                   // tiles whose scores have been issued
       for (uint32_t n = 0; alive && n < count; ++n) {
         const uint32_t s = n & 1u, phase = (n >> 1) & 1u;
         if (scored == n) {
-          if (!mbar_wait(bar(c.full[s]), phase, waits)) break;
+          if (!__all_sync(0xffffffffu, mbar_wait(bar(c.full[s]), phase, waits))) break;
           score(n);
           ++scored;
         }
         // while the weights of tile n are made: the scores of the next tile, if its rows have come
         if (scored == n + 1 && n + 1 < count) {
           const uint32_t s1 = s ^ 1u, phase1 = ((n + 1) >> 1) & 1u;
-          while (!mbar_test(bar(c.weighted), n & 1u)) {
-            if (mbar_test(bar(c.full[s1]), phase1)) {
+          while (!__any_sync(0xffffffffu, mbar_test(bar(c.weighted), n & 1u) || c.abort_flag)) {
+            if (__all_sync(0xffffffffu, mbar_test(bar(c.full[s1]), phase1))) {
               score(n + 1);
               ++scored;
               break;
             }
-            if (c.abort_flag) break;
           }
         }
-        if (!mbar_wait(bar(c.weighted), n & 1u, waits)) break;
-        if (!(c.valid[s][0] | c.valid[s][1])) { commit(bar(c.empty[s])); continue; }   // in order behind the products before
-        fence_after();
-        uint64_t da = operand(base + s * kStageBytes, kPieceBytes), db = operand(base + Layout<kN>::kWeights, 16u);
-        asm volatile("" : "+l"(da), "+l"(db));
-#pragma unroll
-        for (uint32_t m = 0; m < 4; ++m) {
-#pragma unroll
-          for (uint32_t k = 0; k < kTile / 16u; ++k)
-            mma(tmem + kOut + m * kN, da + (2u * m * (kPieceBytes >> 4) + k * 128u), db + k * 128u, kValueDesc, written || k != 0u);
+        if (!__all_sync(0xffffffffu, mbar_wait(bar(c.weighted), n & 1u, waits))) break;
+        if (none(s)) {                       // in order behind the products before
+          if (leader) commit(bar(c.empty[s]));
+          continue;
         }
+        fence_after();
+        const uint64_t da = operand(base + s * kStageBytes, kPieceBytes), db = operand(base + Layout<kN>::kWeights, 16u);
+        if (leader) {
+#pragma unroll
+          for (uint32_t m = 0; m < 4; ++m) {
+#pragma unroll
+            for (uint32_t k = 0; k < kTile / 16u; ++k)
+              mma(tmem + kOut + m * kN, da + (2u * m * (kPieceBytes >> 4) + k * 128u), db + k * 128u, kValueDesc, written || k != 0u);
+          }
+          commit(bar(c.empty[s]));
+        }
+        __syncwarp();
         written = true;
-        commit(bar(c.empty[s]));
       }
     }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegisters));
-    // ================= softmax: rows 16 w + lane / 4 and + 8 of every tile =================
-    constexpr uint32_t kBlocks = kN / 8;     // blocks of eight heads; a thread holds two of each
+    // ================= softmax: rows 16 w + lane / 4 and + 8 of every tile, half of the heads =================
+    constexpr uint32_t kBlocks = kN / 16;    // blocks of eight heads per half; a thread holds two of each
+    const uint32_t side = warp >> 2, w = warp & 3u, head_at = side * (kN / 2u);
     float ref[2 * kBlocks], sum[2 * kBlocks];
 #pragma unroll
     for (uint32_t j = 0; j < 2 * kBlocks; ++j) { ref[j] = -INFINITY; sum[j] = 0.f; }
     const float scale = a.scale * 1.4426950408889634f;
-    const uint32_t quad = (warp * 32u) << 16;
-    const uint32_t row0 = warp * 16u + (lane >> 2);
+    const uint32_t quad = (w * 32u) << 16;
+    const uint32_t row0 = w * 16u + (lane >> 2);
     bool dead = false, written = false;
     for (uint32_t n = 0; n < count; ++n) {
       const uint32_t s = n & 1u, phase = (n >> 1) & 1u;
       bool ok = !dead && mbar_wait(bar(c.scored[s]), phase, waits) && mbar_wait(bar(c.full[s]), phase, waits);
       ok = __all_sync(0xffffffffu, ok);
-      const uint32_t present = c.valid[s][warp >> 1] >> ((warp & 1u) * 16u);
-      const bool empty = ok && !(c.valid[s][0] | c.valid[s][1]);
-      if (empty) { mbar_arrive(bar(c.weighted)); continue; }   // the same for all: the mask belongs to the tile
-      const bool has0 = (present >> (lane >> 2)) & 1u, has1 = (present >> ((lane >> 2) + 8u)) & 1u;
+      if (ok && none(s)) {                     // the same for all: the mask belongs to the tile
+        // as below: a thread arrives for this tile only when all have arrived for the one before
+        if (n && !mbar_wait(bar(c.empty[(n - 1u) & 1u]), ((n - 1u) >> 1) & 1u, waits)) dead = true;
+        else mbar_arrive(bar(c.weighted));
+        continue;
+      }
+      const uint32_t word = c.valid[s][row0 & 3u];
+      const bool has0 = (word >> (row0 >> 2)) & 1u, has1 = (word >> ((row0 >> 2) + 2u)) & 1u;
       uint32_t v[4 * kBlocks];
       if (ok) {
         fence_after();
-#pragma unroll
-        for (uint32_t j = 0; j < kBlocks; j += 2) tmem_ld_scores(tmem + quad + kScores + s * kN + j * 8u, v + 4 * j);
+        tmem_ld_scores<kBlocks>(tmem + quad + kScores + s * kN + head_at, v);
         tmem_ld_done();
       }
-      // d = scale' s - ref; one score more than 2^8 above its reference makes the whole role take the maximum
+      // scores in units of log2; one more than 2^8 above its reference makes the whole half take the maximum
+      float x[4 * kBlocks];
       bool above = false;
 #pragma unroll
-      for (uint32_t j = 0; j < 2 * kBlocks; ++j) {
-        const uint32_t at = (j >> 1) * 4u + (j & 1u);
-        const float x0 = __uint_as_float(v[at]), x1 = __uint_as_float(v[at + 2]);
-        above |= (has0 && fmaf(x0, scale, -ref[j]) > kSlack) || (has1 && fmaf(x1, scale, -ref[j]) > kSlack);
+      for (uint32_t j = 0; j < 4 * kBlocks; ++j) {
+        const bool has = (j & 2u) ? has1 : has0;
+        x[j] = has ? __uint_as_float(v[j]) * scale : -INFINITY;
+        above |= x[j] - ref[(j >> 2) * 2u + (j & 1u)] > kSlack;
       }
-      if (role_any(1u, above || !ok)) {
-        if (role_any(1u, !ok)) { dead = true; break; }
+      if (role_any(1u + side, above || !ok)) {
+        if (role_any(1u + side, !ok)) { dead = true; break; }
 #pragma unroll
         for (uint32_t j = 0; j < 2 * kBlocks; ++j) {
           const uint32_t at = (j >> 1) * 4u + (j & 1u);
-          float top = fmaxf(has0 ? __uint_as_float(v[at]) * scale : -INFINITY, has1 ? __uint_as_float(v[at + 2]) * scale : -INFINITY);
+          float top = fmaxf(x[at], x[at + 2]);
 #pragma unroll
           for (uint32_t o = 4; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-          if (lane < 4) c.reduce[warp][(j >> 1) * 8u + lane * 2u + (j & 1u)] = top;
+          if (lane < 4) c.reduce[w][head_at + (j >> 1) * 8u + lane * 2u + (j & 1u)] = top;
         }
-        role_any(1u, false);
+        role_any(1u + side, false);
 #pragma unroll
         for (uint32_t j = 0; j < 2 * kBlocks; ++j) {
-          const uint32_t h = (j >> 1) * 8u + (lane & 3u) * 2u + (j & 1u);
+          const uint32_t h = head_at + (j >> 1) * 8u + (lane & 3u) * 2u + (j & 1u);
           const float top = fmaxf(fmaxf(c.reduce[0][h], c.reduce[1][h]), fmaxf(c.reduce[2][h], c.reduce[3][h]));
           const float next = fmaxf(ref[j], top);
           const float factor = next == ref[j] ? 1.f : exp2_fast(ref[j] - next);   // 0 the first time
           ref[j] = next;
           sum[j] *= factor;
-          if (warp == 0 && lane < 4) c.factor[h] = factor;
+          if (w == 0 && lane < 4) c.factor[h] = factor;
         }
-        role_any(1u, false);
+        role_any(1u + side, false);
         if (written) {                         // the accumulators hold the tiles before this one, which must be in
           const uint32_t before = n - 1u;      // stages are released in order, an empty tile's too
           ok = mbar_wait(bar(c.empty[before & 1u]), (before >> 1) & 1u, waits);
@@ -440,12 +491,12 @@ attend_tiles(const __grid_constant__ KvipAttentionArgs a, const uint32_t groups,
             fence_after();
             for (uint32_t m = 0; m < 4; ++m) {
 #pragma unroll
-              for (uint32_t h = 0; h < kN; h += 16) {
-                uint32_t o[16];
+              for (uint32_t h = head_at; h < head_at + kN / 2u; h += 8) {
+                uint32_t o[8];
                 tmem_ld_rows(tmem + quad + kOut + m * kN + h, o);
                 tmem_ld_done();
 #pragma unroll
-                for (uint32_t x = 0; x < 16; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * c.factor[h + x]);
+                for (uint32_t i = 0; i < 8; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * c.factor[h + i]);
                 tmem_st_rows(tmem + quad + kOut + m * kN + h, o);
               }
             }
@@ -458,10 +509,8 @@ attend_tiles(const __grid_constant__ KvipAttentionArgs a, const uint32_t groups,
       uint32_t p[2 * kBlocks];                 // weights of a row, two heads in a word: row 0 then row 1
 #pragma unroll
       for (uint32_t j = 0; j < kBlocks; ++j) {
-        const float x0 = has0 ? exp2_fast(fmaf(__uint_as_float(v[4 * j]), scale, -ref[2 * j])) : 0.f;
-        const float y0 = has0 ? exp2_fast(fmaf(__uint_as_float(v[4 * j + 1]), scale, -ref[2 * j + 1])) : 0.f;
-        const float x1 = has1 ? exp2_fast(fmaf(__uint_as_float(v[4 * j + 2]), scale, -ref[2 * j])) : 0.f;
-        const float y1 = has1 ? exp2_fast(fmaf(__uint_as_float(v[4 * j + 3]), scale, -ref[2 * j + 1])) : 0.f;
+        const float x0 = exp2_fast(x[4 * j] - ref[2 * j]), y0 = exp2_fast(x[4 * j + 1] - ref[2 * j + 1]);
+        const float x1 = exp2_fast(x[4 * j + 2] - ref[2 * j]), y1 = exp2_fast(x[4 * j + 3] - ref[2 * j + 1]);
         sum[2 * j] += x0 + x1;
         sum[2 * j + 1] += y0 + y1;
         p[2 * j] = pack_pair<T>(x0, y0);
@@ -473,7 +522,7 @@ attend_tiles(const __grid_constant__ KvipAttentionArgs a, const uint32_t groups,
         const uint32_t to = base + Layout<kN>::kWeights + row0 * 128u + (lane & 3u) * 4u;
 #pragma unroll
         for (uint32_t j = 0; j < kBlocks; ++j) {
-          const uint32_t at = to + ((j ^ (row0 & 7u)) << 4);   // row0 + 8 has the same swizzle
+          const uint32_t at = to + (((side * kBlocks + j) ^ (row0 & 7u)) << 4);   // row0 + 8 has the same swizzle
           asm volatile("st.shared.b32 [%0], %1;" ::"r"(at), "r"(p[2 * j]) : "memory");
           asm volatile("st.shared.b32 [%0], %1;" ::"r"(at + 1024u), "r"(p[2 * j + 1]) : "memory");
         }
@@ -484,56 +533,62 @@ attend_tiles(const __grid_constant__ KvipAttentionArgs a, const uint32_t groups,
       written = true;
     }
     if (count && !dead && !mbar_wait(bar(c.empty[(count - 1u) & 1u]), ((count - 1u) >> 1) & 1u, waits)) dead = true;
-    if (!role_any(1u, dead)) {
-      fence_after();
-      // sums over the rows of all tiles; then one value element per lane and block, heads along the columns
-      float* top = reinterpret_cast<float*>(smem + Layout<kN>::kWeights);   // the weights have been read
-      auto over_rows = [&](float x) {
+    // sums over the rows of all tiles
 #pragma unroll
-        for (uint32_t o = 4; o < 32; o <<= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
-        return x;
-      };
+    for (uint32_t j = 0; j < 2 * kBlocks; ++j) {
+      const uint32_t h = head_at + (j >> 1) * 8u + (lane & 3u) * 2u + (j & 1u);
+      float total = sum[j];
 #pragma unroll
-      for (uint32_t j = 0; j < 2 * kBlocks; ++j) {
-        const uint32_t h = (j >> 1) * 8u + (lane & 3u) * 2u + (j & 1u);
-        const float x = over_rows(sum[j]);
-        if (lane < 4) {
-          c.reduce[warp][h] = x;
-          if (warp == 0) top[h] = ref[j];
-        }
+      for (uint32_t o = 4; o < 32; o <<= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+      if (lane < 4) {
+        c.reduce[w][h] = total;
+        if (w == 0) c.top[h] = ref[j];
       }
-      role_any(1u, false);
+    }
+    if (!role_any<2 * kRole>(3u, dead)) {
       const uint64_t out_row = static_cast<uint64_t>(t) * a.heads + head0;
       const uint64_t part_row = (static_cast<uint64_t>(split) * a.tokens + t) * a.heads + head0;
       if (tid < heads) {
-        const float whole = (c.reduce[0][tid] + c.reduce[1][tid]) + (c.reduce[2][tid] + c.reduce[3][tid]);
+        const float total = (c.reduce[0][tid] + c.reduce[1][tid]) + (c.reduce[2][tid] + c.reduce[3][tid]);
         if (splits == 1) {
-          a.lse[out_row + tid] = written ? (top[tid] + log2f(whole)) * 0.6931471805599453f : -INFINITY;
+          a.lse[out_row + tid] = written ? (c.top[tid] + log2f(total)) * 0.6931471805599453f : -INFINITY;
         } else {
-          a.partial_stats[2 * (part_row + tid)] = written ? top[tid] : -INFINITY;
-          a.partial_stats[2 * (part_row + tid) + 1] = whole;
+          a.partial_stats[2 * (part_row + tid)] = written ? c.top[tid] : -INFINITY;
+          a.partial_stats[2 * (part_row + tid) + 1] = total;
         }
-        c.factor[tid] = written ? 1.f / whole : 0.f;
+        c.factor[tid] = written ? 1.f / total : 0.f;
       }
-      role_any(1u, false);
-      for (uint32_t m = 0; m < 4; ++m) {
-        const uint32_t element = m * 128u + warp * 32u + lane;
+      role_any<2 * kRole>(3u, false);
+      fence_after();
+      // A lane holds one value element of every head. The share of the output, [heads, 512] and contiguous in memory, is laid
+      // out in the stages (all products have read them) and leaves as one copy.
+#pragma unroll
+      for (uint32_t m = 0; m < 2; ++m) {
+        const uint32_t block = 2u * side + m, element = block * 128u + w * 32u + lane;
 #pragma unroll
         for (uint32_t h0 = 0; h0 < kN; h0 += 16) {
           uint32_t o[16];
           if (written) {
-            tmem_ld_rows(tmem + quad + kOut + m * kN + h0, o);
+            tmem_ld_rows(tmem + quad + kOut + block * kN + h0, o);
+            tmem_ld_rows(tmem + quad + kOut + block * kN + h0 + 8u, o + 8);
             tmem_ld_done();
           }
 #pragma unroll
-          for (uint32_t x = 0; x < 16; ++x) {
-            const uint32_t h = h0 + x;
-            if (h >= heads) break;
-            const float y = written ? __uint_as_float(o[x]) * c.factor[h] : 0.f;
-            if (splits == 1) static_cast<T*>(a.out)[(out_row + h) * kValue + element] = round_to<T>(y);
-            else a.partial[(part_row + h) * kValue + element] = y;
+          for (uint32_t i = 0; i < 16; ++i) {
+            const float y = written ? __uint_as_float(o[i]) * c.factor[h0 + i] : 0.f;
+            if (splits == 1) reinterpret_cast<T*>(smem)[(h0 + i) * kValue + element] = round_to<T>(y);
+            else reinterpret_cast<float*>(smem)[(h0 + i) * kValue + element] = y;
           }
         }
+      }
+      fence_async();
+      role_any<2 * kRole>(3u, false);
+      if (tid == 0) {
+        void* to = splits == 1 ? static_cast<void*>(static_cast<T*>(a.out) + out_row * kValue) : static_cast<void*>(a.partial + part_row * kValue);
+        const uint32_t bytes = heads * kValue * (splits == 1 ? 2u : 4u);
+        asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(to), "r"(base), "r"(bytes) : "memory");
+        asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+        asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
       }
       fence_before();
     }
@@ -543,7 +598,7 @@ attend_tiles(const __grid_constant__ KvipAttentionArgs a, const uint32_t groups,
   __syncthreads();
   if (c.abort_flag) {
     if (tid == 0) atomicOr(a.status, static_cast<int32_t>(KVIP_ERR_PIPELINE));
-    for (int i = 0; i < 64; ++i) __nanosleep(2000);   // products in flight end before their memory is released
+    for (int i = 0; i < 64; ++i) __nanosleep(2000);   // copies and products in flight end before their memory is released
     __syncthreads();
   }
   if (warp == kMmaWarp) {
@@ -578,12 +633,51 @@ __global__ void __launch_bounds__(128) join_shares(const __grid_constant__ KvipA
   if (threadIdx.x == 0) a.lse[row] = total == 0.f ? -INFINITY : (top + log2f(total)) * 0.6931471805599453f;
 }
 
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                                  const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeTiledFn encode_fn() {
+  static EncodeTiledFn fn = [] {
+    void* symbol = nullptr;
+    cudaDriverEntryPointQueryResult found;
+    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &symbol, 12000, cudaEnableDefault, &found) != cudaSuccess ||
+        found != cudaDriverEntryPointSuccess)
+      symbol = nullptr;
+    return reinterpret_cast<EncodeTiledFn>(symbol);
+  }();
+  return fn;
+}
+// [planes, rows, 576] elements of two bytes, boxes of 64 elements x box_rows rows in 128-byte swizzle; strides in elements.
+bool encode_map(CUtensorMap* map, bool bf16, const void* base, uint32_t dims, uint64_t rows, uint64_t planes, int64_t row, int64_t plane,
+                uint32_t box_rows) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) return false;
+  const cuuint64_t sizes[3] = {kWidth, rows, planes};
+  const cuuint64_t strides[2] = {static_cast<cuuint64_t>(row) * 2u, static_cast<cuuint64_t>(plane) * 2u};
+  const cuuint32_t box[3] = {64, box_rows, 1}, step[3] = {1, 1, 1};
+  return fn(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, dims, const_cast<void*>(base), sizes, strides, box,
+            step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 template <typename T, uint32_t kN>
 uint32_t launch_tiles(const KvipAttentionArgs& a, KernelSlot slot, uint32_t groups, uint32_t group_heads, uint32_t splits, cudaStream_t stream) {
   if (uint32_t bad = raise_dynamic_smem(slot, reinterpret_cast<const void*>(attend_tiles<T, kN>), static_cast<int>(Layout<kN>::kBytes),
                                         "slot_attention attribute"))
     return bad;
-  attend_tiles<T, kN><<<a.tokens * groups * splits, kAttentionThreads, Layout<kN>::kBytes, stream>>>(a, groups, group_heads, splits);
+  const bool bf16 = __is_same(T, __nv_bfloat16);
+  CUtensorMap query_map, pool_map, draft_map;
+  // strides of a dimension of size one do not matter, but the encoder looks at them
+  const int64_t head = a.heads > 1 ? a.query_head : kWidth, token = a.tokens > 1 ? a.query_token : a.heads * kWidth;
+  const int64_t drafted = a.draft && a.tokens > 1 ? a.draft_token : kWidth;
+  if (!encode_map(&query_map, bf16, a.query, 3, a.heads, a.tokens, head, token, kN) ||
+      !encode_map(&pool_map, bf16, a.pool, 2, a.pool_rows, 1, kWidth, 0, 1) ||
+      !encode_map(&draft_map, bf16, a.draft ? a.draft : a.query, 2, a.tokens, 1, drafted, 0, 1)) {
+    set_error("slot_attention: the strides do not fit a tensor map");
+    return KVIP_BAD_ARGUMENT;
+  }
+  attend_tiles<T, kN><<<a.tokens * groups * splits, kAttentionThreads, Layout<kN>::kBytes, stream>>>(query_map, pool_map, draft_map, a, groups,
+                                                                                                     group_heads, splits);
   count_launch();
   return check_launch("attend_tiles");
 }
@@ -625,11 +719,11 @@ extern "C" uint32_t kvip_b200_slot_attention(const KvipAttentionArgs* a, void* s
   KVIP_REQUIRE(a->tokens >= 1 && a->heads >= 1 && a->heads <= 128 && a->entries >= 1, "slot_attention: tokens, 1..128 heads, entries");
   KVIP_REQUIRE(a->batch >= 1 && (a->requests || (a->queries >= 1 && static_cast<uint64_t>(a->batch) * a->queries >= a->tokens)),
                "slot_attention: requests of the tokens");
-  KVIP_REQUIRE(a->output_stride >= 1 && a->output_stride <= a->pool_rows, "slot_attention: pool geometry");
+  KVIP_REQUIRE(a->output_stride >= 1 && a->output_stride <= a->pool_rows && a->pool_rows <= 0x7fffffffull, "slot_attention: pool geometry");
   KVIP_REQUIRE(!a->draft || a->starts, "slot_attention: drafted rows need the requests' starts");
   KVIP_REQUIRE(a->dtype <= KVIP_FLOAT_FP16, "slot_attention: bf16 or fp16");
   KVIP_REQUIRE(((reinterpret_cast<uintptr_t>(a->query) | reinterpret_cast<uintptr_t>(a->pool) | reinterpret_cast<uintptr_t>(a->out) |
-                 reinterpret_cast<uintptr_t>(a->draft)) & 15u) == 0 && ((a->query_token | a->query_head | a->draft_token) & 7) == 0,
+                 reinterpret_cast<uintptr_t>(a->draft) | reinterpret_cast<uintptr_t>(a->partial)) & 15u) == 0 && ((a->query_token | a->query_head | a->draft_token) & 7) == 0,
                "slot_attention: 16-byte aligned rows");
   KVIP_REQUIRE(a->splits <= 1 || (a->partial && a->partial_stats &&
                                   static_cast<uint64_t>(a->splits) * a->tokens * a->heads <= a->partial_rows),
