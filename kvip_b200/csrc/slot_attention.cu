@@ -32,14 +32,18 @@ constexpr uint32_t kPieceBytes = kTile * 128;           // one piece of every ro
 constexpr uint32_t kStageBytes = kPieces * kPieceBytes; // 73,728
 constexpr uint32_t kStages = 2;
 constexpr uint32_t kGroupHeads = 64;
-// Warps 0-3 and 4-7: softmax of the lower and the upper half of the heads; 8-11: loaders, two per stage; 12: MMA issuer.
-constexpr uint32_t kFirstLoaderWarp = 8, kMmaWarp = 12, kAttentionThreads = 32 * 13;
+constexpr uint32_t kThirds = 3;                         // a stage is filled, read and released in three groups of pieces
+constexpr uint32_t kThirdBytes = kStageBytes / kThirds;
+// Warps 0-3 and 4-7: softmax of the lower and the upper half of the heads; 8-15: loaders, four per stage; 16: MMA issuer.
+constexpr uint32_t kFirstLoaderWarp = 8, kLoaderWarps = 4, kMmaWarp = kFirstLoaderWarp + kStages * kLoaderWarps;
+constexpr uint32_t kAttentionThreads = 32 * (kMmaWarp + 1);
 constexpr uint32_t kRole = 128;                         // threads of one softmax half
+constexpr uint32_t kOutRow = kValue * 2 + 64;           // bytes of an output row while it is laid out: 16 banks further than the last
 constexpr float kSlack = 8.f;                           // log2: p may reach 2^8 before the reference moves
 constexpr uint32_t kDefaultWaitKilocycles = 2000000u;   // about one second of SM clock
 
 struct Control {                                        // behind the tiles in shared memory
-  uint64_t full[kStages], empty[kStages], scored[2], weighted, query_full;
+  uint64_t full[kStages][kThirds], empty[kStages][kThirds], scored[2], weighted, query_full;
   uint32_t valid[kStages][4];                           // row 4 l + c of the tile is there: bit l of word c
   float reduce[4][kGroupHeads];
   float factor[kGroupHeads], top[kGroupHeads];
@@ -175,10 +179,6 @@ template <> __device__ __forceinline__ uint32_t pack_pair<__half>(float x, float
   __half2 v = __floats2half2_rn(x, y);
   return *reinterpret_cast<uint32_t*>(&v);
 }
-template <typename T> __device__ __forceinline__ T round_to(float x);
-template <> __device__ __forceinline__ __nv_bfloat16 round_to(float x) { return __float2bfloat16_rn(x); }
-template <> __device__ __forceinline__ __half round_to(float x) { return __float2half_rn(x); }
-
 // What token t may read.
 struct Rows {
   uint32_t base, limit;       // first pool row of the owner and how many it has (0: none may be read)
@@ -227,43 +227,50 @@ attend_tiles(const __grid_constant__ CUtensorMap query_map, const __grid_constan
   const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u;
   const uint32_t split = blockIdx.x % splits, unit = blockIdx.x / splits, group = unit % groups, t = unit / groups;
   const uint32_t head0 = group * group_heads, heads = min(group_heads, a.heads - head0);
-  const int32_t request = a.requests ? a.requests[t] : static_cast<int32_t>(t / a.queries);
-  if (request < 0) return;
   const int32_t* list = a.slots + static_cast<uint64_t>(t) * a.entries;
   const bool vectors = (a.entries & 3u) == 0u && (reinterpret_cast<uintptr_t>(a.slots) & 15u) == 0u;
+  // lists end in -1 where a context is short: the last entry in use bounds the tiles
+  uint32_t last = 0;
+  if (vectors) {
+    for (uint32_t k = tid; k < a.entries / 4u; k += kAttentionThreads) {
+      const int4 e = __ldg(reinterpret_cast<const int4*>(list) + k);
+      if ((e.x & e.y & e.z & e.w) >= 0) last = 4u * k + (e.w >= 0 ? 4u : e.z >= 0 ? 3u : e.y >= 0 ? 2u : 1u);
+    }
+  } else {
+    for (uint32_t k = tid; k < a.entries; k += kAttentionThreads)
+      if (list[k] >= 0) last = k + 1u;
+  }
+  const int32_t request = a.requests ? a.requests[t] : static_cast<int32_t>(t / a.queries);
+  if (request < 0) return;
 
   auto bar = [&](const uint64_t& b) { return smem_u32(&b); };
-  if (tid == 0) {
-    for (uint32_t s = 0; s < kStages; ++s) { mbar_init(bar(c.full[s]), 2); mbar_init(bar(c.empty[s]), 1); }
-    mbar_init(bar(c.scored[0]), 1); mbar_init(bar(c.scored[1]), 1);
-    mbar_init(bar(c.weighted), 2 * kRole); mbar_init(bar(c.query_full), 1);
-    c.abort_flag = 0;
-    c.last = 0;
-    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    fence_async();
-  }
-  if (warp == kMmaWarp) {  // all of tensor memory: one CTA per SM
+  if (warp == kMmaWarp) {
+    if (lane == 0) {
+      for (uint32_t s = 0; s < kStages; ++s)
+        for (uint32_t third = 0; third < kThirds; ++third) { mbar_init(bar(c.full[s][third]), kLoaderWarps); mbar_init(bar(c.empty[s][third]), 1); }
+      mbar_init(bar(c.scored[0]), 1); mbar_init(bar(c.scored[1]), 1);
+      mbar_init(bar(c.weighted), 2 * kRole / 32); mbar_init(bar(c.query_full), 1);
+      c.abort_flag = 0;
+      c.last = 0;
+      asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+      fence_async();
+    }
+    __syncwarp();
+    // all of tensor memory: one CTA per SM
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&c.tmem)) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
   const Rows rows = rows_of(a, t, request);
-  // lists end in -1 where a context is short: the last entry in use bounds the tiles
-  uint32_t last = 0;
-  if (rows.limit) {
-    if (vectors) {
-      for (uint32_t k = tid; k < a.entries / 4u; k += kAttentionThreads) {
-        const int4 e = __ldg(reinterpret_cast<const int4*>(list) + k);
-        if (e.x >= 0 || e.y >= 0 || e.z >= 0 || e.w >= 0) last = 4u * k + (e.w >= 0 ? 4u : e.z >= 0 ? 3u : e.y >= 0 ? 2u : 1u);
-      }
-    } else {
-      for (uint32_t k = tid; k < a.entries; k += kAttentionThreads)
-        if (list[k] >= 0) last = k + 1u;
-    }
-  }
-  last = __reduce_max_sync(0xffffffffu, last);
+  last = __reduce_max_sync(0xffffffffu, rows.limit ? last : 0u);
   fence_before();
   __syncthreads();
   fence_after();
+  if (warp == kFirstLoaderWarp && elect_one()) {   // waited for in any case: by the issuer, or below where there is no tile
+    expect_bytes(bar(c.query_full), kPieces * kN * 128u);
+    for (uint32_t piece = 0; piece < kPieces; ++piece)
+      load_query(base + Layout<kN>::kQuery + piece * (kN * 128u), &query_map, piece * 64u, head0, t, bar(c.query_full));
+  }
+  __syncwarp();
   if (lane == 0 && last) atomicMax(&c.last, last);
   __syncthreads();
   const uint32_t tmem = c.tmem;
@@ -277,16 +284,11 @@ attend_tiles(const __grid_constant__ CUtensorMap query_map, const __grid_constan
   auto none = [&](uint32_t s) { return (c.valid[s][0] | c.valid[s][1] | c.valid[s][2] | c.valid[s][3]) == 0u; };
 
   if (warp >= kFirstLoaderWarp && warp < kMmaWarp) {
-    // ================= loaders: warps 8, 9 (10, 11) gather the first (last) 32 rows of the tiles 0, 2, .. and 1, 3, .. =======
-    const uint32_t g = (warp - kFirstLoaderWarp) & 1u, half = (warp - kFirstLoaderWarp) >> 1;
+    // ================= loaders: warp 8 + 2 i + g gathers 16 rows, from 16 i on, of the tiles g, g + 2, ... =================
+    const uint32_t g = (warp - kFirstLoaderWarp) & 1u, quarter = (warp - kFirstLoaderWarp) >> 1;
     const bool leader = elect_one();
     int32_t bad = warp == kFirstLoaderWarp ? rows.bad : 0;
     if (count) {
-      if (warp == kFirstLoaderWarp && leader) {
-        expect_bytes(bar(c.query_full), kPieces * kN * 128u);
-        for (uint32_t piece = 0; piece < kPieces; ++piece)
-          load_query(base + Layout<kN>::kQuery + piece * (kN * 128u), &query_map, piece * 64u, head0, t, bar(c.query_full));
-      }
       auto entries_of = [&](uint32_t n) -> int4 {   // entries 4 lane .. + 3 of tile n (lanes 0-15), -1 behind the list
         int4 e = make_int4(-1, -1, -1, -1);
         const uint32_t k = (first + n) * kTile + 4u * lane;
@@ -324,36 +326,49 @@ attend_tiles(const __grid_constant__ CUtensorMap query_map, const __grid_constan
         }
         const uint32_t b0 = __ballot_sync(0xffffffffu, v0), b1 = __ballot_sync(0xffffffffu, v1), b2 = __ballot_sync(0xffffffffu, v2),
                        b3 = __ballot_sync(0xffffffffu, v3);
-        if (!__all_sync(0xffffffffu, mbar_wait(bar(c.empty[g]), ((n >> 1) & 1u) ^ 1u, waits))) break;
-        if (leader && half == 0) { c.valid[g][0] = b0; c.valid[g][1] = b1; c.valid[g][2] = b2; c.valid[g][3] = b3; }
-        const uint32_t any = b0 | b1 | b2 | b3;
-        if (!any) {
-          __syncwarp();
-          if (leader) mbar_arrive(bar(c.full[g]));
-          continue;
-        }
         // a place without a row takes one of the tile's own: its weight is zero, and it holds nothing that the token does not read
+        const uint32_t any = b0 | b1 | b2 | b3, phase = ((n >> 1) & 1u) ^ 1u;
         const int32_t mine = v0 ? e.x : v1 ? e.y : v2 ? e.z : e.w;
-        const int32_t spare = __shfl_sync(0xffffffffu, mine, __ffs(static_cast<int>(any)) - 1);
+        const int32_t spare = __shfl_sync(0xffffffffu, mine, (__ffs(static_cast<int>(any)) - 1) & 31);
         if (!v0) e.x = spare;
         if (!v1) e.y = spare;
         if (!v2) e.z = spare;
         if (!v3) e.w = spare;
-        const CUtensorMap* map = from_list ? &pool_map : &draft_map;
-        if (leader) expect_bytes(bar(c.full[g]), kStageBytes / 2u);
-        __syncwarp();
+        int4 r[4];                                 // four times four rows
 #pragma unroll
-        for (uint32_t q = 0; q < 8u; ++q) {        // four rows each
-          const uint32_t from = half * 8u + q;
-          const int4 r = make_int4(__shfl_sync(0xffffffffu, e.x, from), __shfl_sync(0xffffffffu, e.y, from),
-                                   __shfl_sync(0xffffffffu, e.z, from), __shfl_sync(0xffffffffu, e.w, from));
-          if (leader) {
-#pragma unroll
-            for (uint32_t piece = 0; piece < kPieces; ++piece)
-              load_rows(base + g * kStageBytes + piece * kPieceBytes + from * 512u, map, piece * 64u, r, bar(c.full[g]));
-          }
+        for (uint32_t q = 0; q < 4u; ++q) {
+          const uint32_t from = quarter * 4u + q;
+          r[q] = make_int4(__shfl_sync(0xffffffffu, e.x, from), __shfl_sync(0xffffffffu, e.y, from),
+                           __shfl_sync(0xffffffffu, e.z, from), __shfl_sync(0xffffffffu, e.w, from));
         }
+        const CUtensorMap* map = from_list ? &pool_map : &draft_map;
+        bool alive = true;
+#pragma unroll
+        for (uint32_t third = 0; third < kThirds; ++third) {
+          alive = __all_sync(0xffffffffu, mbar_wait(bar(c.empty[g][third]), phase, waits));
+          if (!alive) break;
+          if (leader) {
+            // every reader of the mask of tile n - 2 has done with it when the first third is released
+            if (third == 0 && quarter == 0) { c.valid[g][0] = b0; c.valid[g][1] = b1; c.valid[g][2] = b2; c.valid[g][3] = b3; }
+            if (any) {
+              expect_bytes(bar(c.full[g][third]), kThirdBytes / kLoaderWarps);
+#pragma unroll
+              for (uint32_t i = 0; i < kPieces / kThirds; ++i) {
+                const uint32_t piece = third * (kPieces / kThirds) + i;
+#pragma unroll
+                for (uint32_t q = 0; q < 4u; ++q)
+                  load_rows(base + g * kStageBytes + piece * kPieceBytes + (quarter * 4u + q) * 512u, map, piece * 64u, r[q], bar(c.full[g][third]));
+              }
+            } else {
+              mbar_arrive(bar(c.full[g][third]));
+            }
+          }
+          __syncwarp();
+        }
+        if (!alive) break;
       }
+    } else if (warp == kFirstLoaderWarp) {
+      mbar_wait(bar(c.query_full), 0, waits);
     }
     if (bad) atomicOr(a.status, bad);
   } else if (warp == kMmaWarp) {
@@ -365,48 +380,56 @@ attend_tiles(const __grid_constant__ CUtensorMap query_map, const __grid_constan
       constexpr uint32_t kValueDesc = kBase | (1u << 15) | (1u << 16) | ((128u >> 4) << 24);   // both operands M/N-major
       const bool leader = elect_one();
       bool written = false, alive = __all_sync(0xffffffffu, mbar_wait(bar(c.query_full), 0, waits));
-      auto score = [&](uint32_t n) {         // S^T of tile n, whose rows are in place
-        const uint32_t s = n & 1u;
+      // S^T of tile n, piece by piece as its thirds come; the first has come when this is called
+      auto score = [&](uint32_t n) -> bool {
+        const uint32_t s = n & 1u, phase = (n >> 1) & 1u;
         if (none(s)) {
-          if (leader) mbar_arrive(bar(c.scored[s]));
-          return;
+          bool ok = true;
+          for (uint32_t third = 1; third < kThirds; ++third) ok = ok && __all_sync(0xffffffffu, mbar_wait(bar(c.full[s][third]), phase, waits));
+          if (leader && ok) mbar_arrive(bar(c.scored[s]));
+          return ok;
         }
-        fence_after();
         const uint32_t d = tmem + kScores + s * kN;
         const uint64_t da = operand(base + s * kStageBytes, 16u), db = operand(base + Layout<kN>::kQuery, 16u);
-        if (leader) {
 #pragma unroll
-          for (uint32_t piece = 0; piece < kPieces; ++piece) {
+        for (uint32_t third = 0; third < kThirds; ++third) {
+          if (third && !__all_sync(0xffffffffu, mbar_wait(bar(c.full[s][third]), phase, waits))) return false;
+          fence_after();
+          if (leader) {
 #pragma unroll
-            for (uint32_t k = 0; k < 4; ++k)
-              mma(d, da + (piece * (kPieceBytes >> 4) + 2u * k), db + (piece * (kN * 8u) + 2u * k), kScoreDesc, (piece | k) != 0u);
+            for (uint32_t piece = third * (kPieces / kThirds); piece < (third + 1u) * (kPieces / kThirds); ++piece) {
+#pragma unroll
+              for (uint32_t k = 0; k < 4; ++k)
+                mma(d, da + (piece * (kPieceBytes >> 4) + 2u * k), db + (piece * (kN * 8u) + 2u * k), kScoreDesc, (piece | k) != 0u);
+            }
+            if (third == kThirds - 1u) commit(bar(c.scored[s]));
           }
-          commit(bar(c.scored[s]));
+          __syncwarp();
         }
-        __syncwarp();
+        return true;
       };
       uint32_t scored = 0;                   // tiles whose scores have been issued
       for (uint32_t n = 0; alive && n < count; ++n) {
         const uint32_t s = n & 1u, phase = (n >> 1) & 1u;
         if (scored == n) {
-          if (!__all_sync(0xffffffffu, mbar_wait(bar(c.full[s]), phase, waits))) break;
-          score(n);
+          if (!__all_sync(0xffffffffu, mbar_wait(bar(c.full[s][0]), phase, waits)) || !score(n)) break;
           ++scored;
         }
-        // while the weights of tile n are made: the scores of the next tile, if its rows have come
+        // while the weights of tile n are made: the scores of the next tile, if its rows are coming
         if (scored == n + 1 && n + 1 < count) {
           const uint32_t s1 = s ^ 1u, phase1 = ((n + 1) >> 1) & 1u;
           while (!__any_sync(0xffffffffu, mbar_test(bar(c.weighted), n & 1u) || c.abort_flag)) {
-            if (__all_sync(0xffffffffu, mbar_test(bar(c.full[s1]), phase1))) {
-              score(n + 1);
+            if (__all_sync(0xffffffffu, mbar_test(bar(c.full[s1][0]), phase1))) {
+              alive = score(n + 1);
               ++scored;
               break;
             }
           }
         }
-        if (!__all_sync(0xffffffffu, mbar_wait(bar(c.weighted), n & 1u, waits))) break;
+        if (!alive || !__all_sync(0xffffffffu, mbar_wait(bar(c.weighted), n & 1u, waits))) break;
         if (none(s)) {                       // in order behind the products before
-          if (leader) commit(bar(c.empty[s]));
+          if (leader)
+            for (uint32_t third = 0; third < kThirds; ++third) commit(bar(c.empty[s][third]));
           continue;
         }
         fence_after();
@@ -417,8 +440,8 @@ attend_tiles(const __grid_constant__ CUtensorMap query_map, const __grid_constan
 #pragma unroll
             for (uint32_t k = 0; k < kTile / 16u; ++k)
               mma(tmem + kOut + m * kN, da + (2u * m * (kPieceBytes >> 4) + k * 128u), db + k * 128u, kValueDesc, written || k != 0u);
+            if (m) commit(bar(c.empty[s][m - 1u]));   // blocks 0-1 end with the pieces 0-2, block 2 with 3-5, block 3 with the rest
           }
-          commit(bar(c.empty[s]));
         }
         __syncwarp();
         written = true;
@@ -437,12 +460,14 @@ attend_tiles(const __grid_constant__ CUtensorMap query_map, const __grid_constan
     bool dead = false, written = false;
     for (uint32_t n = 0; n < count; ++n) {
       const uint32_t s = n & 1u, phase = (n >> 1) & 1u;
-      bool ok = !dead && mbar_wait(bar(c.scored[s]), phase, waits) && mbar_wait(bar(c.full[s]), phase, waits);
+      bool ok = !dead && mbar_wait(bar(c.scored[s]), phase, waits) && mbar_wait(bar(c.full[s][0]), phase, waits);
       ok = __all_sync(0xffffffffu, ok);
       if (ok && none(s)) {                     // the same for all: the mask belongs to the tile
         // as below: a thread arrives for this tile only when all have arrived for the one before
-        if (n && !mbar_wait(bar(c.empty[(n - 1u) & 1u]), ((n - 1u) >> 1) & 1u, waits)) dead = true;
-        else mbar_arrive(bar(c.weighted));
+        if (n && !mbar_wait(bar(c.empty[(n - 1u) & 1u][kThirds - 1u]), ((n - 1u) >> 1) & 1u, waits)) dead = true;
+        __syncwarp();
+        if (__any_sync(0xffffffffu, dead)) dead = true;
+        else if (lane == 0) mbar_arrive(bar(c.weighted));
         continue;
       }
       const uint32_t word = c.valid[s][row0 & 3u];
@@ -486,7 +511,7 @@ attend_tiles(const __grid_constant__ CUtensorMap query_map, const __grid_constan
         role_any(1u + side, false);
         if (written) {                         // the accumulators hold the tiles before this one, which must be in
           const uint32_t before = n - 1u;      // stages are released in order, an empty tile's too
-          ok = mbar_wait(bar(c.empty[before & 1u]), (before >> 1) & 1u, waits);
+          ok = mbar_wait(bar(c.empty[before & 1u][kThirds - 1u]), (before >> 1) & 1u, waits);
           if (__all_sync(0xffffffffu, ok)) {
             fence_after();
             for (uint32_t m = 0; m < 4; ++m) {
@@ -517,7 +542,8 @@ attend_tiles(const __grid_constant__ CUtensorMap query_map, const __grid_constan
         p[2 * j + 1] = pack_pair<T>(x1, y1);
       }
       // the product of the tile before has read its weights
-      if (n && !dead && !mbar_wait(bar(c.empty[(n - 1u) & 1u]), ((n - 1u) >> 1) & 1u, waits)) dead = true;
+      if (n && !dead && !mbar_wait(bar(c.empty[(n - 1u) & 1u][kThirds - 1u]), ((n - 1u) >> 1) & 1u, waits)) dead = true;
+      dead = __any_sync(0xffffffffu, dead);
       if (!dead) {
         const uint32_t to = base + Layout<kN>::kWeights + row0 * 128u + (lane & 3u) * 4u;
 #pragma unroll
@@ -528,11 +554,12 @@ attend_tiles(const __grid_constant__ CUtensorMap query_map, const __grid_constan
         }
         fence_async();
         fence_before();
-        mbar_arrive(bar(c.weighted));
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(c.weighted));
       }
       written = true;
     }
-    if (count && !dead && !mbar_wait(bar(c.empty[(count - 1u) & 1u]), ((count - 1u) >> 1) & 1u, waits)) dead = true;
+    if (count && !dead && !mbar_wait(bar(c.empty[(count - 1u) & 1u][kThirds - 1u]), ((count - 1u) >> 1) & 1u, waits)) dead = true;
     // sums over the rows of all tiles
 #pragma unroll
     for (uint32_t j = 0; j < 2 * kBlocks; ++j) {
@@ -560,8 +587,8 @@ attend_tiles(const __grid_constant__ CUtensorMap query_map, const __grid_constan
       }
       role_any<2 * kRole>(3u, false);
       fence_after();
-      // A lane holds one value element of every head. The share of the output, [heads, 512] and contiguous in memory, is laid
-      // out in the stages (all products have read them) and leaves as one copy.
+      // A lane holds one value element of every head. The share of the output is laid out in the stages (all products have read
+      // them) and leaves by copies of whole rows. In 16 bits two lanes exchange a value, so that each writes a whole word.
 #pragma unroll
       for (uint32_t m = 0; m < 2; ++m) {
         const uint32_t block = 2u * side + m, element = block * 128u + w * 32u + lane;
@@ -574,22 +601,33 @@ attend_tiles(const __grid_constant__ CUtensorMap query_map, const __grid_constan
             tmem_ld_done();
           }
 #pragma unroll
-          for (uint32_t i = 0; i < 16; ++i) {
-            const float y = written ? __uint_as_float(o[i]) * c.factor[h0 + i] : 0.f;
-            if (splits == 1) reinterpret_cast<T*>(smem)[(h0 + i) * kValue + element] = round_to<T>(y);
-            else reinterpret_cast<float*>(smem)[(h0 + i) * kValue + element] = y;
+          for (uint32_t i = 0; i < 16; i += 2) {
+            const float2 f = *reinterpret_cast<const float2*>(&c.factor[h0 + i]);
+            const float y0 = written ? __uint_as_float(o[i]) * f.x : 0.f, y1 = written ? __uint_as_float(o[i + 1]) * f.y : 0.f;
+            if (splits == 1) {
+              const bool odd = lane & 1u;
+              const float other = __shfl_xor_sync(0xffffffffu, odd ? y0 : y1, 1);
+              const uint32_t word = odd ? pack_pair<T>(other, y1) : pack_pair<T>(y0, other);
+              *reinterpret_cast<uint32_t*>(smem + (h0 + i + (odd ? 1u : 0u)) * kOutRow + (element & ~1u) * 2u) = word;
+            } else {
+              reinterpret_cast<float*>(smem)[(h0 + i) * kValue + element] = y0;
+              reinterpret_cast<float*>(smem)[(h0 + i + 1u) * kValue + element] = y1;
+            }
           }
         }
       }
       fence_async();
       role_any<2 * kRole>(3u, false);
-      if (tid == 0) {
-        void* to = splits == 1 ? static_cast<void*>(static_cast<T*>(a.out) + out_row * kValue) : static_cast<void*>(a.partial + part_row * kValue);
-        const uint32_t bytes = heads * kValue * (splits == 1 ? 2u : 4u);
-        asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(to), "r"(base), "r"(bytes) : "memory");
-        asm volatile("cp.async.bulk.commit_group;" ::: "memory");
-        asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+      if (splits == 1) {
+        if (tid < heads)
+          asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;"
+                       ::"l"(static_cast<T*>(a.out) + (out_row + tid) * kValue), "r"(base + tid * kOutRow), "r"(kValue * 2u) : "memory");
+      } else if (tid == 0) {
+        asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;"
+                     ::"l"(a.partial + part_row * kValue), "r"(base), "r"(heads * kValue * 4u) : "memory");
       }
+      asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+      asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
       fence_before();
     }
   }
