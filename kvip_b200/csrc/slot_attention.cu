@@ -34,19 +34,28 @@ constexpr uint32_t kStages = 2;
 constexpr uint32_t kGroupHeads = 64;
 constexpr uint32_t kThirds = 3;                         // a stage is filled, read and released in three groups of pieces
 constexpr uint32_t kThirdBytes = kStageBytes / kThirds;
-// Warps 0-3 and 4-7: softmax of the lower and the upper half of the heads; 8-15: loaders, four per stage; 16: MMA issuer.
-constexpr uint32_t kFirstLoaderWarp = 8, kLoaderWarps = 4, kMmaWarp = kFirstLoaderWarp + kStages * kLoaderWarps;
-constexpr uint32_t kAttentionThreads = 32 * (kMmaWarp + 1);
+// Warps 0-3 and 4-7: softmax of the lower and the upper half of the heads; 8-15: loaders, four per stage; 16, 17: issuers of
+// the first and the second product.
+constexpr uint32_t kFirstLoaderWarp = 8, kLoaderWarps = 4, kScoreWarp = kFirstLoaderWarp + kStages * kLoaderWarps, kValueWarp = kScoreWarp + 1;
+constexpr uint32_t kAttentionThreads = 32 * (kValueWarp + 1);
 constexpr uint32_t kRole = 128;                         // threads of one softmax half
-constexpr uint32_t kOutRow = kValue * 2 + 64;           // bytes of an output row while it is laid out: 16 banks further than the last
+constexpr uint32_t kOutRow = kValue * 2 + 16;           // bytes of an output row while it is laid out: four banks further than the last
 constexpr float kSlack = 8.f;                           // log2: p may reach 2^8 before the reference moves
 constexpr uint32_t kDefaultWaitKilocycles = 2000000u;   // about one second of SM clock
 
+// What token t may read.
+struct Rows {
+  uint32_t base, limit;       // first pool row of the owner and how many it has (0: none may be read)
+  uint32_t draft, drafted;    // first drafted row of the request, and how many of them bound those the token sees
+  uint64_t seen;
+  int32_t bad, request;
+};
 struct Control {                                        // behind the tiles in shared memory
-  uint64_t full[kStages][kThirds], empty[kStages][kThirds], scored[2], weighted, query_full;
+  uint64_t full[kStages][kThirds], empty[kStages][kThirds], scored[2], taken[2], weighted, query_full;
   uint32_t valid[kStages][4];                           // row 4 l + c of the tile is there: bit l of word c
   float reduce[4][kGroupHeads];
   float factor[kGroupHeads], top[kGroupHeads];
+  Rows rows;
   uint32_t tmem, abort_flag, last;
 };
 
@@ -64,12 +73,6 @@ __device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
 }
 __device__ __forceinline__ void mbar_arrive(uint32_t bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
-}
-__device__ __forceinline__ bool mbar_test(uint32_t bar, uint32_t parity) {
-  uint32_t done;
-  asm volatile("{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
-               : "=r"(done) : "r"(bar), "r"(parity) : "memory");
-  return done != 0u;
 }
 __device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
   uint32_t done;
@@ -179,15 +182,11 @@ template <> __device__ __forceinline__ uint32_t pack_pair<__half>(float x, float
   __half2 v = __floats2half2_rn(x, y);
   return *reinterpret_cast<uint32_t*>(&v);
 }
-// What token t may read.
-struct Rows {
-  uint32_t base, limit;       // first pool row of the owner and how many it has (0: none may be read)
-  uint32_t draft, drafted;    // first drafted row of the request, and how many of them bound those the token sees
-  uint64_t seen;
-  int32_t bad;
-};
-__device__ __forceinline__ Rows rows_of(const KvipAttentionArgs& a, uint32_t t, int32_t request) {
-  Rows r{0u, a.output_stride, 0u, 0u, 0ull, 0};
+__device__ __forceinline__ Rows rows_of(const KvipAttentionArgs& a, uint32_t t) {
+  const int32_t request = a.requests ? a.requests[t] : static_cast<int32_t>(t / a.queries);
+  Rows r{0u, a.output_stride, 0u, 0u, 0ull, 0, request};
+  if (request < 0) return r;   // padding
+  const uint64_t mask = a.draft && a.ancestors ? static_cast<uint64_t>(a.ancestors[t]) : 0ull;
   if (static_cast<uint32_t>(request) >= a.batch) {
     r.limit = 0;
     r.bad = static_cast<int32_t>(KVIP_ERR_TOKEN_RANGE);
@@ -208,7 +207,7 @@ __device__ __forceinline__ Rows rows_of(const KvipAttentionArgs& a, uint32_t t, 
     } else {
       const uint32_t nodes = static_cast<uint32_t>(min(static_cast<int64_t>(64), behind - first));
       r.draft = static_cast<uint32_t>(first);
-      r.seen = a.ancestors ? static_cast<uint64_t>(a.ancestors[t]) : (own < 0 ? 0ull : own >= 63 ? ~0ull : (2ull << own) - 1ull);
+      r.seen = a.ancestors ? mask : (own < 0 ? 0ull : own >= 63 ? ~0ull : (2ull << own) - 1ull);
       if (nodes < 64u) r.seen &= (1ull << nodes) - 1ull;
       r.drafted = r.seen ? 64u - static_cast<uint32_t>(__clzll(static_cast<long long>(r.seen))) : 0u;
     }
@@ -229,26 +228,13 @@ attend_tiles(const __grid_constant__ CUtensorMap query_map, const __grid_constan
   const uint32_t head0 = group * group_heads, heads = min(group_heads, a.heads - head0);
   const int32_t* list = a.slots + static_cast<uint64_t>(t) * a.entries;
   const bool vectors = (a.entries & 3u) == 0u && (reinterpret_cast<uintptr_t>(a.slots) & 15u) == 0u;
-  // lists end in -1 where a context is short: the last entry in use bounds the tiles
-  uint32_t last = 0;
-  if (vectors) {
-    for (uint32_t k = tid; k < a.entries / 4u; k += kAttentionThreads) {
-      const int4 e = __ldg(reinterpret_cast<const int4*>(list) + k);
-      if ((e.x & e.y & e.z & e.w) >= 0) last = 4u * k + (e.w >= 0 ? 4u : e.z >= 0 ? 3u : e.y >= 0 ? 2u : 1u);
-    }
-  } else {
-    for (uint32_t k = tid; k < a.entries; k += kAttentionThreads)
-      if (list[k] >= 0) last = k + 1u;
-  }
-  const int32_t request = a.requests ? a.requests[t] : static_cast<int32_t>(t / a.queries);
-  if (request < 0) return;
-
   auto bar = [&](const uint64_t& b) { return smem_u32(&b); };
-  if (warp == kMmaWarp) {
+  uint32_t last = 0;
+  if (warp == kScoreWarp) {
     if (lane == 0) {
       for (uint32_t s = 0; s < kStages; ++s)
         for (uint32_t third = 0; third < kThirds; ++third) { mbar_init(bar(c.full[s][third]), kLoaderWarps); mbar_init(bar(c.empty[s][third]), 1); }
-      mbar_init(bar(c.scored[0]), 1); mbar_init(bar(c.scored[1]), 1);
+      for (uint32_t s = 0; s < 2; ++s) { mbar_init(bar(c.scored[s]), 1); mbar_init(bar(c.taken[s]), 2 * kRole / 32); }
       mbar_init(bar(c.weighted), 2 * kRole / 32); mbar_init(bar(c.query_full), 1);
       c.abort_flag = 0;
       c.last = 0;
@@ -259,31 +245,44 @@ attend_tiles(const __grid_constant__ CUtensorMap query_map, const __grid_constan
     // all of tensor memory: one CTA per SM
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&c.tmem)) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  } else if (warp == kValueWarp) {
+    if (lane == 0) c.rows = rows_of(a, t);         // a chain of loads, beside the others' walk along the list
+    if (lane < 3) {
+      const CUtensorMap* map = lane == 0 ? &query_map : lane == 1 ? &pool_map : &draft_map;
+      asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");
+    }
+  } else if (vectors) {
+    // lists end in -1 where a context is short: the last entry in use bounds the tiles
+    for (uint32_t k = tid; k < a.entries / 4u; k += 32u * kScoreWarp) {
+      const int4 e = __ldg(reinterpret_cast<const int4*>(list) + k);
+      if ((e.x & e.y & e.z & e.w) >= 0) last = 4u * k + (e.w >= 0 ? 4u : e.z >= 0 ? 3u : e.y >= 0 ? 2u : 1u);
+    }
+  } else {
+    for (uint32_t k = tid; k < a.entries; k += 32u * kScoreWarp)
+      if (list[k] >= 0) last = k + 1u;
   }
-  const Rows rows = rows_of(a, t, request);
-  last = __reduce_max_sync(0xffffffffu, rows.limit ? last : 0u);
+  last = __reduce_max_sync(0xffffffffu, last);
   fence_before();
   __syncthreads();
   fence_after();
-  if (warp == kFirstLoaderWarp && elect_one()) {   // waited for in any case: by the issuer, or below where there is no tile
+  const Rows rows = c.rows;
+  if (rows.request >= 0 && warp == kScoreWarp && elect_one()) {   // waited for in any case: by this warp
     expect_bytes(bar(c.query_full), kPieces * kN * 128u);
     for (uint32_t piece = 0; piece < kPieces; ++piece)
       load_query(base + Layout<kN>::kQuery + piece * (kN * 128u), &query_map, piece * 64u, head0, t, bar(c.query_full));
   }
   __syncwarp();
-  if (lane == 0 && last) atomicMax(&c.last, last);
+  if (lane == 0 && last && rows.limit) atomicMax(&c.last, last);
   __syncthreads();
   const uint32_t tmem = c.tmem;
   // tiles of the list, then one of the drafted rows
   const uint32_t listed = c.last, list_tiles = (listed + kTile - 1) / kTile, tiles = list_tiles + (rows.drafted ? 1u : 0u);
-  const uint32_t first = static_cast<uint32_t>(static_cast<uint64_t>(tiles) * split / splits);
-  const uint32_t behind = static_cast<uint32_t>(static_cast<uint64_t>(tiles) * (split + 1) / splits);
-  const uint32_t count = behind - first;
+  const uint32_t first = tiles * split / splits, count = rows.request < 0 ? 0u : tiles * (split + 1u) / splits - first;
   const Waits waits{&c.abort_flag, static_cast<long long>(a.wait_kilocycles ? a.wait_kilocycles : kDefaultWaitKilocycles) << 10};
   constexpr uint32_t kScores = 0, kOut = 2 * kN;   // tensor-memory columns: two score tiles, four value blocks
   auto none = [&](uint32_t s) { return (c.valid[s][0] | c.valid[s][1] | c.valid[s][2] | c.valid[s][3]) == 0u; };
 
-  if (warp >= kFirstLoaderWarp && warp < kMmaWarp) {
+  if (warp >= kFirstLoaderWarp && warp < kScoreWarp) {
     // ================= loaders: warp 8 + 2 i + g gathers 16 rows, from 16 i on, of the tiles g, g + 2, ... =================
     const uint32_t g = (warp - kFirstLoaderWarp) & 1u, quarter = (warp - kFirstLoaderWarp) >> 1;
     const bool leader = elect_one();
@@ -353,10 +352,9 @@ attend_tiles(const __grid_constant__ CUtensorMap query_map, const __grid_constan
             if (any) {
               expect_bytes(bar(c.full[g][third]), kThirdBytes / kLoaderWarps);
 #pragma unroll
-              for (uint32_t i = 0; i < kPieces / kThirds; ++i) {
-                const uint32_t piece = third * (kPieces / kThirds) + i;
+              for (uint32_t q = 0; q < 4u; ++q) {
 #pragma unroll
-                for (uint32_t q = 0; q < 4u; ++q)
+                for (uint32_t piece = third * (kPieces / kThirds); piece < (third + 1u) * (kPieces / kThirds); ++piece)
                   load_rows(base + g * kStageBytes + piece * kPieceBytes + (quarter * 4u + q) * 512u, map, piece * 64u, r[q], bar(c.full[g][third]));
               }
             } else {
@@ -367,84 +365,63 @@ attend_tiles(const __grid_constant__ CUtensorMap query_map, const __grid_constan
         }
         if (!alive) break;
       }
-    } else if (warp == kFirstLoaderWarp) {
-      mbar_wait(bar(c.query_full), 0, waits);
     }
     if (bad) atomicOr(a.status, bad);
-  } else if (warp == kMmaWarp) {
-    // ================= MMA issuer: the warp walks together, one elected thread issues =================
-    if (count) {
-      constexpr uint32_t kFormat = __is_same(T, __nv_bfloat16) ? 1u : 0u;
-      constexpr uint32_t kBase = (1u << 4) | (kFormat << 7) | (kFormat << 10) | ((kN >> 3) << 17);
-      constexpr uint32_t kScoreDesc = kBase | ((64u >> 4) << 24);
-      constexpr uint32_t kValueDesc = kBase | (1u << 15) | (1u << 16) | ((128u >> 4) << 24);   // both operands M/N-major
-      const bool leader = elect_one();
-      bool written = false, alive = __all_sync(0xffffffffu, mbar_wait(bar(c.query_full), 0, waits));
-      // S^T of tile n, piece by piece as its thirds come; the first has come when this is called
-      auto score = [&](uint32_t n) -> bool {
+  } else if (warp >= kScoreWarp) {
+    // ================= issuers: the warp walks together, one elected thread issues =================
+    constexpr uint32_t kFormat = __is_same(T, __nv_bfloat16) ? 1u : 0u;
+    constexpr uint32_t kBase = (1u << 4) | (kFormat << 7) | (kFormat << 10) | ((kN >> 3) << 17);
+    constexpr uint32_t kScoreDesc = kBase | ((64u >> 4) << 24);
+    constexpr uint32_t kValueDesc = kBase | (1u << 15) | (1u << 16) | ((128u >> 4) << 24);   // both operands M/N-major
+    const bool leader = elect_one();
+    auto wait = [&](const uint64_t& b, uint32_t phase) { return __all_sync(0xffffffffu, mbar_wait(bar(b), phase, waits)); };
+    if (warp == kScoreWarp) {                // S^T of tile n, piece by piece as its thirds come
+      bool alive = rows.request < 0 || wait(c.query_full, 0);
+      for (uint32_t n = 0; alive && n < count; ++n) {
         const uint32_t s = n & 1u, phase = (n >> 1) & 1u;
-        if (none(s)) {
-          bool ok = true;
-          for (uint32_t third = 1; third < kThirds; ++third) ok = ok && __all_sync(0xffffffffu, mbar_wait(bar(c.full[s][third]), phase, waits));
-          if (leader && ok) mbar_arrive(bar(c.scored[s]));
-          return ok;
-        }
+        if (!wait(c.taken[s], phase ^ 1u)) break;   // the scores of tile n - 2 have been read
         const uint32_t d = tmem + kScores + s * kN;
         const uint64_t da = operand(base + s * kStageBytes, 16u), db = operand(base + Layout<kN>::kQuery, 16u);
 #pragma unroll
         for (uint32_t third = 0; third < kThirds; ++third) {
-          if (third && !__all_sync(0xffffffffu, mbar_wait(bar(c.full[s][third]), phase, waits))) return false;
+          alive = alive && wait(c.full[s][third], phase);
+          if (!alive) break;
           fence_after();
           if (leader) {
+            if (!none(s)) {
 #pragma unroll
-            for (uint32_t piece = third * (kPieces / kThirds); piece < (third + 1u) * (kPieces / kThirds); ++piece) {
+              for (uint32_t piece = third * (kPieces / kThirds); piece < (third + 1u) * (kPieces / kThirds); ++piece) {
 #pragma unroll
-              for (uint32_t k = 0; k < 4; ++k)
-                mma(d, da + (piece * (kPieceBytes >> 4) + 2u * k), db + (piece * (kN * 8u) + 2u * k), kScoreDesc, (piece | k) != 0u);
+                for (uint32_t k = 0; k < 4; ++k)
+                  mma(d, da + (piece * (kPieceBytes >> 4) + 2u * k), db + (piece * (kN * 8u) + 2u * k), kScoreDesc, (piece | k) != 0u);
+              }
             }
             if (third == kThirds - 1u) commit(bar(c.scored[s]));
           }
           __syncwarp();
         }
-        return true;
-      };
-      uint32_t scored = 0;                   // tiles whose scores have been issued
-      for (uint32_t n = 0; alive && n < count; ++n) {
-        const uint32_t s = n & 1u, phase = (n >> 1) & 1u;
-        if (scored == n) {
-          if (!__all_sync(0xffffffffu, mbar_wait(bar(c.full[s][0]), phase, waits)) || !score(n)) break;
-          ++scored;
-        }
-        // while the weights of tile n are made: the scores of the next tile, if its rows are coming
-        if (scored == n + 1 && n + 1 < count) {
-          const uint32_t s1 = s ^ 1u, phase1 = ((n + 1) >> 1) & 1u;
-          while (!__any_sync(0xffffffffu, mbar_test(bar(c.weighted), n & 1u) || c.abort_flag)) {
-            if (__all_sync(0xffffffffu, mbar_test(bar(c.full[s1][0]), phase1))) {
-              alive = score(n + 1);
-              ++scored;
-              break;
-            }
-          }
-        }
-        if (!alive || !__all_sync(0xffffffffu, mbar_wait(bar(c.weighted), n & 1u, waits))) break;
-        if (none(s)) {                       // in order behind the products before
-          if (leader)
-            for (uint32_t third = 0; third < kThirds; ++third) commit(bar(c.empty[s][third]));
-          continue;
-        }
+      }
+    } else {                                 // O^T += V^T P^T of tile n
+      bool written = false;
+      for (uint32_t n = 0; n < count; ++n) {
+        const uint32_t s = n & 1u;
+        if (!wait(c.weighted, n & 1u)) break;
         fence_after();
+        const bool empty = none(s);
         const uint64_t da = operand(base + s * kStageBytes, kPieceBytes), db = operand(base + Layout<kN>::kWeights, 16u);
         if (leader) {
 #pragma unroll
           for (uint32_t m = 0; m < 4; ++m) {
+            if (!empty) {
 #pragma unroll
-            for (uint32_t k = 0; k < kTile / 16u; ++k)
-              mma(tmem + kOut + m * kN, da + (2u * m * (kPieceBytes >> 4) + k * 128u), db + k * 128u, kValueDesc, written || k != 0u);
+              for (uint32_t k = 0; k < kTile / 16u; ++k)
+                mma(tmem + kOut + m * kN, da + (2u * m * (kPieceBytes >> 4) + k * 128u), db + k * 128u, kValueDesc, written || k != 0u);
+            }
             if (m) commit(bar(c.empty[s][m - 1u]));   // blocks 0-1 end with the pieces 0-2, block 2 with 3-5, block 3 with the rest
           }
         }
         __syncwarp();
-        written = true;
+        written = written || !empty;
       }
     }
   } else {
@@ -462,7 +439,9 @@ attend_tiles(const __grid_constant__ CUtensorMap query_map, const __grid_constan
       const uint32_t s = n & 1u, phase = (n >> 1) & 1u;
       bool ok = !dead && mbar_wait(bar(c.scored[s]), phase, waits) && mbar_wait(bar(c.full[s][0]), phase, waits);
       ok = __all_sync(0xffffffffu, ok);
-      if (ok && none(s)) {                     // the same for all: the mask belongs to the tile
+      if (ok && none(s)) {
+        if (lane == 0) mbar_arrive(bar(c.taken[s]));
+        // the same for all: the mask belongs to the tile
         // as below: a thread arrives for this tile only when all have arrived for the one before
         if (n && !mbar_wait(bar(c.empty[(n - 1u) & 1u][kThirds - 1u]), ((n - 1u) >> 1) & 1u, waits)) dead = true;
         __syncwarp();
@@ -477,6 +456,9 @@ attend_tiles(const __grid_constant__ CUtensorMap query_map, const __grid_constan
         fence_after();
         tmem_ld_scores<kBlocks>(tmem + quad + kScores + s * kN + head_at, v);
         tmem_ld_done();
+        fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(c.taken[s]));
       }
       // scores in units of log2; one more than 2^8 above its reference makes the whole half take the maximum
       float x[4 * kBlocks];
@@ -572,59 +554,84 @@ attend_tiles(const __grid_constant__ CUtensorMap query_map, const __grid_constan
         if (w == 0) c.top[h] = ref[j];
       }
     }
-    if (!role_any<2 * kRole>(3u, dead)) {
+    if (!role_any<2 * kRole>(3u, dead) && rows.request >= 0) {
       const uint64_t out_row = static_cast<uint64_t>(t) * a.heads + head0;
       const uint64_t part_row = (static_cast<uint64_t>(split) * a.tokens + t) * a.heads + head0;
       if (tid < heads) {
         const float total = (c.reduce[0][tid] + c.reduce[1][tid]) + (c.reduce[2][tid] + c.reduce[3][tid]);
         if (splits == 1) {
           a.lse[out_row + tid] = written ? (c.top[tid] + log2f(total)) * 0.6931471805599453f : -INFINITY;
+          c.factor[tid] = written ? 1.f / total : 0.f;
         } else {
-          a.partial_stats[2 * (part_row + tid)] = written ? c.top[tid] : -INFINITY;
-          a.partial_stats[2 * (part_row + tid) + 1] = total;
+          reinterpret_cast<float2*>(a.partial_stats)[part_row + tid] = make_float2(written ? c.top[tid] : -INFINITY, total);
         }
-        c.factor[tid] = written ? 1.f / total : 0.f;
       }
-      role_any<2 * kRole>(3u, false);
       fence_after();
-      // A lane holds one value element of every head. The share of the output is laid out in the stages (all products have read
-      // them) and leaves by copies of whole rows. In 16 bits two lanes exchange a value, so that each writes a whole word.
+      // The output is laid out in the stages (all products have read them) and leaves by copies of whole rows. Accumulators have
+      // value elements as rows and heads as columns: 8 x 8 blocks are transposed on their way into shared memory. A share that
+      // will be joined leaves as it is, in fp32 and undivided.
+      if (splits == 1) {
+        role_any<2 * kRole>(3u, false);
+        float f[4 * kBlocks];                // heads 8 j + 2 (lane % 4) + {0, 1}, all of them
 #pragma unroll
-      for (uint32_t m = 0; m < 2; ++m) {
-        const uint32_t block = 2u * side + m, element = block * 128u + w * 32u + lane;
+        for (uint32_t j = 0; j < 2 * kBlocks; ++j) {
+          const float2 pair = *reinterpret_cast<const float2*>(&c.factor[8u * j + 2u * (lane & 3u)]);
+          f[2 * j] = pair.x;
+          f[2 * j + 1] = pair.y;
+        }
+        // addresses of stored rows: lanes 0-7 give the heads of a block for value elements 0-7, 8-15 for 8-15, 16-31 the next block's
+        const uint32_t store = base + ((lane & 7u) + (lane >> 4) * 8u) * kOutRow + ((lane >> 3) & 1u) * 16u;
 #pragma unroll
-        for (uint32_t h0 = 0; h0 < kN; h0 += 16) {
-          uint32_t o[16];
-          if (written) {
-            tmem_ld_rows(tmem + quad + kOut + block * kN + h0, o);
-            tmem_ld_rows(tmem + quad + kOut + block * kN + h0 + 8u, o + 8);
-            tmem_ld_done();
-          }
+        for (uint32_t m = 0; m < 2; ++m) {
+          const uint32_t block = 2u * side + m;
 #pragma unroll
-          for (uint32_t i = 0; i < 16; i += 2) {
-            const float2 f = *reinterpret_cast<const float2*>(&c.factor[h0 + i]);
-            const float y0 = written ? __uint_as_float(o[i]) * f.x : 0.f, y1 = written ? __uint_as_float(o[i + 1]) * f.y : 0.f;
-            if (splits == 1) {
-              const bool odd = lane & 1u;
-              const float other = __shfl_xor_sync(0xffffffffu, odd ? y0 : y1, 1);
-              const uint32_t word = odd ? pack_pair<T>(other, y1) : pack_pair<T>(y0, other);
-              *reinterpret_cast<uint32_t*>(smem + (h0 + i + (odd ? 1u : 0u)) * kOutRow + (element & ~1u) * 2u) = word;
-            } else {
-              reinterpret_cast<float*>(smem)[(h0 + i) * kValue + element] = y0;
-              reinterpret_cast<float*>(smem)[(h0 + i + 1u) * kValue + element] = y1;
+          for (uint32_t half = 0; half < 2; ++half) {
+            uint32_t o[8 * kBlocks];
+            if (written) {
+              tmem_ld_scores<kBlocks>(tmem + quad + (half << 20) + kOut + block * kN, o);
+              tmem_ld_scores<kBlocks>(tmem + quad + (half << 20) + kOut + block * kN + 8u * kBlocks, o + 4 * kBlocks);
+              tmem_ld_done();
+            }
+            const uint32_t element = block * 128u + w * 32u + half * 16u;
+#pragma unroll
+            for (uint32_t j = 0; j < 2 * kBlocks; j += 2) {
+              uint32_t q[4];
+#pragma unroll
+              for (uint32_t i = 0; i < 2; ++i) {
+                const uint32_t* e = o + 4 * (j + i);
+                const float fx = f[2 * (j + i)], fy = f[2 * (j + i) + 1];
+                q[2 * i] = written ? pack_pair<T>(__uint_as_float(e[0]) * fx, __uint_as_float(e[1]) * fy) : 0u;
+                q[2 * i + 1] = written ? pack_pair<T>(__uint_as_float(e[2]) * fx, __uint_as_float(e[3]) * fy) : 0u;
+              }
+              asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};"
+                           ::"r"(store + j * 8u * kOutRow + element * 2u), "r"(q[0]), "r"(q[1]), "r"(q[2]), "r"(q[3]) : "memory");
             }
           }
         }
-      }
-      fence_async();
-      role_any<2 * kRole>(3u, false);
-      if (splits == 1) {
+        fence_async();
+        role_any<2 * kRole>(3u, false);
         if (tid < heads)
           asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;"
                        ::"l"(static_cast<T*>(a.out) + (out_row + tid) * kValue), "r"(base + tid * kOutRow), "r"(kValue * 2u) : "memory");
-      } else if (tid == 0) {
-        asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;"
-                     ::"l"(a.partial + part_row * kValue), "r"(base), "r"(heads * kValue * 4u) : "memory");
+      } else if (written) {                  // an empty share says so in its statistics, its rows are not read
+#pragma unroll
+        for (uint32_t m = 0; m < 2; ++m) {
+          const uint32_t block = 2u * side + m, element = block * 128u + w * 32u + lane;
+#pragma unroll
+          for (uint32_t h0 = 0; h0 < kN; h0 += 16) {
+            uint32_t o[16];
+            tmem_ld_rows(tmem + quad + kOut + block * kN + h0, o);
+            tmem_ld_rows(tmem + quad + kOut + block * kN + h0 + 8u, o + 8);
+            tmem_ld_done();
+#pragma unroll
+            for (uint32_t i = 0; i < 16; ++i) reinterpret_cast<float*>(smem)[(h0 + i) * kValue + element] = __uint_as_float(o[i]);
+          }
+        }
+        fence_async();
+        role_any<2 * kRole>(3u, false);
+        if (tid == 0)
+          asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;"
+                       ::"l"(a.partial + part_row * kValue), "r"(base), "r"(heads * kValue * 4u) : "memory");
       }
       asm volatile("cp.async.bulk.commit_group;" ::: "memory");
       asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
@@ -639,31 +646,32 @@ attend_tiles(const __grid_constant__ CUtensorMap query_map, const __grid_constan
     for (int i = 0; i < 64; ++i) __nanosleep(2000);   // copies and products in flight end before their memory is released
     __syncthreads();
   }
-  if (warp == kMmaWarp) {
+  if (warp == kScoreWarp) {
     fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
   }
 }
 
-// Joins the shares of one (token, head): out = sum_s w_s o_s / sum_s w_s, w_s = sum of the share * 2^(its reference).
+// Joins the shares of one (token, head): out = sum_s w_s o_s / sum_s w_s l_s, w_s = 2^(reference of the share - the largest).
 template <typename T>
 __global__ void __launch_bounds__(128) join_shares(const __grid_constant__ KvipAttentionArgs a, const uint32_t splits) {
   const uint32_t row = blockIdx.x, t = row / a.heads;
   if (a.requests && a.requests[t] < 0) return;
   const uint64_t rows = static_cast<uint64_t>(a.tokens) * a.heads;
+  const float2* stats = reinterpret_cast<const float2*>(a.partial_stats) + row;
   float top = -INFINITY;
-  for (uint32_t s = 0; s < splits; ++s) top = fmaxf(top, a.partial_stats[2 * (s * rows + row)]);
+  for (uint32_t s = 0; s < splits; ++s) top = fmaxf(top, stats[s * rows].x);
   float total = 0.f;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
   for (uint32_t s = 0; s < splits; ++s) {
-    const float2 stat = reinterpret_cast<const float2*>(a.partial_stats)[s * rows + row];
-    const float weight = stat.x == -INFINITY ? 0.f : stat.y * exp2_fast(stat.x - top);
-    const float4 o = reinterpret_cast<const float4*>(a.partial + (s * rows + row) * kValue)[threadIdx.x];
-    total += weight;
-    if (weight != 0.f) {
-      acc.x = fmaf(weight, o.x, acc.x); acc.y = fmaf(weight, o.y, acc.y);
-      acc.z = fmaf(weight, o.z, acc.z); acc.w = fmaf(weight, o.w, acc.w);
-    }
+    const float2 stat = stats[s * rows];
+    const bool used = stat.x != -INFINITY;
+    const float weight = used ? exp2_fast(stat.x - top) : 0.f;
+    const float4 o = used ? reinterpret_cast<const float4*>(a.partial + (s * rows + row) * kValue)[threadIdx.x] : make_float4(0.f, 0.f, 0.f, 0.f);
+    total = fmaf(weight, used ? stat.y : 0.f, total);
+    acc.x = fmaf(weight, o.x, acc.x); acc.y = fmaf(weight, o.y, acc.y);
+    acc.z = fmaf(weight, o.z, acc.z); acc.w = fmaf(weight, o.w, acc.w);
   }
   const float inverse = total == 0.f ? 0.f : 1.f / total;
   uint2 packed = make_uint2(pack_pair<T>(acc.x * inverse, acc.y * inverse), pack_pair<T>(acc.z * inverse, acc.w * inverse));
