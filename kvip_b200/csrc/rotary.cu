@@ -90,13 +90,197 @@ __global__ void __launch_bounds__(kRotaryThreads) quantise_rows(const KvipRotary
   }
 }
 
+// ---- the vector forms ----
+// A unit is 16 elements of a row in two runs of 8 that make 8 pairs: elements 8 v .. and width/2 + 8 v .. of a rotated row
+// in the half layout, 16 v .. in the interleaved one (and 16 elements that do not turn, behind `width` of a quantised row).
+// A CTA takes `tile` tokens and a range of rows: the angles of its tokens once, into shared memory, then a thread per
+// unit. Bound by memory: two (three) wide loads and stores a unit; the angles of a token serve all of its rows.
+template <typename T> struct Unit;   // 16 elements as they lie in memory
+template <> struct Unit<float> { float4 v[4]; };
+template <> struct Unit<__nv_bfloat16> { uint4 v[2]; };
+template <> struct Unit<__half> { uint4 v[2]; };
+
+template <typename T> __device__ __forceinline__ Unit<T> load_unit(const T* low, const T* high) {
+  Unit<T> u;
+  if constexpr (sizeof(T) == 4) {
+    u.v[0] = __ldcs(reinterpret_cast<const float4*>(low)); u.v[1] = __ldcs(reinterpret_cast<const float4*>(low) + 1);
+    u.v[2] = __ldcs(reinterpret_cast<const float4*>(high)); u.v[3] = __ldcs(reinterpret_cast<const float4*>(high) + 1);
+  } else {
+    u.v[0] = __ldcs(reinterpret_cast<const uint4*>(low));
+    u.v[1] = __ldcs(reinterpret_cast<const uint4*>(high));
+  }
+  return u;
+}
+template <typename T> __device__ __forceinline__ void store_unit(T* low, T* high, const Unit<T>& u) {
+  if constexpr (sizeof(T) == 4) {
+    __stcs(reinterpret_cast<float4*>(low), u.v[0]); __stcs(reinterpret_cast<float4*>(low) + 1, u.v[1]);
+    __stcs(reinterpret_cast<float4*>(high), u.v[2]); __stcs(reinterpret_cast<float4*>(high) + 1, u.v[3]);
+  } else {
+    __stcs(reinterpret_cast<uint4*>(low), u.v[0]);
+    __stcs(reinterpret_cast<uint4*>(high), u.v[1]);
+  }
+}
+template <typename T> __device__ __forceinline__ void widen(const Unit<T>& u, float (&x)[16]) {
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (uint32_t i = 0; i < 16; ++i) x[i] = reinterpret_cast<const float*>(&u)[i];
+  } else {
+#pragma unroll
+    for (uint32_t i = 0; i < 16; ++i) x[i] = to_float(reinterpret_cast<const T*>(&u)[i]);
+  }
+}
+template <typename T> __device__ __forceinline__ Unit<T> narrow(const float (&x)[16]) {
+  Unit<T> u;
+#pragma unroll
+  for (uint32_t i = 0; i < 16; ++i) reinterpret_cast<T*>(&u)[i] = from_float<T>(x[i]);
+  return u;
+}
+// Turns the eight pairs of a unit; cs[i] = (cos, sin) of pair i.
+__device__ __forceinline__ void turn_unit(float (&x)[16], const float2* cs, bool split) {
+#pragma unroll
+  for (uint32_t i = 0; i < 8; i += 2) {
+    const float4 c = *reinterpret_cast<const float4*>(cs + i);
+    const uint32_t a0 = split ? i : 2u * i, b0 = split ? i + 8u : 2u * i + 1u, a1 = split ? i + 1u : 2u * i + 2u, b1 = split ? i + 9u : 2u * i + 3u;
+    const float u0 = x[a0], v0 = x[b0], u1 = x[a1], v1 = x[b1];
+    x[a0] = u0 * c.x - v0 * c.y; x[b0] = v0 * c.x + u0 * c.y;
+    x[a1] = u1 * c.z - v1 * c.w; x[b1] = v1 * c.z + u1 * c.w;
+  }
+}
+// (cos, sin) of `pairs` pairs of the CTA's tokens in shared memory: [tile][stride]
+__device__ __forceinline__ void turn_table(const KvipRotaryArgs& a, float2* table, uint32_t first, uint32_t tile, uint32_t pairs) {
+  for (uint32_t i = threadIdx.x; i < tile * pairs; i += kRotaryThreads) {
+    const uint32_t k = i / pairs, pair = i - k * pairs, token = first + k;
+    if (token < a.tokens) table[i] = cos_sin(a.positions[token], a.turns[pair], a.factor);
+  }
+  __syncthreads();
+}
+
+template <typename T, bool kSplit>
+__global__ void __launch_bounds__(kRotaryThreads) rotate_units(const __grid_constant__ KvipRotaryArgs a, const uint32_t tile, const uint32_t rows_here) {
+  extern __shared__ float2 table[];
+  const uint32_t half = a.width >> 1, units = a.width >> 4, rows = a.heads[0] + a.heads[1];
+  const uint32_t first = blockIdx.x * tile, row0 = blockIdx.y * rows_here, count = min(rows_here, rows - row0);
+  turn_table(a, table, first, tile, half);
+  const uint32_t per_token = count * units;
+  for (uint32_t i = threadIdx.x; i < tile * per_token; i += kRotaryThreads) {
+    const uint32_t k = i / per_token, rest = i - k * per_token, row = row0 + rest / units, v = rest % units, token = first + k;
+    if (token >= a.tokens || a.positions[token] < 0) continue;
+    const uint32_t set = row >= a.heads[0] ? 1u : 0u;
+    const int64_t head = set ? row - a.heads[0] : row;
+    const T* x = static_cast<const T*>(a.x[set]) + token * a.x_token[set] + head * a.x_head[set];
+    T* y = static_cast<T*>(a.y[set]) + token * a.y_token[set] + head * a.y_head[set];
+    const uint32_t low = kSplit ? 8u * v : 16u * v, high = kSplit ? half + low : low + 8u;
+    const Unit<T> u = load_unit(x + low, x + high);
+    float e[16];
+    widen<T>(u, e);
+    turn_unit(e, table + k * half + 8u * v, kSplit);
+    store_unit(y + low, y + high, narrow<T>(e));
+  }
+}
+
+// kLanes threads per row of 16 kLanes elements.
+template <typename T, bool kSplit, uint32_t kLanes>
+__global__ void __launch_bounds__(kRotaryThreads) quantise_units(const __grid_constant__ KvipRotaryArgs a, const uint32_t tile, const uint32_t rows_here) {
+  extern __shared__ float2 table[];
+  const uint32_t half = a.width >> 1, turned = a.width >> 4;
+  const uint32_t first = blockIdx.x * tile, row0 = blockIdx.y * rows_here, count = min(rows_here, a.heads[0] - row0);
+  turn_table(a, table, first, tile, half);
+  const uint32_t v = threadIdx.x % kLanes, items = tile * count;
+  for (uint32_t i0 = 0; i0 < items; i0 += kRotaryThreads / kLanes) {   // whole warps stay together for the shuffles
+    const uint32_t i = i0 + threadIdx.x / kLanes, k = i / count, row = row0 + (i - k * count), token = first + k;
+    const bool live = i < items && token < a.tokens && a.positions[token] >= 0;
+    float e[16];
+    float amax = 0.f;
+    const uint32_t low = kSplit && v < turned ? 8u * v : 16u * v, high = kSplit && v < turned ? half + low : low + 8u;
+    if (live) {
+      const T* x = static_cast<const T*>(a.x[0]) + token * a.x_token[0] + row * a.x_head[0];
+      widen<T>(load_unit(x + low, x + high), e);
+      if (v < turned) turn_unit(e, table + k * half + 8u * v, kSplit);
+#pragma unroll
+      for (uint32_t j = 0; j < 16; ++j) amax = fmaxf(amax, fabsf(e[j]));
+    }
+#pragma unroll
+    for (uint32_t o = kLanes / 2u; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+    if (!live) continue;
+    const float scale = amax > 0.f ? amax / 448.f : 1.f, inverse = 1.f / scale;
+    const uint64_t r = static_cast<uint64_t>(token) * a.heads[0] + row;
+    uint32_t packed[4];
+#pragma unroll
+    for (uint32_t j = 0; j < 4; ++j) {
+      const uint32_t x = __nv_cvt_float2_to_fp8x2(make_float2(e[4 * j] * inverse, e[4 * j + 1] * inverse), __NV_SATFINITE, __NV_E4M3);
+      const uint32_t y = __nv_cvt_float2_to_fp8x2(make_float2(e[4 * j + 2] * inverse, e[4 * j + 3] * inverse), __NV_SATFINITE, __NV_E4M3);
+      packed[j] = x | (y << 16);
+    }
+    uint8_t* codes = a.codes + r * a.dim;
+    __stcs(reinterpret_cast<uint2*>(codes + low), make_uint2(packed[0], packed[1]));
+    __stcs(reinterpret_cast<uint2*>(codes + high), make_uint2(packed[2], packed[3]));
+    if (v == 0) a.scales[r] = scale;
+  }
+}
+
+// Tokens and rows per CTA: about 2048 units of work, tokens first (their angles are shared by all rows), and at least two
+// CTAs per SM where there is that much work.
+void shares(uint32_t tokens, uint32_t rows, uint32_t units, uint32_t half, uint32_t* tile, uint32_t* rows_here) {
+  const uint32_t want = 2u * device_sm_count();
+  *rows_here = rows;
+  while (*rows_here > 1u && (*rows_here * units > 2048u || tokens * ((rows + *rows_here - 1) / *rows_here) < want) &&
+         *rows_here * units > kRotaryThreads)
+    *rows_here = (*rows_here + 1) / 2;
+  *tile = 1;
+  const uint32_t parts = (rows + *rows_here - 1) / *rows_here;
+  while (*tile < 16u && *tile * half <= 2048u && *tile * *rows_here * units < 2048u && ((tokens + 2u * *tile - 1) / (2u * *tile)) * parts >= want) *tile *= 2u;
+}
+
+template <typename T> bool aligned_rows(const void* base, int64_t token, int64_t head) {
+  constexpr uint32_t kRun = sizeof(T) == 4 ? 4u : 8u;   // elements of a 16-byte load
+  return (reinterpret_cast<uintptr_t>(base) & 15u) == 0 && token % kRun == 0 && head % kRun == 0;
+}
+
+template <typename T, bool kSplit>
+uint32_t launch_units(const KvipRotaryArgs& a, cudaStream_t stream) {
+  uint32_t tile, rows_here;
+  const uint32_t rows = a.heads[0] + a.heads[1];
+  if (!a.codes) {
+    shares(a.tokens, rows, a.width / 16u, a.width / 2u, &tile, &rows_here);
+    const dim3 grid((a.tokens + tile - 1) / tile, (rows + rows_here - 1) / rows_here);
+    rotate_units<T, kSplit><<<grid, kRotaryThreads, tile * (a.width / 2u) * sizeof(float2), stream>>>(a, tile, rows_here);
+    return 0;
+  }
+  shares(a.tokens, rows, a.dim / 16u, a.width / 2u, &tile, &rows_here);
+  const dim3 grid((a.tokens + tile - 1) / tile, (rows + rows_here - 1) / rows_here);
+  const uint32_t shared = tile * (a.width / 2u) * sizeof(float2);
+  switch (a.dim / 16u) {
+    case 1: quantise_units<T, kSplit, 1><<<grid, kRotaryThreads, shared, stream>>>(a, tile, rows_here); break;
+    case 2: quantise_units<T, kSplit, 2><<<grid, kRotaryThreads, shared, stream>>>(a, tile, rows_here); break;
+    case 4: quantise_units<T, kSplit, 4><<<grid, kRotaryThreads, shared, stream>>>(a, tile, rows_here); break;
+    case 8: quantise_units<T, kSplit, 8><<<grid, kRotaryThreads, shared, stream>>>(a, tile, rows_here); break;
+    case 16: quantise_units<T, kSplit, 16><<<grid, kRotaryThreads, shared, stream>>>(a, tile, rows_here); break;
+    default: quantise_units<T, kSplit, 32><<<grid, kRotaryThreads, shared, stream>>>(a, tile, rows_here); break;
+  }
+  return 0;
+}
+
 template <typename T>
 uint32_t launch_rotary(const KvipRotaryArgs& a, cudaStream_t stream) {
-  const uint32_t most = device_sm_count() * 16u;
+  // the vector forms want rows of whole units at 16-byte boundaries; what else there is goes element by element
+  bool wide = a.width % 16u == 0;
   if (a.codes) {
+    const uint32_t lanes = a.dim / 16u;
+    wide = wide && a.dim % 16u == 0 && lanes <= 32u && (lanes & (lanes - 1u)) == 0 && aligned_rows<T>(a.x[0], a.x_token[0], a.x_head[0]) &&
+           (reinterpret_cast<uintptr_t>(a.codes) & 7u) == 0;
+  } else {
+    for (uint32_t set = 0; set < 2u && a.heads[set]; ++set)
+      wide = wide && aligned_rows<T>(a.x[set], a.x_token[set], a.x_head[set]) && aligned_rows<T>(a.y[set], a.y_token[set], a.y_head[set]);
+  }
+  if (wide) {
+    if (a.layout == KVIP_ROTARY_HALF) launch_units<T, true>(a, stream);
+    else launch_units<T, false>(a, stream);
+  } else if (a.codes) {
+    const uint32_t most = device_sm_count() * 16u;
     const uint64_t blocks = (static_cast<uint64_t>(a.tokens) * a.heads[0] + 7u) / 8u;
     quantise_rows<T><<<static_cast<uint32_t>(blocks < most ? blocks : most), kRotaryThreads, 0, stream>>>(a);
   } else {
+    const uint32_t most = device_sm_count() * 16u;
     const uint64_t items = static_cast<uint64_t>(a.tokens) * (a.heads[0] + a.heads[1]) * (a.width / 2u);
     const uint64_t blocks = (items + kRotaryThreads - 1) / kRotaryThreads;
     rotate_pairs<T><<<static_cast<uint32_t>(blocks < most ? blocks : most), kRotaryThreads, 0, stream>>>(a);

@@ -168,6 +168,10 @@ __device__ __forceinline__ void load_query(uint32_t to, const CUtensorMap* map, 
 __device__ __forceinline__ void expect_bytes(uint32_t bar, uint32_t bytes) {
   asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
 }
+// Asks L2 for a row that a copy will read soon.
+__device__ __forceinline__ void prefetch_row(const uint8_t* row) {
+  asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(row), "r"(kWidth * 2u) : "memory");
+}
 __device__ __forceinline__ bool elect_one() {
   uint32_t leader;
   asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(leader));
@@ -303,10 +307,22 @@ attend_tiles(const __grid_constant__ CUtensorMap query_map, const __grid_constan
         }
         return e;
       };
-      int4 next = entries_of(g);
+      // Rows are asked for two of this stage's tiles before they are copied: a copy from HBM takes twice as long as one from
+      // L2, and the two stages alone do not keep enough of them in flight.
+      auto ahead = [&](const int4& e) {
+        if ((lane >> 2) != quarter) return;        // 16 rows a warp
+        auto ask = [&](int32_t slot) {
+          if (slot >= 0 && static_cast<uint32_t>(slot) < rows.limit)
+            prefetch_row(static_cast<const uint8_t*>(a.pool) + static_cast<uint64_t>(rows.base + static_cast<uint32_t>(slot)) * (kWidth * 2u));
+        };
+        ask(e.x); ask(e.y); ask(e.z); ask(e.w);
+      };
+      int4 next = entries_of(g), later = entries_of(g + kStages);
       for (uint32_t n = g; n < count; n += kStages) {
         int4 e = next;
-        next = entries_of(n + kStages);            // lands while this tile is fetched
+        next = later;
+        later = entries_of(n + 2u * kStages);      // lands while this tile is fetched
+        ahead(next);
         const bool from_list = first + n < list_tiles;
         bool v0, v1, v2, v3;
         if (from_list) {
