@@ -2,7 +2,10 @@
 //
 // A request's walk down its tree needs single probabilities (gathered up front, all nodes at once), and a pass over the
 // vocabulary only where a drafted token is rejected or the walk ends: the sum of what is left, and then the place where
-// the running sum passes sample * sum. One CTA per request in this form; sums are fp64 and their order is fixed.
+// the running sum passes sample * sum. A cluster of CTAs takes one request. Every CTA makes the whole walk from the same
+// numbers, so all of them take the same turns; a pass is split over the warps of the cluster in contiguous shares, whose sums
+// go to every CTA through distributed shared memory, and the warp whose share holds the border looks for it. Sums are fp64 and
+// their order is fixed. Bound by HBM: one target row (and one draft row behind a rejection) per pass.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include "common.cuh"
@@ -24,29 +27,70 @@ __device__ __forceinline__ double remaining(double p, double q, const double* ma
   return p;
 }
 
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ uint32_t cluster_size() {
+  uint32_t n;
+  asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(n));
+  return n;
+}
+__device__ __forceinline__ void cluster_barrier() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// Stores into the same place of another CTA's shared memory.
+__device__ __forceinline__ void store_remote(const double* where, uint32_t rank, double value) {
+  uint32_t address = static_cast<uint32_t>(__cvta_generic_to_shared(where)), remote;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(address), "r"(rank));
+  asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(remote), "d"(value) : "memory");
+}
+
+constexpr uint32_t kRun = 8;               // consecutive elements that a lane takes at a time
+constexpr uint32_t kMaxCluster = 8;
+
+// kRun probabilities from `row` on, zeros behind `count`; `wide`: the row lies on a 16-byte boundary.
+template <typename T> __device__ __forceinline__ void load_run(const T* row, uint32_t count, bool wide, double (&p)[kRun]) {
+  if (wide && count >= kRun) {
+    alignas(16) T v[kRun];
+#pragma unroll
+    for (uint32_t i = 0; i < kRun * sizeof(T) / 16u; ++i) reinterpret_cast<uint4*>(v)[i] = __ldg(reinterpret_cast<const uint4*>(row) + i);
+#pragma unroll
+    for (uint32_t i = 0; i < kRun; ++i) p[i] = probability(v[i]);
+  } else {
+#pragma unroll
+    for (uint32_t i = 0; i < kRun; ++i) p[i] = i < count ? probability(row[i]) : 0.0;
+  }
+}
+
 template <typename T>
-__global__ void __launch_bounds__(kVerifyThreads) verify_walk(const KvipVerifyArgs a) {
-  __shared__ double s_p[kMaxNodes], s_q[kMaxNodes], s_mass[kMaxNodes + 1], s_part[kVerifyWarps];
+__global__ void __launch_bounds__(kVerifyThreads, 2) verify_walk(const __grid_constant__ KvipVerifyArgs a) {
+  __shared__ double s_p[kMaxNodes], s_q[kMaxNodes], s_mass[kMaxNodes + 1], s_part[2][kMaxCluster * kVerifyWarps];
   __shared__ int64_t s_token[kMaxNodes], s_lost[kMaxNodes];
   __shared__ int32_t s_parent[kMaxNodes];
   __shared__ float s_accept[kMaxNodes];
-  const uint32_t b = blockIdx.x, tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5;
+  const uint32_t rank = cluster_rank(), ctas = cluster_size();
+  const uint32_t b = blockIdx.x / ctas, tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5;
   int64_t* out_tokens = a.out_tokens + static_cast<uint64_t>(b) * (a.depth + 1u);
   int32_t* out_nodes = a.out_nodes + static_cast<uint64_t>(b) * (a.depth + 1u);
   const int64_t first = a.starts[b], behind = a.starts[b + 1];
   uint32_t n = 0;
   int32_t bad = 0;
-  if (first >= 0 && behind >= first && behind <= static_cast<int64_t>(a.rows)) n = static_cast<uint32_t>(behind - first);
+  if (first >= 0 && behind >= first && behind <= static_cast<int64_t>(a.rows)) n = static_cast<uint32_t>(min(behind - first, static_cast<int64_t>(kMaxNodes + 1u)));
   else bad = static_cast<int32_t>(KVIP_ERR_TOKEN_RANGE);
   if (n > kMaxNodes) { n = kMaxNodes; bad = static_cast<int32_t>(KVIP_ERR_TOKEN_RANGE); }
-  for (uint32_t i = tid; i <= a.depth; i += kVerifyThreads) { out_tokens[i] = -1; out_nodes[i] = -1; }
-  if (n == 0) {
-    if (tid == 0) {
-      a.out_counts[b] = 0;
-      if (bad) atomicOr(a.status, bad);
+  if (n == 0) {                            // the same for the whole cluster
+    if (rank == 0) {
+      for (uint32_t i = tid; i <= a.depth; i += kVerifyThreads) { out_tokens[i] = -1; out_nodes[i] = -1; }
+      if (tid == 0) {
+        a.out_counts[b] = 0;
+        if (bad) atomicOr(a.status, bad);
+      }
     }
     return;
   }
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");   // this CTA runs: its shared memory may be written
   const T* target = static_cast<const T*>(a.target) + first * a.target_row;
   const T* draft = a.draft ? static_cast<const T*>(a.draft) + first * a.draft_row : nullptr;
   if (tid < n) {
@@ -65,38 +109,67 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_walk(const KvipVerifyAr
       s_q[tid] = draft ? probability(draft[parent * a.draft_row + token]) : 1.0;
     }
   }
+  if (tid == 0) s_mass[0] = 1.0;
   bad = __syncthreads_or(bad);
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");     // ... and so do the others
 
-  // the vocabulary in contiguous shares, one per warp
-  const uint32_t V = a.vocabulary;
-  const uint32_t share = ((V + kVerifyWarps - 1) / kVerifyWarps + 31u) & ~31u;
-  const uint32_t from = min(V, warp * share), to = min(V, from + share);
-  uint32_t node = 0, length = 0, rejected = 0;
-  bool summed = false;
-  auto left_at = [&](uint32_t v) -> double {
-    const double p = probability(target[node * a.target_row + v]);
-    if (!rejected) return p;
-    if (draft) return remaining(p, probability(draft[node * a.draft_row + v]), s_mass, rejected);
-    for (uint32_t i = 0; i < rejected; ++i)
-      if (s_lost[i] == static_cast<int64_t>(v)) return 0.0;
-    return p;
+  // the vocabulary in contiguous shares of whole runs, one per warp of the cluster
+  const uint32_t V = a.vocabulary, shares = ctas * kVerifyWarps, mine = rank * kVerifyWarps + warp;
+  const uint32_t share = ((V + shares - 1) / shares + kRun - 1u) / kRun * kRun;
+  const uint32_t from = min(V, mine * share), to = min(V, from + share);
+  uint32_t node = 0, length = 0, rejected = 0, pass = 0;
+  // what is left of the probabilities v .. v + kRun - 1
+  auto left_at = [&](uint32_t v, double (&p)[kRun]) {
+    const uint32_t count = v < to ? to - v : 0u;
+    const T* row = target + node * a.target_row + v;
+    load_run(row, count, (reinterpret_cast<uintptr_t>(row) & 15u) == 0, p);
+    if (!rejected) return;
+    if (draft) {
+      double q[kRun];
+      const T* guess = draft + node * a.draft_row + v;
+      load_run(guess, count, (reinterpret_cast<uintptr_t>(guess) & 15u) == 0, q);
+      for (uint32_t i = 0; i < rejected; ++i) {
+        const double mass = s_mass[i];
+#pragma unroll
+        for (uint32_t k = 0; k < kRun; ++k) p[k] = fmax(__dsub_rn(p[k], __dmul_rn(mass, q[k])), 0.0);
+      }
+    } else {
+      for (uint32_t i = 0; i < rejected; ++i) {
+        const int64_t at = s_lost[i] - static_cast<int64_t>(v);
+#pragma unroll
+        for (uint32_t k = 0; k < kRun; ++k)
+          if (at == static_cast<int64_t>(k)) p[k] = 0.0;
+      }
+    }
   };
-  auto sum_all = [&]() -> double {
+  auto sum_all = [&]() -> double {         // leaves the shares' sums in s_part[pass & 1] of every CTA
     double sum = 0.0;
-    for (uint32_t v = from + lane; v < to; v += 32u) sum += left_at(v);
+#pragma unroll 2
+    for (uint32_t v = from + lane * kRun; v < to; v += 32u * kRun) {
+      double p[kRun];
+      left_at(v, p);
+#pragma unroll
+      for (uint32_t k = 0; k < kRun; ++k) sum += p[k];
+    }
 #pragma unroll
     for (uint32_t o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    __syncthreads();
-    if (lane == 0) s_part[warp] = sum;
-    __syncthreads();
+    ++pass;
+    double* part = s_part[pass & 1u];
+    if (lane < ctas) store_remote(&part[mine], lane, sum);
+    cluster_barrier();
     double total = 0.0;
-    for (uint32_t w = 0; w < kVerifyWarps; ++w) total += s_part[w];
+    for (uint32_t k = 0; k < shares; k += 32u) total += k + lane < shares ? part[k + lane] : 0.0;
+#pragma unroll
+    for (uint32_t o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
     return total;
   };
+  bool summed = false;
   double total = 0.0;
+  uint32_t path = 0;                       // lane `i` of warp 0 of the first CTA keeps accepted node i + 1 (two words: up to 63)
+  uint32_t path_high = 0;
   for (uint32_t j = 1; j < n && length < a.depth; ++j) {
     if (s_parent[j] != static_cast<int32_t>(node)) continue;
-    const double mass = rejected ? s_mass[rejected] : 1.0;
+    const double mass = s_mass[rejected];
     double r = s_p[j];
     if (draft) {
       r = remaining(r, s_q[j], s_mass, rejected);
@@ -105,14 +178,13 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_walk(const KvipVerifyAr
         if (s_lost[i] == s_token[j]) r = 0.0;
     }
     if (__dmul_rn(__dmul_rn(static_cast<double>(s_accept[j]), s_q[j]), mass) < r) {
-      if (tid == 0) { out_tokens[length] = s_token[j]; out_nodes[length + 1] = static_cast<int32_t>(j); }
+      if (lane == (length & 31u)) { if (length < 32u) path = j; else path_high = j; }
       node = j;
       ++length;
       rejected = 0;
       summed = false;
     } else {
-      __syncthreads();
-      if (tid == 0) { s_mass[0] = 1.0; s_lost[rejected] = s_token[j]; }
+      if (tid == 0) s_lost[rejected] = s_token[j];
       __syncthreads();
       ++rejected;
       total = sum_all();
@@ -123,42 +195,105 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_walk(const KvipVerifyAr
     }
   }
   if (!summed) total = sum_all();
-  // the first share whose running sum passes the limit; where rounding leaves none, the last one that holds anything
-  const double limit = __dmul_rn(static_cast<double>(a.sample[b]), total);
-  double running = 0.0, base = 0.0;
-  uint32_t chosen = 0;
-  for (uint32_t w = 0; w < kVerifyWarps; ++w) {
-    if (s_part[w] > 0.0) { chosen = w; base = running; }
-    running += s_part[w];
-    if (running > limit) break;
-  }
-  if (warp == chosen) {
-    double before = base;
-    uint32_t picked = 0;
-    bool found = false;
-    for (uint32_t v0 = from; v0 < to; v0 += 32u) {
-      const uint32_t v = v0 + lane;
-      const double mine = v < to ? left_at(v) : 0.0;
-      double scan = mine;
-#pragma unroll
-      for (uint32_t d = 1; d < 32u; d <<= 1) {
-        const double other = __shfl_up_sync(0xffffffffu, scan, d);
-        if (lane >= d) scan += other;
-      }
-      const uint32_t holds = __ballot_sync(0xffffffffu, mine > 0.0);
-      const uint32_t passed = __ballot_sync(0xffffffffu, mine > 0.0 && before + scan > limit);
-      if (passed) { picked = v0 + static_cast<uint32_t>(__ffs(static_cast<int>(passed))) - 1u; found = true; break; }
-      if (holds) picked = v0 + 31u - static_cast<uint32_t>(__clz(static_cast<int>(holds)));
-      before += __shfl_sync(0xffffffffu, scan, 31);
+  if (rank == 0 && warp == 0) {            // what has been accepted; the drawn token's place is another warp's
+    for (uint32_t i = lane; i <= a.depth; i += 32u) {
+      const uint32_t at = i < 32u ? path : path_high;
+      if (i != length) out_tokens[i] = i < length ? s_token[at] : -1;
+      if (i < a.depth) out_nodes[i + 1u] = i < length ? static_cast<int32_t>(at) : -1;
     }
-    (void)found;
     if (lane == 0) {
-      out_tokens[length] = picked;
       out_nodes[0] = 0;
       a.out_counts[b] = static_cast<int32_t>(length + 1u);
       if (bad) atomicOr(a.status, bad);
     }
   }
+  // the first share whose running sum passes the limit; where rounding leaves none, the last one that holds anything
+  const double limit = __dmul_rn(static_cast<double>(a.sample[b]), total);
+  const double* part = s_part[pass & 1u];
+  double base = 0.0, before_last = 0.0, running = 0.0;
+  uint32_t chosen = 0;
+  bool passed_any = false;
+  for (uint32_t k = 0; k < shares && !passed_any; k += 32u) {
+    const double own = k + lane < shares ? part[k + lane] : 0.0;
+    double scan = own;
+#pragma unroll
+    for (uint32_t d = 1; d < 32u; d <<= 1) {
+      const double other = __shfl_up_sync(0xffffffffu, scan, d);
+      if (lane >= d) scan += other;
+    }
+    const uint32_t holds = __ballot_sync(0xffffffffu, own > 0.0);
+    const uint32_t passed = __ballot_sync(0xffffffffu, own > 0.0 && running + scan > limit);
+    const uint32_t pick = passed ? static_cast<uint32_t>(__ffs(static_cast<int>(passed))) - 1u : holds ? 31u - static_cast<uint32_t>(__clz(static_cast<int>(holds))) : 0u;
+    if (passed || holds) {
+      chosen = k + pick;
+      before_last = running + __shfl_sync(0xffffffffu, scan - own, pick);
+      base = before_last;
+    }
+    passed_any = passed != 0u;
+    running += __shfl_sync(0xffffffffu, scan, 31);
+  }
+  if (mine == chosen) {
+    double before = base;
+    uint32_t picked = 0;
+    for (uint32_t v0 = from; v0 < to; v0 += 32u * kRun) {
+      const uint32_t v = v0 + lane * kRun;
+      double p[kRun];
+      left_at(v, p);
+      double own = 0.0;
+#pragma unroll
+      for (uint32_t k = 0; k < kRun; ++k) own += p[k];
+      double scan = own;
+#pragma unroll
+      for (uint32_t d = 1; d < 32u; d <<= 1) {
+        const double other = __shfl_up_sync(0xffffffffu, scan, d);
+        if (lane >= d) scan += other;
+      }
+      // within the run: the first element whose running sum passes, else the last that holds anything
+      double sum = before + (scan - own);
+      uint32_t at = 0, last = 0;
+      bool found = false;
+#pragma unroll
+      for (uint32_t k = 0; k < kRun; ++k) {
+        sum += p[k];
+        if (p[k] > 0.0) {
+          last = k;
+          if (!found && sum > limit) { found = true; at = k; }
+        }
+      }
+      const uint32_t passed = __ballot_sync(0xffffffffu, found), holds = __ballot_sync(0xffffffffu, own > 0.0);
+      if (passed) {
+        const uint32_t who = static_cast<uint32_t>(__ffs(static_cast<int>(passed))) - 1u;
+        picked = v0 + who * kRun + __shfl_sync(0xffffffffu, at, who);
+        break;
+      }
+      if (holds) {
+        const uint32_t who = 31u - static_cast<uint32_t>(__clz(static_cast<int>(holds)));
+        picked = v0 + who * kRun + __shfl_sync(0xffffffffu, last, who);
+      }
+      before += __shfl_sync(0xffffffffu, scan, 31);
+    }
+    if (lane == 0) out_tokens[length] = picked;
+  }
+}
+
+template <typename T>
+uint32_t launch_verify(const KvipVerifyArgs& a, cudaStream_t stream) {
+  // eight CTAs a request (64 requests fill the SMs four deep), fewer where the batch does that by itself
+  uint32_t ctas = kMaxCluster;
+  while (ctas > 1u && a.batch * ctas > 8u * device_sm_count()) ctas /= 2u;
+  cudaLaunchConfig_t config{};
+  config.gridDim = dim3(a.batch * ctas);
+  config.blockDim = dim3(kVerifyThreads);
+  config.stream = stream;
+  cudaLaunchAttribute attribute{};
+  attribute.id = cudaLaunchAttributeClusterDimension;
+  attribute.val.clusterDim.x = ctas;
+  attribute.val.clusterDim.y = attribute.val.clusterDim.z = 1;
+  config.attrs = &attribute;
+  config.numAttrs = 1;
+  cudaLaunchKernelEx(&config, verify_walk<T>, a);
+  count_launch();
+  return check_launch("verify_walk");
 }
 
 }  // namespace
@@ -174,9 +309,7 @@ extern "C" uint32_t kvip_b200_verify_drafts(const KvipVerifyArgs* a, void* strea
   KVIP_REQUIRE(a->depth >= 1 && a->depth < kMaxNodes, "verify_drafts: a depth of 1..63");
   KVIP_REQUIRE(a->dtype <= KVIP_FLOAT_FP32, "verify_drafts: unknown type");
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (a->dtype == KVIP_FLOAT_BF16) verify_walk<__nv_bfloat16><<<a->batch, kVerifyThreads, 0, s>>>(*a);
-  else if (a->dtype == KVIP_FLOAT_FP16) verify_walk<__half><<<a->batch, kVerifyThreads, 0, s>>>(*a);
-  else verify_walk<float><<<a->batch, kVerifyThreads, 0, s>>>(*a);
-  count_launch();
-  return check_launch("verify_walk");
+  if (a->dtype == KVIP_FLOAT_BF16) return launch_verify<__nv_bfloat16>(*a, s);
+  if (a->dtype == KVIP_FLOAT_FP16) return launch_verify<__half>(*a, s);
+  return launch_verify<float>(*a, s);
 }
