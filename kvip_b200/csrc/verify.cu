@@ -13,7 +13,7 @@
 namespace kvip {
 namespace {
 
-constexpr uint32_t kVerifyThreads = 512, kVerifyWarps = kVerifyThreads / 32;
+constexpr uint32_t kMostThreads = 1024, kMostWarps = kMostThreads / 32;
 constexpr uint32_t kMaxNodes = 64;
 
 template <typename T> __device__ __forceinline__ double probability(T v);
@@ -50,14 +50,37 @@ __device__ __forceinline__ void store_remote(const double* where, uint32_t rank,
 constexpr uint32_t kRun = 8;               // consecutive elements that a lane takes at a time
 constexpr uint32_t kMaxCluster = 8;
 
-// kRun probabilities from `row` on, zeros behind `count`; `wide`: the row lies on a 16-byte boundary.
-template <typename T> __device__ __forceinline__ void load_run(const T* row, uint32_t count, bool wide, double (&p)[kRun]) {
-  if (wide && count >= kRun) {
-    alignas(16) T v[kRun];
+// kRun probabilities from `row` on, zeros behind `count`. A row of odd length starts anywhere: the aligned vectors round the
+// run are read and shifted. Each of them holds an element of the run, and memory is allocated in whole vectors.
+template <typename T> __device__ __forceinline__ void load_run(const T* row, uint32_t count, double (&p)[kRun]) {
+  if (count >= kRun) {
+    constexpr uint32_t kVectors = kRun * sizeof(T) / 16u;
+    const uint32_t off = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(row)) & 15u;
+    const uint4* from = reinterpret_cast<const uint4*>(reinterpret_cast<uintptr_t>(row) - off);
+    uint32_t w[4 * kVectors + 4];
 #pragma unroll
-    for (uint32_t i = 0; i < kRun * sizeof(T) / 16u; ++i) reinterpret_cast<uint4*>(v)[i] = __ldg(reinterpret_cast<const uint4*>(row) + i);
+    for (uint32_t i = 0; i < kVectors; ++i) {
+      const uint4 x = __ldg(from + i);
+      w[4 * i] = x.x; w[4 * i + 1] = x.y; w[4 * i + 2] = x.z; w[4 * i + 3] = x.w;
+    }
+    if (off) {                             // the same for a whole row
+      const uint4 x = __ldg(from + kVectors);
+      w[4 * kVectors] = x.x; w[4 * kVectors + 1] = x.y; w[4 * kVectors + 2] = x.z; w[4 * kVectors + 3] = x.w;
+      if (off & 8u) {
 #pragma unroll
-    for (uint32_t i = 0; i < kRun; ++i) p[i] = probability(v[i]);
+        for (uint32_t i = 0; i + 2 < 4 * kVectors + 4; ++i) w[i] = w[i + 2];
+      }
+      if (off & 4u) {
+#pragma unroll
+        for (uint32_t i = 0; i + 3 < 4 * kVectors + 4; ++i) w[i] = w[i + 1];
+      }
+      if (off & 2u) {
+#pragma unroll
+        for (uint32_t i = 0; i < 4 * kVectors; ++i) w[i] = __funnelshift_r(w[i], w[i + 1], 16);
+      }
+    }
+#pragma unroll
+    for (uint32_t i = 0; i < kRun; ++i) p[i] = probability(reinterpret_cast<const T*>(w)[i]);
   } else {
 #pragma unroll
     for (uint32_t i = 0; i < kRun; ++i) p[i] = i < count ? probability(row[i]) : 0.0;
@@ -65,8 +88,8 @@ template <typename T> __device__ __forceinline__ void load_run(const T* row, uin
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kVerifyThreads, 2) verify_walk(const __grid_constant__ KvipVerifyArgs a) {
-  __shared__ double s_p[kMaxNodes], s_q[kMaxNodes], s_mass[kMaxNodes + 1], s_part[2][kMaxCluster * kVerifyWarps];
+__global__ void __launch_bounds__(kMostThreads, 1) verify_walk(const __grid_constant__ KvipVerifyArgs a) {
+  __shared__ double s_p[kMaxNodes], s_q[kMaxNodes], s_mass[kMaxNodes + 1], s_part[2][kMaxCluster * kMostWarps];
   __shared__ int64_t s_token[kMaxNodes], s_lost[kMaxNodes];
   __shared__ int32_t s_parent[kMaxNodes];
   __shared__ float s_accept[kMaxNodes];
@@ -82,7 +105,7 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_walk(const __grid_co
   if (n > kMaxNodes) { n = kMaxNodes; bad = static_cast<int32_t>(KVIP_ERR_TOKEN_RANGE); }
   if (n == 0) {                            // the same for the whole cluster
     if (rank == 0) {
-      for (uint32_t i = tid; i <= a.depth; i += kVerifyThreads) { out_tokens[i] = -1; out_nodes[i] = -1; }
+      for (uint32_t i = tid; i <= a.depth; i += blockDim.x) { out_tokens[i] = -1; out_nodes[i] = -1; }
       if (tid == 0) {
         a.out_counts[b] = 0;
         if (bad) atomicOr(a.status, bad);
@@ -114,7 +137,7 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_walk(const __grid_co
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");     // ... and so do the others
 
   // the vocabulary in contiguous shares of whole runs, one per warp of the cluster
-  const uint32_t V = a.vocabulary, shares = ctas * kVerifyWarps, mine = rank * kVerifyWarps + warp;
+  const uint32_t V = a.vocabulary, warps = blockDim.x >> 5, shares = ctas * warps, mine = rank * warps + warp;
   const uint32_t share = ((V + shares - 1) / shares + kRun - 1u) / kRun * kRun;
   const uint32_t from = min(V, mine * share), to = min(V, from + share);
   uint32_t node = 0, length = 0, rejected = 0, pass = 0;
@@ -122,12 +145,12 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_walk(const __grid_co
   auto left_at = [&](uint32_t v, double (&p)[kRun]) {
     const uint32_t count = v < to ? to - v : 0u;
     const T* row = target + node * a.target_row + v;
-    load_run(row, count, (reinterpret_cast<uintptr_t>(row) & 15u) == 0, p);
+    load_run(row, count, p);
     if (!rejected) return;
     if (draft) {
       double q[kRun];
       const T* guess = draft + node * a.draft_row + v;
-      load_run(guess, count, (reinterpret_cast<uintptr_t>(guess) & 15u) == 0, q);
+      load_run(guess, count, q);
       for (uint32_t i = 0; i < rejected; ++i) {
         const double mass = s_mass[i];
 #pragma unroll
@@ -278,12 +301,15 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_walk(const __grid_co
 
 template <typename T>
 uint32_t launch_verify(const KvipVerifyArgs& a, cudaStream_t stream) {
-  // eight CTAs a request (64 requests fill the SMs four deep), fewer where the batch does that by itself
-  uint32_t ctas = kMaxCluster;
-  while (ctas > 1u && a.batch * ctas > 8u * device_sm_count()) ctas /= 2u;
+  // Eight CTAs a request, of as many threads as leave all of them resident at once (a pass is a chain of latencies, and
+  // requests wait for nothing but their own); fewer CTAs where the batch fills the SMs by itself.
+  const uint32_t sms = device_sm_count();
+  uint32_t ctas = kMaxCluster, threads = kMostThreads;
+  while (ctas > 1u && a.batch * ctas > 8u * sms) ctas /= 2u;
+  while (threads > 256u && a.batch * ctas > sms * (kMostThreads / threads)) threads /= 2u;
   cudaLaunchConfig_t config{};
   config.gridDim = dim3(a.batch * ctas);
-  config.blockDim = dim3(kVerifyThreads);
+  config.blockDim = dim3(threads);
   config.stream = stream;
   cudaLaunchAttribute attribute{};
   attribute.id = cudaLaunchAttributeClusterDimension;
