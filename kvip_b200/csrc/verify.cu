@@ -6,6 +6,7 @@
 // numbers, so all of them take the same turns; a pass is split over the warps of the cluster in contiguous shares, whose sums
 // go to every CTA through distributed shared memory, and the warp whose share holds the border looks for it. Sums are fp64 and
 // their order is fixed. Bound by HBM: one target row (and one draft row behind a rejection) per pass.
+#include <type_traits>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include "common.cuh"
@@ -16,10 +17,12 @@ namespace {
 constexpr uint32_t kMostThreads = 1024, kMostWarps = kMostThreads / 32;
 constexpr uint32_t kMaxNodes = 64;
 
-template <typename T> __device__ __forceinline__ double probability(T v);
-template <> __device__ __forceinline__ double probability(float v) { return v > 0.f ? static_cast<double>(v) : 0.0; }
-template <> __device__ __forceinline__ double probability(__nv_bfloat16 v) { return probability(__bfloat162float(v)); }
-template <> __device__ __forceinline__ double probability(__half v) { return probability(__half2float(v)); }
+// A probability as it counts: what is negative or NaN is nothing.
+template <typename T> __device__ __forceinline__ float clean(T v);
+template <> __device__ __forceinline__ float clean(float v) { return fmaxf(v, 0.f); }
+template <> __device__ __forceinline__ float clean(__nv_bfloat16 v) { return fmaxf(__bfloat162float(v), 0.f); }
+template <> __device__ __forceinline__ float clean(__half v) { return fmaxf(__half2float(v), 0.f); }
+template <typename T> __device__ __forceinline__ double probability(T v) { return static_cast<double>(clean(v)); }
 
 // What is left of probability p after the rejections so far: r = max(r - Z_i q, 0) for each of them.
 __device__ __forceinline__ double remaining(double p, double q, const double* mass, uint32_t rejected) {
@@ -47,44 +50,130 @@ __device__ __forceinline__ void store_remote(const double* where, uint32_t rank,
   asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(remote), "d"(value) : "memory");
 }
 
-constexpr uint32_t kRun = 8;               // consecutive elements that a lane takes at a time
 constexpr uint32_t kMaxCluster = 8;
 
-// kRun probabilities from `row` on, zeros behind `count`. A row of odd length starts anywhere: the aligned vectors round the
-// run are read and shifted. Each of them holds an element of the run, and memory is allocated in whole vectors.
-template <typename T> __device__ __forceinline__ void load_run(const T* row, uint32_t count, double (&p)[kRun]) {
-  if (count >= kRun) {
-    constexpr uint32_t kVectors = kRun * sizeof(T) / 16u;
-    const uint32_t off = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(row)) & 15u;
-    const uint4* from = reinterpret_cast<const uint4*>(reinterpret_cast<uintptr_t>(row) - off);
-    uint32_t w[4 * kVectors + 4];
+// A lane takes the probabilities of one 16-byte run at a time. A row of odd length starts anywhere: the two aligned vectors
+// round the run are read and shifted. A vector is read only where it holds an element of the run (memory is allocated in whole
+// vectors); `off` is the same for a whole row.
+template <typename T> struct Run {
+  static constexpr uint32_t kCount = 16u / sizeof(T);
+  uint4 low, high;
+};
+template <typename T, bool kAligned> __device__ __forceinline__ Run<T> load_run(const T* row, uint32_t count) {
+  Run<T> r;
+  r.low = r.high = make_uint4(0u, 0u, 0u, 0u);
+  const uint32_t off = kAligned ? 0u : static_cast<uint32_t>(reinterpret_cast<uintptr_t>(row)) & 15u;
+  const uint4* from = reinterpret_cast<const uint4*>(reinterpret_cast<uintptr_t>(row) - off);
+  if (count) r.low = __ldg(from);
+  if (!kAligned && off + count * sizeof(T) > 16u) r.high = __ldg(from + 1);
+  return r;
+}
+// The run's first word into place, zeros behind its elements: nothing stays nothing, whatever is taken from it.
+template <typename T, bool kAligned> __device__ __forceinline__ void settle_run(Run<T>& r, uint32_t off, uint32_t count) {
+  uint32_t w[8] = {r.low.x, r.low.y, r.low.z, r.low.w, r.high.x, r.high.y, r.high.z, r.high.w};
+  if (!kAligned) {
+    if (off & 8u) {
 #pragma unroll
-    for (uint32_t i = 0; i < kVectors; ++i) {
-      const uint4 x = __ldg(from + i);
-      w[4 * i] = x.x; w[4 * i + 1] = x.y; w[4 * i + 2] = x.z; w[4 * i + 3] = x.w;
+      for (uint32_t i = 0; i < 6; ++i) w[i] = w[i + 2];
     }
-    if (off) {                             // the same for a whole row
-      const uint4 x = __ldg(from + kVectors);
-      w[4 * kVectors] = x.x; w[4 * kVectors + 1] = x.y; w[4 * kVectors + 2] = x.z; w[4 * kVectors + 3] = x.w;
-      if (off & 8u) {
+    if (off & 4u) {
 #pragma unroll
-        for (uint32_t i = 0; i + 2 < 4 * kVectors + 4; ++i) w[i] = w[i + 2];
-      }
-      if (off & 4u) {
-#pragma unroll
-        for (uint32_t i = 0; i + 3 < 4 * kVectors + 4; ++i) w[i] = w[i + 1];
-      }
-      if (off & 2u) {
-#pragma unroll
-        for (uint32_t i = 0; i < 4 * kVectors; ++i) w[i] = __funnelshift_r(w[i], w[i + 1], 16);
-      }
+      for (uint32_t i = 0; i < 5; ++i) w[i] = w[i + 1];
     }
+    if (off & 2u) {
 #pragma unroll
-    for (uint32_t i = 0; i < kRun; ++i) p[i] = probability(reinterpret_cast<const T*>(w)[i]);
-  } else {
-#pragma unroll
-    for (uint32_t i = 0; i < kRun; ++i) p[i] = i < count ? probability(row[i]) : 0.0;
+      for (uint32_t i = 0; i < 4; ++i) w[i] = __funnelshift_r(w[i], w[i + 1], 16);
+    }
   }
+  if (count < Run<T>::kCount) {            // the last run of the vocabulary
+#pragma unroll
+    for (uint32_t i = 0; i < 4; ++i) {
+      const uint32_t bytes = count * sizeof(T);
+      w[i] = bytes >= 4u * i + 4u ? w[i] : bytes > 4u * i ? w[i] & 0xffffu : 0u;
+    }
+  }
+  r.low = make_uint4(w[0], w[1], w[2], w[3]);
+}
+template <typename T> __device__ __forceinline__ float value_of(const Run<T>& r, uint32_t k) { return clean(reinterpret_cast<const T*>(&r.low)[k]); }
+
+// What a pass has to take from the target's row.
+struct Losses {
+  const double* mass;      // s_mass: mass[i] before rejection i, the first is 1
+  const int64_t* lost;     // rejected tokens where the draft was certain
+  uint32_t rejected;
+  bool drafted;
+};
+// What is left of a run at v: r = max(r - mass q, 0) for each rejection, or nothing at a lost token.
+template <typename T> __device__ __forceinline__ void left_of_run(const Run<T>& rp, const Run<T>& rq, uint32_t v, const Losses& l, double (&r)[Run<T>::kCount]) {
+  constexpr uint32_t kRun = Run<T>::kCount;
+#pragma unroll
+  for (uint32_t k = 0; k < kRun; ++k) r[k] = static_cast<double>(value_of(rp, k));
+  for (uint32_t i = 0; i < l.rejected; ++i) {
+    if (l.drafted) {
+      const double mass = l.mass[i];
+#pragma unroll
+      for (uint32_t k = 0; k < kRun; ++k) {
+        const double d = __dsub_rn(r[k], __dmul_rn(mass, static_cast<double>(value_of(rq, k))));
+        r[k] = d > 0.0 ? d : 0.0;
+      }
+    } else {
+      const int64_t at = l.lost[i] - static_cast<int64_t>(v);
+#pragma unroll
+      for (uint32_t k = 0; k < kRun; ++k)
+        if (at == static_cast<int64_t>(k)) r[k] = 0.0;
+    }
+  }
+}
+// This lane's part of the sum between `from` and `to`: kMode 0: nothing rejected; 1: one rejection by a draft row, the common
+// one, decided in fp32 (p > q) and subtracted in fp64; 2: anything. kAtOnce runs are on their way at a time.
+template <typename T, bool kAligned, uint32_t kMode>
+__device__ __forceinline__ double sum_runs(const T* row, const T* guess, uint32_t from, uint32_t to, const Losses& l) {
+  constexpr uint32_t kRun = Run<T>::kCount, kAtOnce = kMode == 2u ? 1u : kAligned ? 4u : 2u;
+  const uint32_t off_p = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(row)) & 15u, off_q = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(guess)) & 15u;
+  double sums[2] = {0.0, 0.0};
+  for (uint32_t v0 = from + (threadIdx.x & 31u) * kRun; v0 < to; v0 += 32u * kRun * kAtOnce) {
+    Run<T> rp[kAtOnce], rq[kAtOnce];
+#pragma unroll
+    for (uint32_t u = 0; u < kAtOnce; ++u) {
+      const uint32_t v = v0 + u * 32u * kRun, count = v < to ? min(kRun, to - v) : 0u;
+      rp[u] = load_run<T, kAligned>(row + v, count);
+      if (kMode == 1u || (kMode == 2u && l.drafted)) rq[u] = load_run<T, kAligned>(guess + v, count);
+    }
+#pragma unroll
+    for (uint32_t u = 0; u < kAtOnce; ++u) {
+      const uint32_t v = v0 + u * 32u * kRun, count = v < to ? min(kRun, to - v) : 0u;
+      settle_run<T, kAligned>(rp[u], off_p, count);
+      if constexpr (kMode == 0u) {
+#pragma unroll
+        for (uint32_t k = 0; k < kRun; ++k) sums[k & 1u] += static_cast<double>(value_of(rp[u], k));
+      } else {
+        if (kMode == 1u || l.drafted) settle_run<T, kAligned>(rq[u], off_q, count);
+        if constexpr (kMode == 1u) {
+#pragma unroll
+          for (uint32_t k = 0; k < kRun; ++k) {
+            const float p = value_of(rp[u], k), q = value_of(rq[u], k);
+            const bool more = p > q;
+            sums[k & 1u] += __dsub_rn(static_cast<double>(more ? p : 0.f), static_cast<double>(more ? q : 0.f));
+          }
+        } else {
+          double r[kRun];
+          left_of_run<T>(rp[u], rq[u], v, l, r);
+#pragma unroll
+          for (uint32_t k = 0; k < kRun; ++k) sums[k & 1u] += r[k];
+        }
+      }
+    }
+  }
+  double sum = sums[0] + sums[1];
+#pragma unroll
+  for (uint32_t o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  return sum;
+}
+template <typename T, bool kAligned>
+__device__ __forceinline__ double sum_mode(const T* row, const T* guess, uint32_t from, uint32_t to, const Losses& l) {
+  if (l.rejected == 0u) return sum_runs<T, kAligned, 0u>(row, row, from, to, l);
+  if (l.rejected == 1u && l.drafted) return sum_runs<T, kAligned, 1u>(row, guess, from, to, l);
+  return sum_runs<T, kAligned, 2u>(row, guess, from, to, l);
 }
 
 template <typename T>
@@ -137,45 +226,20 @@ __global__ void __launch_bounds__(kMostThreads, 1) verify_walk(const __grid_cons
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");     // ... and so do the others
 
   // the vocabulary in contiguous shares of whole runs, one per warp of the cluster
-  const uint32_t V = a.vocabulary, warps = blockDim.x >> 5, shares = ctas * warps, mine = rank * warps + warp;
+  constexpr uint32_t kRun = Run<T>::kCount;
+  const uint32_t V = a.vocabulary, warps = blockDim.x >> 5, shares = ctas * warps;
   const uint32_t share = ((V + shares - 1) / shares + kRun - 1u) / kRun * kRun;
-  const uint32_t from = min(V, mine * share), to = min(V, from + share);
   uint32_t node = 0, length = 0, rejected = 0, pass = 0;
-  // what is left of the probabilities v .. v + kRun - 1
-  auto left_at = [&](uint32_t v, double (&p)[kRun]) {
-    const uint32_t count = v < to ? to - v : 0u;
-    const T* row = target + node * a.target_row + v;
-    load_run(row, count, p);
-    if (!rejected) return;
-    if (draft) {
-      double q[kRun];
-      const T* guess = draft + node * a.draft_row + v;
-      load_run(guess, count, q);
-      for (uint32_t i = 0; i < rejected; ++i) {
-        const double mass = s_mass[i];
-#pragma unroll
-        for (uint32_t k = 0; k < kRun; ++k) p[k] = fmax(__dsub_rn(p[k], __dmul_rn(mass, q[k])), 0.0);
-      }
-    } else {
-      for (uint32_t i = 0; i < rejected; ++i) {
-        const int64_t at = s_lost[i] - static_cast<int64_t>(v);
-#pragma unroll
-        for (uint32_t k = 0; k < kRun; ++k)
-          if (at == static_cast<int64_t>(k)) p[k] = 0.0;
-      }
-    }
+  auto losses = [&]() { return Losses{s_mass, s_lost, rejected, draft != nullptr}; };
+  auto sum_between = [&](uint32_t from, uint32_t to) -> double {
+    const T* row = target + node * a.target_row;
+    const T* guess = draft ? draft + node * a.draft_row : row;
+    return ((reinterpret_cast<uintptr_t>(row) | reinterpret_cast<uintptr_t>(guess)) & 15u) == 0 ? sum_mode<T, true>(row, guess, from, to, losses())
+                                                                                              : sum_mode<T, false>(row, guess, from, to, losses());
   };
   auto sum_all = [&]() -> double {         // leaves the shares' sums in s_part[pass & 1] of every CTA
-    double sum = 0.0;
-#pragma unroll 2
-    for (uint32_t v = from + lane * kRun; v < to; v += 32u * kRun) {
-      double p[kRun];
-      left_at(v, p);
-#pragma unroll
-      for (uint32_t k = 0; k < kRun; ++k) sum += p[k];
-    }
-#pragma unroll
-    for (uint32_t o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    const uint32_t mine = rank * warps + warp, from = min(V, mine * share);
+    const double sum = sum_between(from, min(V, from + share));
     ++pass;
     double* part = s_part[pass & 1u];
     if (lane < ctas) store_remote(&part[mine], lane, sum);
@@ -185,6 +249,30 @@ __global__ void __launch_bounds__(kMostThreads, 1) verify_walk(const __grid_cons
 #pragma unroll
     for (uint32_t o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
     return total;
+  };
+  // Of `count` sums in order, the first one whose running sum, from `running` on, passes the limit; where rounding leaves none,
+  // the last one that holds anything. `running` becomes the sum before it.
+  auto passing = [&](const double* sums, uint32_t count, double limit, double& running) -> uint32_t {
+    double so_far = running;
+    uint32_t chosen = 0;
+    for (uint32_t k = 0; k < count; k += 32u) {
+      const double own = k + lane < count ? sums[k + lane] : 0.0;
+      double scan = own;
+#pragma unroll
+      for (uint32_t d = 1; d < 32u; d <<= 1) {
+        const double other = __shfl_up_sync(0xffffffffu, scan, d);
+        if (lane >= d) scan += other;
+      }
+      const uint32_t holds = __ballot_sync(0xffffffffu, own > 0.0), passed = __ballot_sync(0xffffffffu, own > 0.0 && so_far + scan > limit);
+      if (holds) {
+        const uint32_t pick = passed ? static_cast<uint32_t>(__ffs(static_cast<int>(passed))) - 1u : 31u - static_cast<uint32_t>(__clz(static_cast<int>(holds)));
+        chosen = k + pick;
+        running = so_far + __shfl_sync(0xffffffffu, scan - own, pick);
+      }
+      if (passed) break;
+      so_far += __shfl_sync(0xffffffffu, scan, 31);
+    }
+    return chosen;
   };
   bool summed = false;
   double total = 0.0;
@@ -230,73 +318,62 @@ __global__ void __launch_bounds__(kMostThreads, 1) verify_walk(const __grid_cons
       if (bad) atomicOr(a.status, bad);
     }
   }
-  // the first share whose running sum passes the limit; where rounding leaves none, the last one that holds anything
+  // The share that holds the border is looked through once more, by all warps of its CTA: a part each, then a run per lane.
   const double limit = __dmul_rn(static_cast<double>(a.sample[b]), total);
-  const double* part = s_part[pass & 1u];
-  double base = 0.0, before_last = 0.0, running = 0.0;
-  uint32_t chosen = 0;
-  bool passed_any = false;
-  for (uint32_t k = 0; k < shares && !passed_any; k += 32u) {
-    const double own = k + lane < shares ? part[k + lane] : 0.0;
+  double running = 0.0;
+  const uint32_t chosen = passing(s_part[pass & 1u], shares, limit, running);
+  if (chosen / warps != rank) return;
+  const uint32_t begin = min(V, chosen * share), end = min(V, begin + share);
+  const uint32_t part = ((end - begin + warps - 1u) / warps + kRun - 1u) / kRun * kRun;
+  double* sums = s_part[(pass & 1u) ^ 1u];   // the other CTAs have done with it, and write to it no more
+  const uint32_t from = min(end, begin + warp * part);
+  const double sum = sum_between(from, min(end, from + part));
+  if (lane == 0) sums[warp] = sum;
+  __syncthreads();
+  if (warp) return;
+  const uint32_t place = passing(sums, warps, limit, running);
+  const T* row = target + node * a.target_row;
+  const T* guess = draft ? draft + node * a.draft_row : row;
+  const uint32_t off_p = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(row)) & 15u, off_q = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(guess)) & 15u;
+  const uint32_t first_run = min(end, begin + place * part), behind_run = min(end, first_run + part);
+  uint32_t picked = 0;
+  for (uint32_t v0 = first_run; v0 < behind_run; v0 += 32u * kRun) {
+    const uint32_t v = v0 + lane * kRun, count = v < behind_run ? min(kRun, behind_run - v) : 0u;
+    Run<T> rp = load_run<T, false>(row + v, count), rq = load_run<T, false>(guess + v, count);
+    settle_run<T, false>(rp, off_p, count);
+    settle_run<T, false>(rq, off_q, count);
+    double p[kRun];
+    left_of_run<T>(rp, rq, v, losses(), p);
+    double own = 0.0;
+#pragma unroll
+    for (uint32_t k = 0; k < kRun; ++k) own += p[k];
     double scan = own;
 #pragma unroll
     for (uint32_t d = 1; d < 32u; d <<= 1) {
       const double other = __shfl_up_sync(0xffffffffu, scan, d);
       if (lane >= d) scan += other;
     }
-    const uint32_t holds = __ballot_sync(0xffffffffu, own > 0.0);
-    const uint32_t passed = __ballot_sync(0xffffffffu, own > 0.0 && running + scan > limit);
-    const uint32_t pick = passed ? static_cast<uint32_t>(__ffs(static_cast<int>(passed))) - 1u : holds ? 31u - static_cast<uint32_t>(__clz(static_cast<int>(holds))) : 0u;
-    if (passed || holds) {
-      chosen = k + pick;
-      before_last = running + __shfl_sync(0xffffffffu, scan - own, pick);
-      base = before_last;
+    // within the run: the first element whose running sum passes, else the last that holds anything
+    double so_far = running + (scan - own);
+    uint32_t at = 0, last = 0;
+    bool found = false;
+#pragma unroll
+    for (uint32_t k = 0; k < kRun; ++k) {
+      so_far += p[k];
+      if (p[k] > 0.0) {
+        last = k;
+        if (!found && so_far > limit) { found = true; at = k; }
+      }
     }
-    passed_any = passed != 0u;
+    const uint32_t passed = __ballot_sync(0xffffffffu, found), holds = __ballot_sync(0xffffffffu, own > 0.0);
+    if (passed || holds) {
+      const uint32_t who = passed ? static_cast<uint32_t>(__ffs(static_cast<int>(passed))) - 1u : 31u - static_cast<uint32_t>(__clz(static_cast<int>(holds)));
+      picked = v0 + who * kRun + __shfl_sync(0xffffffffu, passed ? at : last, who);
+    }
+    if (passed) break;
     running += __shfl_sync(0xffffffffu, scan, 31);
   }
-  if (mine == chosen) {
-    double before = base;
-    uint32_t picked = 0;
-    for (uint32_t v0 = from; v0 < to; v0 += 32u * kRun) {
-      const uint32_t v = v0 + lane * kRun;
-      double p[kRun];
-      left_at(v, p);
-      double own = 0.0;
-#pragma unroll
-      for (uint32_t k = 0; k < kRun; ++k) own += p[k];
-      double scan = own;
-#pragma unroll
-      for (uint32_t d = 1; d < 32u; d <<= 1) {
-        const double other = __shfl_up_sync(0xffffffffu, scan, d);
-        if (lane >= d) scan += other;
-      }
-      // within the run: the first element whose running sum passes, else the last that holds anything
-      double sum = before + (scan - own);
-      uint32_t at = 0, last = 0;
-      bool found = false;
-#pragma unroll
-      for (uint32_t k = 0; k < kRun; ++k) {
-        sum += p[k];
-        if (p[k] > 0.0) {
-          last = k;
-          if (!found && sum > limit) { found = true; at = k; }
-        }
-      }
-      const uint32_t passed = __ballot_sync(0xffffffffu, found), holds = __ballot_sync(0xffffffffu, own > 0.0);
-      if (passed) {
-        const uint32_t who = static_cast<uint32_t>(__ffs(static_cast<int>(passed))) - 1u;
-        picked = v0 + who * kRun + __shfl_sync(0xffffffffu, at, who);
-        break;
-      }
-      if (holds) {
-        const uint32_t who = 31u - static_cast<uint32_t>(__clz(static_cast<int>(holds)));
-        picked = v0 + who * kRun + __shfl_sync(0xffffffffu, last, who);
-      }
-      before += __shfl_sync(0xffffffffu, scan, 31);
-    }
-    if (lane == 0) out_tokens[length] = picked;
-  }
+  if (lane == 0) out_tokens[length] = picked;
 }
 
 template <typename T>
