@@ -5,7 +5,9 @@
 // the running sum passes sample * sum. A cluster of CTAs takes one request. Every CTA makes the whole walk from the same
 // numbers, so all of them take the same turns; a pass is split over the warps of the cluster in contiguous shares, whose sums
 // go to every CTA through distributed shared memory, and the warp whose share holds the border looks for it. Sums are fp64 and
-// their order is fixed. Bound by HBM: one target row (and one draft row behind a rejection) per pass.
+// their order is fixed. The rejections at one node need no pass of their own over each other's results: where r - Z q is not
+// cut off, r = max(target - C draft, 0) with C = 1 + Z_1 + .. + Z_(k-1), and what was cut off stays below. So a pass costs one fp64
+// fma, one add and two conversions (the slowest of them, 16 a clock and SM) per element, however many rejections. Bound by HBM: one target row (and one draft row behind a rejection) per pass.
 #include <type_traits>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -24,10 +26,10 @@ template <> __device__ __forceinline__ float clean(__nv_bfloat16 v) { return fma
 template <> __device__ __forceinline__ float clean(__half v) { return fmaxf(__half2float(v), 0.f); }
 template <typename T> __device__ __forceinline__ double probability(T v) { return static_cast<double>(clean(v)); }
 
-// What is left of probability p after the rejections so far: r = max(r - Z_i q, 0) for each of them.
-__device__ __forceinline__ double remaining(double p, double q, const double* mass, uint32_t rejected) {
-  for (uint32_t i = 0; i < rejected; ++i) p = fmax(__dsub_rn(p, __dmul_rn(mass[i], q)), 0.0);
-  return p;
+// What is left of probability p where the masses taken so far sum up to `taken`: max(p - taken q, 0).
+__device__ __forceinline__ double remaining(double p, double q, double taken) {
+  const double d = __fma_rn(-taken, q, p);
+  return __double2hiint(d) < 0 ? 0.0 : d;   // the sign by the integer units: the fp64 ones are the scarce ones
 }
 
 __device__ __forceinline__ uint32_t cluster_rank() {
@@ -98,34 +100,30 @@ template <typename T> __device__ __forceinline__ float value_of(const Run<T>& r,
 
 // What a pass has to take from the target's row.
 struct Losses {
-  const double* mass;      // s_mass: mass[i] before rejection i, the first is 1
-  const int64_t* lost;     // rejected tokens where the draft was certain
+  double taken;            // drafted: sum of the masses, 0 where nothing was rejected
+  const int64_t* lost;     // else the rejected tokens
   uint32_t rejected;
   bool drafted;
 };
-// What is left of a run at v: r = max(r - mass q, 0) for each rejection, or nothing at a lost token.
+// What is left of a run at v.
 template <typename T> __device__ __forceinline__ void left_of_run(const Run<T>& rp, const Run<T>& rq, uint32_t v, const Losses& l, double (&r)[Run<T>::kCount]) {
   constexpr uint32_t kRun = Run<T>::kCount;
 #pragma unroll
   for (uint32_t k = 0; k < kRun; ++k) r[k] = static_cast<double>(value_of(rp, k));
+  if (l.drafted) {
+#pragma unroll
+    for (uint32_t k = 0; k < kRun; ++k) r[k] = remaining(r[k], static_cast<double>(value_of(rq, k)), l.taken);
+    return;
+  }
   for (uint32_t i = 0; i < l.rejected; ++i) {
-    if (l.drafted) {
-      const double mass = l.mass[i];
+    const int64_t at = l.lost[i] - static_cast<int64_t>(v);
 #pragma unroll
-      for (uint32_t k = 0; k < kRun; ++k) {
-        const double d = __dsub_rn(r[k], __dmul_rn(mass, static_cast<double>(value_of(rq, k))));
-        r[k] = d > 0.0 ? d : 0.0;
-      }
-    } else {
-      const int64_t at = l.lost[i] - static_cast<int64_t>(v);
-#pragma unroll
-      for (uint32_t k = 0; k < kRun; ++k)
-        if (at == static_cast<int64_t>(k)) r[k] = 0.0;
-    }
+    for (uint32_t k = 0; k < kRun; ++k)
+      if (at == static_cast<int64_t>(k)) r[k] = 0.0;
   }
 }
-// This lane's part of the sum between `from` and `to`: kMode 0: nothing rejected; 1: one rejection by a draft row, the common
-// one, decided in fp32 (p > q) and subtracted in fp64; 2: anything. kAtOnce runs are on their way at a time.
+// This lane's part of the sum between `from` and `to`; kMode 0: nothing rejected, 1: by a draft row, 2: certain tokens.
+// kAtOnce runs are on their way at a time.
 template <typename T, bool kAligned, uint32_t kMode>
 __device__ __forceinline__ double sum_runs(const T* row, const T* guess, uint32_t from, uint32_t to, const Losses& l) {
   constexpr uint32_t kRun = Run<T>::kCount, kAtOnce = kMode == 2u ? 1u : kAligned ? 4u : 2u;
@@ -137,7 +135,7 @@ __device__ __forceinline__ double sum_runs(const T* row, const T* guess, uint32_
     for (uint32_t u = 0; u < kAtOnce; ++u) {
       const uint32_t v = v0 + u * 32u * kRun, count = v < to ? min(kRun, to - v) : 0u;
       rp[u] = load_run<T, kAligned>(row + v, count);
-      if (kMode == 1u || (kMode == 2u && l.drafted)) rq[u] = load_run<T, kAligned>(guess + v, count);
+      if (kMode == 1u) rq[u] = load_run<T, kAligned>(guess + v, count);
     }
 #pragma unroll
     for (uint32_t u = 0; u < kAtOnce; ++u) {
@@ -146,21 +144,16 @@ __device__ __forceinline__ double sum_runs(const T* row, const T* guess, uint32_
       if constexpr (kMode == 0u) {
 #pragma unroll
         for (uint32_t k = 0; k < kRun; ++k) sums[k & 1u] += static_cast<double>(value_of(rp[u], k));
+      } else if constexpr (kMode == 1u) {
+        settle_run<T, kAligned>(rq[u], off_q, count);
+#pragma unroll
+        for (uint32_t k = 0; k < kRun; ++k)
+          sums[k & 1u] += remaining(static_cast<double>(value_of(rp[u], k)), static_cast<double>(value_of(rq[u], k)), l.taken);
       } else {
-        if (kMode == 1u || l.drafted) settle_run<T, kAligned>(rq[u], off_q, count);
-        if constexpr (kMode == 1u) {
+        double r[kRun];
+        left_of_run<T>(rp[u], rp[u], v, l, r);
 #pragma unroll
-          for (uint32_t k = 0; k < kRun; ++k) {
-            const float p = value_of(rp[u], k), q = value_of(rq[u], k);
-            const bool more = p > q;
-            sums[k & 1u] += __dsub_rn(static_cast<double>(more ? p : 0.f), static_cast<double>(more ? q : 0.f));
-          }
-        } else {
-          double r[kRun];
-          left_of_run<T>(rp[u], rq[u], v, l, r);
-#pragma unroll
-          for (uint32_t k = 0; k < kRun; ++k) sums[k & 1u] += r[k];
-        }
+        for (uint32_t k = 0; k < kRun; ++k) sums[k & 1u] += r[k];
       }
     }
   }
@@ -172,21 +165,56 @@ __device__ __forceinline__ double sum_runs(const T* row, const T* guess, uint32_
 template <typename T, bool kAligned>
 __device__ __forceinline__ double sum_mode(const T* row, const T* guess, uint32_t from, uint32_t to, const Losses& l) {
   if (l.rejected == 0u) return sum_runs<T, kAligned, 0u>(row, row, from, to, l);
-  if (l.rejected == 1u && l.drafted) return sum_runs<T, kAligned, 1u>(row, guess, from, to, l);
+  if (l.drafted) return sum_runs<T, kAligned, 1u>(row, guess, from, to, l);
   return sum_runs<T, kAligned, 2u>(row, guess, from, to, l);
+}
+template <typename T> __device__ __forceinline__ double sum_between(const T* row, const T* guess, uint32_t from, uint32_t to, const Losses l) {
+  return ((reinterpret_cast<uintptr_t>(row) | reinterpret_cast<uintptr_t>(guess)) & 15u) == 0 ? sum_mode<T, true>(row, guess, from, to, l)
+                                                                                            : sum_mode<T, false>(row, guess, from, to, l);
+}
+// Of `count` sums in order, the first one whose running sum, from `running` on, passes the limit; where rounding leaves none,
+// the last one that holds anything. `running` becomes the sum before it. A lane takes `each` sums in a row; sum k lies at
+// place_of(k, each), where the lanes' reads meet no bank twice.
+__device__ __forceinline__ uint32_t place_of(uint32_t k, uint32_t each) { return (k % each) * 32u + k / each; }
+struct Place { double running; uint32_t chosen; };
+__device__ __forceinline__ Place passing(const double* sums, uint32_t count, double limit, double running) {
+  const uint32_t lane = threadIdx.x & 31u, each = (count + 31u) / 32u, first = lane * each;
+  double own = 0.0;
+  for (uint32_t i = 0; i < each; ++i) own += first + i < count ? sums[i * 32u + lane] : 0.0;
+  double scan = own;
+#pragma unroll
+  for (uint32_t d = 1; d < 32u; d <<= 1) {
+    const double other = __shfl_up_sync(0xffffffffu, scan, d);
+    if (lane >= d) scan += other;
+  }
+  const uint32_t holds = __ballot_sync(0xffffffffu, own > 0.0), passed = __ballot_sync(0xffffffffu, own > 0.0 && running + scan > limit);
+  const uint32_t pick = passed ? static_cast<uint32_t>(__ffs(static_cast<int>(passed))) - 1u : holds ? 31u - static_cast<uint32_t>(__clz(static_cast<int>(holds))) : 0u;
+  Place at{running + (scan - own), first};   // this lane's, should it be the one
+  double before = at.running;
+  for (uint32_t i = 0; i < each; ++i) {
+    const double x = first + i < count ? sums[i * 32u + lane] : 0.0;
+    if (x > 0.0) { at.running = before; at.chosen = first + i; }
+    before += x;
+    if (x > 0.0 && before > limit) break;
+  }
+  at.running = __shfl_sync(0xffffffffu, at.running, pick);
+  at.chosen = __shfl_sync(0xffffffffu, at.chosen, pick);
+  return at;
 }
 
 template <typename T>
 __global__ void __launch_bounds__(kMostThreads, 1) verify_walk(const __grid_constant__ KvipVerifyArgs a) {
-  __shared__ double s_p[kMaxNodes], s_q[kMaxNodes], s_mass[kMaxNodes + 1], s_part[2][kMaxCluster * kMostWarps];
+  __shared__ double s_p[kMaxNodes], s_q[kMaxNodes], s_part[2][kMaxCluster * kMostWarps];
   __shared__ int64_t s_token[kMaxNodes], s_lost[kMaxNodes];
   __shared__ int32_t s_parent[kMaxNodes];
   __shared__ float s_accept[kMaxNodes];
+  __shared__ Place s_border;
   const uint32_t rank = cluster_rank(), ctas = cluster_size();
   const uint32_t b = blockIdx.x / ctas, tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5;
   int64_t* out_tokens = a.out_tokens + static_cast<uint64_t>(b) * (a.depth + 1u);
   int32_t* out_nodes = a.out_nodes + static_cast<uint64_t>(b) * (a.depth + 1u);
   const int64_t first = a.starts[b], behind = a.starts[b + 1];
+  const double sample = static_cast<double>(a.sample[b]);
   uint32_t n = 0;
   int32_t bad = 0;
   if (first >= 0 && behind >= first && behind <= static_cast<int64_t>(a.rows)) n = static_cast<uint32_t>(min(behind - first, static_cast<int64_t>(kMaxNodes + 1u)));
@@ -221,7 +249,6 @@ __global__ void __launch_bounds__(kMostThreads, 1) verify_walk(const __grid_cons
       s_q[tid] = draft ? probability(draft[parent * a.draft_row + token]) : 1.0;
     }
   }
-  if (tid == 0) s_mass[0] = 1.0;
   bad = __syncthreads_or(bad);
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");     // ... and so do the others
 
@@ -230,49 +257,25 @@ __global__ void __launch_bounds__(kMostThreads, 1) verify_walk(const __grid_cons
   const uint32_t V = a.vocabulary, warps = blockDim.x >> 5, shares = ctas * warps;
   const uint32_t share = ((V + shares - 1) / shares + kRun - 1u) / kRun * kRun;
   uint32_t node = 0, length = 0, rejected = 0, pass = 0;
-  auto losses = [&]() { return Losses{s_mass, s_lost, rejected, draft != nullptr}; };
-  auto sum_between = [&](uint32_t from, uint32_t to) -> double {
+  double mass = 1.0, taken = 0.0;          // of what is left at the node, and of all before
+  auto losses = [&]() { return Losses{taken, s_lost, rejected, draft != nullptr}; };
+  auto part_sum = [&](uint32_t from, uint32_t to) -> double {
     const T* row = target + node * a.target_row;
-    const T* guess = draft ? draft + node * a.draft_row : row;
-    return ((reinterpret_cast<uintptr_t>(row) | reinterpret_cast<uintptr_t>(guess)) & 15u) == 0 ? sum_mode<T, true>(row, guess, from, to, losses())
-                                                                                              : sum_mode<T, false>(row, guess, from, to, losses());
+    return sum_between<T>(row, draft ? draft + node * a.draft_row : row, from, to, losses());
   };
   auto sum_all = [&]() -> double {         // leaves the shares' sums in s_part[pass & 1] of every CTA
     const uint32_t mine = rank * warps + warp, from = min(V, mine * share);
-    const double sum = sum_between(from, min(V, from + share));
+    const double sum = part_sum(from, min(V, from + share));
     ++pass;
     double* part = s_part[pass & 1u];
-    if (lane < ctas) store_remote(&part[mine], lane, sum);
+    const uint32_t each = (shares + 31u) / 32u;
+    if (lane < ctas) store_remote(&part[place_of(mine, each)], lane, sum);
     cluster_barrier();
     double total = 0.0;
-    for (uint32_t k = 0; k < shares; k += 32u) total += k + lane < shares ? part[k + lane] : 0.0;
+    for (uint32_t i = 0; i < each; ++i) total += lane * each + i < shares ? part[i * 32u + lane] : 0.0;
 #pragma unroll
     for (uint32_t o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
     return total;
-  };
-  // Of `count` sums in order, the first one whose running sum, from `running` on, passes the limit; where rounding leaves none,
-  // the last one that holds anything. `running` becomes the sum before it.
-  auto passing = [&](const double* sums, uint32_t count, double limit, double& running) -> uint32_t {
-    double so_far = running;
-    uint32_t chosen = 0;
-    for (uint32_t k = 0; k < count; k += 32u) {
-      const double own = k + lane < count ? sums[k + lane] : 0.0;
-      double scan = own;
-#pragma unroll
-      for (uint32_t d = 1; d < 32u; d <<= 1) {
-        const double other = __shfl_up_sync(0xffffffffu, scan, d);
-        if (lane >= d) scan += other;
-      }
-      const uint32_t holds = __ballot_sync(0xffffffffu, own > 0.0), passed = __ballot_sync(0xffffffffu, own > 0.0 && so_far + scan > limit);
-      if (holds) {
-        const uint32_t pick = passed ? static_cast<uint32_t>(__ffs(static_cast<int>(passed))) - 1u : 31u - static_cast<uint32_t>(__clz(static_cast<int>(holds)));
-        chosen = k + pick;
-        running = so_far + __shfl_sync(0xffffffffu, scan - own, pick);
-      }
-      if (passed) break;
-      so_far += __shfl_sync(0xffffffffu, scan, 31);
-    }
-    return chosen;
   };
   bool summed = false;
   double total = 0.0;
@@ -280,10 +283,9 @@ __global__ void __launch_bounds__(kMostThreads, 1) verify_walk(const __grid_cons
   uint32_t path_high = 0;
   for (uint32_t j = 1; j < n && length < a.depth; ++j) {
     if (s_parent[j] != static_cast<int32_t>(node)) continue;
-    const double mass = s_mass[rejected];
     double r = s_p[j];
     if (draft) {
-      r = remaining(r, s_q[j], s_mass, rejected);
+      r = remaining(r, s_q[j], taken);
     } else {
       for (uint32_t i = 0; i < rejected; ++i)
         if (s_lost[i] == s_token[j]) r = 0.0;
@@ -293,19 +295,20 @@ __global__ void __launch_bounds__(kMostThreads, 1) verify_walk(const __grid_cons
       node = j;
       ++length;
       rejected = 0;
+      mass = 1.0;
+      taken = 0.0;
       summed = false;
     } else {
       if (tid == 0) s_lost[rejected] = s_token[j];
       __syncthreads();
       ++rejected;
-      total = sum_all();
+      taken += mass;
+      mass = total = sum_all();
       summed = true;
-      if (tid == 0) s_mass[rejected] = total;
-      __syncthreads();
-      if (total == 0.0) { rejected = 0; summed = false; break; }
+      if (total == 0.0) { rejected = 0; taken = 0.0; summed = false; break; }
     }
   }
-  if (!summed) total = sum_all();
+  if (!summed) total = sum_all();          // nothing rejected at the last node
   if (rank == 0 && warp == 0) {            // what has been accepted; the drawn token's place is another warp's
     for (uint32_t i = lane; i <= a.depth; i += 32u) {
       const uint32_t at = i < 32u ? path : path_high;
@@ -319,19 +322,26 @@ __global__ void __launch_bounds__(kMostThreads, 1) verify_walk(const __grid_cons
     }
   }
   // The share that holds the border is looked through once more, by all warps of its CTA: a part each, then a run per lane.
-  const double limit = __dmul_rn(static_cast<double>(a.sample[b]), total);
-  double running = 0.0;
-  const uint32_t chosen = passing(s_part[pass & 1u], shares, limit, running);
+  const double limit = __dmul_rn(sample, total);
+  if (warp == 0) {
+    const Place border = passing(s_part[pass & 1u], shares, limit, 0.0);
+    if (lane == 0) { s_border.running = border.running; s_border.chosen = border.chosen; }
+  }
+  __syncthreads();
+  const Place border{s_border.running, s_border.chosen};
+  const uint32_t chosen = border.chosen;
   if (chosen / warps != rank) return;
   const uint32_t begin = min(V, chosen * share), end = min(V, begin + share);
   const uint32_t part = ((end - begin + warps - 1u) / warps + kRun - 1u) / kRun * kRun;
   double* sums = s_part[(pass & 1u) ^ 1u];   // the other CTAs have done with it, and write to it no more
   const uint32_t from = min(end, begin + warp * part);
-  const double sum = sum_between(from, min(end, from + part));
+  const double sum = part_sum(from, min(end, from + part));
   if (lane == 0) sums[warp] = sum;
   __syncthreads();
   if (warp) return;
-  const uint32_t place = passing(sums, warps, limit, running);
+  const Place inner = passing(sums, warps, limit, border.running);
+  const uint32_t place = inner.chosen;
+  double running = inner.running;
   const T* row = target + node * a.target_row;
   const T* guess = draft ? draft + node * a.draft_row : row;
   const uint32_t off_p = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(row)) & 15u, off_q = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(guess)) & 15u;
