@@ -126,7 +126,7 @@ template <typename T> __device__ __forceinline__ void left_of_run(const Run<T>& 
 // kAtOnce runs are on their way at a time.
 template <typename T, bool kAligned, uint32_t kMode>
 __device__ __forceinline__ double sum_runs(const T* row, const T* guess, uint32_t from, uint32_t to, const Losses& l) {
-  constexpr uint32_t kRun = Run<T>::kCount, kAtOnce = kMode == 2u ? 1u : kAligned ? 4u : 2u;
+  constexpr uint32_t kRun = Run<T>::kCount, kAtOnce = kMode == 2u ? 1u : kAligned && kRun == 4u ? 4u : 2u;
   const uint32_t off_p = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(row)) & 15u, off_q = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(guess)) & 15u;
   double sums[2] = {0.0, 0.0};
   for (uint32_t v0 = from + (threadIdx.x & 31u) * kRun; v0 < to; v0 += 32u * kRun * kAtOnce) {
@@ -393,7 +393,8 @@ uint32_t launch_verify(const KvipVerifyArgs& a, cudaStream_t stream) {
   const uint32_t sms = device_sm_count();
   uint32_t ctas = kMaxCluster, threads = kMostThreads;
   while (ctas > 1u && a.batch * ctas > 8u * sms) ctas /= 2u;
-  while (threads > 256u && a.batch * ctas > sms * (kMostThreads / threads)) threads /= 2u;
+const uint32_t resident = (a.batch * ctas + sms - 1) / sms;   // CTAs per SM
+  if (resident > 1u) threads = resident >= 4u ? 256u : kMostThreads / resident / 32u * 32u;
   cudaLaunchConfig_t config{};
   config.gridDim = dim3(a.batch * ctas);
   config.blockDim = dim3(threads);
