@@ -252,20 +252,6 @@ def last_error(library=None):
     return lib.kvip_b200_last_error().decode(errors="replace")
 
 
-def enqueue(function, args, device, what):
-    """One entry point on the current stream of `device` (an index), which need not be the current device."""
-    import torch
-
-    stream = torch.cuda.current_stream(device).cuda_stream
-    if torch.cuda.current_device() == device:
-        code = function(ctypes.byref(args), stream)
-    else:
-        with torch.cuda.device(device):
-            code = function(ctypes.byref(args), stream)
-    if code:
-        check(code, what)
-
-
 def check(code, what, library=None):
     """Map the C return convention to the reference's Python errors (ValueError for contract
     violations, RuntimeError for a failed launch; operators/lifetch/streaming.py:129-131)."""

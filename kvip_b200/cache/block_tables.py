@@ -4,7 +4,7 @@ The reference receives `metadata.slot_mapping`, positions and block tables from 
 that follows a verification of drafted tokens knows its lengths only on the GPU; `BlockTables` makes the maps from
 them in one launch, with no copy to the host and none from it: blocks from a free list, packed positions, slots and
 requests, and (for `QueryInputs.prepare_device`) the layout of the query slots."""
-from .. import _lib
+from .. import _lib, _launch
 
 
 class BlockTables:
@@ -42,12 +42,14 @@ class BlockTables:
         self.taken, self.status = torch.zeros(1, **i32), torch.zeros(1, **i32)
         self.layout = torch.zeros((4, batch * queries), **i64) if queries else None
         self.device, self.index = self.table.device, self.table.get_device()
-        self.function = _lib.load_library().kvip_b200_slot_maps
+        self.launch = _launch.Launcher("kvip_b200_slot_maps")
         outputs = (self.table, self.positions, self.slot_mapping, self.requests, self.starts, self.ends, self.held_after, self.taken,
                    self.status)
-        self._outputs = tuple(t.data_ptr() for t in outputs) + (self.layout.data_ptr() if queries else None,)
-        self._state = (self.held.data_ptr(), self.free.data_ptr(), self.head.data_ptr())
-        self._sizes = (batch, pages, blocks, tokens, block, queries)
+        pointers = tuple(t.data_ptr() for t in outputs) + (self.layout.data_ptr() if queries else 0,)
+        # the record behind `counts`: every buffer is this object's own
+        self._rest = (self.held.data_ptr(), self.free.data_ptr(), self.head.data_ptr(), *pointers, batch, pages, blocks, tokens,
+                      block, queries)
+        self._lengths = self.lengths.data_ptr()
 
     @property
     def nbytes(self):
@@ -74,8 +76,7 @@ class BlockTables:
         if (counts.dtype != self.torch.int32 or counts.ndim != 1 or counts.numel() != self.batch or counts.get_device() != self.index
                 or not counts.is_contiguous()):
             raise ValueError("BlockTables counts must be contiguous int32 [batch] on the tables' device")
-        args = _lib.SlotMapsArgs(self.lengths.data_ptr(), counts.data_ptr(), *self._state, *self._outputs, *self._sizes)
-        _lib.enqueue(self.function, args, self.index, "slot_maps")
+        self.launch(self.index, self._lengths, counts.data_ptr(), *self._rest)
         return self
 
     def commit(self, kept):

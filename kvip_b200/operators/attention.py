@@ -3,7 +3,7 @@
 The reference leaves attention to the serving framework; `slot_output` and the resident pool are its interface to it.
 `SlotAttention` reads both where they lie: no dense gather is needed, every token's rows go from the pool into the
 kernel once."""
-from .. import _lib
+from .. import _lib, _launch
 
 
 class SlotAttention:
@@ -47,7 +47,7 @@ class SlotAttention:
         self.partial = torch.empty((self.partial_rows, _lib.ATTENTION_VALUE), dtype=torch.float32, device=device)
         self.partial_stats = torch.empty((self.partial_rows, 2), dtype=torch.float32, device=device)
         self._fixed = (self.partial.data_ptr(), self.partial_stats.data_ptr(), self.status.data_ptr())
-        self.function = _lib.load_library().kvip_b200_slot_attention
+        self.launch = _launch.Launcher("kvip_b200_slot_attention")
 
     @property
     def nbytes(self):
@@ -85,14 +85,14 @@ class SlotAttention:
             batch = starts.numel() - 1
         else:
             batch = rows // output_stride
-        requests_ptr = None if requests is None else self._flat(requests, "requests", torch.int32, requests.numel())
+        requests_ptr = 0 if requests is None else self._flat(requests, "requests", torch.int32, requests.numel())
         if requests is None:
             if queries < 1 or batch * queries < tokens:
                 raise ValueError("SlotAttention tokens without requests belong to request t // queries")
         elif requests.numel() < tokens:
             raise ValueError("SlotAttention requests must cover the tokens")
-        owners_ptr = None if row_owners is None else self._flat(row_owners, "row_owners", torch.int32, batch)
-        draft_ptr = starts_ptr = ancestors_ptr = None
+        owners_ptr = 0 if row_owners is None else self._flat(row_owners, "row_owners", torch.int32, batch)
+        draft_ptr = starts_ptr = ancestors_ptr = 0
         draft_token = 0
         if draft is not None:
             if starts is None:
@@ -119,10 +119,9 @@ class SlotAttention:
             lse_ptr = lse.data_ptr()
         else:
             lse_ptr = self._flat(lse, "lse", torch.float32, tokens * heads)
-        args = _lib.AttentionArgs(
-            query.data_ptr(), pool.data_ptr(), slots.data_ptr(), requests_ptr, owners_ptr, starts_ptr, draft_ptr, ancestors_ptr,
+        self.launch(
+            index, query.data_ptr(), pool.data_ptr(), slots.data_ptr(), requests_ptr, owners_ptr, starts_ptr, draft_ptr, ancestors_ptr,
             out_ptr, lse_ptr, *self._fixed, query.stride(0), query.stride(1), draft_token, rows, tokens, heads, entries, batch,
             queries, output_stride, _lib.FLOAT_BF16 if self.dtype == torch.bfloat16 else _lib.FLOAT_FP16, splits, self.partial_rows,
             wait_kilocycles, scale, 0)
-        _lib.enqueue(self.function, args, index, "slot_attention")
         return out, lse

@@ -3,7 +3,7 @@
 The reference's query slots carry up to four tokens of a speculative step and leave their verification to the serving
 framework. `DraftVerifier` walks every request's tree of drafted tokens on the GPU in one launch; the counts it returns
 are what `BlockTables.commit` and the next step's maps take."""
-from .. import _lib
+from .. import _lib, _launch
 
 
 class DraftVerifier:
@@ -34,7 +34,7 @@ class DraftVerifier:
         self.device, self.index = self.counts.device, self.counts.get_device()
         self._outputs = tuple(t.data_ptr() for t in (self.tokens, self.nodes, self.counts, self.status))
         self.types = {torch.bfloat16: _lib.FLOAT_BF16, torch.float16: _lib.FLOAT_FP16, torch.float32: _lib.FLOAT_FP32}
-        self.function = _lib.load_library().kvip_b200_verify_drafts
+        self.launch = _launch.Launcher("kvip_b200_verify_drafts")
 
     def _flat(self, tensor, name, dtype, count):
         if tensor.dtype != dtype or tensor.ndim != 1 or tensor.numel() < count or tensor.get_device() != self.index or not tensor.is_contiguous():
@@ -49,17 +49,16 @@ class DraftVerifier:
         rows, vocabulary = target.shape
         if rows < 1 or not 1 <= vocabulary <= 1 << 24:
             raise ValueError("DraftVerifier: at least one row, a vocabulary of 1..2^24")
-        draft_ptr, draft_row = None, 0
+        draft_ptr, draft_row = 0, 0
         if draft is not None:
             if draft.shape != target.shape or draft.dtype != target.dtype or draft.stride(1) != 1 or draft.get_device() != index:
                 raise ValueError("DraftVerifier draft must match the target")
             draft_ptr, draft_row = draft.data_ptr(), draft.stride(0)
         if starts.numel() != self.batch + 1:
             raise ValueError("DraftVerifier starts must be [batch + 1]")
-        args = _lib.VerifyArgs(
-            target.data_ptr(), draft_ptr, self._flat(tokens, "tokens", torch.int64, rows), self._flat(parents, "parents", torch.int32, rows),
+        self.launch(
+            index, target.data_ptr(), draft_ptr, self._flat(tokens, "tokens", torch.int64, rows), self._flat(parents, "parents", torch.int32, rows),
             self._flat(starts, "starts", torch.int32, self.batch + 1), self._flat(accept, "accept", torch.float32, rows),
             self._flat(sample, "sample", torch.float32, self.batch), *self._outputs, target.stride(0), draft_row, rows, vocabulary,
             self.batch, self.depth, kind, 0)
-        _lib.enqueue(self.function, args, index, "verify_drafts")
         return self.tokens, self.nodes, self.counts

@@ -7,7 +7,7 @@ before `ingest_decode`), or the first `width` elements of longer Index rows that
 scale per row in the same pass (`quantise`)."""
 import math
 
-from . import _lib
+from . import _lib, _launch
 
 LAYOUTS = {"half": 0, "interleaved": 1}
 
@@ -59,9 +59,9 @@ class Rotary:
         pairs, self.factor = frequencies(width, base, scaling)
         self.width, self.layout = width, LAYOUTS[layout]
         self.turns = torch.tensor([f / (2 * math.pi) for f in pairs], dtype=torch.float64, device=self.device)
-        self.index = self.turns.device.index
+        self.index, self._table = self.turns.get_device(), self.turns.data_ptr()
         self.types = {torch.bfloat16: _lib.FLOAT_BF16, torch.float16: _lib.FLOAT_FP16, torch.float32: _lib.FLOAT_FP32}
-        self.function = _lib.load_library().kvip_b200_rotary
+        self.launch = _launch.Launcher("kvip_b200_rotary")
 
     def _rows(self, tensor, tokens, what, kind=None):
         """(pointer, token stride, head stride, heads) of rows [tokens, heads, width] or [tokens, width]."""
@@ -90,7 +90,7 @@ class Rotary:
         query_out = query if query_out is None else query_out
         x0, xt0, xh0, heads0 = self._rows(query, tokens, "query")
         y0, yt0, yh0, out0 = self._rows(query_out, tokens, "query_out", kind)
-        x1 = y1 = None
+        x1 = y1 = 0
         xt1 = xh1 = yt1 = yh1 = heads1 = out1 = 0
         if key is not None:
             key_out = key if key_out is None else key_out
@@ -105,11 +105,9 @@ class Rotary:
                 raise ValueError("Rotary query needs at least one head")
             return query_out, key_out
         if heads1 == 0:
-            x1 = y1 = None
-        args = _lib.RotaryArgs(positions.data_ptr(), self.turns.data_ptr(), x0, x1, y0, y1, None, None, xt0, xt1, xh0, xh1,
-                               yt0, yt1, yh0, yh1, heads0, heads1, tokens, self.width, self.width, self.layout,
-                               self.types[kind], self.factor)
-        _lib.enqueue(self.function, args, self.index, "rotary")
+            x1 = y1 = 0
+        self.launch(self.index, positions.data_ptr(), self._table, x0, x1, y0, y1, 0, 0, xt0, xt1, xh0, xh1, yt0, yt1, yh0, yh1,
+                    heads0, heads1, tokens, self.width, self.width, self.layout, self.types[kind], self.factor)
         return query_out, key_out
 
     def quantise(self, positions, rows, codes=None, scales=None):
@@ -134,8 +132,7 @@ class Rotary:
             raise ValueError("Rotary scales must be contiguous float32 [tokens, heads]")
         if tokens == 0 or heads == 0:
             return codes, scales
-        args = _lib.RotaryArgs(positions.data_ptr(), self.turns.data_ptr(), rows.data_ptr(), None, None, None, codes.data_ptr(),
-                               scales.data_ptr(), rows.stride(0), 0, rows.stride(1), 0, 0, 0, 0, 0, heads, 0, tokens,
-                               self.width, dim, self.layout, self.types[rows.dtype], self.factor)
-        _lib.enqueue(self.function, args, self.index, "rotary.quantise")
+        self.launch(self.index, positions.data_ptr(), self._table, rows.data_ptr(), 0, 0, 0, codes.data_ptr(), scales.data_ptr(),
+                    rows.stride(0), 0, rows.stride(1), 0, 0, 0, 0, 0, heads, 0, tokens, self.width, dim, self.layout,
+                    self.types[rows.dtype], self.factor)
         return codes, scales
