@@ -14,25 +14,16 @@ constexpr uint32_t kMapBatch = 1024;              // requests per launch
 constexpr uint32_t kPerThread = kMapBatch / kMapThreads;
 constexpr uint32_t kTokensPerThread = 4;
 
-struct Request {
-  int32_t length, count, held, fresh;   // count: tokens that are numbered; fresh: new blocks
-  bool placed;                          // false: its tokens get no slot
-};
-
-__global__ void __launch_bounds__(kMapThreads) slot_map_rows(const KvipSlotMapsArgs a) {
-  __shared__ uint32_t s_start[kMapBatch + 1], s_off[kMapBatch];
+__global__ void __launch_bounds__(kMapThreads) slot_map_rows(const __grid_constant__ KvipSlotMapsArgs a) {
+  __shared__ uint32_t s_start[kMapBatch + 1], s_off[kMapBatch], s_fresh[kMapBatch];
   __shared__ int32_t s_length[kMapBatch], s_held[kMapBatch];
   __shared__ uint8_t s_placed[kMapBatch];
-  __shared__ uint32_t scratch[33];
-  const uint32_t tid = threadIdx.x;
-  const int32_t head = a.head[0];
-  const int64_t available = head < 0 ? 0 : static_cast<int64_t>(a.blocks) - head;
-  const int64_t room = static_cast<int64_t>(a.pages) * a.block;
-  int32_t bad = 0;
+  __shared__ uint64_t s_warp[kMapThreads / 32u];
+  __shared__ uint32_t s_taken;
+  const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5;
 
-  // requests tid * kPerThread + i: consecutive per thread, so one block scan of the threads' sums orders them all
+  // requests tid * kPerThread + i: consecutive per thread, so one scan of the threads' sums orders them all
   int32_t length[kPerThread], count[kPerThread], held[kPerThread];
-  uint32_t fresh[kPerThread], tokens_here = 0, fresh_here = 0;
 #pragma unroll
   for (uint32_t i = 0; i < kPerThread; ++i) {
     const uint32_t b = tid * kPerThread + i;
@@ -41,6 +32,12 @@ __global__ void __launch_bounds__(kMapThreads) slot_map_rows(const KvipSlotMapsA
     count[i] = live ? a.counts[b] : 0;
     held[i] = live ? a.held[b] : 0;
   }
+  const int32_t head = a.head[0];
+  const int64_t available = head < 0 ? 0 : static_cast<int64_t>(a.blocks) - head;
+  const int64_t room = static_cast<int64_t>(a.pages) * a.block;   // fits 31 bits
+  int32_t bad = 0;
+  uint32_t fresh[kPerThread];
+  uint64_t sum = 0;                     // tokens in the low half, new blocks in the high one
 #pragma unroll
   for (uint32_t i = 0; i < kPerThread; ++i) {
     fresh[i] = 0;
@@ -50,15 +47,28 @@ __global__ void __launch_bounds__(kMapThreads) slot_map_rows(const KvipSlotMapsA
       bad |= static_cast<int32_t>(KVIP_ERR_TOKEN_RANGE);
       count[i] = 0;
     } else if (count[i] > 0) {
-      const int64_t need = (end + a.block - 1) / a.block;
-      if (need > held[i]) fresh[i] = static_cast<uint32_t>(need - held[i]);
+      const uint32_t need = (static_cast<uint32_t>(end) - 1u) / a.block + 1u;
+      if (need > static_cast<uint32_t>(held[i])) fresh[i] = need - static_cast<uint32_t>(held[i]);
     }
-    tokens_here += static_cast<uint32_t>(count[i]);
-    fresh_here += fresh[i];
+    sum += static_cast<uint32_t>(count[i]) | (static_cast<uint64_t>(fresh[i]) << 32);
   }
-  uint32_t total_tokens = 0;
-  uint32_t start = block_exclusive_scan(tokens_here, scratch, &total_tokens);
-  uint32_t off = block_exclusive_scan(fresh_here, scratch, nullptr);
+  uint64_t scan = sum;
+#pragma unroll
+  for (uint32_t d = 1; d < 32u; d <<= 1) {
+    const uint64_t other = __shfl_up_sync(0xffffffffu, scan, d);
+    if (lane >= d) scan += other;
+  }
+  if (lane == 31u) s_warp[warp] = scan;
+  if (tid == 0) s_taken = 0;
+  __syncthreads();
+  uint64_t before = scan - sum, all = 0;
+#pragma unroll
+  for (uint32_t w = 0; w < kMapThreads / 32u; ++w) {
+    if (w < warp) before += s_warp[w];
+    all += s_warp[w];
+  }
+  uint32_t start = static_cast<uint32_t>(before), off = static_cast<uint32_t>(before >> 32);
+  const uint32_t total_tokens = static_cast<uint32_t>(all);
   // entries used: the requests up to the first one that the list cannot serve
   uint32_t served = 0;
 #pragma unroll
@@ -68,41 +78,46 @@ __global__ void __launch_bounds__(kMapThreads) slot_map_rows(const KvipSlotMapsA
     if (!placed) bad |= static_cast<int32_t>(KVIP_ERR_NO_SLOT);
     else if (fresh[i]) served = off + fresh[i];
     if (b < a.batch) {
-      s_start[b] = start; s_off[b] = off; s_length[b] = length[i]; s_held[b] = held[i];
+      s_start[b] = start; s_off[b] = off; s_fresh[b] = placed ? fresh[i] : 0u; s_length[b] = length[i]; s_held[b] = held[i];
       s_placed[b] = placed ? 1u : 0u;
       if (blockIdx.x == 0) {
         a.starts[b] = static_cast<int32_t>(min(start, a.tokens));
         a.ends[b] = length[i] + (placed ? count[i] : 0);
         a.held_after[b] = held[i] + (placed ? static_cast<int32_t>(fresh[i]) : 0);
       }
-      if (b + 1 == a.batch) s_start[a.batch] = start + static_cast<uint32_t>(count[i]);
     }
     start += static_cast<uint32_t>(count[i]);
     off += fresh[i];
   }
-  if (total_tokens > a.tokens) bad |= static_cast<int32_t>(KVIP_ERR_TOKEN_RANGE);
-  const int any_bad = __syncthreads_or(bad);   // also publishes the shared tables
   if (blockIdx.x == 0) {
-    // max over the block of `served`
-    const uint32_t most = __reduce_max_sync(0xffffffffu, served);
-    if ((tid & 31u) == 0) scratch[tid >> 5] = most;
-    __syncthreads();
-    if (tid == 0) {
-      uint32_t taken = 0;
-      for (uint32_t w = 0; w < kMapThreads / 32u; ++w) taken = max(taken, scratch[w]);
-      a.taken[0] = static_cast<int32_t>(taken);
-      a.starts[a.batch] = static_cast<int32_t>(min(total_tokens, a.tokens));
-    }
-    if (any_bad && bad) atomicOr(a.status, bad);
+    served = __reduce_max_sync(0xffffffffu, served);
+    if (lane == 0 && served) atomicMax(&s_taken, served);
+    if (total_tokens > a.tokens) bad |= static_cast<int32_t>(KVIP_ERR_TOKEN_RANGE);
+    if (bad) atomicOr(a.status, bad);
+  }
+  if (tid == 0) s_start[a.batch] = total_tokens;
+  __syncthreads();
+  if (blockIdx.x == 0 && tid == 0) {
+    a.taken[0] = static_cast<int32_t>(s_taken);
+    a.starts[a.batch] = static_cast<int32_t>(min(total_tokens, a.tokens));
   }
 
-  // the appended entries of the table rows: a warp per request
-  for (uint32_t b = blockIdx.x * (kMapThreads / 32u) + (tid >> 5); b < a.batch; b += gridDim.x * (kMapThreads / 32u)) {
-    if (!s_placed[b]) continue;
-    const int64_t end = static_cast<int64_t>(s_length[b]) + (s_start[b + 1] - s_start[b]);
-    const int32_t need = s_start[b + 1] == s_start[b] ? 0 : static_cast<int32_t>((end + a.block - 1) / a.block);
-    for (int32_t p = s_held[b] + static_cast<int32_t>(tid & 31u); p < need; p += 32)
-      a.table[static_cast<uint64_t>(b) * a.pages + p] = a.free_blocks[head + s_off[b] + (p - s_held[b])];
+  // the appended entries of the table rows: requests in turn over the CTAs, a thread each; long appendages by the whole warp
+  for (uint32_t b0 = 0; b0 < a.batch; b0 += gridDim.x * kMapThreads) {
+    const uint32_t b = b0 + tid * gridDim.x + blockIdx.x;
+    const uint32_t mine = b < a.batch ? s_fresh[b] : 0u;
+    auto append = [&](uint32_t r, uint32_t p) {
+      a.table[static_cast<uint64_t>(r) * a.pages + static_cast<uint32_t>(s_held[r]) + p] = a.free_blocks[static_cast<uint32_t>(head) + s_off[r] + p];
+    };
+    if (mine <= 2u)
+      for (uint32_t p = 0; p < mine; ++p) append(b, p);
+    uint32_t todo = __ballot_sync(0xffffffffu, mine > 2u);
+    while (todo) {
+      const uint32_t from = static_cast<uint32_t>(__ffs(static_cast<int>(todo))) - 1u;
+      const uint32_t r = __shfl_sync(0xffffffffu, b, from), n = __shfl_sync(0xffffffffu, mine, from);
+      todo &= todo - 1u;
+      for (uint32_t p = lane; p < n; p += 32u) append(r, p);
+    }
   }
 
   // packed tokens: four consecutive ones per thread, one search for the first
