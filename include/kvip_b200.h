@@ -688,15 +688,12 @@ typedef struct KvipAttentionArgs {
   const int64_t* ancestors;    /* [tokens], or NULL: every drafted row up to the token's own (a chain) */
   void* out;                   /* [tokens, heads, 512] same type as the query */
   float* lse;                  /* [tokens, heads] */
-  float* partial;              /* [partial_rows, 512] workspace of the shares, or NULL: every token in one piece */
-  float* partial_stats;        /* [partial_rows, 2] */
   int32_t* status;             /* [1] OR-ed KVIP_ERR_* */
   int64_t query_token, query_head;   /* strides of query in elements, multiples of 8 */
   int64_t draft_token;               /* stride of draft in elements, a multiple of 8 */
   uint64_t pool_rows;
   uint32_t tokens, heads, entries, batch, queries, output_stride, dtype;
-  uint32_t splits;             /* shares of a token's rows that are computed apart and joined (splits * tokens * heads <= */
-  uint32_t partial_rows;       /* partial_rows); 0 = by the sizes */
+  uint32_t splits;             /* CTAs that share the rows of a token (1, 2, 4 or 8); 0 = by the sizes */
   uint32_t wait_kilocycles;    /* limit of every barrier wait, in units of 1024 SM clock cycles; 0 = about one second */
   float scale;
   uint32_t reserved0;

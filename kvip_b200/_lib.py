@@ -154,10 +154,10 @@ class RotaryArgs(ctypes.Structure):
 
 
 AttentionArgs = _struct("AttentionArgs", (
-    "query", "pool", "slots", "requests", "row_owners", "starts", "draft", "ancestors", "out", "lse", "partial",
-    "partial_stats", "status"), [(n, i64) for n in ("query_token", "query_head", "draft_token")] + [("pool_rows", u64)] + [
-        (n, u32) for n in ("tokens", "heads", "entries", "batch", "queries", "output_stride", "dtype", "splits", "partial_rows",
-                           "wait_kilocycles")] + [("scale", f32), ("reserved0", u32)])
+    "query", "pool", "slots", "requests", "row_owners", "starts", "draft", "ancestors", "out", "lse", "status"),
+    [(n, i64) for n in ("query_token", "query_head", "draft_token")] + [("pool_rows", u64)] + [(n, u32) for n in (
+        "tokens", "heads", "entries", "batch", "queries", "output_stride", "dtype", "splits", "wait_kilocycles")] + [
+            ("scale", f32), ("reserved0", u32)])
 
 VerifyArgs = _struct("VerifyArgs", (
     "target", "draft", "tokens", "parents", "starts", "accept", "sample", "out_tokens", "out_nodes", "out_counts", "status"),

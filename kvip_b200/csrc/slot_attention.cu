@@ -32,13 +32,17 @@ constexpr uint32_t kPieceBytes = kTile * 128;           // one piece of every ro
 constexpr uint32_t kStageBytes = kPieces * kPieceBytes; // 73,728
 constexpr uint32_t kStages = 2;
 constexpr uint32_t kGroupHeads = 64;
+constexpr uint32_t kAhead = 2;                          // tiles whose list entries a loader holds
 constexpr uint32_t kThirds = 3;                         // a stage is filled, read and released in three groups of pieces
 constexpr uint32_t kThirdBytes = kStageBytes / kThirds;
-// Warps 0-3 and 4-7: softmax of the lower and the upper half of the heads; 8-15: loaders, four per stage; 16, 17: issuers of
-// the first and the second product.
-constexpr uint32_t kFirstLoaderWarp = 8, kLoaderWarps = 4, kScoreWarp = kFirstLoaderWarp + kStages * kLoaderWarps, kValueWarp = kScoreWarp + 1;
-constexpr uint32_t kAttentionThreads = 32 * (kValueWarp + 1);
-constexpr uint32_t kRole = 128;                         // threads of one softmax half
+// Softmax: four warps per 16 heads. Behind them four loaders and an issuer for each product. Tiles are loaded in order: the copy
+// engine takes about ten clocks for 128 bytes of four rows, so one tile at a time keeps it busy.
+constexpr uint32_t kLoaderWarps = 4, kRole = 128, kSideHeads = 16;
+constexpr uint32_t kMaxSplits = 8;                      // CTAs of a cluster
+template <uint32_t kN> struct Warps {
+  static constexpr uint32_t kSides = kN / kSideHeads, kLoader = 4 * kSides, kScore = kLoader + kLoaderWarps, kValue = kScore + 1;
+  static constexpr uint32_t kThreads = 32 * (kValue + 1);
+};
 constexpr uint32_t kOutRow = kValue * 2 + 16;           // bytes of an output row while it is laid out: four banks further than the last
 constexpr float kSlack = 8.f;                           // log2: p may reach 2^8 before the reference moves
 constexpr uint32_t kDefaultWaitKilocycles = 2000000u;   // about one second of SM clock
@@ -121,22 +125,11 @@ __device__ __forceinline__ uint64_t operand(uint32_t address, uint32_t pieces) {
   return static_cast<uint64_t>((address & 0x3ffffu) >> 4) | (static_cast<uint64_t>(pieces >> 4) << 16) |
          (static_cast<uint64_t>(1024u >> 4) << 32) | (1ull << 46) | (2ull << 61);
 }
-// 16 lanes x 8 kBlocks fp32 columns: a thread holds rows lane/4 (v[4j], v[4j + 1]) and lane/4 + 8 (v[4j + 2], v[4j + 3]),
-// columns 8j + 2 (lane%4) + {0, 1}.
-template <uint32_t kBlocks> __device__ __forceinline__ void tmem_ld_scores(uint32_t address, uint32_t* v) {
-  if constexpr (kBlocks == 4) {
-    asm volatile("tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
-                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
-                   "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
-                 : "r"(address) : "memory");
-  } else if constexpr (kBlocks >= 2) {
-    asm volatile("tcgen05.ld.sync.aligned.16x256b.x2.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
-                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]) : "r"(address) : "memory");
-    if constexpr (kBlocks == 3) tmem_ld_scores<1>(address + 16u, v + 8);
-  } else {
-    asm volatile("tcgen05.ld.sync.aligned.16x256b.x1.b32 {%0, %1, %2, %3}, [%4];"
-                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(address) : "memory");
-  }
+// 16 lanes x 16 fp32 columns: a thread holds rows lane/4 (v[4j], v[4j + 1]) and lane/4 + 8 (v[4j + 2], v[4j + 3]), columns
+// 8j + 2 (lane%4) + {0, 1}.
+__device__ __forceinline__ void tmem_ld_blocks(uint32_t address, uint32_t* v) {
+  asm volatile("tcgen05.ld.sync.aligned.16x256b.x2.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]) : "r"(address) : "memory");
 }
 // 32 lanes x 8 fp32 columns: a thread holds its lane's row.
 __device__ __forceinline__ void tmem_ld_rows(uint32_t address, uint32_t* v) {
@@ -168,9 +161,23 @@ __device__ __forceinline__ void load_query(uint32_t to, const CUtensorMap* map, 
 __device__ __forceinline__ void expect_bytes(uint32_t bar, uint32_t bytes) {
   asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
 }
-// Asks L2 for a row that a copy will read soon.
-__device__ __forceinline__ void prefetch_row(const uint8_t* row) {
-  asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(row), "r"(kWidth * 2u) : "memory");
+__device__ __forceinline__ void cluster_barrier() {
+  asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t remote(uint32_t address, uint32_t rank) {
+  uint32_t there;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(address), "r"(rank));
+  return there;
+}
+__device__ __forceinline__ float load_remote(uint32_t address) {
+  float x;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x) : "r"(address) : "memory");
+  return x;
+}
+__device__ __forceinline__ float4 load_remote4(uint32_t address) {
+  float4 x;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(x.x), "=f"(x.y), "=f"(x.z), "=f"(x.w) : "r"(address) : "memory");
+  return x;
 }
 __device__ __forceinline__ bool elect_one() {
   uint32_t leader;
@@ -197,6 +204,7 @@ __device__ __forceinline__ Rows rows_of(const KvipAttentionArgs& a, uint32_t t) 
     return r;
   }
   const int32_t owner = a.row_owners ? a.row_owners[request] : request;
+  const int64_t first = a.draft ? a.starts[request] : 0, behind = a.draft ? a.starts[request + 1] : 0;
   const uint64_t base = static_cast<uint64_t>(static_cast<uint32_t>(owner)) * a.output_stride;
   if (owner < 0 || base + a.output_stride > a.pool_rows) {
     r.limit = 0;
@@ -205,7 +213,7 @@ __device__ __forceinline__ Rows rows_of(const KvipAttentionArgs& a, uint32_t t) 
     r.base = static_cast<uint32_t>(base);
   }
   if (a.draft) {
-    const int64_t first = a.starts[request], behind = a.starts[request + 1], own = static_cast<int64_t>(t) - first;
+    const int64_t own = static_cast<int64_t>(t) - first;
     if (first < 0 || behind < first || behind > static_cast<int64_t>(a.tokens)) {
       r.bad |= static_cast<int32_t>(KVIP_ERR_TOKEN_RANGE);
     } else {
@@ -220,10 +228,11 @@ __device__ __forceinline__ Rows rows_of(const KvipAttentionArgs& a, uint32_t t) 
 }
 
 template <typename T, uint32_t kN>
-__global__ void __launch_bounds__(kAttentionThreads, 1)
+__global__ void __launch_bounds__(Warps<kN>::kThreads, 1)
 attend_tiles(const __grid_constant__ CUtensorMap query_map, const __grid_constant__ CUtensorMap pool_map,
              const __grid_constant__ CUtensorMap draft_map, const __grid_constant__ KvipAttentionArgs a, const uint32_t groups,
              const uint32_t group_heads, const uint32_t splits) {
+  constexpr uint32_t kSides = Warps<kN>::kSides, kFirstLoaderWarp = Warps<kN>::kLoader, kScoreWarp = Warps<kN>::kScore, kValueWarp = Warps<kN>::kValue;
   extern __shared__ __align__(1024) uint8_t smem[];
   const uint32_t base = smem_u32(smem);
   Control& c = *reinterpret_cast<Control*>(smem + Layout<kN>::kControl);
@@ -236,10 +245,12 @@ attend_tiles(const __grid_constant__ CUtensorMap query_map, const __grid_constan
   uint32_t last = 0;
   if (warp == kScoreWarp) {
     if (lane == 0) {
+      for (const CUtensorMap* map : {&query_map, &pool_map, &draft_map})
+        asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");
       for (uint32_t s = 0; s < kStages; ++s)
         for (uint32_t third = 0; third < kThirds; ++third) { mbar_init(bar(c.full[s][third]), kLoaderWarps); mbar_init(bar(c.empty[s][third]), 1); }
-      for (uint32_t s = 0; s < 2; ++s) { mbar_init(bar(c.scored[s]), 1); mbar_init(bar(c.taken[s]), 2 * kRole / 32); }
-      mbar_init(bar(c.weighted), 2 * kRole / 32); mbar_init(bar(c.query_full), 1);
+      for (uint32_t s = 0; s < 2; ++s) { mbar_init(bar(c.scored[s]), 1); mbar_init(bar(c.taken[s]), 4 * kSides); }
+      mbar_init(bar(c.weighted), 4 * kSides); mbar_init(bar(c.query_full), 1);
       c.abort_flag = 0;
       c.last = 0;
       asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -251,10 +262,6 @@ attend_tiles(const __grid_constant__ CUtensorMap query_map, const __grid_constan
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   } else if (warp == kValueWarp) {
     if (lane == 0) c.rows = rows_of(a, t);         // a chain of loads, beside the others' walk along the list
-    if (lane < 3) {
-      const CUtensorMap* map = lane == 0 ? &query_map : lane == 1 ? &pool_map : &draft_map;
-      asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");
-    }
   } else if (vectors) {
     // lists end in -1 where a context is short: the last entry in use bounds the tiles
     for (uint32_t k = tid; k < a.entries / 4u; k += 32u * kScoreWarp) {
@@ -287,8 +294,8 @@ attend_tiles(const __grid_constant__ CUtensorMap query_map, const __grid_constan
   auto none = [&](uint32_t s) { return (c.valid[s][0] | c.valid[s][1] | c.valid[s][2] | c.valid[s][3]) == 0u; };
 
   if (warp >= kFirstLoaderWarp && warp < kScoreWarp) {
-    // ================= loaders: warp 8 + 2 i + g gathers 16 rows, from 16 i on, of the tiles g, g + 2, ... =================
-    const uint32_t g = (warp - kFirstLoaderWarp) & 1u, quarter = (warp - kFirstLoaderWarp) >> 1;
+    // ================= loaders: warp 8 + i gathers 16 rows, from 16 i on, of every tile =================
+    const uint32_t quarter = warp - kFirstLoaderWarp;
     const bool leader = elect_one();
     int32_t bad = warp == kFirstLoaderWarp ? rows.bad : 0;
     if (count) {
@@ -307,22 +314,15 @@ attend_tiles(const __grid_constant__ CUtensorMap query_map, const __grid_constan
         }
         return e;
       };
-      // Rows are asked for two of this stage's tiles before they are copied: a copy from HBM takes twice as long as one from
-      // L2, and the two stages alone do not keep enough of them in flight.
-      auto ahead = [&](const int4& e) {
-        if ((lane >> 2) != quarter) return;        // 16 rows a warp
-        auto ask = [&](int32_t slot) {
-          if (slot >= 0 && static_cast<uint32_t>(slot) < rows.limit)
-            prefetch_row(static_cast<const uint8_t*>(a.pool) + static_cast<uint64_t>(rows.base + static_cast<uint32_t>(slot)) * (kWidth * 2u));
-        };
-        ask(e.x); ask(e.y); ask(e.z); ask(e.w);
-      };
-      int4 next = entries_of(g), later = entries_of(g + kStages);
-      for (uint32_t n = g; n < count; n += kStages) {
-        int4 e = next;
-        next = later;
-        later = entries_of(n + 2u * kStages);      // lands while this tile is fetched
-        ahead(next);
+      int4 queue[kAhead];                          // entries of the tiles n + 1 .. n + kAhead
+#pragma unroll
+      for (uint32_t k = 0; k < kAhead; ++k) queue[k] = entries_of(k);
+      for (uint32_t n = 0; n < count; ++n) {
+        const uint32_t g = n & 1u;
+        int4 e = queue[0];
+#pragma unroll
+        for (uint32_t k = 0; k + 1 < kAhead; ++k) queue[k] = queue[k + 1];
+        queue[kAhead - 1] = entries_of(n + kAhead);   // lands while tiles are fetched
         const bool from_list = first + n < list_tiles;
         bool v0, v1, v2, v3;
         if (from_list) {
@@ -441,9 +441,9 @@ attend_tiles(const __grid_constant__ CUtensorMap query_map, const __grid_constan
       }
     }
   } else {
-    // ================= softmax: rows 16 w + lane / 4 and + 8 of every tile, half of the heads =================
-    constexpr uint32_t kBlocks = kN / 16;    // blocks of eight heads per half; a thread holds two of each
-    const uint32_t side = warp >> 2, w = warp & 3u, head_at = side * (kN / 2u);
+    // ================= softmax: rows 16 w + lane / 4 and + 8 of every tile, 16 heads =================
+    constexpr uint32_t kBlocks = 2;          // blocks of eight heads; a thread holds two heads of each, for two rows
+    const uint32_t side = warp >> 2, w = warp & 3u, head_at = side * kSideHeads;
     float ref[2 * kBlocks], sum[2 * kBlocks];
 #pragma unroll
     for (uint32_t j = 0; j < 2 * kBlocks; ++j) { ref[j] = -INFINITY; sum[j] = 0.f; }
@@ -470,13 +470,13 @@ attend_tiles(const __grid_constant__ CUtensorMap query_map, const __grid_constan
       uint32_t v[4 * kBlocks];
       if (ok) {
         fence_after();
-        tmem_ld_scores<kBlocks>(tmem + quad + kScores + s * kN + head_at, v);
+        tmem_ld_blocks(tmem + quad + kScores + s * kN + head_at, v);
         tmem_ld_done();
         fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(bar(c.taken[s]));
       }
-      // scores in units of log2; one more than 2^8 above its reference makes the whole half take the maximum
+      // scores in units of log2; one more than 2^8 above its reference makes the whole side take the maximum
       float x[4 * kBlocks];
       bool above = false;
 #pragma unroll
@@ -514,7 +514,7 @@ attend_tiles(const __grid_constant__ CUtensorMap query_map, const __grid_constan
             fence_after();
             for (uint32_t m = 0; m < 4; ++m) {
 #pragma unroll
-              for (uint32_t h = head_at; h < head_at + kN / 2u; h += 8) {
+              for (uint32_t h = head_at; h < head_at + kSideHeads; h += 8) {
                 uint32_t o[8];
                 tmem_ld_rows(tmem + quad + kOut + m * kN + h, o);
                 tmem_ld_done();
@@ -570,89 +570,115 @@ attend_tiles(const __grid_constant__ CUtensorMap query_map, const __grid_constan
         if (w == 0) c.top[h] = ref[j];
       }
     }
-    if (!role_any<2 * kRole>(3u, dead) && rows.request >= 0) {
-      const uint64_t out_row = static_cast<uint64_t>(t) * a.heads + head0;
-      const uint64_t part_row = (static_cast<uint64_t>(split) * a.tokens + t) * a.heads + head0;
-      if (tid < heads) {
-        const float total = (c.reduce[0][tid] + c.reduce[1][tid]) + (c.reduce[2][tid] + c.reduce[3][tid]);
-        if (splits == 1) {
-          a.lse[out_row + tid] = written ? (c.top[tid] + log2f(total)) * 0.6931471805599453f : -INFINITY;
-          c.factor[tid] = written ? 1.f / total : 0.f;
-        } else {
-          reinterpret_cast<float2*>(a.partial_stats)[part_row + tid] = make_float2(written ? c.top[tid] : -INFINITY, total);
-        }
-      }
-      fence_after();
-      // The output is laid out in the stages (all products have read them) and leaves by copies of whole rows. Accumulators have
-      // value elements as rows and heads as columns: 8 x 8 blocks are transposed on their way into shared memory. A share that
-      // will be joined leaves as it is, in fp32 and undivided.
-      if (splits == 1) {
-        role_any<2 * kRole>(3u, false);
-        float f[4 * kBlocks];                // heads 8 j + 2 (lane % 4) + {0, 1}, all of them
-#pragma unroll
-        for (uint32_t j = 0; j < 2 * kBlocks; ++j) {
-          const float2 pair = *reinterpret_cast<const float2*>(&c.factor[8u * j + 2u * (lane & 3u)]);
-          f[2 * j] = pair.x;
-          f[2 * j + 1] = pair.y;
-        }
+    if (!written && w == 0 && lane < 4)
+      for (uint32_t j = 0; j < 2 * kBlocks; ++j) c.top[head_at + (j >> 1) * 8u + lane * 2u + (j & 1u)] = -INFINITY;
+    dead = role_any<kSides * kRole>(kSides + 1u, dead);
+    if (dead || rows.request < 0) {
+      written = false;                       // a share that cannot be trusted counts as empty; the status says so
+      if (tid < kN) c.top[tid] = -INFINITY;
+    }
+    fence_after();
+    if (tid < heads) {
+      const float total = (c.reduce[0][tid] + c.reduce[1][tid]) + (c.reduce[2][tid] + c.reduce[3][tid]);
+      if (splits > 1) c.factor[tid] = total;
+      else c.factor[tid] = written ? 1.f / total : 0.f;
+      if (splits == 1 && rows.request >= 0 && !dead)
+        a.lse[static_cast<uint64_t>(t) * a.heads + head0 + tid] = written ? (c.top[tid] + log2f(total)) * 0.6931471805599453f : -INFINITY;
+    }
+    // The output is laid out in the stages (all products have read them). Accumulators have value elements as rows and heads as
+    // columns: 8 x 8 blocks are transposed on their way into shared memory, and whole rows leave by copies. A share that
+    // will be joined stays here as it is, in fp32 and undivided.
+    if (splits == 1) {
+      role_any<kSides * kRole>(kSides + 1u, false);
+      if (rows.request >= 0 && !dead) {
         // addresses of stored rows: lanes 0-7 give the heads of a block for value elements 0-7, 8-15 for 8-15, 16-31 the next block's
         const uint32_t store = base + ((lane & 7u) + (lane >> 4) * 8u) * kOutRow + ((lane >> 3) & 1u) * 16u;
-#pragma unroll
-        for (uint32_t m = 0; m < 2; ++m) {
-          const uint32_t block = 2u * side + m;
+        for (uint32_t block = side; block < 4u; block += kSides) {
 #pragma unroll
           for (uint32_t half = 0; half < 2; ++half) {
-            uint32_t o[8 * kBlocks];
+            uint32_t o[kN / 2];
             if (written) {
-              tmem_ld_scores<kBlocks>(tmem + quad + (half << 20) + kOut + block * kN, o);
-              tmem_ld_scores<kBlocks>(tmem + quad + (half << 20) + kOut + block * kN + 8u * kBlocks, o + 4 * kBlocks);
+#pragma unroll
+              for (uint32_t h = 0; h < kN; h += 16) tmem_ld_blocks(tmem + quad + (half << 20) + kOut + block * kN + h, o + h / 2);
               tmem_ld_done();
             }
             const uint32_t element = block * 128u + w * 32u + half * 16u;
 #pragma unroll
-            for (uint32_t j = 0; j < 2 * kBlocks; j += 2) {
+            for (uint32_t j = 0; j < kN / 8u; j += 2) {
               uint32_t q[4];
 #pragma unroll
               for (uint32_t i = 0; i < 2; ++i) {
                 const uint32_t* e = o + 4 * (j + i);
-                const float fx = f[2 * (j + i)], fy = f[2 * (j + i) + 1];
-                q[2 * i] = written ? pack_pair<T>(__uint_as_float(e[0]) * fx, __uint_as_float(e[1]) * fy) : 0u;
-                q[2 * i + 1] = written ? pack_pair<T>(__uint_as_float(e[2]) * fx, __uint_as_float(e[3]) * fy) : 0u;
+                const float2 f = *reinterpret_cast<const float2*>(&c.factor[8u * (j + i) + 2u * (lane & 3u)]);
+                q[2 * i] = written ? pack_pair<T>(__uint_as_float(e[0]) * f.x, __uint_as_float(e[1]) * f.y) : 0u;
+                q[2 * i + 1] = written ? pack_pair<T>(__uint_as_float(e[2]) * f.x, __uint_as_float(e[3]) * f.y) : 0u;
               }
               asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};"
                            ::"r"(store + j * 8u * kOutRow + element * 2u), "r"(q[0]), "r"(q[1]), "r"(q[2]), "r"(q[3]) : "memory");
             }
           }
         }
-        fence_async();
-        role_any<2 * kRole>(3u, false);
-        if (tid < heads)
-          asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;"
-                       ::"l"(static_cast<T*>(a.out) + (out_row + tid) * kValue), "r"(base + tid * kOutRow), "r"(kValue * 2u) : "memory");
-      } else if (written) {                  // an empty share says so in its statistics, its rows are not read
-#pragma unroll
-        for (uint32_t m = 0; m < 2; ++m) {
-          const uint32_t block = 2u * side + m, element = block * 128u + w * 32u + lane;
-#pragma unroll
-          for (uint32_t h0 = 0; h0 < kN; h0 += 16) {
-            uint32_t o[16];
-            tmem_ld_rows(tmem + quad + kOut + block * kN + h0, o);
-            tmem_ld_rows(tmem + quad + kOut + block * kN + h0 + 8u, o + 8);
-            tmem_ld_done();
-#pragma unroll
-            for (uint32_t i = 0; i < 16; ++i) reinterpret_cast<float*>(smem)[(h0 + i) * kValue + element] = __uint_as_float(o[i]);
-          }
-        }
-        fence_async();
-        role_any<2 * kRole>(3u, false);
-        if (tid == 0)
-          asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;"
-                       ::"l"(a.partial + part_row * kValue), "r"(base), "r"(heads * kValue * 4u) : "memory");
       }
-      asm volatile("cp.async.bulk.commit_group;" ::: "memory");
-      asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
-      fence_before();
+      fence_async();
+      role_any<kSides * kRole>(kSides + 1u, false);
+      if (tid < heads && rows.request >= 0 && !dead) {
+        asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;"
+                     ::"l"(static_cast<T*>(a.out) + (static_cast<uint64_t>(t) * a.heads + head0 + tid) * kValue), "r"(base + tid * kOutRow), "r"(kValue * 2u)
+                     : "memory");
+        asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+        asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+      }
+    } else if (written) {
+      for (uint32_t block = side; block < 4u; block += kSides) {
+        const uint32_t element = block * 128u + w * 32u + lane;
+#pragma unroll
+        for (uint32_t h0 = 0; h0 < kN; h0 += 16) {
+          uint32_t o[16];
+          tmem_ld_rows(tmem + quad + kOut + block * kN + h0, o);
+          tmem_ld_rows(tmem + quad + kOut + block * kN + h0 + 8u, o + 8);
+          tmem_ld_done();
+#pragma unroll
+          for (uint32_t i = 0; i < 16; ++i) reinterpret_cast<float*>(smem)[(h0 + i) * kValue + element] = __uint_as_float(o[i]);
+        }
+      }
     }
+    fence_before();
+  }
+
+  // ---- shares of one unit, a CTA each: every CTA joins the heads rank, rank + splits, .. out of all of them -------------
+  //   out = sum_s w_s o_s / sum_s w_s l_s, w_s = 2^(reference of share s - the largest)
+  if (splits > 1) {
+    cluster_barrier();
+    if (rows.request >= 0) {
+      for (uint32_t item = warp; ; item += Warps<kN>::kThreads / 32u) {   // half a row per warp
+        const uint32_t h = split + (item >> 1) * splits, element = (item & 1u) * 256u + lane * 4u;
+        if (h >= heads) break;
+        float tops[kMaxSplits], top = -INFINITY;
+#pragma unroll
+        for (uint32_t s = 0; s < kMaxSplits; ++s) {
+          tops[s] = s < splits ? load_remote(remote(smem_u32(&c.top[h]), s)) : -INFINITY;
+          top = fmaxf(top, tops[s]);
+        }
+        float total = 0.f, y[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (uint32_t s = 0; s < kMaxSplits; ++s) {
+          if (tops[s] == -INFINITY) continue;                             // an empty share has written nothing
+          const float weight = exp2_fast(tops[s] - top);
+          total = fmaf(weight, load_remote(remote(smem_u32(&c.factor[h]), s)), total);
+          const uint32_t from = remote(base + (h * kValue + element) * 4u, s);
+          const float4 low = load_remote4(from), high = load_remote4(from + 512u);
+          y[0] = fmaf(weight, low.x, y[0]); y[1] = fmaf(weight, low.y, y[1]); y[2] = fmaf(weight, low.z, y[2]); y[3] = fmaf(weight, low.w, y[3]);
+          y[4] = fmaf(weight, high.x, y[4]); y[5] = fmaf(weight, high.y, y[5]); y[6] = fmaf(weight, high.z, y[6]); y[7] = fmaf(weight, high.w, y[7]);
+        }
+        const float inverse = top == -INFINITY ? 0.f : 1.f / total;
+        const uint64_t row = static_cast<uint64_t>(t) * a.heads + head0 + h;
+        T* out = static_cast<T*>(a.out) + row * kValue + element;
+        *reinterpret_cast<uint2*>(out) = make_uint2(pack_pair<T>(y[0] * inverse, y[1] * inverse), pack_pair<T>(y[2] * inverse, y[3] * inverse));
+        *reinterpret_cast<uint2*>(out + 128) = make_uint2(pack_pair<T>(y[4] * inverse, y[5] * inverse), pack_pair<T>(y[6] * inverse, y[7] * inverse));
+        if (!(item & 1u) && lane == 0) a.lse[row] = top == -INFINITY ? -INFINITY : (top + log2f(total)) * 0.6931471805599453f;
+      }
+    }
+    cluster_barrier();                       // nobody leaves while its share is being read
   }
 
   // ---- teardown ----------------------------------------------------------------------------
@@ -666,33 +692,6 @@ attend_tiles(const __grid_constant__ CUtensorMap query_map, const __grid_constan
     fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
   }
-}
-
-// Joins the shares of one (token, head): out = sum_s w_s o_s / sum_s w_s l_s, w_s = 2^(reference of the share - the largest).
-template <typename T>
-__global__ void __launch_bounds__(128) join_shares(const __grid_constant__ KvipAttentionArgs a, const uint32_t splits) {
-  const uint32_t row = blockIdx.x, t = row / a.heads;
-  if (a.requests && a.requests[t] < 0) return;
-  const uint64_t rows = static_cast<uint64_t>(a.tokens) * a.heads;
-  const float2* stats = reinterpret_cast<const float2*>(a.partial_stats) + row;
-  float top = -INFINITY;
-  for (uint32_t s = 0; s < splits; ++s) top = fmaxf(top, stats[s * rows].x);
-  float total = 0.f;
-  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-  for (uint32_t s = 0; s < splits; ++s) {
-    const float2 stat = stats[s * rows];
-    const bool used = stat.x != -INFINITY;
-    const float weight = used ? exp2_fast(stat.x - top) : 0.f;
-    const float4 o = used ? reinterpret_cast<const float4*>(a.partial + (s * rows + row) * kValue)[threadIdx.x] : make_float4(0.f, 0.f, 0.f, 0.f);
-    total = fmaf(weight, used ? stat.y : 0.f, total);
-    acc.x = fmaf(weight, o.x, acc.x); acc.y = fmaf(weight, o.y, acc.y);
-    acc.z = fmaf(weight, o.z, acc.z); acc.w = fmaf(weight, o.w, acc.w);
-  }
-  const float inverse = total == 0.f ? 0.f : 1.f / total;
-  uint2 packed = make_uint2(pack_pair<T>(acc.x * inverse, acc.y * inverse), pack_pair<T>(acc.z * inverse, acc.w * inverse));
-  reinterpret_cast<uint2*>(static_cast<T*>(a.out) + static_cast<uint64_t>(row) * kValue)[threadIdx.x] = packed;
-  if (threadIdx.x == 0) a.lse[row] = total == 0.f ? -INFINITY : (top + log2f(total)) * 0.6931471805599453f;
 }
 
 typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
@@ -738,38 +737,56 @@ uint32_t launch_tiles(const KvipAttentionArgs& a, KernelSlot slot, uint32_t grou
     set_error("slot_attention: the strides do not fit a tensor map");
     return KVIP_BAD_ARGUMENT;
   }
-  attend_tiles<T, kN><<<a.tokens * groups * splits, kAttentionThreads, Layout<kN>::kBytes, stream>>>(query_map, pool_map, draft_map, a, groups,
-                                                                                                     group_heads, splits);
+  cudaLaunchConfig_t config{};
+  config.gridDim = dim3(a.tokens * groups * splits);
+  config.blockDim = dim3(Warps<kN>::kThreads);
+  config.dynamicSmemBytes = Layout<kN>::kBytes;
+  config.stream = stream;
+  cudaLaunchAttribute cluster{};
+  cluster.id = cudaLaunchAttributeClusterDimension;
+  cluster.val.clusterDim.x = splits;
+  cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
+  config.attrs = &cluster;
+  config.numAttrs = 1;
+  cudaLaunchKernelEx(&config, attend_tiles<T, kN>, query_map, pool_map, draft_map, a, groups, group_heads, splits);
   count_launch();
   return check_launch("attend_tiles");
 }
 
+// How a call is cut: heads per CTA (all up to 64, or fewer, which read the rows more often) and CTAs that share the rows of a
+// token. Few tokens are cut finely, because the SMs would stand idle; each cut costs the rows' copies once more or the joining of the
+// shares. Counted in clocks, from measurements on full lists (below): a tile takes kTileClocks, and a CTA what it spends
+// before its first and behind its last tile.
+struct Cut { uint32_t groups, group_heads, splits; };
+Cut cut_of(const KvipAttentionArgs& a) {
+  const uint32_t tiles = (a.entries + kTile - 1) / kTile + (a.draft ? 1u : 0u), sms = device_sm_count();
+  Cut best{};
+  uint64_t least = ~0ull;
+  for (uint32_t width = 64; width >= 16; width /= 2) {
+    const uint32_t groups = (a.heads + width - 1) / width, group_heads = (a.heads + groups - 1) / groups;
+    const uint64_t units = static_cast<uint64_t>(a.tokens) * groups;
+    for (uint32_t splits = 1; splits <= kMaxSplits; splits *= 2) {
+      if (a.splits && a.splits != splits) continue;
+      if (!a.splits && splits > tiles) break;
+      const uint64_t resident = (splits <= 2u ? sms : sms * 7u / 8u) / splits;      // clusters at once: they stay within a part of the GPU
+      const uint64_t waves = (units + resident - 1) / resident;
+      const uint64_t clocks = waves * (static_cast<uint64_t>((tiles + splits - 1) / splits) * (2900u + 12u * group_heads) + 11000u +
+                                       (splits > 1 ? 2000u + 60u * group_heads : 30u * group_heads));
+      if (clocks < least) { least = clocks; best = {groups, group_heads, splits}; }
+    }
+  }
+  return best;
+}
+
 template <typename T>
 uint32_t launch_attention(const KvipAttentionArgs& a, uint32_t first_slot, cudaStream_t stream) {
-  const uint32_t groups = (a.heads + kGroupHeads - 1) / kGroupHeads, group_heads = (a.heads + groups - 1) / groups;
-  const uint64_t units = static_cast<uint64_t>(a.tokens) * groups;
-  uint32_t splits = a.splits;
-  if (!splits) {
-    // few tokens: shares of at least two tiles, as many as the SMs take at once
-    const uint32_t tiles = (a.entries + (a.draft ? 64u : 0u) + kTile - 1) / kTile, sms = device_sm_count();
-    splits = units < sms ? static_cast<uint32_t>(sms / units) : 1u;
-    if (splits > tiles / 2u) splits = tiles / 2u;
-    if (!a.partial || !a.partial_stats) splits = 1;
-    const uint64_t room = a.partial_rows / (static_cast<uint64_t>(a.tokens) * a.heads);
-    if (splits > room) splits = static_cast<uint32_t>(room);
-    if (splits < 1) splits = 1;
-  }
-  if (units * splits > 0x7fffffffull) { set_error("slot_attention: too many tokens in one call"); return KVIP_BAD_ARGUMENT; }
-  uint32_t bad;
-  const KernelSlot slot = static_cast<KernelSlot>(first_slot + (group_heads + 15u) / 16u - 1u);
-  if (group_heads <= 16) bad = launch_tiles<T, 16>(a, slot, groups, group_heads, splits, stream);
-  else if (group_heads <= 32) bad = launch_tiles<T, 32>(a, slot, groups, group_heads, splits, stream);
-  else if (group_heads <= 48) bad = launch_tiles<T, 48>(a, slot, groups, group_heads, splits, stream);
-  else bad = launch_tiles<T, 64>(a, slot, groups, group_heads, splits, stream);
-  if (bad || splits == 1) return bad;
-  join_shares<T><<<a.tokens * a.heads, 128, 0, stream>>>(a, splits);
-  count_launch();
-  return check_launch("join_shares");
+  const Cut cut = cut_of(a);
+  if (static_cast<uint64_t>(a.tokens) * cut.groups * cut.splits > 0x7fffffffull) { set_error("slot_attention: too many tokens in one call"); return KVIP_BAD_ARGUMENT; }
+  const KernelSlot slot = static_cast<KernelSlot>(first_slot + (cut.group_heads + 15u) / 16u - 1u);
+  if (cut.group_heads <= 16) return launch_tiles<T, 16>(a, slot, cut.groups, cut.group_heads, cut.splits, stream);
+  if (cut.group_heads <= 32) return launch_tiles<T, 32>(a, slot, cut.groups, cut.group_heads, cut.splits, stream);
+  if (cut.group_heads <= 48) return launch_tiles<T, 48>(a, slot, cut.groups, cut.group_heads, cut.splits, stream);
+  return launch_tiles<T, 64>(a, slot, cut.groups, cut.group_heads, cut.splits, stream);
 }
 
 }  // namespace
@@ -785,11 +802,9 @@ extern "C" uint32_t kvip_b200_slot_attention(const KvipAttentionArgs* a, void* s
   KVIP_REQUIRE(!a->draft || a->starts, "slot_attention: drafted rows need the requests' starts");
   KVIP_REQUIRE(a->dtype <= KVIP_FLOAT_FP16, "slot_attention: bf16 or fp16");
   KVIP_REQUIRE(((reinterpret_cast<uintptr_t>(a->query) | reinterpret_cast<uintptr_t>(a->pool) | reinterpret_cast<uintptr_t>(a->out) |
-                 reinterpret_cast<uintptr_t>(a->draft) | reinterpret_cast<uintptr_t>(a->partial)) & 15u) == 0 && ((a->query_token | a->query_head | a->draft_token) & 7) == 0,
+                 reinterpret_cast<uintptr_t>(a->draft)) & 15u) == 0 && ((a->query_token | a->query_head | a->draft_token) & 7) == 0,
                "slot_attention: 16-byte aligned rows");
-  KVIP_REQUIRE(a->splits <= 1 || (a->partial && a->partial_stats &&
-                                  static_cast<uint64_t>(a->splits) * a->tokens * a->heads <= a->partial_rows),
-               "slot_attention: the workspace does not hold the shares");
+  KVIP_REQUIRE(a->splits <= kMaxSplits && (a->splits & (a->splits - 1u)) == 0, "slot_attention: 0, 1, 2, 4 or 8 shares");
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   return a->dtype == KVIP_FLOAT_BF16 ? launch_attention<__nv_bfloat16>(*a, kSlotAttentionBf16, s) : launch_attention<__half>(*a, kSlotAttentionFp16, s);
 }

@@ -23,8 +23,8 @@ class SlotAttention:
     -inf; a token with a negative request is padding and its outputs are left as they are. `status` collects KVIP_ERR_*
     bits of slots or requests out of range, which are skipped.
 
-    Workspace and default outputs belong to this object: calls of one object, and graphs captured from it, must follow
-    one another. Two streams need two objects."""
+    There is no workspace; the outputs belong to this object unless the call gives its own, so calls without `out` and `lse`,
+    and graphs captured from them, must follow one another."""
 
     def __init__(self, torch, device, *, tokens, heads, entries=_lib.TOPK, dtype=None):
         self.torch = torch
@@ -41,17 +41,12 @@ class SlotAttention:
         self.lse = torch.full((tokens, heads), float("-inf"), dtype=torch.float32, device=device)
         self.status = torch.zeros(1, dtype=torch.int32, device=device)
         self.device, self.index = self.out.device, self.out.get_device()
-        # shares of tokens that do not fill the GPU by themselves: at most one block of 64 heads per SM
-        sms = torch.cuda.get_device_properties(self.device).multi_processor_count
-        self.partial_rows = sms * min(heads, 64)
-        self.partial = torch.empty((self.partial_rows, _lib.ATTENTION_VALUE), dtype=torch.float32, device=device)
-        self.partial_stats = torch.empty((self.partial_rows, 2), dtype=torch.float32, device=device)
-        self._fixed = (self.partial.data_ptr(), self.partial_stats.data_ptr(), self.status.data_ptr())
+        self._status = self.status.data_ptr()
         self.launch = _launch.Launcher("kvip_b200_slot_attention")
 
     @property
     def nbytes(self):
-        return sum(t.numel() * t.element_size() for t in (self.out, self.lse, self.status, self.partial, self.partial_stats))
+        return sum(t.numel() * t.element_size() for t in (self.out, self.lse, self.status))
 
     def _flat(self, tensor, name, dtype, count):
         if tensor.dtype != dtype or tensor.numel() != count or tensor.get_device() != self.index or not tensor.is_contiguous():
@@ -121,7 +116,7 @@ class SlotAttention:
             lse_ptr = self._flat(lse, "lse", torch.float32, tokens * heads)
         self.launch(
             index, query.data_ptr(), pool.data_ptr(), slots.data_ptr(), requests_ptr, owners_ptr, starts_ptr, draft_ptr, ancestors_ptr,
-            out_ptr, lse_ptr, *self._fixed, query.stride(0), query.stride(1), draft_token, rows, tokens, heads, entries, batch,
-            queries, output_stride, _lib.FLOAT_BF16 if self.dtype == torch.bfloat16 else _lib.FLOAT_FP16, splits, self.partial_rows,
+            out_ptr, lse_ptr, self._status, query.stride(0), query.stride(1), draft_token, rows, tokens, heads, entries, batch,
+            queries, output_stride, _lib.FLOAT_BF16 if self.dtype == torch.bfloat16 else _lib.FLOAT_FP16, splits,
             wait_kilocycles, scale, 0)
         return out, lse
