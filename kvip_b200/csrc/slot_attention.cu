@@ -17,6 +17,7 @@
 //
 // p is rounded to the rows' type for the second product (half a step, as the output is); its sum is taken before the
 // rounding, in fp32, because the log-sum is an output too.
+#include <atomic>
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -33,8 +34,9 @@ constexpr uint32_t kStageBytes = kPieces * kPieceBytes; // 73,728
 constexpr uint32_t kStages = 2;
 constexpr uint32_t kGroupHeads = 64;
 constexpr uint32_t kAhead = 2;                          // tiles whose list entries a loader holds
-constexpr uint32_t kThirds = 3;                         // a stage is filled, read and released in three groups of pieces
-constexpr uint32_t kThirdBytes = kStageBytes / kThirds;
+constexpr uint32_t kParts = 4;                          // a stage is filled, read and released in four groups of pieces: two for each block
+                                                        // of 128 value elements, and with the last the piece behind the value
+__host__ __device__ constexpr uint32_t part_end(uint32_t part) { return part + 1 == kParts ? kPieces : 2 * part + 2; }
 // Softmax: four warps per 16 heads. Behind them four loaders and an issuer for each product. Tiles are loaded in order: the copy
 // engine takes about ten clocks for 128 bytes of four rows, so one tile at a time keeps it busy.
 constexpr uint32_t kLoaderWarps = 4, kRole = 128, kSideHeads = 16;
@@ -55,7 +57,7 @@ struct Rows {
   int32_t bad, request;
 };
 struct Control {                                        // behind the tiles in shared memory
-  uint64_t full[kStages][kThirds], empty[kStages][kThirds], scored[2], taken[2], weighted, query_full;
+  uint64_t full[kStages][kParts], empty[kStages][kParts], scored[2], taken[2], weighted, query_full;
   uint32_t valid[kStages][4];                           // row 4 l + c of the tile is there: bit l of word c
   float reduce[4][kGroupHeads];
   float factor[kGroupHeads], top[kGroupHeads];
@@ -248,7 +250,7 @@ attend_tiles(const __grid_constant__ CUtensorMap query_map, const __grid_constan
       for (const CUtensorMap* map : {&query_map, &pool_map, &draft_map})
         asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");
       for (uint32_t s = 0; s < kStages; ++s)
-        for (uint32_t third = 0; third < kThirds; ++third) { mbar_init(bar(c.full[s][third]), kLoaderWarps); mbar_init(bar(c.empty[s][third]), 1); }
+        for (uint32_t part = 0; part < kParts; ++part) { mbar_init(bar(c.full[s][part]), kLoaderWarps); mbar_init(bar(c.empty[s][part]), 1); }
       for (uint32_t s = 0; s < 2; ++s) { mbar_init(bar(c.scored[s]), 1); mbar_init(bar(c.taken[s]), 4 * kSides); }
       mbar_init(bar(c.weighted), 4 * kSides); mbar_init(bar(c.query_full), 1);
       c.abort_flag = 0;
@@ -359,22 +361,22 @@ attend_tiles(const __grid_constant__ CUtensorMap query_map, const __grid_constan
         const CUtensorMap* map = from_list ? &pool_map : &draft_map;
         bool alive = true;
 #pragma unroll
-        for (uint32_t third = 0; third < kThirds; ++third) {
-          alive = __all_sync(0xffffffffu, mbar_wait(bar(c.empty[g][third]), phase, waits));
+        for (uint32_t part = 0; part < kParts; ++part) {
+          alive = __all_sync(0xffffffffu, mbar_wait(bar(c.empty[g][part]), phase, waits));
           if (!alive) break;
           if (leader) {
-            // every reader of the mask of tile n - 2 has done with it when the first third is released
-            if (third == 0 && quarter == 0) { c.valid[g][0] = b0; c.valid[g][1] = b1; c.valid[g][2] = b2; c.valid[g][3] = b3; }
+            // every reader of the mask of tile n - 2 has done with it when the first part is released
+            if (part == 0 && quarter == 0) { c.valid[g][0] = b0; c.valid[g][1] = b1; c.valid[g][2] = b2; c.valid[g][3] = b3; }
             if (any) {
-              expect_bytes(bar(c.full[g][third]), kThirdBytes / kLoaderWarps);
+              expect_bytes(bar(c.full[g][part]), (part_end(part) - 2u * part) * kPieceBytes / kLoaderWarps);
 #pragma unroll
               for (uint32_t q = 0; q < 4u; ++q) {
 #pragma unroll
-                for (uint32_t piece = third * (kPieces / kThirds); piece < (third + 1u) * (kPieces / kThirds); ++piece)
-                  load_rows(base + g * kStageBytes + piece * kPieceBytes + (quarter * 4u + q) * 512u, map, piece * 64u, r[q], bar(c.full[g][third]));
+                for (uint32_t piece = 2u * part; piece < part_end(part); ++piece)
+                  load_rows(base + g * kStageBytes + piece * kPieceBytes + (quarter * 4u + q) * 512u, map, piece * 64u, r[q], bar(c.full[g][part]));
               }
             } else {
-              mbar_arrive(bar(c.full[g][third]));
+              mbar_arrive(bar(c.full[g][part]));
             }
           }
           __syncwarp();
@@ -391,7 +393,7 @@ attend_tiles(const __grid_constant__ CUtensorMap query_map, const __grid_constan
     constexpr uint32_t kValueDesc = kBase | (1u << 15) | (1u << 16) | ((128u >> 4) << 24);   // both operands M/N-major
     const bool leader = elect_one();
     auto wait = [&](const uint64_t& b, uint32_t phase) { return __all_sync(0xffffffffu, mbar_wait(bar(b), phase, waits)); };
-    if (warp == kScoreWarp) {                // S^T of tile n, piece by piece as its thirds come
+    if (warp == kScoreWarp) {                // S^T of tile n, part by part as they come
       bool alive = rows.request < 0 || wait(c.query_full, 0);
       for (uint32_t n = 0; alive && n < count; ++n) {
         const uint32_t s = n & 1u, phase = (n >> 1) & 1u;
@@ -399,20 +401,20 @@ attend_tiles(const __grid_constant__ CUtensorMap query_map, const __grid_constan
         const uint32_t d = tmem + kScores + s * kN;
         const uint64_t da = operand(base + s * kStageBytes, 16u), db = operand(base + Layout<kN>::kQuery, 16u);
 #pragma unroll
-        for (uint32_t third = 0; third < kThirds; ++third) {
-          alive = alive && wait(c.full[s][third], phase);
+        for (uint32_t part = 0; part < kParts; ++part) {
+          alive = alive && wait(c.full[s][part], phase);
           if (!alive) break;
           fence_after();
           if (leader) {
             if (!none(s)) {
 #pragma unroll
-              for (uint32_t piece = third * (kPieces / kThirds); piece < (third + 1u) * (kPieces / kThirds); ++piece) {
+              for (uint32_t piece = 2u * part; piece < part_end(part); ++piece) {
 #pragma unroll
                 for (uint32_t k = 0; k < 4; ++k)
                   mma(d, da + (piece * (kPieceBytes >> 4) + 2u * k), db + (piece * (kN * 8u) + 2u * k), kScoreDesc, (piece | k) != 0u);
               }
             }
-            if (third == kThirds - 1u) commit(bar(c.scored[s]));
+            if (part == kParts - 1u) commit(bar(c.scored[s]));
           }
           __syncwarp();
         }
@@ -433,7 +435,7 @@ attend_tiles(const __grid_constant__ CUtensorMap query_map, const __grid_constan
               for (uint32_t k = 0; k < kTile / 16u; ++k)
                 mma(tmem + kOut + m * kN, da + (2u * m * (kPieceBytes >> 4) + k * 128u), db + k * 128u, kValueDesc, written || k != 0u);
             }
-            if (m) commit(bar(c.empty[s][m - 1u]));   // blocks 0-1 end with the pieces 0-2, block 2 with 3-5, block 3 with the rest
+            commit(bar(c.empty[s][m]));
           }
         }
         __syncwarp();
@@ -459,7 +461,7 @@ attend_tiles(const __grid_constant__ CUtensorMap query_map, const __grid_constan
         if (lane == 0) mbar_arrive(bar(c.taken[s]));
         // the same for all: the mask belongs to the tile
         // as below: a thread arrives for this tile only when all have arrived for the one before
-        if (n && !mbar_wait(bar(c.empty[(n - 1u) & 1u][kThirds - 1u]), ((n - 1u) >> 1) & 1u, waits)) dead = true;
+        if (n && !mbar_wait(bar(c.empty[(n - 1u) & 1u][kParts - 1u]), ((n - 1u) >> 1) & 1u, waits)) dead = true;
         __syncwarp();
         if (__any_sync(0xffffffffu, dead)) dead = true;
         else if (lane == 0) mbar_arrive(bar(c.weighted));
@@ -509,7 +511,7 @@ attend_tiles(const __grid_constant__ CUtensorMap query_map, const __grid_constan
         role_any(1u + side, false);
         if (written) {                         // the accumulators hold the tiles before this one, which must be in
           const uint32_t before = n - 1u;      // stages are released in order, an empty tile's too
-          ok = mbar_wait(bar(c.empty[before & 1u][kThirds - 1u]), (before >> 1) & 1u, waits);
+          ok = mbar_wait(bar(c.empty[before & 1u][kParts - 1u]), (before >> 1) & 1u, waits);
           if (__all_sync(0xffffffffu, ok)) {
             fence_after();
             for (uint32_t m = 0; m < 4; ++m) {
@@ -540,7 +542,7 @@ attend_tiles(const __grid_constant__ CUtensorMap query_map, const __grid_constan
         p[2 * j + 1] = pack_pair<T>(x1, y1);
       }
       // the product of the tile before has read its weights
-      if (n && !dead && !mbar_wait(bar(c.empty[(n - 1u) & 1u][kThirds - 1u]), ((n - 1u) >> 1) & 1u, waits)) dead = true;
+      if (n && !dead && !mbar_wait(bar(c.empty[(n - 1u) & 1u][kParts - 1u]), ((n - 1u) >> 1) & 1u, waits)) dead = true;
       dead = __any_sync(0xffffffffu, dead);
       if (!dead) {
         const uint32_t to = base + Layout<kN>::kWeights + row0 * 128u + (lane & 3u) * 4u;
@@ -557,7 +559,7 @@ attend_tiles(const __grid_constant__ CUtensorMap query_map, const __grid_constan
       }
       written = true;
     }
-    if (count && !dead && !mbar_wait(bar(c.empty[(count - 1u) & 1u][kThirds - 1u]), ((count - 1u) >> 1) & 1u, waits)) dead = true;
+    if (count && !dead && !mbar_wait(bar(c.empty[(count - 1u) & 1u][kParts - 1u]), ((count - 1u) >> 1) & 1u, waits)) dead = true;
     // sums over the rows of all tiles
 #pragma unroll
     for (uint32_t j = 0; j < 2 * kBlocks; ++j) {
@@ -722,10 +724,26 @@ bool encode_map(CUtensorMap* map, bool bf16, const void* base, uint32_t dims, ui
 }
 
 template <typename T, uint32_t kN>
-uint32_t launch_tiles(const KvipAttentionArgs& a, KernelSlot slot, uint32_t groups, uint32_t group_heads, uint32_t splits, cudaStream_t stream) {
+uint32_t configure(cudaLaunchConfig_t& config, cudaLaunchAttribute& cluster, KernelSlot slot, uint32_t ctas, uint32_t splits, cudaStream_t stream) {
   if (uint32_t bad = raise_dynamic_smem(slot, reinterpret_cast<const void*>(attend_tiles<T, kN>), static_cast<int>(Layout<kN>::kBytes),
                                         "slot_attention attribute"))
     return bad;
+  config = cudaLaunchConfig_t{};
+  config.gridDim = dim3(ctas);
+  config.blockDim = dim3(Warps<kN>::kThreads);
+  config.dynamicSmemBytes = Layout<kN>::kBytes;
+  config.stream = stream;
+  cluster = cudaLaunchAttribute{};
+  cluster.id = cudaLaunchAttributeClusterDimension;
+  cluster.val.clusterDim.x = splits;
+  cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
+  config.attrs = &cluster;
+  config.numAttrs = 1;
+  return 0;
+}
+
+template <typename T, uint32_t kN>
+uint32_t launch_tiles(const KvipAttentionArgs& a, KernelSlot slot, uint32_t groups, uint32_t group_heads, uint32_t splits, cudaStream_t stream) {
   const bool bf16 = __is_same(T, __nv_bfloat16);
   CUtensorMap query_map, pool_map, draft_map;
   // strides of a dimension of size one do not matter, but the encoder looks at them
@@ -737,41 +755,55 @@ uint32_t launch_tiles(const KvipAttentionArgs& a, KernelSlot slot, uint32_t grou
     set_error("slot_attention: the strides do not fit a tensor map");
     return KVIP_BAD_ARGUMENT;
   }
-  cudaLaunchConfig_t config{};
-  config.gridDim = dim3(a.tokens * groups * splits);
-  config.blockDim = dim3(Warps<kN>::kThreads);
-  config.dynamicSmemBytes = Layout<kN>::kBytes;
-  config.stream = stream;
-  cudaLaunchAttribute cluster{};
-  cluster.id = cudaLaunchAttributeClusterDimension;
-  cluster.val.clusterDim.x = splits;
-  cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
-  config.attrs = &cluster;
-  config.numAttrs = 1;
+  cudaLaunchConfig_t config;
+  cudaLaunchAttribute cluster;
+  if (uint32_t bad = configure<T, kN>(config, cluster, slot, a.tokens * groups * splits, splits, stream)) return bad;
   cudaLaunchKernelEx(&config, attend_tiles<T, kN>, query_map, pool_map, draft_map, a, groups, group_heads, splits);
   count_launch();
   return check_launch("attend_tiles");
 }
 
+// Clusters of `splits` CTAs that run at once on the current device (one CTA per SM; a cluster stays within a part of the GPU, so
+// large ones leave SMs idle). Asked once per device.
+uint32_t resident_clusters(uint32_t splits) {
+  static std::atomic<uint32_t> known[64][4];
+  const uint32_t at = splits == 1u ? 0u : splits == 2u ? 1u : splits == 4u ? 2u : 3u;
+  int device = 0;
+  if (cudaGetDevice(&device) != cudaSuccess || device < 0 || device >= 64) device = -1;
+  if (device >= 0) {
+    const uint32_t n = known[device][at].load(std::memory_order_relaxed);
+    if (n) return n;
+  }
+  cudaLaunchConfig_t config;
+  cudaLaunchAttribute cluster;
+  int n = 0;
+  if (configure<__nv_bfloat16, 64>(config, cluster, static_cast<KernelSlot>(kSlotAttentionBf16 + 3), splits, splits, nullptr) ||
+      cudaOccupancyMaxActiveClusters(&n, attend_tiles<__nv_bfloat16, 64>, &config) != cudaSuccess || n < 1) {
+    cudaGetLastError();
+    return device_sm_count() * 3u / (4u * splits) + 1u;
+  }
+  if (device >= 0) known[device][at].store(static_cast<uint32_t>(n), std::memory_order_relaxed);
+  return static_cast<uint32_t>(n);
+}
+
 // How a call is cut: heads per CTA (all up to 64, or fewer, which read the rows more often) and CTAs that share the rows of a
-// token. Few tokens are cut finely, because the SMs would stand idle; each cut costs the rows' copies once more or the joining of the
-// shares. Counted in clocks, from measurements on full lists (below): a tile takes kTileClocks, and a CTA what it spends
-// before its first and behind its last tile.
+// token. Few tokens are cut finely, because the SMs would stand idle; each cut costs the rows' copies once more or the joining of
+// the shares. Counted in clocks of full lists: a tile of 64 rows takes 2350 + 7 per head, a CTA 12700 + 228 per head before its
+// first and behind its last tile (fitted to 1 token x 128 heads x 2048 slots: 16 heads x 8 CTAs 15.0 us, 16 x 4 19.8, 16 x 2 30.2,
+// 32 x 8 16.4, 64 x 8 21.6, 64 x 1 61.9; 16 tokens: 64 x 4 28.4 against 64 x 2 38.8; 100 tokens: 64 x 2 126 against 64 x 1 137).
 struct Cut { uint32_t groups, group_heads, splits; };
 Cut cut_of(const KvipAttentionArgs& a) {
-  const uint32_t tiles = (a.entries + kTile - 1) / kTile + (a.draft ? 1u : 0u), sms = device_sm_count();
+  const uint32_t tiles = (a.entries + kTile - 1) / kTile + (a.draft ? 1u : 0u);
   Cut best{};
   uint64_t least = ~0ull;
-  for (uint32_t width = 64; width >= 16; width /= 2) {
+  for (uint32_t width = kGroupHeads; width >= 16; width /= 2) {
     const uint32_t groups = (a.heads + width - 1) / width, group_heads = (a.heads + groups - 1) / groups;
+    if (width < kGroupHeads && groups == (a.heads + 2 * width - 1) / (2 * width)) continue;   // the wider cut again
     const uint64_t units = static_cast<uint64_t>(a.tokens) * groups;
     for (uint32_t splits = 1; splits <= kMaxSplits; splits *= 2) {
-      if (a.splits && a.splits != splits) continue;
-      if (!a.splits && splits > tiles) break;
-      const uint64_t resident = (splits <= 2u ? sms : sms * 7u / 8u) / splits;      // clusters at once: they stay within a part of the GPU
-      const uint64_t waves = (units + resident - 1) / resident;
-      const uint64_t clocks = waves * (static_cast<uint64_t>((tiles + splits - 1) / splits) * (2900u + 12u * group_heads) + 11000u +
-                                       (splits > 1 ? 2000u + 60u * group_heads : 30u * group_heads));
+      if (a.splits ? a.splits != splits : splits > 1 && splits > tiles) continue;
+      const uint64_t waves = (units + resident_clusters(splits) - 1) / resident_clusters(splits);
+      const uint64_t clocks = waves * (static_cast<uint64_t>((tiles + splits - 1) / splits) * (2350u + 7u * group_heads) + 12700u + 228u * group_heads);
       if (clocks < least) { least = clocks; best = {groups, group_heads, splits}; }
     }
   }
