@@ -658,19 +658,32 @@ attend_tiles(const __grid_constant__ CUtensorMap query_map, const __grid_constan
         float tops[kMaxSplits], top = -INFINITY;
 #pragma unroll
         for (uint32_t s = 0; s < kMaxSplits; ++s) {
-          tops[s] = s < splits ? load_remote(remote(smem_u32(&c.top[h]), s)) : -INFINITY;
-          top = fmaxf(top, tops[s]);
+          tops[s] = load_remote(remote(smem_u32(&c.top[h]), min(s, splits - 1u)));
+          if (s >= splits) tops[s] = -INFINITY;
         }
+#pragma unroll
+        for (uint32_t s = 0; s < kMaxSplits; ++s) top = fmaxf(top, tops[s]);
         float total = 0.f, y[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (uint32_t s = 0; s < kMaxSplits; ++s) {
-          if (tops[s] == -INFINITY) continue;                             // an empty share has written nothing
-          const float weight = exp2_fast(tops[s] - top);
-          total = fmaf(weight, load_remote(remote(smem_u32(&c.factor[h]), s)), total);
-          const uint32_t from = remote(base + (h * kValue + element) * 4u, s);
-          const float4 low = load_remote4(from), high = load_remote4(from + 512u);
-          y[0] = fmaf(weight, low.x, y[0]); y[1] = fmaf(weight, low.y, y[1]); y[2] = fmaf(weight, low.z, y[2]); y[3] = fmaf(weight, low.w, y[3]);
-          y[4] = fmaf(weight, high.x, y[4]); y[5] = fmaf(weight, high.y, y[5]); y[6] = fmaf(weight, high.z, y[6]); y[7] = fmaf(weight, high.w, y[7]);
+        for (uint32_t s0 = 0; s0 < kMaxSplits; s0 += 4) {                  // four shares' numbers on their way at a time
+          if (s0 >= splits) break;
+          float4 low[4], high[4];
+          float sums[4];
+#pragma unroll
+          for (uint32_t i = 0; i < 4; ++i) {
+            const uint32_t s = min(s0 + i, splits - 1u), from = remote(base + (h * kValue + element) * 4u, s);
+            sums[i] = load_remote(remote(smem_u32(&c.factor[h]), s));
+            low[i] = load_remote4(from);
+            high[i] = load_remote4(from + 512u);
+          }
+#pragma unroll
+          for (uint32_t i = 0; i < 4; ++i) {
+            if (tops[s0 + i] == -INFINITY) continue;                      // no such share, or an empty one: it has written nothing
+            const float weight = exp2_fast(tops[s0 + i] - top);
+            total = fmaf(weight, sums[i], total);
+            y[0] = fmaf(weight, low[i].x, y[0]); y[1] = fmaf(weight, low[i].y, y[1]); y[2] = fmaf(weight, low[i].z, y[2]); y[3] = fmaf(weight, low[i].w, y[3]);
+            y[4] = fmaf(weight, high[i].x, y[4]); y[5] = fmaf(weight, high[i].y, y[5]); y[6] = fmaf(weight, high[i].z, y[6]); y[7] = fmaf(weight, high[i].w, y[7]);
+          }
         }
         const float inverse = top == -INFINITY ? 0.f : 1.f / total;
         const uint64_t row = static_cast<uint64_t>(t) * a.heads + head0 + h;
