@@ -104,16 +104,19 @@ class IndexSelector:
     `LIFetch` and returns the logical TopK per query token; prefill rows of a mixed batch are selected by the
     model-side indexer over its own paged cache. `slots(n)` are the resident slots for the attention kernel.
 
-    The caller binds `inputs.bind_positions(positions)` before the call, as in the reference."""
+    The caller binds `inputs.bind_positions(positions)` before the call, as in the reference. With `rotary` (a
+    `kvip.Rotary`), Index queries may come unrotated in the model's type and without scales: they are rotated by
+    `positions`, one per query token, and quantised here. `attend` runs the attention of the decode rows over the slots."""
 
     def __init__(self, torch, *, inputs, rotating, update, logical_ids, row_owners, storage=None, forward=None,
-                 lru=None):
+                 lru=None, rotary=None):
         from .operators.lifetch import LIFetch
 
         self.torch = torch
         self.inputs, self.rotating, self.update = inputs, rotating, update
         self.forward = forward if forward is not None else LIFetch(rotating, update, lru=lru)
         self.logical_ids, self.row_owners, self.storage = logical_ids, row_owners, storage
+        self.rotary = rotary
         self.positions = None
         if logical_ids.ndim != 2 or not logical_ids.is_contiguous() or logical_ids.dtype != torch.int64:
             raise ValueError("LIFetch logical IDs require contiguous int64 owner/history rows")
@@ -142,8 +145,14 @@ class IndexSelector:
         if self.row_owners.data_ptr() != self.inputs.row_owners.data_ptr():
             self.row_owners.copy_(self.inputs.row_owners)
 
-    def __call__(self, query, weights, indexer, metadata, query_scale):
+    def __call__(self, query, weights, indexer, metadata, query_scale=None):
         torch = self.torch
+        if self.rotary is not None and query_scale is None:
+            if self.positions is None:
+                raise ValueError("LIFetch queries are rotated by `positions`, which are not set")
+            query, query_scale = self.rotary.quantise(self.positions, query.view(weights.shape[0], self.inputs.index_heads, 128))
+        elif query_scale is None:
+            raise ValueError("LIFetch queries without scales need a Rotary to quantise them")
         mixed = bool(self.plans) and len(self.decodes) != len(self.plans)
         if self.storage is not None:
             if mixed:
@@ -183,6 +192,20 @@ class IndexSelector:
                 query_rows[plan.begin:plan.stop], weights[plan.begin:plan.stop], prefill,
                 scale_rows[plan.begin:plan.stop]))
         return result
+
+    def attend(self, attention, query, *, scale, tables=None, requests=None, starts=None, draft=None, ancestors=None, out=None, lse=None):
+        """Attention of the decode rows over the slots the selection has returned, straight from the resident pool:
+        `attention` a `kvip.SlotAttention`, `query` [tokens, heads, 576] in packed order. `tables` (the `BlockTables` that
+        planned the step) names the request of every token and where a request's tokens start; without it `requests` and,
+        for drafted rows, `starts` do, or the layout of the step is read."""
+        if tables is not None:
+            requests, starts = tables.requests, tables.starts
+        elif requests is None:
+            inputs = self.inputs
+            requests = self.torch.where(inputs.output_valid > 0, inputs.unpack_indices // inputs.queries, -1).to(self.torch.int32)
+        return attention(query, self.rotating.output, self.slots(query.shape[0]), scale=scale, requests=requests,
+                         row_owners=self.row_owners, output_stride=self.rotating.output_stride, starts=starts if draft is not None else None,
+                         draft=draft, ancestors=ancestors, out=out, lse=lse)
 
     def slots(self, token_count):
         if self.attention_indices is None:

@@ -122,12 +122,31 @@ class QueryInputs:
             pending.synchronize()          # the copy that last used this staging block (two steps ago) has finished
         self.host[ring].numpy()[...] = layout
         self.metadata.copy_(self.host[ring], non_blocking=True)
-        if self.block_offsets.numel():     # per-owner contiguous Index storage: page p of a request = owner * pages + p
-            self.torch.mul(self.row_owners[:, None], self.block_offsets.numel(), out=self.block_bases)
-            self.torch.add(self.block_bases, self.block_offsets, out=self.block_table)
+        self._owner_pages()
         if pending is None:
             pending = self.host_events[ring] = self.torch.cuda.Event()
         pending.record(self.torch.cuda.current_stream(self.device))
+
+    def prepare_device(self, layout, query_owners):
+        """The layout of a step whose query counts are known on the device alone (behind a verification of drafted tokens):
+        `layout` int64 [4, batch * queries] as `BlockTables.plan` writes it, `query_owners` int32 [batch]. Device copies
+        only, capturable. The number of packed tokens stays on the device: output rows behind the last one are -1."""
+        if layout.dtype != self.torch.int64 or tuple(layout.shape) != (4, self.batch * self.queries):
+            raise ValueError("LIFetch layouts are int64 [4, batch * queries]")
+        if query_owners.dtype != self.torch.int32 or tuple(query_owners.shape) != (self.batch,):
+            raise ValueError("LIFetch owners are int32 [batch]")
+        self._on_device(layout, "layout")
+        self._on_device(query_owners, "owners")
+        self.metadata[:OWNERS].copy_(layout)
+        if query_owners.data_ptr() != self.row_owners.data_ptr():
+            self.row_owners.copy_(query_owners)
+        self.token_count = self.batch * self.queries
+        self._owner_pages()
+
+    def _owner_pages(self):
+        if self.block_offsets.numel():     # per-owner contiguous Index storage: page p of a request = owner * pages + p
+            self.torch.mul(self.row_owners[:, None], self.block_offsets.numel(), out=self.block_bases)
+            self.torch.add(self.block_bases, self.block_offsets, out=self.block_table)
 
     def _gather(self, *, query=None, weights=None, scale=None, positions=None, tokens):
         """One gather launch on the bound device (kvip_b200_pack_inputs)."""
