@@ -32,14 +32,14 @@ class BlockTables:
         if not 0 <= queries <= _lib.MAX_QUERIES:
             raise ValueError("BlockTables: zero to four query slots per request")
         self.batch, self.pages, self.blocks, self.tokens, self.block, self.queries = batch, pages, blocks, tokens, block, queries
+        # one block of int32 and one of int64 words: a table is made in a few launches
         i32, i64 = dict(dtype=torch.int32, device=device), dict(dtype=torch.int64, device=device)
-        self.lengths, self.held = torch.zeros(batch, **i32), torch.zeros(batch, **i32)
+        words = torch.zeros(5 * batch + 4 + tokens, **i32)
+        (self.lengths, self.held, self.ends, self.held_after, self.starts, self.head, self.taken, self.status, self.requests) = words.split(
+            (batch, batch, batch, batch, batch + 1, 1, 1, 1, tokens))
+        self.positions, self.slot_mapping = torch.full((2, tokens), -1, **i64).unbind(0)
         self.table = torch.full((batch, pages), -1, **i32)
-        self.free, self.head = torch.arange(max(1, blocks), **i32), torch.zeros(1, **i32)
-        self.positions, self.slot_mapping = torch.full((tokens,), -1, **i64), torch.full((tokens,), -1, **i64)
-        self.requests, self.starts = torch.full((tokens,), -1, **i32), torch.zeros(batch + 1, **i32)
-        self.ends, self.held_after = torch.zeros(batch, **i32), torch.zeros(batch, **i32)
-        self.taken, self.status = torch.zeros(1, **i32), torch.zeros(1, **i32)
+        self.free = torch.arange(max(1, blocks), **i32)
         self.layout = torch.zeros((4, batch * queries), **i64) if queries else None
         self.device, self.index = self.table.device, self.table.get_device()
         self.launch = _launch.Launcher("kvip_b200_slot_maps")

@@ -290,7 +290,10 @@ attend_tiles(const __grid_constant__ CUtensorMap query_map, const __grid_constan
   const uint32_t tmem = c.tmem;
   // tiles of the list, then one of the drafted rows
   const uint32_t listed = c.last, list_tiles = (listed + kTile - 1) / kTile, tiles = list_tiles + (rows.drafted ? 1u : 0u);
-  const uint32_t first = tiles * split / splits, count = rows.request < 0 ? 0u : tiles * (split + 1u) / splits - first;
+  // A list may be far shorter than its entries. Up to three tiles are one CTA's: joining shares takes as long as two more of them.
+  const uint32_t shares = tiles <= 3u ? 1u : splits;
+  const bool idle = rows.request < 0 || split >= shares;
+  const uint32_t first = idle ? 0u : tiles * split / shares, count = idle ? 0u : tiles * (split + 1u) / shares - first;
   const Waits waits{&c.abort_flag, static_cast<long long>(a.wait_kilocycles ? a.wait_kilocycles : kDefaultWaitKilocycles) << 10};
   constexpr uint32_t kScores = 0, kOut = 2 * kN;   // tensor-memory columns: two score tiles, four value blocks
   auto none = [&](uint32_t s) { return (c.valid[s][0] | c.valid[s][1] | c.valid[s][2] | c.valid[s][3]) == 0u; };
@@ -575,24 +578,24 @@ attend_tiles(const __grid_constant__ CUtensorMap query_map, const __grid_constan
     if (!written && w == 0 && lane < 4)
       for (uint32_t j = 0; j < 2 * kBlocks; ++j) c.top[head_at + (j >> 1) * 8u + lane * 2u + (j & 1u)] = -INFINITY;
     dead = role_any<kSides * kRole>(kSides + 1u, dead);
-    if (dead || rows.request < 0) {
+    if (dead || idle) {
       written = false;                       // a share that cannot be trusted counts as empty; the status says so
       if (tid < kN) c.top[tid] = -INFINITY;
     }
     fence_after();
     if (tid < heads) {
       const float total = (c.reduce[0][tid] + c.reduce[1][tid]) + (c.reduce[2][tid] + c.reduce[3][tid]);
-      if (splits > 1) c.factor[tid] = total;
+      if (shares > 1) c.factor[tid] = total;
       else c.factor[tid] = written ? 1.f / total : 0.f;
-      if (splits == 1 && rows.request >= 0 && !dead)
+      if (shares == 1 && !idle && !dead)
         a.lse[static_cast<uint64_t>(t) * a.heads + head0 + tid] = written ? (c.top[tid] + log2f(total)) * 0.6931471805599453f : -INFINITY;
     }
     // The output is laid out in the stages (all products have read them). Accumulators have value elements as rows and heads as
     // columns: 8 x 8 blocks are transposed on their way into shared memory, and whole rows leave by copies. A share that
     // will be joined stays here as it is, in fp32 and undivided.
-    if (splits == 1) {
+    if (shares == 1) {
       role_any<kSides * kRole>(kSides + 1u, false);
-      if (rows.request >= 0 && !dead) {
+      if (!idle && !dead) {
         // addresses of stored rows: lanes 0-7 give the heads of a block for value elements 0-7, 8-15 for 8-15, 16-31 the next block's
         const uint32_t store = base + ((lane & 7u) + (lane >> 4) * 8u) * kOutRow + ((lane >> 3) & 1u) * 16u;
         for (uint32_t block = side; block < 4u; block += kSides) {
@@ -623,7 +626,7 @@ attend_tiles(const __grid_constant__ CUtensorMap query_map, const __grid_constan
       }
       fence_async();
       role_any<kSides * kRole>(kSides + 1u, false);
-      if (tid < heads && rows.request >= 0 && !dead) {
+      if (tid < heads && !idle && !dead) {
         asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;"
                      ::"l"(static_cast<T*>(a.out) + (static_cast<uint64_t>(t) * a.heads + head0 + tid) * kValue), "r"(base + tid * kOutRow), "r"(kValue * 2u)
                      : "memory");
@@ -649,29 +652,29 @@ attend_tiles(const __grid_constant__ CUtensorMap query_map, const __grid_constan
 
   // ---- shares of one unit, a CTA each: every CTA joins the heads rank, rank + splits, .. out of all of them -------------
   //   out = sum_s w_s o_s / sum_s w_s l_s, w_s = 2^(reference of share s - the largest)
-  if (splits > 1) {
+  if (shares > 1) {
     cluster_barrier();
     if (rows.request >= 0) {
       for (uint32_t item = warp; ; item += Warps<kN>::kThreads / 32u) {   // half a row per warp
-        const uint32_t h = split + (item >> 1) * splits, element = (item & 1u) * 256u + lane * 4u;
+        const uint32_t h = split + (item >> 1) * shares, element = (item & 1u) * 256u + lane * 4u;
         if (h >= heads) break;
         float tops[kMaxSplits], top = -INFINITY;
 #pragma unroll
         for (uint32_t s = 0; s < kMaxSplits; ++s) {
-          tops[s] = load_remote(remote(smem_u32(&c.top[h]), min(s, splits - 1u)));
-          if (s >= splits) tops[s] = -INFINITY;
+          tops[s] = load_remote(remote(smem_u32(&c.top[h]), min(s, shares - 1u)));
+          if (s >= shares) tops[s] = -INFINITY;
         }
 #pragma unroll
         for (uint32_t s = 0; s < kMaxSplits; ++s) top = fmaxf(top, tops[s]);
         float total = 0.f, y[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (uint32_t s0 = 0; s0 < kMaxSplits; s0 += 4) {                  // four shares' numbers on their way at a time
-          if (s0 >= splits) break;
+          if (s0 >= shares) break;
           float4 low[4], high[4];
           float sums[4];
 #pragma unroll
           for (uint32_t i = 0; i < 4; ++i) {
-            const uint32_t s = min(s0 + i, splits - 1u), from = remote(base + (h * kValue + element) * 4u, s);
+            const uint32_t s = min(s0 + i, shares - 1u), from = remote(base + (h * kValue + element) * 4u, s);
             sums[i] = load_remote(remote(smem_u32(&c.factor[h]), s));
             low[i] = load_remote4(from);
             high[i] = load_remote4(from + 512u);

@@ -5,6 +5,8 @@ The reference leaves attention to the serving framework; `slot_output` and the r
 kernel once."""
 from .. import _lib, _launch
 
+WIDTH, VALUE = _lib.ATTENTION_WIDTH, _lib.ATTENTION_VALUE
+
 
 class SlotAttention:
     """Attention of up to `tokens` packed query tokens with up to `heads` heads over `entries` slots each.
@@ -37,86 +39,85 @@ class SlotAttention:
         if tokens < 1 or not 1 <= heads <= 128 or not 1 <= entries <= 1 << 20:
             raise ValueError("SlotAttention: at least one token, 1..128 heads, 1..2^20 entries")
         self.tokens, self.heads, self.entries = tokens, heads, entries
-        self.out = torch.zeros((tokens, heads, _lib.ATTENTION_VALUE), dtype=self.dtype, device=device)
+        self.out = torch.zeros((tokens, heads, VALUE), dtype=self.dtype, device=device)
         self.lse = torch.full((tokens, heads), float("-inf"), dtype=torch.float32, device=device)
         self.status = torch.zeros(1, dtype=torch.int32, device=device)
         self.device, self.index = self.out.device, self.out.get_device()
-        self._status = self.status.data_ptr()
+        self._out, self._lse, self._status = self.out.data_ptr(), self.lse.data_ptr(), self.status.data_ptr()
+        self.kind = _lib.FLOAT_BF16 if self.dtype == torch.bfloat16 else _lib.FLOAT_FP16
         self.launch = _launch.Launcher("kvip_b200_slot_attention")
 
     @property
     def nbytes(self):
         return sum(t.numel() * t.element_size() for t in (self.out, self.lse, self.status))
 
-    def _flat(self, tensor, name, dtype, count):
-        if tensor.dtype != dtype or tensor.numel() != count or tensor.get_device() != self.index or not tensor.is_contiguous():
-            raise ValueError(f"SlotAttention {name} must be contiguous {dtype} with {count} elements on {self.device}")
+    def _flat(self, tensor, name, dtype, least, exact=False):
+        """Address of a contiguous tensor of at least (or exactly) `least` elements."""
+        count = tensor.numel()
+        if count < least or (exact and count != least) or tensor.dtype != dtype or tensor.get_device() != self.index or not tensor.is_contiguous():
+            raise ValueError(f"SlotAttention {name} must be contiguous {dtype} with {least} elements on {self.device}")
         return tensor.data_ptr()
 
     def __call__(self, query, pool, slots, *, scale, output_stride, requests=None, row_owners=None, queries=1, starts=None,
                  draft=None, ancestors=None, out=None, lse=None, splits=0, wait_kilocycles=0):
-        torch, index, width = self.torch, self.index, _lib.ATTENTION_WIDTH
-        if query.ndim != 3 or query.shape[2] != width or query.dtype != self.dtype or query.stride(2) != 1 or query.get_device() != index:
-            raise ValueError(f"SlotAttention query must be {self.dtype} [tokens, heads, {width}], innermost stride 1, on {self.device}")
-        tokens, heads = query.shape[0], query.shape[1]
+        torch, index, dtype = self.torch, self.index, self.dtype
+        shape, strides = query.shape, query.stride()
+        if len(shape) != 3 or shape[2] != WIDTH or strides[2] != 1 or query.dtype != dtype or query.get_device() != index:
+            raise ValueError(f"SlotAttention query must be {dtype} [tokens, heads, {WIDTH}], innermost stride 1, on {self.device}")
+        tokens, heads, _ = shape
         if tokens > self.tokens or heads > self.heads or heads < 1:
             raise ValueError("SlotAttention query exceeds the bound tokens or heads")
-        if (pool.shape[-1] * pool.element_size() != 2 * width or pool.dtype not in (torch.uint8, self.dtype) or pool.get_device() != index
+        size = 1 if pool.dtype == torch.uint8 else 2
+        rows, rest = divmod(pool.numel() * size, 2 * WIDTH)
+        if (rest or pool.shape[-1] * size != 2 * WIDTH or (size == 2 and pool.dtype != dtype) or pool.get_device() != index
                 or not pool.is_contiguous()):
-            raise ValueError(f"SlotAttention pool must be contiguous uint8 [rows, {2 * width}] or {self.dtype} [rows, {width}]")
-        if slots.dtype != torch.int32 or not slots.is_contiguous() or slots.get_device() != index or slots.shape[0] != tokens:
-            raise ValueError("SlotAttention slots must be contiguous int32 [tokens, entries]")
-        entries = slots.shape[-1]
-        if slots.numel() != tokens * entries or not 1 <= entries <= self.entries:
-            raise ValueError("SlotAttention slots must be [tokens, entries] (or [tokens, 1, entries]) within the bound entries")
-        rows = pool.numel() * pool.element_size() // (2 * width)
+            raise ValueError(f"SlotAttention pool must be contiguous uint8 [rows, {2 * WIDTH}] or {dtype} [rows, {WIDTH}]")
+        listed = slots.shape
+        entries = listed[-1]
+        if (slots.dtype != torch.int32 or listed[0] != tokens or slots.numel() != tokens * entries or not 1 <= entries <= self.entries
+                or slots.get_device() != index or not slots.is_contiguous()):
+            raise ValueError("SlotAttention slots must be contiguous int32 [tokens, entries] (or [tokens, 1, entries]) within the bound entries")
         if not 1 <= output_stride <= rows:
             raise ValueError("SlotAttention output_stride must lie within the pool")
         if tokens == 0:
             return (self.out[:0, :heads] if out is None else out), (self.lse[:0, :heads] if lse is None else lse)
-        if row_owners is not None:
-            batch = row_owners.numel()
-        elif starts is not None:
-            batch = starts.numel() - 1
+        batch = row_owners.numel() if row_owners is not None else starts.numel() - 1 if starts is not None else rows // output_stride
+        if requests is not None:
+            requests_ptr = self._flat(requests, "requests", torch.int32, tokens)
+        elif queries < 1 or batch * queries < tokens:
+            raise ValueError("SlotAttention tokens without requests belong to request t // queries")
         else:
-            batch = rows // output_stride
-        requests_ptr = 0 if requests is None else self._flat(requests, "requests", torch.int32, requests.numel())
-        if requests is None:
-            if queries < 1 or batch * queries < tokens:
-                raise ValueError("SlotAttention tokens without requests belong to request t // queries")
-        elif requests.numel() < tokens:
-            raise ValueError("SlotAttention requests must cover the tokens")
+            requests_ptr = 0
         owners_ptr = 0 if row_owners is None else self._flat(row_owners, "row_owners", torch.int32, batch)
-        draft_ptr = starts_ptr = ancestors_ptr = 0
-        draft_token = 0
+        draft_ptr = starts_ptr = ancestors_ptr = draft_token = 0
         if draft is not None:
             if starts is None:
                 raise ValueError("SlotAttention draft rows need the requests' starts")
-            starts_ptr = self._flat(starts, "starts", torch.int32, batch + 1)
-            if draft.ndim != 2 or draft.shape[0] < tokens or draft.shape[1] != width or draft.dtype != self.dtype or draft.stride(1) != 1 \
-                    or draft.get_device() != index:
-                raise ValueError(f"SlotAttention draft must be {self.dtype} [tokens, {width}], innermost stride 1")
-            draft_ptr, draft_token = draft.data_ptr(), draft.stride(0)
+            starts_ptr = self._flat(starts, "starts", torch.int32, batch + 1, True)
+            drafted = draft.shape
+            if len(drafted) != 2 or drafted[0] < tokens or drafted[1] != WIDTH or draft.dtype != dtype or draft.get_device() != index:
+                raise ValueError(f"SlotAttention draft must be {dtype} [tokens, {WIDTH}]")
+            draft_token, inner = draft.stride()
+            if inner != 1:
+                raise ValueError("SlotAttention draft needs an innermost stride of 1")
+            draft_ptr = draft.data_ptr()
             if ancestors is not None:
-                if ancestors.numel() < tokens:
-                    raise ValueError("SlotAttention ancestors must cover the tokens")
-                ancestors_ptr = self._flat(ancestors, "ancestors", torch.int64, ancestors.numel())
+                ancestors_ptr = self._flat(ancestors, "ancestors", torch.int64, tokens)
         elif ancestors is not None:
             raise ValueError("SlotAttention ancestors need draft rows")
+        whole = tokens == self.tokens and heads == self.heads
         if out is None:
-            out = self.out if tokens == self.tokens and heads == self.heads else self.out.view(-1)[
-                :tokens * heads * _lib.ATTENTION_VALUE].view(tokens, heads, _lib.ATTENTION_VALUE)
-            out_ptr = out.data_ptr()
+            out = self.out if whole else self.out.view(-1)[:tokens * heads * VALUE].view(tokens, heads, VALUE)
+            out_ptr = self._out
         else:
-            out_ptr = self._flat(out, "out", self.dtype, tokens * heads * _lib.ATTENTION_VALUE)
+            out_ptr = self._flat(out, "out", dtype, tokens * heads * VALUE, True)
         if lse is None:
-            lse = self.lse if tokens == self.tokens and heads == self.heads else self.lse.view(-1)[:tokens * heads].view(tokens, heads)
-            lse_ptr = lse.data_ptr()
+            lse = self.lse if whole else self.lse.view(-1)[:tokens * heads].view(tokens, heads)
+            lse_ptr = self._lse
         else:
-            lse_ptr = self._flat(lse, "lse", torch.float32, tokens * heads)
+            lse_ptr = self._flat(lse, "lse", torch.float32, tokens * heads, True)
         self.launch(
             index, query.data_ptr(), pool.data_ptr(), slots.data_ptr(), requests_ptr, owners_ptr, starts_ptr, draft_ptr, ancestors_ptr,
-            out_ptr, lse_ptr, self._status, query.stride(0), query.stride(1), draft_token, rows, tokens, heads, entries, batch,
-            queries, output_stride, _lib.FLOAT_BF16 if self.dtype == torch.bfloat16 else _lib.FLOAT_FP16, splits,
-            wait_kilocycles, scale, 0)
+            out_ptr, lse_ptr, self._status, strides[0], strides[1], draft_token, rows, tokens, heads, entries, batch, queries,
+            output_stride, self.kind, splits, wait_kilocycles, scale, 0)
         return out, lse

@@ -37,28 +37,29 @@ class DraftVerifier:
         self.launch = _launch.Launcher("kvip_b200_verify_drafts")
 
     def _flat(self, tensor, name, dtype, count):
-        if tensor.dtype != dtype or tensor.ndim != 1 or tensor.numel() < count or tensor.get_device() != self.index or not tensor.is_contiguous():
+        if tensor.numel() < count or tensor.dtype != dtype or tensor.ndim != 1 or tensor.get_device() != self.index or not tensor.is_contiguous():
             raise ValueError(f"DraftVerifier {name} must be contiguous {dtype} with at least {count} elements on {self.device}")
         return tensor.data_ptr()
 
     def __call__(self, target, draft, tokens, parents, starts, accept, sample):
-        torch, index = self.torch, self.index
-        kind = self.types.get(target.dtype)
-        if kind is None or target.ndim != 2 or target.stride(1) != 1 or target.get_device() != index:
+        torch, index, flat = self.torch, self.index, self._flat
+        kind, shape, strides = self.types.get(target.dtype), target.shape, target.stride()
+        if kind is None or len(shape) != 2 or strides[1] != 1 or target.get_device() != index:
             raise ValueError(f"DraftVerifier target must be [rows, vocabulary] float32, bfloat16 or float16, innermost stride 1, on {self.device}")
-        rows, vocabulary = target.shape
+        rows, vocabulary = shape
         if rows < 1 or not 1 <= vocabulary <= 1 << 24:
             raise ValueError("DraftVerifier: at least one row, a vocabulary of 1..2^24")
         draft_ptr, draft_row = 0, 0
         if draft is not None:
-            if draft.shape != target.shape or draft.dtype != target.dtype or draft.stride(1) != 1 or draft.get_device() != index:
+            draft_row, inner = draft.stride() if draft.ndim == 2 else (0, 0)
+            if draft.shape != shape or draft.dtype != target.dtype or inner != 1 or draft.get_device() != index:
                 raise ValueError("DraftVerifier draft must match the target")
-            draft_ptr, draft_row = draft.data_ptr(), draft.stride(0)
+            draft_ptr = draft.data_ptr()
         if starts.numel() != self.batch + 1:
             raise ValueError("DraftVerifier starts must be [batch + 1]")
         self.launch(
-            index, target.data_ptr(), draft_ptr, self._flat(tokens, "tokens", torch.int64, rows), self._flat(parents, "parents", torch.int32, rows),
-            self._flat(starts, "starts", torch.int32, self.batch + 1), self._flat(accept, "accept", torch.float32, rows),
-            self._flat(sample, "sample", torch.float32, self.batch), *self._outputs, target.stride(0), draft_row, rows, vocabulary,
+            index, target.data_ptr(), draft_ptr, flat(tokens, "tokens", torch.int64, rows), flat(parents, "parents", torch.int32, rows),
+            flat(starts, "starts", torch.int32, self.batch + 1), flat(accept, "accept", torch.float32, rows),
+            flat(sample, "sample", torch.float32, self.batch), *self._outputs, strides[0], draft_row, rows, vocabulary,
             self.batch, self.depth, kind, 0)
         return self.tokens, self.nodes, self.counts
