@@ -651,7 +651,7 @@ uint32_t kvip_b200_slot_maps(const KvipSlotMapsArgs* args, void* stream);
 /* Rotary positions. Pair i of a rotated row (elements i and i + width/2 in the half layout, 2i and 2i + 1 in the
  * interleaved one) turns by the angle position * frequency_i; turns[i] = frequency_i / 2 pi. Rows of tokens with a
  * negative position are not written. `x[s]`: two sets of rows [tokens, heads[s], width] with their own strides (in
- * elements, innermost stride 1); y may be x. */
+ * elements, innermost stride 1). y may be x; rows of y must not overlap one another, nor other rows of x. */
 enum { KVIP_ROTARY_HALF = 0, KVIP_ROTARY_INTERLEAVED = 1 };
 enum { KVIP_FLOAT_BF16 = 0, KVIP_FLOAT_FP16 = 1, KVIP_FLOAT_FP32 = 2 };
 typedef struct KvipRotaryArgs {
@@ -671,7 +671,8 @@ uint32_t kvip_b200_rotary(const KvipRotaryArgs* args, void* stream);
 /* Attention of packed query tokens over selected rows of the resident pool and, for a tree of drafted tokens, over
  * the drafted rows of their own request. Token t of request r = requests[t] sees the pool rows
  *   owner(r) * output_stride + slots[t, k]   for every slots[t, k] >= 0, and
- *   drafted row starts[r] + j                for every set bit j of ancestors[t] (j < starts[r+1] - starts[r], j < 64).
+ *   drafted row starts[r] + j                for every set bit j of ancestors[t] (j < starts[r+1] - starts[r], j < 64; a
+ *                                            request with more drafted rows is a KVIP_ERR_TOKEN_RANGE).
  * A row has 576 elements, its first 512 are also the value:
  *   out[t,h] = sum p v, p = softmax(scale * query[t,h] . row); lse[t,h] = log of the sum of exp(scale * query . row).
  * A token that sees no row gets zeros and lse = -inf; a token with requests[t] < 0 is padding, its outputs are left as they are. */

@@ -289,6 +289,15 @@ uint32_t launch_rotary(const KvipRotaryArgs& a, cudaStream_t stream) {
   return check_launch("rotary");
 }
 
+// Whether rows of `width` elements at these strides lie apart: each is written by one thread or another, in no order.
+bool apart(uint64_t tokens, uint64_t heads, int64_t token, int64_t head, int64_t width) {
+  if (tokens == 1) token = INT64_MAX;
+  if (heads == 1) head = INT64_MAX;
+  const int64_t near = token < head ? token : head, far = token < head ? head : token;
+  const int64_t count = static_cast<int64_t>(token < head ? tokens : heads);
+  return near >= width && (far == INT64_MAX || far >= near * (count - 1) + width);
+}
+
 }  // namespace
 }  // namespace kvip
 
@@ -303,6 +312,8 @@ extern "C" uint32_t kvip_b200_rotary(const KvipRotaryArgs* a, void* stream) {
   KVIP_REQUIRE(a->codes || (a->heads[1] == 0) == (a->x[1] == nullptr), "rotary: the second set needs rows and heads");
   KVIP_REQUIRE(a->codes || a->heads[1] == 0 || a->y[1], "rotary: null output pointer");
   KVIP_REQUIRE(a->layout <= KVIP_ROTARY_INTERLEAVED && a->dtype <= KVIP_FLOAT_FP32, "rotary: unknown layout or type");
+  for (uint32_t set = 0; !a->codes && set < 2u && a->heads[set]; ++set)
+    KVIP_REQUIRE(apart(a->tokens, a->heads[set], a->y_token[set], a->y_head[set], a->width), "rotary: output rows overlap");
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (a->dtype == KVIP_FLOAT_BF16) return launch_rotary<__nv_bfloat16>(*a, s);
   if (a->dtype == KVIP_FLOAT_FP16) return launch_rotary<__half>(*a, s);

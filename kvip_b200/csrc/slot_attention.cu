@@ -220,6 +220,7 @@ __device__ __forceinline__ Rows rows_of(const KvipAttentionArgs& a, uint32_t t) 
       r.bad |= static_cast<int32_t>(KVIP_ERR_TOKEN_RANGE);
     } else {
       const uint32_t nodes = static_cast<uint32_t>(min(static_cast<int64_t>(64), behind - first));
+      if (behind - first > 64) r.bad |= static_cast<int32_t>(KVIP_ERR_TOKEN_RANGE);   // what lies behind the 64th is not seen
       r.draft = static_cast<uint32_t>(first);
       r.seen = a.ancestors ? mask : (own < 0 ? 0ull : own >= 63 ? ~0ull : (2ull << own) - 1ull);
       if (nodes < 64u) r.seen &= (1ull << nodes) - 1ull;

@@ -207,6 +207,25 @@ def test_rotary_leaves_padding_rows_alone(device):
     assert (scales[[1, 4]] == 3.0).all() and (codes.view(torch.uint8)[[1, 4]] == 5).all() and (scales[[0, 2, 3]] != 3.0).all()
 
 
+def test_rotary_head_major_and_broadcast_rows(device):
+    """Rows whose heads lie further apart than their tokens; an input that is one row for all heads; an output that would be."""
+    import kvip_b200 as kvip
+    g = torch.Generator(device=device)
+    g.manual_seed(6)
+    rope = kvip.Rotary(torch, 64, device, layout="interleaved")
+    positions = torch.randint(0, 1 << 20, (10,), generator=g, device=device)
+    rows = torch.randn((6, 10, 64), generator=g, device=device).to(torch.bfloat16).transpose(0, 1)
+    out = torch.empty((6, 10, 64), dtype=torch.bfloat16, device=device).transpose(0, 1)
+    rope(positions, rows, query_out=out)
+    expected, size = reference.rotary(host(rows), positions.cpu().numpy(), 64, "interleaved")
+    assert (np.abs(host(out) - expected) <= rotary_tolerance(expected, size, torch.bfloat16, 1 << 20)).all()
+    one = rows[:, :1].expand(10, 6, 64)
+    rope(positions, one, query_out=out)
+    assert torch.equal(out[:, 0], out[:, 5])
+    with pytest.raises(ValueError, match="overlap"):
+        rope(positions, one)
+
+
 @pytest.mark.parametrize("tokens,heads,dim,width,layout,kind,stride", [
     (1, 64, 128, 64, "half", torch.bfloat16, 0), (64, 64, 128, 64, "half", torch.bfloat16, 0), (33, 32, 128, 128, "interleaved", torch.float16, 0),
     (7, 3, 130, 64, "half", torch.bfloat16, 0), (65, 1, 128, 32, "half", torch.float32, 8), (5, 64, 128, 64, "interleaved", torch.bfloat16, 1),
@@ -283,7 +302,8 @@ def attention_case(device, seed, *, counts, heads, entries, stride, context, kin
     for t in range(tokens):
         j = t - starts[requests[t]]
         parent = (j - 1 if not tree else int(rng.integers(0, j))) if j else -1
-        ancestors[t] = (1 << int(j)) - (1 << 64 if j == 63 else 0) | (int(ancestors[starts[requests[t]] + parent]) if j else 0)
+        own = 0 if j > 63 else (1 << int(j)) - (1 << 64 if j == 63 else 0)
+        ancestors[t] = own | (int(ancestors[starts[requests[t]] + parent]) if j else 0)
     case = dict(
         query=(torch.randn((tokens, heads, 576), generator=g, device=device) * spread).to(kind), pool=pool,
         slots=torch.from_numpy(slots).to(device), requests=torch.from_numpy(requests).to(device),
@@ -461,6 +481,50 @@ def test_attention_reports_and_skips_what_is_out_of_range(device):
     case["requests"][2] = 3
     attend, out, lse = run_attention(dict(case, draft=None, starts=None, ancestors=None), device)
     assert int(attend.status.item()) & 1 and (out[2] == 0).all()
+
+
+def test_attention_more_drafted_rows_than_a_mask_holds(device):
+    case = attention_case(device, 37, counts=[70, 2], heads=16, entries=64, stride=64, context=[10, 64], draft=False)
+    g = torch.Generator(device=device)
+    g.manual_seed(1)
+    case.update(starts=torch.tensor([0, 70, 72], dtype=torch.int32, device=device),
+                draft=torch.randn((72, 576), generator=g, device=device).to(torch.bfloat16), ancestors=None)
+    attend, out, lse = run_attention(case, device)
+    assert int(attend.status.item()) == 1
+    check_attention(case, out, lse)
+
+
+def test_attention_bounded_waits_give_up_and_report(device):
+    """A wait limit far below a tile's loading time: the call ends by itself, says so (unless everything came at once), and the next
+    call is right again. In one piece and in shares."""
+    import kvip_b200 as kvip
+    case = attention_case(device, 38, counts=[2], heads=64, entries=2048, stride=4096, context=[2048])
+    for splits in (1, 4):
+        attend = kvip.SlotAttention(torch, device, tokens=2, heads=64)
+        attend(**case, splits=splits, wait_kilocycles=1)
+        torch.cuda.synchronize()
+        assert int(attend.status.item()) in (0, 32)
+        attend.status.zero_()
+        out, lse = attend(**case, splits=splits)
+        check_attention(case, out, lse)
+        assert int(attend.status.item()) == 0
+
+
+def test_attention_on_two_streams_with_outputs_of_their_own(device):
+    """One object, two streams, outputs given by the caller: nothing is shared."""
+    import kvip_b200 as kvip
+    case = attention_case(device, 39, counts=[1, 2, 1], heads=128, entries=700, stride=1024, context=[700, 3, 650])
+    attend = kvip.SlotAttention(torch, device, tokens=4, heads=128, entries=700)
+    streams = [torch.cuda.Stream(device) for _ in range(2)]
+    outs = [(torch.empty((4, 128, 512), dtype=torch.bfloat16, device=device), torch.empty((4, 128), device=device)) for _ in range(2)]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for stream, (out, lse) in zip(streams, outs):
+            with torch.cuda.stream(stream):
+                attend(**case, out=out, lse=lse)
+    torch.cuda.synchronize()
+    check_attention(case, *outs[0])
+    assert torch.equal(outs[0][0], outs[1][0]) and torch.equal(outs[0][1], outs[1][1])
 
 
 def test_attention_offsets_beyond_32_bits(device):

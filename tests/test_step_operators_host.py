@@ -44,7 +44,8 @@ def test_slot_maps_refusals(library, bad, word):
     refused(library, "kvip_b200_slot_maps", filled(_lib.SlotMapsArgs, **{**MAPS, **bad}), word)
 
 
-ROTARY = dict(codes=None, heads0=4, heads1=1, tokens=3, width=64, dim=64, layout=0, dtype=0, factor=1.0)
+ROTARY = dict(codes=None, heads0=4, heads1=1, tokens=3, width=64, dim=64, layout=0, dtype=0, factor=1.0, x_token0=256, x_head0=64, y_token0=256,
+              y_head0=64, x_token1=64, y_token1=64)
 
 
 @pytest.mark.parametrize("bad,word", [
@@ -52,7 +53,8 @@ ROTARY = dict(codes=None, heads0=4, heads1=1, tokens=3, width=64, dim=64, layout
     (dict(heads1=0), "second set"), (dict(tokens=0), "token"), (dict(heads0=0), "head"), (dict(width=63), "even"), (dict(width=0), "even"),
     (dict(width=1026), "even"), (dict(layout=2), "layout"), (dict(dtype=3), "type"), (dict(codes=4096, scales=None), "null output"),
     (dict(codes=4096, dim=32, heads1=0), "quantised"), (dict(codes=4096, dim=5000, heads1=0), "quantised"), (dict(codes=4096, dim=128), "quantised"),
-    (dict(heads0=65537), "65536")])
+    (dict(heads0=65537), "65536"), (dict(y_head0=0), "overlap"), (dict(y_token0=0), "overlap"), (dict(y_head0=63), "overlap"),
+    (dict(y_token0=255), "overlap"), (dict(y_token1=32), "overlap"), (dict(y_token0=64, y_head0=128), "overlap")])
 def test_rotary_refusals(library, bad, word):
     refused(library, "kvip_b200_rotary", filled(_lib.RotaryArgs, **{**ROTARY, **bad}), word)
 
