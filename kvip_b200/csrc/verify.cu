@@ -53,6 +53,7 @@ __device__ __forceinline__ void store_remote(const double* where, uint32_t rank,
 }
 
 constexpr uint32_t kMaxCluster = 8;
+constexpr uint32_t kRunsInARow = 4;        // of a lane, where one warp looks through a share
 
 // A lane takes the probabilities of one 16-byte run at a time. A row of odd length starts anywhere: the two aligned vectors
 // round the run are read and shifted. A vector is read only where it holds an element of the run (memory is allocated in whole
@@ -321,69 +322,73 @@ __global__ void __launch_bounds__(kMostThreads, 1) verify_walk(const __grid_cons
       if (bad) atomicOr(a.status, bad);
     }
   }
-  // The share that holds the border is looked through once more, by all warps of its CTA: a part each, then a run per lane.
+  // The share that holds the border is looked through once more: a long one by all warps of its CTA, a part each; then a lane
+  // takes a few runs in a row.
   const double limit = __dmul_rn(sample, total);
   if (warp == 0) {
     const Place border = passing(s_part[pass & 1u], shares, limit, 0.0);
     if (lane == 0) { s_border.running = border.running; s_border.chosen = border.chosen; }
   }
   __syncthreads();
-  const Place border{s_border.running, s_border.chosen};
-  const uint32_t chosen = border.chosen;
-  if (chosen / warps != rank) return;
-  const uint32_t begin = min(V, chosen * share), end = min(V, begin + share);
-  const uint32_t part = ((end - begin + warps - 1u) / warps + kRun - 1u) / kRun * kRun;
-  double* sums = s_part[(pass & 1u) ^ 1u];   // the other CTAs have done with it, and write to it no more
-  const uint32_t from = min(end, begin + warp * part);
-  const double sum = part_sum(from, min(end, from + part));
-  if (lane == 0) sums[warp] = sum;
-  __syncthreads();
-  if (warp) return;
-  const Place inner = passing(sums, warps, limit, border.running);
-  const uint32_t place = inner.chosen;
-  double running = inner.running;
+  double running = s_border.running;
+  const uint32_t chosen = s_border.chosen;
+  if (chosen - rank * warps >= warps) return;   // another CTA's
+  uint32_t begin = min(V, chosen * share), end = min(V, begin + share);
+  if (share > 32u * kRun * kRunsInARow) {
+    const uint32_t part = ((end - begin + warps - 1u) / warps + kRun - 1u) / kRun * kRun;
+    double* sums = s_part[(pass & 1u) ^ 1u];   // the other CTAs have done with it, and write to it no more
+    const uint32_t from = min(end, begin + warp * part);
+    const double sum = part_sum(from, min(end, from + part));
+    if (lane == 0) sums[warp] = sum;
+    __syncthreads();
+    if (warp) return;
+    const Place inner = passing(sums, warps, limit, running);
+    running = inner.running;
+    begin = min(end, begin + inner.chosen * part);
+    end = min(end, begin + part);
+  } else if (warp) {
+    return;
+  }
   const T* row = target + node * a.target_row;
   const T* guess = draft ? draft + node * a.draft_row : row;
   const uint32_t off_p = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(row)) & 15u, off_q = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(guess)) & 15u;
-  const uint32_t first_run = min(end, begin + place * part), behind_run = min(end, first_run + part);
-  uint32_t picked = 0;
-  for (uint32_t v0 = first_run; v0 < behind_run; v0 += 32u * kRun) {
-    const uint32_t v = v0 + lane * kRun, count = v < behind_run ? min(kRun, behind_run - v) : 0u;
-    Run<T> rp = load_run<T, false>(row + v, count), rq = load_run<T, false>(guess + v, count);
-    settle_run<T, false>(rp, off_p, count);
-    settle_run<T, false>(rq, off_q, count);
-    double p[kRun];
-    left_of_run<T>(rp, rq, v, losses(), p);
-    double own = 0.0;
+  const uint32_t each = ((end - begin + 31u) / 32u + kRun - 1u) / kRun * kRun;   // elements of a lane
+  const uint32_t mine = min(end, begin + lane * each), behind_mine = min(end, mine + each);
+  auto runs = [&](auto&& visit) {              // this lane's runs in order
+    for (uint32_t v = mine; v < behind_mine; v += kRun) {
+      const uint32_t count = min(kRun, behind_mine - v);
+      Run<T> rp = load_run<T, false>(row + v, count), rq = load_run<T, false>(guess + v, count);
+      settle_run<T, false>(rp, off_p, count);
+      settle_run<T, false>(rq, off_q, count);
+      double p[kRun];
+      left_of_run<T>(rp, rq, v, losses(), p);
 #pragma unroll
-    for (uint32_t k = 0; k < kRun; ++k) own += p[k];
-    double scan = own;
+      for (uint32_t k = 0; k < kRun; ++k) visit(v + k, p[k]);
+    }
+  };
+  double own = 0.0;
+  runs([&](uint32_t, double p) { own += p; });
+  double scan = own;
 #pragma unroll
-    for (uint32_t d = 1; d < 32u; d <<= 1) {
-      const double other = __shfl_up_sync(0xffffffffu, scan, d);
-      if (lane >= d) scan += other;
-    }
-    // within the run: the first element whose running sum passes, else the last that holds anything
-    double so_far = running + (scan - own);
-    uint32_t at = 0, last = 0;
-    bool found = false;
-#pragma unroll
-    for (uint32_t k = 0; k < kRun; ++k) {
-      so_far += p[k];
-      if (p[k] > 0.0) {
-        last = k;
-        if (!found && so_far > limit) { found = true; at = k; }
-      }
-    }
-    const uint32_t passed = __ballot_sync(0xffffffffu, found), holds = __ballot_sync(0xffffffffu, own > 0.0);
-    if (passed || holds) {
-      const uint32_t who = passed ? static_cast<uint32_t>(__ffs(static_cast<int>(passed))) - 1u : 31u - static_cast<uint32_t>(__clz(static_cast<int>(holds)));
-      picked = v0 + who * kRun + __shfl_sync(0xffffffffu, passed ? at : last, who);
-    }
-    if (passed) break;
-    running += __shfl_sync(0xffffffffu, scan, 31);
+  for (uint32_t d = 1; d < 32u; d <<= 1) {
+    const double other = __shfl_up_sync(0xffffffffu, scan, d);
+    if (lane >= d) scan += other;
   }
-  if (lane == 0) out_tokens[length] = picked;
+  const uint32_t passed = __ballot_sync(0xffffffffu, own > 0.0 && running + scan > limit), holds = __ballot_sync(0xffffffffu, own > 0.0);
+  const uint32_t who = passed ? static_cast<uint32_t>(__ffs(static_cast<int>(passed))) - 1u : holds ? 31u - static_cast<uint32_t>(__clz(static_cast<int>(holds))) : 0u;
+  if (lane == who) {                           // the first element whose running sum passes, else the last that holds anything
+    double so_far = running + (scan - own);
+    uint32_t picked = 0;
+    bool found = false;
+    runs([&](uint32_t v, double p) {
+      so_far += p;
+      if (p > 0.0 && !found) {
+        picked = v;
+        found = so_far > limit;
+      }
+    });
+    out_tokens[length] = picked;
+  }
 }
 
 template <typename T>
@@ -393,7 +398,7 @@ uint32_t launch_verify(const KvipVerifyArgs& a, cudaStream_t stream) {
   const uint32_t sms = device_sm_count();
   uint32_t ctas = kMaxCluster, threads = kMostThreads;
   while (ctas > 1u && a.batch * ctas > 8u * sms) ctas /= 2u;
-const uint32_t resident = (a.batch * ctas + sms - 1) / sms;   // CTAs per SM
+  const uint32_t resident = (a.batch * ctas + sms - 1) / sms;   // CTAs per SM
   if (resident > 1u) threads = resident >= 4u ? 256u : kMostThreads / resident / 32u * 32u;
   cudaLaunchConfig_t config{};
   config.gridDim = dim3(a.batch * ctas);
