@@ -67,7 +67,7 @@ struct Control {                                        // behind the tiles in s
   float reduce[4][kGroupHeads];
   float factor[kGroupHeads], top[kGroupHeads];
   Rows rows;
-  uint32_t tmem, abort_flag, last;
+  uint32_t tmem, abort_flag, last[32];                  // per warp
 };
 
 template <uint32_t kN> struct Layout {
@@ -260,9 +260,11 @@ attend_tiles(const __grid_constant__ CUtensorMap query_map, const __grid_constan
       for (uint32_t s = 0; s < 2; ++s) { mbar_init(bar(c.scored[s]), 1); mbar_init(bar(c.taken[s]), 4 * kSides); }
       mbar_init(bar(c.weighted), 4 * kSides); mbar_init(bar(c.query_full), 1);
       c.abort_flag = 0;
-      c.last = 0;
       asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
       fence_async();
+      expect_bytes(bar(c.query_full), kPieces * kN * 128u);   // waited for in any case: by this warp
+      for (uint32_t piece = 0; piece < kPieces; ++piece)
+        load_query(base + Layout<kN>::kQuery + piece * (kN * 128u), &query_map, piece * 64u, head0, t, bar(c.query_full));
     }
     __syncwarp();
     // all of tensor memory: one CTA per SM
@@ -281,21 +283,15 @@ attend_tiles(const __grid_constant__ CUtensorMap query_map, const __grid_constan
       if (list[k] >= 0) last = k + 1u;
   }
   last = __reduce_max_sync(0xffffffffu, last);
+  if (lane == 0) c.last[warp] = last;
   fence_before();
   __syncthreads();
   fence_after();
   const Rows rows = c.rows;
-  if (rows.request >= 0 && warp == kScoreWarp && elect_one()) {   // waited for in any case: by this warp
-    expect_bytes(bar(c.query_full), kPieces * kN * 128u);
-    for (uint32_t piece = 0; piece < kPieces; ++piece)
-      load_query(base + Layout<kN>::kQuery + piece * (kN * 128u), &query_map, piece * 64u, head0, t, bar(c.query_full));
-  }
-  __syncwarp();
-  if (lane == 0 && last && rows.limit) atomicMax(&c.last, last);
-  __syncthreads();
+  last = __reduce_max_sync(0xffffffffu, lane < kScoreWarp ? c.last[lane] : 0u);
   const uint32_t tmem = c.tmem;
   // tiles of the list, then one of the drafted rows
-  const uint32_t listed = c.last, list_tiles = (listed + kTile - 1) / kTile, tiles = list_tiles + (rows.drafted ? 1u : 0u);
+  const uint32_t listed = rows.limit ? last : 0u, list_tiles = (listed + kTile - 1) / kTile, tiles = list_tiles + (rows.drafted ? 1u : 0u);
   // A list may be far shorter than its entries. Up to three tiles are one CTA's: joining shares takes as long as two more of them.
   const uint32_t shares = tiles <= 3u ? 1u : splits;
   const bool idle = rows.request < 0 || split >= shares;
@@ -403,7 +399,7 @@ attend_tiles(const __grid_constant__ CUtensorMap query_map, const __grid_constan
     const bool leader = elect_one();
     auto wait = [&](const uint64_t& b, uint32_t phase) { return __all_sync(0xffffffffu, mbar_wait(bar(b), phase, waits)); };
     if (warp == kScoreWarp) {                // S^T of tile n, part by part as they come
-      bool alive = rows.request < 0 || wait(c.query_full, 0);
+      bool alive = wait(c.query_full, 0);
       for (uint32_t n = 0; alive && n < count; ++n) {
         const uint32_t s = n & 1u, phase = (n >> 1) & 1u;
         if (!wait(c.taken[s], phase ^ 1u)) break;   // the scores of tile n - 2 have been read
@@ -568,7 +564,6 @@ attend_tiles(const __grid_constant__ CUtensorMap query_map, const __grid_constan
       }
       written = true;
     }
-    if (count && !dead && !mbar_wait(bar(c.empty[(count - 1u) & 1u][kParts - 1u]), ((count - 1u) >> 1) & 1u, waits)) dead = true;
     // sums over the rows of all tiles
 #pragma unroll
     for (uint32_t j = 0; j < 2 * kBlocks; ++j) {
@@ -583,6 +578,7 @@ attend_tiles(const __grid_constant__ CUtensorMap query_map, const __grid_constan
     }
     if (!written && w == 0 && lane < 4)
       for (uint32_t j = 0; j < 2 * kBlocks; ++j) c.top[head_at + (j >> 1) * 8u + lane * 2u + (j & 1u)] = -INFINITY;
+    if (count && !dead && !mbar_wait(bar(c.empty[(count - 1u) & 1u][kParts - 1u]), ((count - 1u) >> 1) & 1u, waits)) dead = true;
     dead = role_any<kSides * kRole>(kSides + 1u, dead);
     if (dead || idle) {
       written = false;                       // a share that cannot be trusted counts as empty; the status says so
