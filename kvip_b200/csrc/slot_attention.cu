@@ -38,12 +38,10 @@ constexpr uint32_t kPieceBytes = kTile * 128;           // one piece of every ro
 constexpr uint32_t kStageBytes = kPieces * kPieceBytes; // 73,728
 constexpr uint32_t kStages = 2;
 constexpr uint32_t kGroupHeads = 64;
-constexpr uint32_t kAhead = 2;                          // tiles whose list entries a loader holds
 constexpr uint32_t kParts = 4;                          // a stage is filled, read and released in four groups of pieces: two for each block
                                                         // of 128 value elements, and with the last the piece behind the value
 __host__ __device__ constexpr uint32_t part_end(uint32_t part) { return part + 1 == kParts ? kPieces : 2 * part + 2; }
-// Softmax: four warps per 16 heads. Behind them four loaders and an issuer for each product. Tiles are loaded in order: the copy
-// engine takes about ten clocks for 128 bytes of four rows, so one tile at a time keeps it busy.
+// Softmax: four warps per 16 heads. Behind them four loaders and an issuer for each product.
 constexpr uint32_t kLoaderWarps = 4, kRole = 128, kSideHeads = 16;
 constexpr uint32_t kMaxSplits = 8;                      // CTAs of a cluster
 template <uint32_t kN> struct Warps {
@@ -63,7 +61,7 @@ struct Rows {
 };
 struct Control {                                        // behind the tiles in shared memory
   uint64_t full[kStages][kParts], empty[kStages][kParts], scored[2], taken[2], weighted, query_full;
-  uint32_t valid[kStages][4];                           // row 4 l + c of the tile is there: bit l of word c
+  uint32_t valid[kStages][kLoaderWarps];                // row 16 i + b of the tile is there: bit b of word i
   float reduce[4][kGroupHeads];
   float factor[kGroupHeads], top[kGroupHeads];
   Rows rows;
@@ -154,12 +152,13 @@ __device__ __forceinline__ float exp2_fast(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-// Four rows of a [rows, 576] tensor, 64 elements from `x` on, to `to` and the three 128-byte rows behind it (swizzled).
-__device__ __forceinline__ void load_rows(uint32_t to, const CUtensorMap* map, uint32_t x, int4 rows, uint32_t bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5, %6}], [%7];"
-      ::"r"(to), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(rows.x), "r"(rows.y), "r"(rows.z), "r"(rows.w), "r"(bar)
-      : "memory");
+// 16 bytes into shared memory, zeros where `present` is false.
+__device__ __forceinline__ void copy16(uint32_t to, uint64_t from, bool present) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(present ? 16u : 0u) : "memory");
+}
+// Arrives at the barrier when this thread's copies so far have landed.
+__device__ __forceinline__ void arrive_after_copies(uint32_t bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
 }
 __device__ __forceinline__ void load_query(uint32_t to, const CUtensorMap* map, uint32_t x, uint32_t head, uint32_t token, uint32_t bar) {
   asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
@@ -237,8 +236,7 @@ __device__ __forceinline__ Rows rows_of(const KvipAttentionArgs& a, uint32_t t) 
 
 template <typename T, uint32_t kN>
 __global__ void __launch_bounds__(Warps<kN>::kThreads, 1)
-attend_tiles(const __grid_constant__ CUtensorMap query_map, const __grid_constant__ CUtensorMap pool_map,
-             const __grid_constant__ CUtensorMap draft_map, const __grid_constant__ KvipAttentionArgs a, const uint32_t groups,
+attend_tiles(const __grid_constant__ CUtensorMap query_map, const __grid_constant__ KvipAttentionArgs a, const uint32_t groups,
              const uint32_t group_heads, const uint32_t splits) {
   constexpr uint32_t kSides = Warps<kN>::kSides, kFirstLoaderWarp = Warps<kN>::kLoader, kScoreWarp = Warps<kN>::kScore, kValueWarp = Warps<kN>::kValue;
   extern __shared__ __align__(1024) uint8_t smem[];
@@ -253,10 +251,9 @@ attend_tiles(const __grid_constant__ CUtensorMap query_map, const __grid_constan
   uint32_t last = 0;
   if (warp == kScoreWarp) {
     if (lane == 0) {
-      for (const CUtensorMap* map : {&query_map, &pool_map, &draft_map})
-        asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");
+      asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&query_map)) : "memory");
       for (uint32_t s = 0; s < kStages; ++s)
-        for (uint32_t part = 0; part < kParts; ++part) { mbar_init(bar(c.full[s][part]), kLoaderWarps); mbar_init(bar(c.empty[s][part]), 1); }
+        for (uint32_t part = 0; part < kParts; ++part) { mbar_init(bar(c.full[s][part]), 32 * kLoaderWarps + (part ? 0 : kLoaderWarps)); mbar_init(bar(c.empty[s][part]), 1); }
       for (uint32_t s = 0; s < 2; ++s) { mbar_init(bar(c.scored[s]), 1); mbar_init(bar(c.taken[s]), 4 * kSides); }
       mbar_init(bar(c.weighted), 4 * kSides); mbar_init(bar(c.query_full), 1);
       c.abort_flag = 0;
@@ -301,94 +298,64 @@ attend_tiles(const __grid_constant__ CUtensorMap query_map, const __grid_constan
   auto none = [&](uint32_t s) { return (c.valid[s][0] | c.valid[s][1] | c.valid[s][2] | c.valid[s][3]) == 0u; };
 
   if (warp >= kFirstLoaderWarp && warp < kScoreWarp) {
-    // ================= loaders: warp 8 + i gathers 16 rows, from 16 i on, of every tile =================
-    const uint32_t quarter = warp - kFirstLoaderWarp;
-    const bool leader = elect_one();
-    int32_t bad = warp == kFirstLoaderWarp ? rows.bad : 0;
-    if (count) {
-      auto entries_of = [&](uint32_t n) -> int4 {   // entries 4 lane .. + 3 of tile n (lanes 0-15), -1 behind the list
-        int4 e = make_int4(-1, -1, -1, -1);
-        const uint32_t k = (first + n) * kTile + 4u * lane;
-        if (lane < 16u && n < count && k < listed) {
-          if (vectors) {
-            e = __ldg(reinterpret_cast<const int4*>(list + k));
-          } else {
-            e.x = list[k];
-            if (k + 1u < listed) e.y = list[k + 1u];
-            if (k + 2u < listed) e.z = list[k + 2u];
-            if (k + 3u < listed) e.w = list[k + 3u];
-          }
+    // ================= loaders: each copies 16 rows of every tile =================
+    // A lane copies 16 bytes of one of four rows, so that an instruction takes whole 128-byte lines and fills all banks of
+    // four swizzled rows. Measured alone: 1253 clocks a tile from L2 on all SMs, 6.2 TB/s from HBM (tensor-map gathers of four rows: 1466
+    // and 6.1; they also hold the products back more, 67.6 against 66.5 us for 64 tokens x 128 heads).
+    const uint32_t loader = warp - kFirstLoaderWarp;
+    int32_t bad = warp == kFirstLoaderWarp && lane == 0 ? rows.bad : 0;
+    const uint64_t pool = reinterpret_cast<uint64_t>(a.pool), pool_row = pool + static_cast<uint64_t>(rows.base) * (kWidth * 2u);
+    const uint64_t draft_bytes = static_cast<uint64_t>(a.draft_token) * 2u;
+    const uint64_t draft_row = reinterpret_cast<uint64_t>(a.draft) + rows.draft * draft_bytes;
+    auto entry_of = [&](uint32_t n) -> int32_t {     // list entry of row 16 loader + lane of tile n, -1 behind the list
+      const uint32_t k = (first + n) * kTile + loader * 16u + lane;
+      return lane < 16u && n < count && k < listed ? __ldg(list + k) : -1;
+    };
+    const uint32_t unit = lane & 7u, to = base + (loader * 16u + (lane >> 3)) * 128u;
+    int32_t next = entry_of(0);
+    for (uint32_t n = 0; n < count; ++n) {
+      const uint32_t g = n & 1u, phase = ((n >> 1) & 1u) ^ 1u;
+      const int32_t slot = next;
+      next = entry_of(n + 1u);                       // lands while this tile is copied
+      uint64_t source = 0;                           // of row 16 loader + lane
+      if (first + n < list_tiles) {
+        if (slot >= 0) {
+          if (static_cast<uint32_t>(slot) < rows.limit) source = pool_row + static_cast<uint64_t>(static_cast<uint32_t>(slot)) * (kWidth * 2u);
+          else bad |= static_cast<int32_t>(KVIP_ERR_SOURCE);
         }
-        return e;
-      };
-      int4 queue[kAhead];                          // entries of the tiles n + 1 .. n + kAhead
+      } else if (lane < 16u && ((rows.seen >> (loader * 16u + lane)) & 1ull)) {
+        source = draft_row + (loader * 16u + lane) * draft_bytes;
+      }
+      const uint32_t present = __ballot_sync(0xffffffffu, source != 0);
+      uint64_t from[4];
+      bool there[4];
 #pragma unroll
-      for (uint32_t k = 0; k < kAhead; ++k) queue[k] = entries_of(k);
-      for (uint32_t n = 0; n < count; ++n) {
-        const uint32_t g = n & 1u;
-        int4 e = queue[0];
+      for (uint32_t q = 0; q < 4u; ++q) {
+        const uint64_t row = __shfl_sync(0xffffffffu, source, q * 4u + (lane >> 3));
+        there[q] = row != 0;
+        from[q] = (there[q] ? row : pool) + unit * 16u;
+      }
+      bool alive = true;
 #pragma unroll
-        for (uint32_t k = 0; k + 1 < kAhead; ++k) queue[k] = queue[k + 1];
-        queue[kAhead - 1] = entries_of(n + kAhead);   // lands while tiles are fetched
-        const bool from_list = first + n < list_tiles;
-        bool v0, v1, v2, v3;
-        if (from_list) {
-          auto check = [&](int32_t& slot) {
-            if (slot < 0) return false;
-            if (static_cast<uint32_t>(slot) >= rows.limit) { bad |= static_cast<int32_t>(KVIP_ERR_SOURCE); return false; }
-            slot = static_cast<int32_t>(rows.base + static_cast<uint32_t>(slot));
-            return true;
-          };
-          v0 = check(e.x); v1 = check(e.y); v2 = check(e.z); v3 = check(e.w);
-        } else {
-          const uint32_t bits = lane < 16u ? static_cast<uint32_t>(rows.seen >> (4u * lane)) & 15u : 0u;
-          const int32_t row = static_cast<int32_t>(rows.draft + 4u * lane);
-          e = make_int4(row, row + 1, row + 2, row + 3);
-          v0 = bits & 1u; v1 = bits & 2u; v2 = bits & 4u; v3 = bits & 8u;
+      for (uint32_t part = 0; part < kParts; ++part) {
+        alive = __all_sync(0xffffffffu, mbar_wait(bar(c.empty[g][part]), phase, waits));
+        if (!alive) break;
+        if (part == 0 && lane == 0) {                // every reader of the mask of tile n - 2 has done with it
+          c.valid[g][loader] = present;
+          mbar_arrive(bar(c.full[g][0]));
         }
-        const uint32_t b0 = __ballot_sync(0xffffffffu, v0), b1 = __ballot_sync(0xffffffffu, v1), b2 = __ballot_sync(0xffffffffu, v2),
-                       b3 = __ballot_sync(0xffffffffu, v3);
-        // a place without a row takes one of the tile's own: its weight is zero, and it holds nothing that the token does not read
-        const uint32_t any = b0 | b1 | b2 | b3, phase = ((n >> 1) & 1u) ^ 1u;
-        const int32_t mine = v0 ? e.x : v1 ? e.y : v2 ? e.z : e.w;
-        const int32_t spare = __shfl_sync(0xffffffffu, mine, (__ffs(static_cast<int>(any)) - 1) & 31);
-        if (!v0) e.x = spare;
-        if (!v1) e.y = spare;
-        if (!v2) e.z = spare;
-        if (!v3) e.w = spare;
-        int4 r[4];                                 // four times four rows
 #pragma unroll
         for (uint32_t q = 0; q < 4u; ++q) {
-          const uint32_t from = quarter * 4u + q;
-          r[q] = make_int4(__shfl_sync(0xffffffffu, e.x, from), __shfl_sync(0xffffffffu, e.y, from),
-                           __shfl_sync(0xffffffffu, e.z, from), __shfl_sync(0xffffffffu, e.w, from));
+          const uint32_t row = loader * 16u + q * 4u + (lane >> 3);
+#pragma unroll
+          for (uint32_t piece = 2u * part; piece < part_end(part); ++piece)
+            copy16(to + g * kStageBytes + piece * kPieceBytes + q * 512u + ((unit ^ (row & 7u)) << 4), from[q] + piece * 128u, there[q]);
         }
-        const CUtensorMap* map = from_list ? &pool_map : &draft_map;
-        bool alive = true;
-#pragma unroll
-        for (uint32_t part = 0; part < kParts; ++part) {
-          alive = __all_sync(0xffffffffu, mbar_wait(bar(c.empty[g][part]), phase, waits));
-          if (!alive) break;
-          if (leader) {
-            // every reader of the mask of tile n - 2 has done with it when the first part is released
-            if (part == 0 && quarter == 0) { c.valid[g][0] = b0; c.valid[g][1] = b1; c.valid[g][2] = b2; c.valid[g][3] = b3; }
-            if (any) {
-              expect_bytes(bar(c.full[g][part]), (part_end(part) - 2u * part) * kPieceBytes / kLoaderWarps);
-#pragma unroll
-              for (uint32_t q = 0; q < 4u; ++q) {
-#pragma unroll
-                for (uint32_t piece = 2u * part; piece < part_end(part); ++piece)
-                  load_rows(base + g * kStageBytes + piece * kPieceBytes + (quarter * 4u + q) * 512u, map, piece * 64u, r[q], bar(c.full[g][part]));
-              }
-            } else {
-              mbar_arrive(bar(c.full[g][part]));
-            }
-          }
-          __syncwarp();
-        }
-        if (!alive) break;
+        arrive_after_copies(bar(c.full[g][part]));
       }
+      if (!alive) break;
     }
+    asm volatile("cp.async.wait_all;" ::: "memory");
     if (bad) atomicOr(a.status, bad);
   } else if (warp >= kScoreWarp) {
     // ================= issuers: the warp walks together, one elected thread issues =================
@@ -411,6 +378,7 @@ attend_tiles(const __grid_constant__ CUtensorMap query_map, const __grid_constan
           if (!alive) break;
           fence_after();
           if (leader) {
+            fence_async();                   // the rows were written by ordinary copies
             if (!none(s)) {
 #pragma unroll
               for (uint32_t piece = 2u * part; piece < part_end(part); ++piece) {
@@ -472,8 +440,8 @@ attend_tiles(const __grid_constant__ CUtensorMap query_map, const __grid_constan
         else if (lane == 0) mbar_arrive(bar(c.weighted));
         continue;
       }
-      const uint32_t word = c.valid[s][row0 & 3u];
-      const bool has0 = (word >> (row0 >> 2)) & 1u, has1 = (word >> ((row0 >> 2) + 2u)) & 1u;
+      const uint32_t word = c.valid[s][w] >> (lane >> 2);
+      const bool has0 = word & 1u, has1 = (word >> 8) & 1u;
       uint32_t v[4 * kBlocks];
       if (ok) {
         fence_after();
@@ -728,16 +696,15 @@ EncodeTiledFn encode_fn() {
   }();
   return fn;
 }
-// [planes, rows, 576] elements of two bytes, boxes of 64 elements x box_rows rows in 128-byte swizzle; strides in elements.
-bool encode_map(CUtensorMap* map, bool bf16, const void* base, uint32_t dims, uint64_t rows, uint64_t planes, int64_t row, int64_t plane,
-                uint32_t box_rows) {
+// Queries [tokens, heads, 576] of two-byte elements, boxes of 64 elements x box_heads in 128-byte swizzle; strides in elements.
+bool encode_queries(CUtensorMap* map, bool bf16, const void* base, uint64_t heads, uint64_t tokens, int64_t head, int64_t token, uint32_t box_heads) {
   EncodeTiledFn fn = encode_fn();
   if (!fn) return false;
-  const cuuint64_t sizes[3] = {kWidth, rows, planes};
-  const cuuint64_t strides[2] = {static_cast<cuuint64_t>(row) * 2u, static_cast<cuuint64_t>(plane) * 2u};
-  const cuuint32_t box[3] = {64, box_rows, 1}, step[3] = {1, 1, 1};
-  return fn(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, dims, const_cast<void*>(base), sizes, strides, box,
-            step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+  const cuuint64_t sizes[3] = {kWidth, heads, tokens};
+  const cuuint64_t strides[2] = {static_cast<cuuint64_t>(head) * 2u, static_cast<cuuint64_t>(token) * 2u};
+  const cuuint32_t box[3] = {64, box_heads, 1}, step[3] = {1, 1, 1};
+  return fn(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void*>(base), sizes, strides, box, step,
+            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
@@ -763,20 +730,17 @@ uint32_t configure(cudaLaunchConfig_t& config, cudaLaunchAttribute& cluster, Ker
 template <typename T, uint32_t kN>
 uint32_t launch_tiles(const KvipAttentionArgs& a, KernelSlot slot, uint32_t groups, uint32_t group_heads, uint32_t splits, cudaStream_t stream) {
   const bool bf16 = __is_same(T, __nv_bfloat16);
-  CUtensorMap query_map, pool_map, draft_map;
+  CUtensorMap query_map;
   // strides of a dimension of size one do not matter, but the encoder looks at them
   const int64_t head = a.heads > 1 ? a.query_head : kWidth, token = a.tokens > 1 ? a.query_token : a.heads * kWidth;
-  const int64_t drafted = a.draft && a.tokens > 1 ? a.draft_token : kWidth;
-  if (!encode_map(&query_map, bf16, a.query, 3, a.heads, a.tokens, head, token, kN) ||
-      !encode_map(&pool_map, bf16, a.pool, 2, a.pool_rows, 1, kWidth, 0, 1) ||
-      !encode_map(&draft_map, bf16, a.draft ? a.draft : a.query, 2, a.tokens, 1, drafted, 0, 1)) {
+  if (!encode_queries(&query_map, bf16, a.query, a.heads, a.tokens, head, token, kN)) {
     set_error("slot_attention: the strides do not fit a tensor map");
     return KVIP_BAD_ARGUMENT;
   }
   cudaLaunchConfig_t config;
   cudaLaunchAttribute cluster;
   if (uint32_t bad = configure<T, kN>(config, cluster, slot, a.tokens * groups * splits, splits, stream)) return bad;
-  cudaLaunchKernelEx(&config, attend_tiles<T, kN>, query_map, pool_map, draft_map, a, groups, group_heads, splits);
+  cudaLaunchKernelEx(&config, attend_tiles<T, kN>, query_map, a, groups, group_heads, splits);
   count_launch();
   return check_launch("attend_tiles");
 }
