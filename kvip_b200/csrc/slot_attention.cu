@@ -18,11 +18,11 @@
 // p is rounded to the rows' type for the second product (half a step, as the output is); its sum is taken before the
 // rounding, in fp32, because the log-sum is an output too.
 //
-// Bound, at 64 heads per CTA, by the loop of the two stages that shared memory holds beside the queries: a tile's rows need 3300
-// clocks to land while the other tile's products read shared memory (1253 alone), 1200 more until its scores are complete, 1300 for the
-// softmax and 700 until the value product lets go: 6460 clocks for two tiles, the tensor pipe busy in 52 % of them, operand reads in 48 %.
-// At 16 heads by HBM. Measured on one B200: 64 tokens x 128 heads x 2048 rows 66.5 us (36.5 GFLOP, 169 MB once; 45 us with the loads
-// alone), 128 tokens x 16 heads 62 us (4.9 TB/s of rows), one token x 128 heads 14.6 us.
+// Bound, at 64 heads per CTA, by the loop of the two stages that shared memory holds beside the queries: a tile's rows need 3370
+// clocks to land while the other tile's products run (1253 for the copies alone), 1080 more until its scores are complete, 1340 for
+// the softmax and 680 until the value product lets go: 6470 clocks for two tiles. The tensor pipe is busy in 53 % of a CTA's cycles. At
+// 16 heads by HBM. Measured on one B200: 64 tokens x 128 heads x 2048 rows 66.4 us (36.5 GFLOP, 169 MB once), 128 tokens x 16 heads
+// 61.7 us (4.9 TB/s of rows), one token x 128 heads 14.5 us.
 #include <atomic>
 #include <cuda.h>
 #include <cuda_bf16.h>
