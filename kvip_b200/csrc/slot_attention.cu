@@ -431,24 +431,17 @@ attend_tiles(const __grid_constant__ CUtensorMap query_map, const __grid_constan
       const uint32_t s = n & 1u, phase = (n >> 1) & 1u;
       bool ok = !dead && mbar_wait(bar(c.scored[s]), phase, waits) && mbar_wait(bar(c.full[s][0]), phase, waits);
       ok = __all_sync(0xffffffffu, ok);
-      if (ok && none(s)) {
-        if (lane == 0) mbar_arrive(bar(c.taken[s]));
-        // the same for all: the mask belongs to the tile
-        // as below: a thread arrives for this tile only when all have arrived for the one before
-        if (n && !mbar_wait(bar(c.empty[(n - 1u) & 1u][kParts - 1u]), ((n - 1u) >> 1) & 1u, waits)) dead = true;
-        __syncwarp();
-        if (__any_sync(0xffffffffu, dead)) dead = true;
-        else if (lane == 0) mbar_arrive(bar(c.weighted));
-        continue;
-      }
+      const bool empty = ok && none(s);        // the same for all that could wait: the mask belongs to the tile
       const uint32_t word = c.valid[s][w] >> (lane >> 2);
       const bool has0 = word & 1u, has1 = (word >> 8) & 1u;
       uint32_t v[4 * kBlocks];
       if (ok) {
-        fence_after();
-        tmem_ld_blocks(tmem + quad + kScores + s * kN + head_at, v);
-        tmem_ld_done();
-        fence_before();
+        if (!empty) {
+          fence_after();
+          tmem_ld_blocks(tmem + quad + kScores + s * kN + head_at, v);
+          tmem_ld_done();
+          fence_before();
+        }
         __syncwarp();
         if (lane == 0) mbar_arrive(bar(c.taken[s]));
       }
@@ -457,10 +450,11 @@ attend_tiles(const __grid_constant__ CUtensorMap query_map, const __grid_constan
       bool above = false;
 #pragma unroll
       for (uint32_t j = 0; j < 4 * kBlocks; ++j) {
-        const bool has = (j & 2u) ? has1 : has0;
+        const bool has = ok && ((j & 2u) ? has1 : has0);
         x[j] = has ? __uint_as_float(v[j]) * scale : -INFINITY;
         above |= x[j] - ref[(j >> 2) * 2u + (j & 1u)] > kSlack;
       }
+      // an empty tile is voted on too: a warp whose wait ran out does not know that it is one
       if (role_any(1u + side, above || !ok)) {
         if (role_any(1u + side, !ok)) { dead = true; break; }
 #pragma unroll
@@ -504,6 +498,13 @@ attend_tiles(const __grid_constant__ CUtensorMap query_map, const __grid_constan
             dead = true;
           }
         }
+      }
+      if (empty) {
+        // as below: a thread arrives for this tile only when all have arrived for the one before
+        if (n && !dead && !mbar_wait(bar(c.empty[(n - 1u) & 1u][kParts - 1u]), ((n - 1u) >> 1) & 1u, waits)) dead = true;
+        dead = __any_sync(0xffffffffu, dead);
+        if (!dead && lane == 0) mbar_arrive(bar(c.weighted));
+        continue;
       }
       uint32_t p[2 * kBlocks];                 // weights of a row, two heads in a word: row 0 then row 1
 #pragma unroll

@@ -510,6 +510,25 @@ def test_attention_bounded_waits_give_up_and_report(device):
         assert int(attend.status.item()) == 0
 
 
+@pytest.mark.parametrize("heads", [16, 64])
+def test_attention_bounded_waits_over_tiles_without_rows(device, heads):
+    """Whole tiles of slots that name no row, the last one too, under wait limits from nothing to enough: warps whose wait ran out and warps
+    that found the tile empty end the call together."""
+    import kvip_b200 as kvip
+    case = attention_case(device, 40, counts=[2, 1], heads=heads, entries=1024, stride=1024, context=[1024, 1024], draft=False)
+    for tile in (0, 3, 4, 9, 15):
+        case["slots"][:, 64 * tile:64 * tile + 64] = 1024 + 7            # behind the request's slots
+    attend = kvip.SlotAttention(torch, device, tokens=3, heads=heads)
+    for splits in (1, 4):
+        for limit in (1, 2, 3, 5, 8, 13, 21):
+            attend(**case, splits=splits, wait_kilocycles=limit)
+            torch.cuda.synchronize()
+            attend.status.zero_()
+        out, lse = attend(**case, splits=splits)
+        check_attention(case, out, lse)
+        assert int(attend.status.item()) == 64        # KVIP_ERR_SOURCE: a slot outside the request
+
+
 def test_attention_on_two_streams_with_outputs_of_their_own(device):
     """One object, two streams, outputs given by the caller: nothing is shared."""
     import kvip_b200 as kvip
