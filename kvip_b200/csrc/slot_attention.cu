@@ -21,8 +21,8 @@
 // Bound, at 64 heads per CTA, by the loop of the two stages that shared memory holds beside the queries: a tile's rows need 3370
 // clocks to land while the other tile's products run (1253 for the copies alone), 1080 more until its scores are complete, 1340 for
 // the softmax and 680 until the value product lets go: 6470 clocks for two tiles. The tensor pipe is busy in 53 % of a CTA's cycles. At
-// 16 heads by HBM. Measured on one B200: 64 tokens x 128 heads x 2048 rows 66.4 us (36.5 GFLOP, 169 MB once), 128 tokens x 16 heads
-// 61.7 us (4.9 TB/s of rows), one token x 128 heads 14.5 us.
+// 16 heads by HBM. Measured on one B200: 64 tokens x 128 heads x 2048 rows 64.9 us (36.5 GFLOP, 169 MB once), 128 tokens x 16 heads
+// 61.7 us (4.9 TB/s of rows), one token x 128 heads 14.3 us.
 #include <atomic>
 #include <cuda.h>
 #include <cuda_bf16.h>
@@ -454,6 +454,12 @@ attend_tiles(const __grid_constant__ CUtensorMap query_map, const __grid_constan
         x[j] = has ? __uint_as_float(v[j]) * scale : -INFINITY;
         above |= x[j] - ref[(j >> 2) * 2u + (j & 1u)] > kSlack;
       }
+      // Weights against the reference as it stands: on their way while the warps agree that it may stand.
+      float e[4 * kBlocks];
+#pragma unroll
+      for (uint32_t j = 0; j < 4 * kBlocks; ++j) e[j] = exp2_fast(x[j] - ref[(j >> 2) * 2u + (j & 1u)]);
+      // the product of the tile before has read its weights, and every tile before is in the accumulators
+      if (n && ok) ok = mbar_wait(bar(c.empty[(n - 1u) & 1u][kParts - 1u]), ((n - 1u) >> 1) & 1u, waits);
       // an empty tile is voted on too: a warp whose wait ran out does not know that it is one
       if (role_any(1u + side, above || !ok)) {
         if (role_any(1u + side, !ok)) { dead = true; break; }
@@ -477,61 +483,47 @@ attend_tiles(const __grid_constant__ CUtensorMap query_map, const __grid_constan
           if (w == 0 && lane < 4) c.factor[h] = factor;
         }
         role_any(1u + side, false);
-        if (written) {                         // the accumulators hold the tiles before this one, which must be in
-          const uint32_t before = n - 1u;      // stages are released in order, an empty tile's too
-          ok = mbar_wait(bar(c.empty[before & 1u][kParts - 1u]), (before >> 1) & 1u, waits);
-          if (__all_sync(0xffffffffu, ok)) {
-            fence_after();
-            for (uint32_t m = 0; m < 4; ++m) {
+        if (written) {                         // the accumulators hold the tiles before this one
+          fence_after();
+          for (uint32_t m = 0; m < 4; ++m) {
 #pragma unroll
-              for (uint32_t h = head_at; h < head_at + kSideHeads; h += 8) {
-                uint32_t o[8];
-                tmem_ld_rows(tmem + quad + kOut + m * kN + h, o);
-                tmem_ld_done();
+            for (uint32_t h = head_at; h < head_at + kSideHeads; h += 8) {
+              uint32_t o[8];
+              tmem_ld_rows(tmem + quad + kOut + m * kN + h, o);
+              tmem_ld_done();
 #pragma unroll
-                for (uint32_t i = 0; i < 8; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * c.factor[h + i]);
-                tmem_st_rows(tmem + quad + kOut + m * kN + h, o);
-              }
+              for (uint32_t i = 0; i < 8; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * c.factor[h + i]);
+              tmem_st_rows(tmem + quad + kOut + m * kN + h, o);
             }
-            tmem_st_done();
-          } else {
-            dead = true;
           }
+          tmem_st_done();
         }
+#pragma unroll
+        for (uint32_t j = 0; j < 4 * kBlocks; ++j) e[j] = exp2_fast(x[j] - ref[(j >> 2) * 2u + (j & 1u)]);
       }
       if (empty) {
-        // as below: a thread arrives for this tile only when all have arrived for the one before
-        if (n && !dead && !mbar_wait(bar(c.empty[(n - 1u) & 1u][kParts - 1u]), ((n - 1u) >> 1) & 1u, waits)) dead = true;
-        dead = __any_sync(0xffffffffu, dead);
-        if (!dead && lane == 0) mbar_arrive(bar(c.weighted));
+        if (lane == 0) mbar_arrive(bar(c.weighted));
         continue;
       }
       uint32_t p[2 * kBlocks];                 // weights of a row, two heads in a word: row 0 then row 1
 #pragma unroll
       for (uint32_t j = 0; j < kBlocks; ++j) {
-        const float x0 = exp2_fast(x[4 * j] - ref[2 * j]), y0 = exp2_fast(x[4 * j + 1] - ref[2 * j + 1]);
-        const float x1 = exp2_fast(x[4 * j + 2] - ref[2 * j]), y1 = exp2_fast(x[4 * j + 3] - ref[2 * j + 1]);
-        sum[2 * j] += x0 + x1;
-        sum[2 * j + 1] += y0 + y1;
-        p[2 * j] = pack_pair<T>(x0, y0);
-        p[2 * j + 1] = pack_pair<T>(x1, y1);
+        sum[2 * j] += e[4 * j] + e[4 * j + 2];
+        sum[2 * j + 1] += e[4 * j + 1] + e[4 * j + 3];
+        p[2 * j] = pack_pair<T>(e[4 * j], e[4 * j + 1]);
+        p[2 * j + 1] = pack_pair<T>(e[4 * j + 2], e[4 * j + 3]);
       }
-      // the product of the tile before has read its weights
-      if (n && !dead && !mbar_wait(bar(c.empty[(n - 1u) & 1u][kParts - 1u]), ((n - 1u) >> 1) & 1u, waits)) dead = true;
-      dead = __any_sync(0xffffffffu, dead);
-      if (!dead) {
-        const uint32_t to = base + Layout<kN>::kWeights + row0 * 128u + (lane & 3u) * 4u;
+      const uint32_t to = base + Layout<kN>::kWeights + row0 * 128u + (lane & 3u) * 4u;
 #pragma unroll
-        for (uint32_t j = 0; j < kBlocks; ++j) {
-          const uint32_t at = to + (((side * kBlocks + j) ^ (row0 & 7u)) << 4);   // row0 + 8 has the same swizzle
-          asm volatile("st.shared.b32 [%0], %1;" ::"r"(at), "r"(p[2 * j]) : "memory");
-          asm volatile("st.shared.b32 [%0], %1;" ::"r"(at + 1024u), "r"(p[2 * j + 1]) : "memory");
-        }
-        fence_async();
-        fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(bar(c.weighted));
+      for (uint32_t j = 0; j < kBlocks; ++j) {
+        const uint32_t at = to + (((side * kBlocks + j) ^ (row0 & 7u)) << 4);   // row0 + 8 has the same swizzle
+        asm volatile("st.shared.b32 [%0], %1;" ::"r"(at), "r"(p[2 * j]) : "memory");
+        asm volatile("st.shared.b32 [%0], %1;" ::"r"(at + 1024u), "r"(p[2 * j + 1]) : "memory");
       }
+      fence_async();
+      fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar(c.weighted));
       written = true;
     }
     // sums over the rows of all tiles
