@@ -258,9 +258,10 @@ __global__ void __launch_bounds__(kMostThreads, 1) verify_walk(const __grid_cons
   constexpr uint32_t kRun = Run<T>::kCount;
   const uint32_t V = a.vocabulary, warps = blockDim.x >> 5, shares = ctas * warps;
   const uint32_t share = ((V + shares - 1) / shares + kRun - 1u) / kRun * kRun;
-  uint32_t node = 0, length = 0, rejected = 0, pass = 0;
+  // A node's rejected tokens lie behind those of the nodes before it: a warp that is still at an earlier test finds its own untouched.
+  uint32_t node = 0, length = 0, rejected = 0, lost = 0, pass = 0;
   double mass = 1.0, taken = 0.0;          // of what is left at the node, and of all before
-  auto losses = [&]() { return Losses{taken, s_lost, rejected, draft != nullptr}; };
+  auto losses = [&]() { return Losses{taken, s_lost + lost, rejected, draft != nullptr}; };
   auto part_sum = [&](uint32_t from, uint32_t to) -> double {
     const T* row = target + node * a.target_row;
     return sum_between<T>(row, draft ? draft + node * a.draft_row : row, from, to, losses());
@@ -272,6 +273,7 @@ __global__ void __launch_bounds__(kMostThreads, 1) verify_walk(const __grid_cons
     double* part = s_part[pass & 1u];
     const uint32_t each = (shares + 31u) / 32u;
     if (lane < ctas) store_remote(&part[place_of(mine, each)], lane, sum);
+    __syncwarp();
     cluster_barrier();
     double total = 0.0;
     for (uint32_t i = 0; i < each; ++i) total += lane * each + i < shares ? part[i * 32u + lane] : 0.0;
@@ -290,18 +292,19 @@ __global__ void __launch_bounds__(kMostThreads, 1) verify_walk(const __grid_cons
       r = remaining(r, s_q[j], taken);
     } else {
       for (uint32_t i = 0; i < rejected; ++i)
-        if (s_lost[i] == s_token[j]) r = 0.0;
+        if (s_lost[lost + i] == s_token[j]) r = 0.0;
     }
     if (__dmul_rn(__dmul_rn(static_cast<double>(s_accept[j]), s_q[j]), mass) < r) {
       if (lane == (length & 31u)) { if (length < 32u) path = j; else path_high = j; }
       node = j;
       ++length;
+      lost += rejected;
       rejected = 0;
       mass = 1.0;
       taken = 0.0;
       summed = false;
     } else {
-      if (tid == 0) s_lost[rejected] = s_token[j];
+      if (tid == 0) s_lost[lost + rejected] = s_token[j];
       __syncthreads();
       ++rejected;
       taken += mass;

@@ -643,6 +643,26 @@ def test_verify_matches_the_walk(device, counts, vocabulary, kind, draft, tree, 
                                  near=(0.1, 0.7, 3.0)[seed], pad=pad), device, depth)
 
 
+@pytest.mark.parametrize("lift,most,deepest", [(2.5, 1.0, 2), (6.0, 0.4, 4)])
+def test_verify_without_draft_rows_repeated_tokens(device, lift, most, deepest):
+    """Deep trees over three tokens with certain drafts: every request accepts and rejects in turn, siblings and levels repeat tokens, so the
+    rejected tokens of a node decide the next test. Passes over 24 tokens are short, so warps run close behind one another."""
+    rng = np.random.default_rng(77)
+    g = torch.Generator(device=device)
+    g.manual_seed(77)
+    counts = [64] * 48
+    case = verify_case(device, 77, counts=counts, vocabulary=24, draft=False)
+    logits = torch.randn((64 * 48, 24), generator=g, device=device)
+    logits[:, :3] += lift
+    case["target"].copy_(torch.softmax(logits, 1))
+    case["tokens"] = torch.from_numpy(rng.integers(0, 3, 64 * 48)).to(device)
+    accepted = 0
+    for _ in range(20):
+        case["accept"] = torch.rand(64 * 48, generator=g, device=device) * most
+        accepted = max(accepted, int(check_verify(case, device, 63)[2].max()) - 1)
+    assert accepted >= deepest             # walks that go on behind rejections
+
+
 def test_verify_borders(device):
     """Numbers at the ends of [0, 1), distributions with one token, a draft equal to its target, rows of nothing."""
     counts, vocabulary = [3] * 8, 300
