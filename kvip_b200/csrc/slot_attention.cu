@@ -549,7 +549,7 @@ attend_tiles(const __grid_constant__ CUtensorMap query_map, const __grid_constan
     fence_after();
     if (tid < heads) {
       const float total = (c.reduce[0][tid] + c.reduce[1][tid]) + (c.reduce[2][tid] + c.reduce[3][tid]);
-      if (shares > 1) c.factor[tid] = total;
+      if (shares > 1) c.factor[tid] = written ? total : 0.f;   // no rows: no mass; scores of NaN have a mass of NaN
       else c.factor[tid] = written ? 1.f / total : 0.f;
       if (shares == 1 && !idle && !dead)
         a.lse[static_cast<uint64_t>(t) * a.heads + head0 + tid] = written ? (c.top[tid] + log2f(total)) * 0.6931471805599453f : -INFINITY;
@@ -645,19 +645,19 @@ attend_tiles(const __grid_constant__ CUtensorMap query_map, const __grid_constan
           }
 #pragma unroll
           for (uint32_t i = 0; i < 4; ++i) {
-            if (tops[s0 + i] == -INFINITY) continue;                      // no such share, or an empty one: it has written nothing
+            if (s0 + i >= shares || sums[i] == 0.f) continue;             // no such share, or an empty one: it has written nothing
             const float weight = exp2_fast(tops[s0 + i] - top);
             total = fmaf(weight, sums[i], total);
             y[0] = fmaf(weight, low[i].x, y[0]); y[1] = fmaf(weight, low[i].y, y[1]); y[2] = fmaf(weight, low[i].z, y[2]); y[3] = fmaf(weight, low[i].w, y[3]);
             y[4] = fmaf(weight, high[i].x, y[4]); y[5] = fmaf(weight, high[i].y, y[5]); y[6] = fmaf(weight, high[i].z, y[6]); y[7] = fmaf(weight, high[i].w, y[7]);
           }
         }
-        const float inverse = top == -INFINITY ? 0.f : 1.f / total;
+        const float inverse = total == 0.f ? 0.f : 1.f / total;
         const uint64_t row = static_cast<uint64_t>(t) * a.heads + head0 + h;
         T* out = static_cast<T*>(a.out) + row * kValue + element;
         *reinterpret_cast<uint2*>(out) = make_uint2(pack_pair<T>(y[0] * inverse, y[1] * inverse), pack_pair<T>(y[2] * inverse, y[3] * inverse));
         *reinterpret_cast<uint2*>(out + 128) = make_uint2(pack_pair<T>(y[4] * inverse, y[5] * inverse), pack_pair<T>(y[6] * inverse, y[7] * inverse));
-        if (!(item & 1u) && lane == 0) a.lse[row] = top == -INFINITY ? -INFINITY : (top + log2f(total)) * 0.6931471805599453f;
+        if (!(item & 1u) && lane == 0) a.lse[row] = total == 0.f ? -INFINITY : (top + log2f(total)) * 0.6931471805599453f;
       }
     }
     cluster_barrier();                       // nobody leaves while its share is being read

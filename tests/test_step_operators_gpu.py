@@ -529,6 +529,27 @@ def test_attention_bounded_waits_over_tiles_without_rows(device, heads):
         assert int(attend.status.item()) == 64        # KVIP_ERR_SOURCE: a slot outside the request
 
 
+@pytest.mark.parametrize("splits", [1, 2, 8])
+@pytest.mark.parametrize("heads", [16, 64])
+def test_attention_a_query_of_nan_stays_one(device, heads, splits):
+    """NaN in one head's query makes that head's row and lse NaN, however its rows are shared out; the other heads do not notice."""
+    import kvip_b200 as kvip
+    case = attention_case(device, 41, counts=[2, 1], heads=heads, entries=640, stride=1024, context=[640, 500])
+    clean = dict(case, query=case["query"].clone())
+    case["query"][1, 5, 17] = float("nan")
+    case["query"][2, 0] = float("nan")
+    attend = kvip.SlotAttention(torch, device, tokens=3, heads=heads)
+    out, lse = attend(**case, splits=splits)
+    hit = torch.zeros((3, heads), dtype=torch.bool, device=device)
+    hit[1, 5] = hit[2, 0] = True
+    assert torch.equal(out.isnan().all(-1), hit) and torch.equal(out.isnan().any(-1), hit) and torch.equal(lse.isnan(), hit)
+    out, lse = out.clone(), lse.clone()
+    fine_out, fine_lse = attend(**clean, splits=splits)
+    check_attention(clean, fine_out, fine_lse)
+    out[hit], lse[hit] = fine_out[hit], fine_lse[hit]
+    check_attention(clean, out, lse)
+
+
 def test_attention_on_two_streams_with_outputs_of_their_own(device):
     """One object, two streams, outputs given by the caller: nothing is shared."""
     import kvip_b200 as kvip
