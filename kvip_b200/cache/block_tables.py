@@ -88,7 +88,8 @@ class BlockTables:
 
     def release(self, rows):
         """Requests that have ended (host list of row numbers): their blocks return to the free list, their rows are
-        empty. Fixed shapes, no device read on the host."""
+        empty. Fixed shapes, no device read on the host. Blocks that the list has no place for (rows of `load` that hold more than was
+        taken from it, or a block twice) are dropped, and `status` says KVIP_ERR_NO_SLOT."""
         rows = sorted(set(int(r) for r in rows))
         if not rows:
             return
@@ -101,12 +102,16 @@ class BlockTables:
         mine = (page[None, :] < held[:, None]).reshape(-1)
         order = mine.cumsum(0)
         total = order[-1:]
-        # the list grows downwards from head; entries that are no block go to a place that is written back as it was
-        place = torch.where(mine, self.head.long() - total + order - 1, self.blocks)
+        # the list grows downwards from head; entries that are no block, and blocks that the list has no place for (a state
+        # whose rows hold more than was taken from it), go to a place behind it
+        place = self.head.long() - total + order - 1
+        fits = mine & (place >= 0) & (place < self.blocks)
         longer = torch.cat((self.free[:self.blocks], self.free[:1]))
-        longer.scatter_(0, place, torch.where(mine, table.reshape(-1), longer[-1]))
+        longer.scatter_(0, torch.where(fits, place, self.blocks), torch.where(fits, table.reshape(-1), longer[-1]))
         self.free[:self.blocks].copy_(longer[:-1])
-        self.head.sub_(total.to(torch.int32))
+        self.head.sub_(total.to(torch.int32)).clamp_(min=0)
+        lost = (mine & ~fits).any().to(torch.int32) * _lib.ERR_NO_SLOT
+        self.status.bitwise_or_(lost)
         self.table[index] = -1
         self.held[index] = 0
         self.lengths[index] = 0

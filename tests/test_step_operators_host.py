@@ -108,6 +108,29 @@ def test_objects_refuse_the_cpu_and_bad_geometry():
             make()
 
 
+@pytest.mark.parametrize("head,status", [(3, 0), (2, 4), (0, 4), (9, 4)])
+def test_released_blocks_find_a_place_in_the_list_or_are_reported(head, status):
+    """`release` with host tensors: a list that has handed out three blocks takes three back; one that has handed out fewer (rows loaded
+    with blocks from elsewhere), or whose head lies behind its end, drops what has no place and says so."""
+    from kvip_b200 import BlockTables
+    tables = BlockTables.__new__(BlockTables)
+    tables.torch, tables.device, tables.batch, tables.blocks, tables.pages = torch, torch.device("cpu"), 2, 6, 4
+    tables.table = torch.tensor([[7, 8, -1, -1], [9, -1, -1, -1]], dtype=torch.int32)
+    tables.held, tables.lengths = torch.tensor([2, 1], dtype=torch.int32), torch.tensor([20, 3], dtype=torch.int32)
+    tables.free, tables.head = torch.arange(100, 106, dtype=torch.int32), torch.tensor([head], dtype=torch.int32)
+    tables.status = torch.zeros(1, dtype=torch.int32)
+    tables.release([0, 1])
+    assert int(tables.status) == status
+    assert int(tables.head) == max(0, head - 3) and int(tables.held.sum()) == 0 and int(tables.table.max()) == -1
+    free = tables.free.tolist()
+    if head == 3:
+        assert free == [7, 8, 9, 103, 104, 105]
+    elif head == 2:
+        assert free == [8, 9, 102, 103, 104, 105]
+    else:
+        assert free == list(range(100, 106))
+
+
 def test_rotary_frequencies():
     for width in (2, 64, 128):
         for scaling in (None, {"kind": "linear", "factor": 8.0}, {"kind": "yarn", "factor": 40.0, "original": 4096},
