@@ -660,7 +660,7 @@ typedef struct KvipRotaryArgs {
   const void* x[2];            /* the second may be NULL */
   void* y[2];                  /* rows of the same type; with codes NULL */
   uint8_t* codes;              /* [tokens, heads[0], dim] FP8 e4m3: rotate the first `width` of `dim` elements of x[0] and */
-  float* scales;               /* [tokens, heads[0]] quantise the row with scale = amax / 448 (1 for a row of zeros) */
+  float* scales;               /* [tokens, heads[0]] quantise the row with scale = amax / 448, at least 2^-126 (1 for a row of zeros) */
   int64_t x_token[2], x_head[2], y_token[2], y_head[2];
   uint32_t heads[2];
   uint32_t tokens, width, dim, layout, dtype;

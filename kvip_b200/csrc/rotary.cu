@@ -15,6 +15,8 @@ namespace kvip {
 namespace {
 
 constexpr uint32_t kRotaryThreads = 256;
+// Scale of a quantised row. Not below 2^-126, whose reciprocal is finite: beneath it zeros would become 0 * inf.
+__device__ __forceinline__ float row_scale(float amax) { return amax > 0.f ? fmaxf(amax / 448.f, 1.17549435e-38f) : 1.f; }
 
 template <typename T> __device__ __forceinline__ float to_float(T v);
 template <> __device__ __forceinline__ float to_float(float v) { return v; }
@@ -86,7 +88,8 @@ __global__ void __launch_bounds__(kRotaryThreads) quantise_rows(const KvipRotary
       if (pass == 0) {
 #pragma unroll
         for (uint32_t o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-        if (amax > 0.f) { scale = amax / 448.f; inverse = 1.f / scale; }
+        scale = row_scale(amax);
+        inverse = 1.f / scale;
         if (lane == 0) a.scales[r] = scale;
       }
     }
@@ -205,7 +208,7 @@ __global__ void __launch_bounds__(kRotaryThreads) quantise_units(const __grid_co
 #pragma unroll
     for (uint32_t o = kLanes / 2u; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
     if (!live) continue;
-    const float scale = amax > 0.f ? amax / 448.f : 1.f, inverse = 1.f / scale;
+    const float scale = row_scale(amax), inverse = 1.f / scale;
     const uint64_t r = static_cast<uint64_t>(token) * a.heads[0] + row;
     uint32_t packed[4];
 #pragma unroll

@@ -82,7 +82,8 @@ class Rotary:
     def __call__(self, positions, query, key=None, *, query_out=None, key_out=None):
         """Rotate `query` (and `key`), in place or into `query_out` / `key_out`. Rows are [tokens, heads, width] or
         [tokens, width] views with any strides (bf16, fp16 or fp32); positions int64 [tokens], and the rows of a token with
-        a negative position (padding) are not written. Returns (query_out, key_out)."""
+        a negative position (padding) are not written. Outputs that are not in place, and query and key, have no
+        element in common. Returns (query_out, key_out)."""
         tokens = self._tokens(positions)
         kind = query.dtype
         if kind not in self.types:
@@ -112,7 +113,7 @@ class Rotary:
 
     def quantise(self, positions, rows, codes=None, scales=None):
         """Rotate the first `width` elements of every row and quantise the whole row: rows [tokens, heads, dim] ->
-        (codes [tokens, heads, dim] float8_e4m3fn, scales [tokens, heads] float32) with scale = amax / 448 (1 for a row of
+        (codes [tokens, heads, dim] float8_e4m3fn, scales [tokens, heads] float32) with scale = amax / 448, at least 2^-126 (1 for a row of
         zeros), the rule of `IndexCacheStorage.ingest_decode`. Rows of tokens with a negative position are not written.
         Without `codes` / `scales` the outputs are allocated."""
         torch = self.torch

@@ -254,6 +254,27 @@ def test_rotary_quantised_rows(device, tokens, heads, dim, width, layout, kind, 
     assert (np.abs(got).max(-1)[amax > 0] == 448).all() and (got[-1, -1] == 0).all() and got_scale[-1, -1] == 1
 
 
+@pytest.mark.parametrize("dim", [128, 70])
+@pytest.mark.parametrize("kind", [torch.bfloat16, torch.float32])
+def test_rotary_quantised_rows_near_the_smallest_numbers(device, kind, dim):
+    """Rows whose largest element is anything from 2^-133 to 2^-110, among zeros, at position 0 (nothing turns: cos 1, sin 0). Zeros stay
+    zeros; every element comes back within its e4m3 rounding, 2^-4 relative or half of the smallest step 2^-9 in units of the scale, and
+    two fp32 roundings (the reciprocal and the product, 2^-23 together)."""
+    import kvip_b200 as kvip
+    exponents = torch.arange(-133, -109, dtype=torch.float64)
+    rows = torch.zeros((exponents.numel(), 2, dim), dtype=torch.float64)
+    rows[:, 0, ::3] = torch.linspace(-1, 1, len(range(0, dim, 3)), dtype=torch.float64)
+    rows[:, 1, 5] = 1.0
+    rows = (rows * torch.exp2(exponents)[:, None, None]).to(kind).to(device)
+    turn = kvip.Rotary(torch, 64 if dim == 128 else 6, device)
+    codes, scales = turn.quantise(torch.zeros(exponents.numel(), dtype=torch.int64, device=device), rows)
+    exact, most = rows.double(), rows.float().abs().amax(-1)
+    assert torch.equal(scales, torch.where(most > 0, (most / 448).clamp(min=2.0 ** -126), 1.0))
+    back = codes.float().double() * scales.double()[..., None]
+    assert bool(((back - exact).abs() <= exact.abs() * (2.0 ** -4 + 2.0 ** -22) + scales.double()[..., None] * 2.0 ** -10 * (1 + 2.0 ** -22)).all())
+    assert bool((codes.float()[exact == 0] == 0).all())
+
+
 def test_rotary_feeds_the_ingested_index_keys(device):
     """Keys rotated in place and ingested equal the rows that `quantise` makes (one rule of quantisation)."""
     from types import SimpleNamespace
