@@ -803,7 +803,8 @@ uint32_t launch_attention(const KvipAttentionArgs& a, uint32_t first_slot, cudaS
 extern "C" uint32_t kvip_b200_slot_attention(const KvipAttentionArgs* a, void* stream) {
   using namespace kvip;
   KVIP_REQUIRE(a && a->query && a->pool && a->slots && a->out && a->lse && a->status, "slot_attention: null pointer");
-  KVIP_REQUIRE(a->tokens >= 1 && a->heads >= 1 && a->heads <= 128 && a->entries >= 1, "slot_attention: tokens, 1..128 heads, entries");
+  KVIP_REQUIRE(a->tokens >= 1 && a->heads >= 1 && a->heads <= 128 && a->entries >= 1 && a->entries <= (1u << 20),
+               "slot_attention: tokens, 1..128 heads, 1..2^20 entries");
   KVIP_REQUIRE(a->batch >= 1 && (a->requests || (a->queries >= 1 && static_cast<uint64_t>(a->batch) * a->queries >= a->tokens)),
                "slot_attention: requests of the tokens");
   KVIP_REQUIRE(a->output_stride >= 1 && a->output_stride <= a->pool_rows && a->pool_rows <= 0x7fffffffull, "slot_attention: pool geometry");

@@ -82,6 +82,8 @@ class SlotAttention:
         if tokens == 0:
             return (self.out[:0, :heads] if out is None else out), (self.lse[:0, :heads] if lse is None else lse)
         batch = row_owners.numel() if row_owners is not None else starts.numel() - 1 if starts is not None else rows // output_stride
+        if batch < 1:
+            raise ValueError("SlotAttention needs at least one request")
         if requests is not None:
             requests_ptr = self._flat(requests, "requests", torch.int32, tokens)
         elif queries < 1 or batch * queries < tokens:

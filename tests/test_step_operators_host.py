@@ -68,7 +68,7 @@ ATTENTION = dict(query_token=128 * 576, query_head=576, draft_token=576, pool_ro
     (dict(entries=0), "entries"), (dict(batch=0), "requests"), (dict(requests=None, batch=1), "requests"), (dict(output_stride=0), "pool"),
     (dict(output_stride=8193), "pool"), (dict(starts=None), "starts"), (dict(dtype=2), "bf16"), (dict(query=4104), "aligned"),
     (dict(query_token=4), "aligned"), (dict(draft=4104), "aligned"), (dict(draft_token=578), "aligned"),
-    (dict(splits=3), "shares"), (dict(splits=16), "shares"), (dict(pool_rows=1 << 31), "pool")])
+    (dict(splits=3), "shares"), (dict(splits=16), "shares"), (dict(pool_rows=1 << 31), "pool"), (dict(entries=(1 << 20) + 1), "entries")])
 def test_attention_refusals(library, bad, word):
     refused(library, "kvip_b200_slot_attention", filled(_lib.AttentionArgs, **{**ATTENTION, **bad}), word)
 
