@@ -625,7 +625,7 @@ uint32_t kvip_prepare_shape(KvipRuntimeShape* shape);    /* include/api.h:9 */
  * position lengths + i and slot row[position / block] * block + position % block. Rows t >= starts[batch] of the token
  * outputs are -1. A request whose range does not fit its row (or is negative) adds no token and sets
  * KVIP_ERR_TOKEN_RANGE; one that the free list cannot serve keeps its packed tokens, with position and slot -1, and
- * takes no block (KVIP_ERR_NO_SLOT); a packed token behind the last output row is dropped (KVIP_ERR_TOKEN_RANGE).
+ * takes no block (KVIP_ERR_NO_SLOT); a negative block, of the row or of the list, gives slot -1 (KVIP_ERR_NO_SLOT); a packed token behind the last output row is dropped (KVIP_ERR_TOKEN_RANGE).
  * lengths, held, counts and head are not written: the call can be repeated. */
 typedef struct KvipSlotMapsArgs {
   const int32_t* lengths;      /* [batch] */
@@ -693,7 +693,7 @@ typedef struct KvipAttentionArgs {
   int64_t query_token, query_head;   /* strides of query in elements, multiples of 8 */
   int64_t draft_token;               /* stride of draft in elements, a multiple of 8 */
   uint64_t pool_rows;
-  uint32_t tokens, heads, entries, batch, queries, output_stride, dtype;
+  uint32_t tokens, heads, entries, batch, queries, output_stride, dtype;   /* 1..128 heads, entries up to 2^20 */
   uint32_t splits;             /* CTAs that share the rows of a token (1, 2, 4 or 8); 0 = by the sizes */
   uint32_t wait_kilocycles;    /* limit of every barrier wait, in units of 1024 SM clock cycles; 0 = about one second */
   float scale;

@@ -122,6 +122,7 @@ __global__ void __launch_bounds__(kMapThreads) slot_map_rows(const __grid_consta
   }
 
   // packed tokens: four consecutive ones per thread, one search for the first
+  bool hole = false;
   for (uint32_t t0 = (blockIdx.x * kMapThreads + tid) * kTokensPerThread; t0 < a.tokens;
        t0 += gridDim.x * kMapThreads * kTokensPerThread) {
     uint32_t lo = 0, hi = a.batch;   // largest b with s_start[b] <= t0
@@ -146,6 +147,7 @@ __global__ void __launch_bounds__(kMapThreads) slot_map_rows(const __grid_consta
                                               : a.free_blocks[head + s_off[b] + (page - held_b)];
           position = p;
           if (block >= 0) slot = static_cast<int64_t>(block) * a.block + (p - page * a.block);
+          else hole = true;
         }
       }
       a.positions[t] = position;
@@ -153,6 +155,8 @@ __global__ void __launch_bounds__(kMapThreads) slot_map_rows(const __grid_consta
       a.requests[t] = request;
     }
   }
+
+  if (hole) atomicOr(a.status, static_cast<int32_t>(KVIP_ERR_NO_SLOT));
 
   if (a.layout) {   // rows GATHER, QUERY_VALID, UNPACK, OUTPUT_VALID of the query slots
     const uint32_t slots = a.batch * a.queries;

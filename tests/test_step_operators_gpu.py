@@ -94,6 +94,17 @@ def test_slot_maps_report_what_does_not_fit(device, counts, lengths, held, spare
     check_maps(tables, expected)
 
 
+def test_slot_maps_report_rows_and_lists_with_holes(device):
+    """A row that lacks a block it is said to hold, and a free list with no block in a place: slot -1, position as ever, and the status."""
+    import kvip_b200 as kvip
+    tables = kvip.BlockTables(torch, device, batch=2, pages=4, blocks=4, tokens=8, block=4)
+    tables.load(lengths=torch.tensor([3, 0]), held=torch.tensor([2, 0]), table=torch.tensor([[5, -1, -1, -1], [-1] * 4]), free=torch.tensor([6, -1, 8]))
+    tables.plan(torch.tensor([3, 5], dtype=torch.int32, device=device))
+    assert tables.positions.tolist() == [3, 4, 5, 0, 1, 2, 3, 4]
+    assert tables.slot_mapping.tolist() == [23, -1, -1, 24, 25, 26, 27, -1]
+    assert int(tables.status) == 4 and int(tables.taken) == 2
+
+
 def test_slot_maps_layout_is_the_query_inputs_layout(device):
     from kvip_b200.inputs import slot_layout
     rng = np.random.default_rng(9)
