@@ -237,14 +237,15 @@ __device__ __forceinline__ Rows rows_of(const KvipAttentionArgs& a, uint32_t t) 
 
 template <typename T, uint32_t kN>
 __global__ void __launch_bounds__(Warps<kN>::kThreads, 1)
-attend_tiles(const __grid_constant__ CUtensorMap query_map, const __grid_constant__ KvipAttentionArgs a, const uint32_t groups,
-             const uint32_t group_heads, const uint32_t splits) {
+attend_tiles(const __grid_constant__ CUtensorMap query_map, const __grid_constant__ KvipAttentionArgs a, const uint32_t group_heads,
+             const uint32_t splits_log) {
   constexpr uint32_t kSides = Warps<kN>::kSides, kFirstLoaderWarp = Warps<kN>::kLoader, kScoreWarp = Warps<kN>::kScore, kValueWarp = Warps<kN>::kValue;
   extern __shared__ __align__(1024) uint8_t smem[];
   const uint32_t base = smem_u32(smem);
   Control& c = *reinterpret_cast<Control*>(smem + Layout<kN>::kControl);
   const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u;
-  const uint32_t split = blockIdx.x % splits, unit = blockIdx.x / splits, group = unit % groups, t = unit / groups;
+  const uint32_t splits = 1u << splits_log, split = blockIdx.x & (splits - 1u), group = blockIdx.x >> splits_log, t = blockIdx.z * gridDim.y + blockIdx.y;
+  if (t >= a.tokens) return;                 // behind the last token: whole clusters
   const uint32_t head0 = group * group_heads, heads = min(group_heads, a.heads - head0);
   const int32_t* list = a.slots + static_cast<uint64_t>(t) * a.entries;
   const bool vectors = (a.entries & 3u) == 0u && (reinterpret_cast<uintptr_t>(a.slots) & 15u) == 0u;
@@ -291,9 +292,9 @@ attend_tiles(const __grid_constant__ CUtensorMap query_map, const __grid_constan
   // tiles of the list, then one of the drafted rows
   const uint32_t listed = rows.limit ? last : 0u, list_tiles = (listed + kTile - 1) / kTile, tiles = list_tiles + (rows.drafted ? 1u : 0u);
   // A list may be far shorter than its entries. Up to three tiles are one CTA's: joining shares takes as long as two more of them.
-  const uint32_t shares = tiles <= 3u ? 1u : splits;
+  const uint32_t shares_log = tiles <= 3u ? 0u : splits_log, shares = 1u << shares_log;
   const bool idle = rows.request < 0 || split >= shares;
-  const uint32_t first = idle ? 0u : tiles * split / shares, count = idle ? 0u : tiles * (split + 1u) / shares - first;
+  const uint32_t first = idle ? 0u : tiles * split >> shares_log, count = idle ? 0u : (tiles * (split + 1u) >> shares_log) - first;
   const Waits waits{&c.abort_flag, static_cast<long long>(a.wait_kilocycles ? a.wait_kilocycles : kDefaultWaitKilocycles) << 10};
   constexpr uint32_t kScores = 0, kOut = 2 * kN;   // tensor-memory columns: two score tiles, four value blocks
   auto none = [&](uint32_t s) { return (c.valid[s][0] | c.valid[s][1] | c.valid[s][2] | c.valid[s][3]) == 0u; };
@@ -703,12 +704,12 @@ bool encode_queries(CUtensorMap* map, bool bf16, const void* base, uint64_t head
 }
 
 template <typename T, uint32_t kN>
-uint32_t configure(cudaLaunchConfig_t& config, cudaLaunchAttribute& cluster, KernelSlot slot, uint32_t ctas, uint32_t splits, cudaStream_t stream) {
+uint32_t configure(cudaLaunchConfig_t& config, cudaLaunchAttribute& cluster, KernelSlot slot, dim3 ctas, uint32_t splits, cudaStream_t stream) {
   if (uint32_t bad = raise_dynamic_smem(slot, reinterpret_cast<const void*>(attend_tiles<T, kN>), static_cast<int>(Layout<kN>::kBytes),
                                         "slot_attention attribute"))
     return bad;
   config = cudaLaunchConfig_t{};
-  config.gridDim = dim3(ctas);
+  config.gridDim = ctas;
   config.blockDim = dim3(Warps<kN>::kThreads);
   config.dynamicSmemBytes = Layout<kN>::kBytes;
   config.stream = stream;
@@ -731,10 +732,12 @@ uint32_t launch_tiles(const KvipAttentionArgs& a, KernelSlot slot, uint32_t grou
     set_error("slot_attention: the strides do not fit a tensor map");
     return KVIP_BAD_ARGUMENT;
   }
+  // tokens in y and z, shares as a power of two: the kernel finds its place without a division (one token 14.1 -> 13.8 us)
+  const uint32_t y = a.tokens < 32768u ? a.tokens : 32768u, splits_log = splits == 8u ? 3u : splits / 2u;
   cudaLaunchConfig_t config;
   cudaLaunchAttribute cluster;
-  if (uint32_t bad = configure<T, kN>(config, cluster, slot, a.tokens * groups * splits, splits, stream)) return bad;
-  cudaLaunchKernelEx(&config, attend_tiles<T, kN>, query_map, a, groups, group_heads, splits);
+  if (uint32_t bad = configure<T, kN>(config, cluster, slot, dim3(groups * splits, y, (a.tokens + y - 1u) / y), splits, stream)) return bad;
+  cudaLaunchKernelEx(&config, attend_tiles<T, kN>, query_map, a, group_heads, splits_log);
   count_launch();
   return check_launch("attend_tiles");
 }
@@ -753,7 +756,7 @@ uint32_t resident_clusters(uint32_t splits) {
   cudaLaunchConfig_t config;
   cudaLaunchAttribute cluster;
   int n = 0;
-  if (configure<__nv_bfloat16, 64>(config, cluster, static_cast<KernelSlot>(kSlotAttentionBf16 + 3), splits, splits, nullptr) ||
+  if (configure<__nv_bfloat16, 64>(config, cluster, static_cast<KernelSlot>(kSlotAttentionBf16 + 3), dim3(splits), splits, nullptr) ||
       cudaOccupancyMaxActiveClusters(&n, attend_tiles<__nv_bfloat16, 64>, &config) != cudaSuccess || n < 1) {
     cudaGetLastError();
     return device_sm_count() * 3u / (4u * splits) + 1u;
@@ -789,7 +792,7 @@ Cut cut_of(const KvipAttentionArgs& a) {
 template <typename T>
 uint32_t launch_attention(const KvipAttentionArgs& a, uint32_t first_slot, cudaStream_t stream) {
   const Cut cut = cut_of(a);
-  if (static_cast<uint64_t>(a.tokens) * cut.groups * cut.splits > 0x7fffffffull) { set_error("slot_attention: too many tokens in one call"); return KVIP_BAD_ARGUMENT; }
+  if (a.tokens > (1u << 30)) { set_error("slot_attention: too many tokens in one call"); return KVIP_BAD_ARGUMENT; }
   const KernelSlot slot = static_cast<KernelSlot>(first_slot + (cut.group_heads + 15u) / 16u - 1u);
   if (cut.group_heads <= 16) return launch_tiles<T, 16>(a, slot, cut.groups, cut.group_heads, cut.splits, stream);
   if (cut.group_heads <= 32) return launch_tiles<T, 32>(a, slot, cut.groups, cut.group_heads, cut.splits, stream);

@@ -582,6 +582,26 @@ def test_attention_a_query_of_nan_stays_one(device, heads, splits):
     check_attention(clean, out, lse)
 
 
+def test_attention_of_more_tokens_than_one_grid_dimension(device):
+    """40001 tokens of two heads over six slots each: the tokens fill two planes of the grid, the second in part."""
+    import kvip_b200 as kvip
+    tokens = 40001
+    g = torch.Generator(device=device)
+    g.manual_seed(43)
+    query = torch.randn((tokens, 2, 576), generator=g, device=device).to(torch.bfloat16)
+    pool = torch.randn((256, 576), generator=g, device=device).to(torch.bfloat16)
+    slots = torch.randint(-1, 64, (tokens, 6), generator=g, device=device, dtype=torch.int32)
+    requests = torch.arange(tokens, device=device, dtype=torch.int32) % 4
+    case = dict(query=query, pool=pool, slots=slots, requests=requests, row_owners=torch.tensor([2, 0, 3, 1], dtype=torch.int32, device=device),
+                output_stride=64, scale=0.05)
+    attend = kvip.SlotAttention(torch, device, tokens=tokens, heads=2, entries=6)
+    out, lse = attend(**case)
+    rows = torch.cat([torch.arange(0, tokens, 997), torch.tensor([32766, 32767, 32768, 32769, 40000])]).to(device)
+    few = dict(case, query=query[rows], slots=slots[rows], requests=requests[rows])
+    check_attention(few, out[rows], lse[rows])
+    assert int(attend.status.item()) == 0 and not bool(out.isnan().any())
+
+
 def test_attention_on_two_streams_with_outputs_of_their_own(device):
     """One object, two streams, outputs given by the caller: nothing is shared."""
     import kvip_b200 as kvip
