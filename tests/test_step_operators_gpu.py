@@ -582,6 +582,26 @@ def test_attention_a_query_of_nan_stays_one(device, heads, splits):
     check_attention(clean, out, lse)
 
 
+@pytest.mark.parametrize("requests,heads,entries", [(78, 128, 700), (151, 64, 512), (170, 16, 1100)])
+def test_attention_of_a_wave_and_a_few_tokens(device, requests, heads, entries):
+    """A little more than one CTA per SM: the tokens behind the first wave may be cut on their own. All of them are compared, drafted
+    rows and padding among them, and what is padding stays as it was."""
+    import kvip_b200 as kvip
+    rng = np.random.default_rng(requests)
+    case = attention_case(device, 44, counts=[1] * (requests - 2) + [3, 1], heads=heads, entries=entries, stride=1200,
+                          context=rng.integers(1, entries + 1, requests))
+    tokens = requests + 2
+    padding = torch.tensor([3, tokens - 1], device=device)
+    case["requests"][padding] = -1
+    attend = kvip.SlotAttention(torch, device, tokens=tokens, heads=heads, entries=entries)
+    attend.out.fill_(7.0)
+    attend.lse.fill_(7.0)
+    out, lse = attend(**case)
+    assert bool((out[padding] == 7).all()) and bool((lse[padding] == 7).all())
+    check_attention(case, out, lse, [t for t in range(tokens) if t not in padding.tolist()])
+    assert int(attend.status.item()) == 0
+
+
 def test_attention_of_more_tokens_than_one_grid_dimension(device):
     """40001 tokens of two heads over six slots each: the tokens fill two planes of the grid, the second in part."""
     import kvip_b200 as kvip
