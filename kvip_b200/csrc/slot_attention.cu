@@ -770,8 +770,9 @@ uint32_t resident_clusters(uint32_t splits) {
 // How a call is cut: heads per CTA (all up to 64, or fewer, which read the rows more often) and CTAs that share the rows of a
 // token. Few tokens are cut finely, because the SMs would stand idle; each cut costs the rows' copies once more or the joining of
 // the shares. Counted in clocks of full lists: a tile of 64 rows takes 2350 + 7 per head, a CTA 12700 + 228 per head before its
-// first and behind its last tile (fitted to 1 token x 128 heads x 2048 slots: 16 heads x 8 CTAs 15.0 us, 16 x 4 19.8, 16 x 2 30.2,
-// 32 x 8 16.4, 64 x 8 21.6, 64 x 1 61.9; 16 tokens: 64 x 4 28.4 against 64 x 2 38.8; 100 tokens: 64 x 2 126 against 64 x 1 137).
+// first and behind its last tile (fitted to an earlier form of the kernel; the order still holds: 1 token x 128 heads x 2048 slots in
+// 16 heads x 8 CTAs 14.2 us, 16 x 4 18.5, 16 x 2 28.8, 32 x 8 15.7, 64 x 8 20.6; 16 tokens 64 x 4 27.3 against 64 x 2 40.2; 64 tokens 64 x 1
+// 65.0 against 64 x 2 84.6).
 uint64_t clocks_of(uint32_t tiles, uint32_t group_heads, uint32_t splits) {
   return static_cast<uint64_t>((tiles + splits - 1) / splits) * (2350u + 7u * group_heads) + 12700u + 228u * group_heads;
 }
