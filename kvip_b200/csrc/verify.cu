@@ -8,7 +8,7 @@
 // their order is fixed. The rejections at one node need no pass of their own over each other's results: where r - Z q is not
 // cut off, r = max(target - C draft, 0) with C = 1 + Z_1 + .. + Z_(k-1), and what was cut off stays below. So a pass costs one fp64
 // fma, one add and two conversions (the slowest of them, 16 a clock and SM) per element, however many rejections. Bound by HBM: one
-// target row (and one draft row behind a rejection) per pass. Measured: 64 chains of 4 over 131072 tokens in fp32 18.5 us (67 MB, half of the
+// target row (and one draft row behind a rejection) per pass. Measured: 64 chains of 4 over 131072 tokens in fp32 18.8 us (67 MB, half of the
 // time in the pass), one request 9.7 us (latency), 48 trees of up to 16 nodes over 100003 bf16 tokens 31 us (five passes in one of them).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
