@@ -379,7 +379,7 @@ uint32_t kvip_b200_exchange(const KvipExchangeArgs* args, void* stream);
 /* ---- paged Index-cache update (new tokens) -----------------------------------------
  * keys[owner, query_end-1] = src[slot_mapping[gather[row]]], same for scales; invalid rows
  * write row `row` of owner 0. With bf16 sources the row is quantised to FP8 e4m3 with a
- * per-token scale amax/448. Replaces VllmIndexCacheStorage.ingest_decode
+ * per-token scale amax/448, at least 2^-126. Replaces VllmIndexCacheStorage.ingest_decode
  * (python/kvip/adapters/vllm/index_import.py:38-52). */
 typedef struct KvipIngestArgs {
   const void* source_keys;       /* [source_rows, 128] u8 (fp8) or bf16 */

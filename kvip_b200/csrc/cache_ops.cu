@@ -178,7 +178,7 @@ __global__ void __launch_bounds__(128) ingest_rows(const KvipIngestArgs a) {
     if (d == 0) a.scales[target] = a.source_scales[source];
     return;
   }
-  // bf16 row -> FP8 e4m3 with one scale per token: scale = amax / 448 (1 for an all-zero row)
+  // bf16 row -> FP8 e4m3 with one scale per token: scale = amax / 448, at least 2^-126 (1 for an all-zero row)
   __shared__ float warp_max[4];
   const float x = __uint_as_float(static_cast<uint32_t>(
                       reinterpret_cast<const uint16_t*>(a.source_keys)[static_cast<uint64_t>(source) * 128u + d]) << 16);
@@ -188,7 +188,7 @@ __global__ void __launch_bounds__(128) ingest_rows(const KvipIngestArgs a) {
   if ((d & 31u) == 0) warp_max[d >> 5] = m;
   __syncthreads();
   const float amax = fmaxf(fmaxf(warp_max[0], warp_max[1]), fmaxf(warp_max[2], warp_max[3]));
-  const float scale = amax > 0.f ? amax / 448.f : 1.f;
+  const float scale = index_row_scale(amax);
   a.keys[target * 128u + d] = static_cast<uint8_t>(__nv_cvt_float_to_fp8(x / scale, __NV_SATFINITE, __NV_E4M3));
   if (d == 0) a.scales[target] = scale;
 }

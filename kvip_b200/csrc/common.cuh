@@ -38,6 +38,10 @@ uint32_t device_sm_count();   // SMs of the current device (148 when the query f
     }                                           \
   } while (0)
 
+// Scale of an Index row in FP8 e4m3: its codes are x / scale, correctly rounded. Not below 2^-126: the quotients of the smallest rows
+// then stay within the type, and the reciprocal of a scale is finite.
+__device__ __forceinline__ float index_row_scale(float amax) { return amax > 0.f ? fmaxf(amax / 448.f, 1.17549435e-38f) : 1.f; }
+
 // fp32 -> unsigned key with the same order (larger float = larger key).
 // NaN sorts above +inf, like the reference's sortable-u16 map (score_common.h:66-97).
 __host__ __device__ inline uint32_t sortable_key(float value) {

@@ -4,8 +4,8 @@
 // part (exact subtraction in fp64) goes to sincospi in fp32. A position of 2^21 keeps 32 bits behind the point that way,
 // where an fp32 angle would have none. The rotation is fp32, rounded once to the row's type.
 //
-// Bound by HBM: 8192 tokens x 129 rows of 64 inside rows of 576 take 50 us (5.4 TB/s), 16411 x 64 rows of 128 to FP8 82 us (5.0 TB/s, and
-// issue slots 69 % busy); one pair per thread instead of a unit of eight took 204 and 473.
+// Bound by HBM: 8192 tokens x 129 rows of 64 inside rows of 576 take 50 us (5.4 TB/s), 16411 x 64 rows of 128 to FP8 87.6 us (4.65 TB/s); one
+// pair per thread instead of a unit of eight took 204 and 473.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
@@ -15,8 +15,6 @@ namespace kvip {
 namespace {
 
 constexpr uint32_t kRotaryThreads = 256;
-// Scale of a quantised row. Not below 2^-126, whose reciprocal is finite: beneath it zeros would become 0 * inf.
-__device__ __forceinline__ float row_scale(float amax) { return amax > 0.f ? fmaxf(amax / 448.f, 1.17549435e-38f) : 1.f; }
 
 template <typename T> __device__ __forceinline__ float to_float(T v);
 template <> __device__ __forceinline__ float to_float(float v) { return v; }
@@ -70,12 +68,12 @@ __global__ void __launch_bounds__(kRotaryThreads) quantise_rows(const KvipRotary
     if (position < 0) continue;
     const T* x = static_cast<const T*>(a.x[0]) + token * a.x_token[0] + head * a.x_head[0];
     const bool split = a.layout == KVIP_ROTARY_HALF;
-    float amax = 0.f, scale = 1.f, inverse = 1.f;
+    float amax = 0.f, scale = 1.f;
     for (uint32_t pass = 0; pass < 2u; ++pass) {
       uint8_t* codes = a.codes + r * a.dim;
       auto emit = [&](uint32_t at, float value) {
         if (pass == 0) amax = fmaxf(amax, fabsf(value));
-        else codes[at] = static_cast<uint8_t>(__nv_cvt_float_to_fp8(value * inverse, __NV_SATFINITE, __NV_E4M3));
+        else codes[at] = static_cast<uint8_t>(__nv_cvt_float_to_fp8(value / scale, __NV_SATFINITE, __NV_E4M3));
       };
       for (uint32_t pair = lane; pair < half; pair += 32u) {
         const uint32_t at = split ? pair : 2u * pair, other = split ? pair + half : at + 1u;
@@ -88,8 +86,7 @@ __global__ void __launch_bounds__(kRotaryThreads) quantise_rows(const KvipRotary
       if (pass == 0) {
 #pragma unroll
         for (uint32_t o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-        scale = row_scale(amax);
-        inverse = 1.f / scale;
+        scale = index_row_scale(amax);
         if (lane == 0) a.scales[r] = scale;
       }
     }
@@ -152,6 +149,26 @@ __device__ __forceinline__ void turn_unit(float (&x)[16], const float2* cs, bool
     x[a1] = u1 * c.z - v1 * c.w; x[b1] = v1 * c.z + u1 * c.w;
   }
 }
+// FP8 codes of e[i] / scale, the quotient rounded to fp32 and then to the code. A product with the reciprocal would give codes next to a
+// border wrongly; one correction by the remainder, q + (e - q scale) / scale, makes q the rounded quotient (P. Markstein, "Computation of
+// elementary functions on the IBM RISC System/6000 processor", 1990). It wants remainders above the smallest numbers, so the elements of
+// a row with a tiny scale are multiplied by 2^64 first. 16411 x 64 rows: 83 us with products alone, 87.6 so, 118 with
+// divisions.
+__device__ __forceinline__ uint32_t two_codes(float x, float y, float2 minus_scale, float2 inverse) {
+  const float2 e = make_float2(x, y), q = __fmul2_rn(e, inverse);
+  return __nv_cvt_float2_to_fp8x2(__ffma2_rn(__ffma2_rn(q, minus_scale, e), inverse, q), __NV_SATFINITE, __NV_E4M3);
+}
+__device__ __forceinline__ void codes_of(float (&e)[16], float scale, uint32_t (&packed)[4]) {
+  if (scale < 0x1p-60f) {
+#pragma unroll
+    for (uint32_t i = 0; i < 16; ++i) e[i] *= 0x1p64f;
+    scale *= 0x1p64f;
+  }
+  const float inverse = 1.f / scale, minus = scale < INFINITY ? -scale : 0.f;   // beside an infinity finite elements are 0, not a remainder of NaN
+  const float2 i = make_float2(inverse, inverse), s = make_float2(minus, minus);
+#pragma unroll
+  for (uint32_t j = 0; j < 4; ++j) packed[j] = two_codes(e[4 * j], e[4 * j + 1], s, i) | (two_codes(e[4 * j + 2], e[4 * j + 3], s, i) << 16);
+}
 // (cos, sin) of `pairs` pairs of the CTA's tokens in shared memory: [tile][stride]
 __device__ __forceinline__ void turn_table(const KvipRotaryArgs& a, float2* table, uint32_t first, uint32_t tile, uint32_t pairs) {
   for (uint32_t i = threadIdx.x; i < tile * pairs; i += kRotaryThreads) {
@@ -185,8 +202,9 @@ __global__ void __launch_bounds__(kRotaryThreads) rotate_units(const __grid_cons
 }
 
 // kLanes threads per row of 16 kLanes elements.
+// Six CTAs per SM: without the bound the compiler takes 42 registers, which leave five (16411 x 64 rows 92.5 us instead of 87.6).
 template <typename T, bool kSplit, uint32_t kLanes>
-__global__ void __launch_bounds__(kRotaryThreads) quantise_units(const __grid_constant__ KvipRotaryArgs a, const uint32_t tile, const uint32_t rows_here) {
+__global__ void __launch_bounds__(kRotaryThreads, 6) quantise_units(const __grid_constant__ KvipRotaryArgs a, const uint32_t tile, const uint32_t rows_here) {
   extern __shared__ float2 table[];
   const uint32_t half = a.width >> 1, turned = a.width >> 4;
   const uint32_t first = blockIdx.x * tile, row0 = blockIdx.y * rows_here, count = min(rows_here, a.heads[0] - row0);
@@ -208,15 +226,10 @@ __global__ void __launch_bounds__(kRotaryThreads) quantise_units(const __grid_co
 #pragma unroll
     for (uint32_t o = kLanes / 2u; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
     if (!live) continue;
-    const float scale = row_scale(amax), inverse = 1.f / scale;
+    const float scale = index_row_scale(amax);
     const uint64_t r = static_cast<uint64_t>(token) * a.heads[0] + row;
     uint32_t packed[4];
-#pragma unroll
-    for (uint32_t j = 0; j < 4; ++j) {
-      const uint32_t x = __nv_cvt_float2_to_fp8x2(make_float2(e[4 * j] * inverse, e[4 * j + 1] * inverse), __NV_SATFINITE, __NV_E4M3);
-      const uint32_t y = __nv_cvt_float2_to_fp8x2(make_float2(e[4 * j + 2] * inverse, e[4 * j + 3] * inverse), __NV_SATFINITE, __NV_E4M3);
-      packed[j] = x | (y << 16);
-    }
+    codes_of(e, scale, packed);
     uint8_t* codes = a.codes + r * a.dim;
     __stcs(reinterpret_cast<uint2*>(codes + low), make_uint2(packed[0], packed[1]));
     __stcs(reinterpret_cast<uint2*>(codes + high), make_uint2(packed[2], packed[3]));
@@ -224,7 +237,8 @@ __global__ void __launch_bounds__(kRotaryThreads) quantise_units(const __grid_co
   }
 }
 
-// Tokens and rows per CTA: about 1024 units of work (512 and 2048 are slower: 16411 x 64 rows to FP8 take 88, 82 and 84 us), tokens first (their angles are shared by all rows), and at least two
+// Tokens and rows per CTA: about 1024 units of work (512 and 2048 are slower: 16411 x 64 rows to FP8 took 88, 82 and 84 us
+// before codes were quotients), tokens first (their angles are shared by all rows), and at least two
 // CTAs per SM where there is that much work.
 void shares(uint32_t tokens, uint32_t rows, uint32_t units, uint32_t half, uint32_t* tile, uint32_t* rows_here) {
   const uint32_t want = 2u * device_sm_count();

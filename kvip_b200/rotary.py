@@ -114,7 +114,7 @@ class Rotary:
     def quantise(self, positions, rows, codes=None, scales=None):
         """Rotate the first `width` elements of every row and quantise the whole row: rows [tokens, heads, dim] ->
         (codes [tokens, heads, dim] float8_e4m3fn, scales [tokens, heads] float32) with scale = amax / 448, at least 2^-126 (1 for a row of
-        zeros), the rule of `IndexCacheStorage.ingest_decode`. Rows of tokens with a negative position are not written.
+        zeros), and codes of the quotients by it, the rule of `IndexCacheStorage.ingest_decode`. Rows of tokens with a negative position are not written.
         Without `codes` / `scales` the outputs are allocated."""
         torch = self.torch
         tokens = self._tokens(positions)

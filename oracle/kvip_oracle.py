@@ -424,7 +424,7 @@ def gather(pool, slots, owners, queries, output_stride):
 def quantize_rows(rows_bf16_bits):
     x = bf16_to_f32(rows_bf16_bits)
     amax = np.abs(x).max(axis=-1)
-    scale = np.where(amax > 0, (amax / np.float32(448.0)).astype(np.float32), np.float32(1.0)).astype(np.float32)
+    scale = np.where(amax > 0, np.maximum((amax / np.float32(448.0)).astype(np.float32), np.float32(2.0 ** -126)), np.float32(1.0)).astype(np.float32)
     return encode_e4m3((x / scale[..., None]).astype(np.float32)), scale
 
 
