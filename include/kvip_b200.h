@@ -625,7 +625,8 @@ uint32_t kvip_prepare_shape(KvipRuntimeShape* shape);    /* include/api.h:9 */
  * position lengths + i and slot row[position / block] * block + position % block. Rows t >= starts[batch] of the token
  * outputs are -1. A request whose range does not fit its row (or is negative) adds no token and sets
  * KVIP_ERR_TOKEN_RANGE; one that the free list cannot serve keeps its packed tokens, with position and slot -1, and
- * takes no block (KVIP_ERR_NO_SLOT); a negative block, of the row or of the list, gives slot -1 (KVIP_ERR_NO_SLOT); a packed token behind the last output row is dropped (KVIP_ERR_TOKEN_RANGE).
+ * takes no block (KVIP_ERR_NO_SLOT); a negative block, of the row or of the list, gives slot -1 (KVIP_ERR_NO_SLOT); a packed token behind the last output row is dropped (KVIP_ERR_TOKEN_RANGE)
+ * from all outputs but `ends` and the blocks, which the request keeps.
  * lengths, held, counts and head are not written: the call can be repeated. */
 typedef struct KvipSlotMapsArgs {
   const int32_t* lengths;      /* [batch] */

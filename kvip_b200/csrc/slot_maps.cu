@@ -158,15 +158,15 @@ __global__ void __launch_bounds__(kMapThreads) slot_map_rows(const __grid_consta
 
   if (hole) atomicOr(a.status, static_cast<int32_t>(KVIP_ERR_NO_SLOT));
 
-  if (a.layout) {   // rows GATHER, QUERY_VALID, UNPACK, OUTPUT_VALID of the query slots
-    const uint32_t slots = a.batch * a.queries;
+  if (a.layout) {   // rows GATHER, QUERY_VALID, UNPACK, OUTPUT_VALID of the query slots: packed tokens behind the last output row are not there
+    const uint32_t slots = a.batch * a.queries, kept = min(total_tokens, a.tokens);
     for (uint32_t s = blockIdx.x * kMapThreads + tid; s < slots; s += gridDim.x * kMapThreads) {
       const uint32_t b = s / a.queries, q = s - b * a.queries;
-      const bool live = q < s_start[b + 1] - s_start[b];
+      const bool live = q < s_start[b + 1] - s_start[b] && s_start[b] + q < kept;
       a.layout[s] = live ? static_cast<int64_t>(s_start[b] + q) : 0;
       a.layout[slots + s] = live ? 1 : 0;
       int64_t from = 0;
-      if (s < total_tokens) {
+      if (s < kept) {
         uint32_t lo = 0, hi = a.batch;
         while (hi - lo > 1u) {
           const uint32_t mid = (lo + hi) >> 1;
@@ -176,7 +176,7 @@ __global__ void __launch_bounds__(kMapThreads) slot_map_rows(const __grid_consta
         from = static_cast<int64_t>(lo) * a.queries + (s - s_start[lo]);
       }
       a.layout[2 * slots + s] = from;
-      a.layout[3 * slots + s] = s < total_tokens ? 1 : 0;
+      a.layout[3 * slots + s] = s < kept ? 1 : 0;
     }
   }
 }

@@ -67,3 +67,21 @@ def test_ingested_keys_are_the_quantised_rows(device, smallest):
     at = (positions + 1, positions)
     assert torch.equal(storage.scales[at], scales[:, 0])
     assert torch.equal(storage.keys[at].view(torch.float8_e4m3fn).float(), codes[:, 0].float())
+
+
+# ---- slot maps and the layout of the query slots -----------------------------------------------------------------------
+@pytest.mark.parametrize("counts,tokens", [([4] * 8, 16), ([4, 0, 3, 4, 1], 9), ([3, 3, 3], 8), ([4, 4], 1), ([2, 1], 3), ([2, 1], 11)])
+def test_layout_ends_where_the_packed_tokens_end(device, counts, tokens):
+    """Fewer output rows than packed tokens: what is dropped from positions, slots and starts is dropped from the layout as well."""
+    import kvip_b200 as kvip
+    batch, queries = len(counts), 4
+    tables = kvip.BlockTables(torch, device, batch=batch, pages=2, blocks=2 * batch, tokens=tokens, block=16, queries=queries)
+    tables.plan(torch.tensor(counts, dtype=torch.int32, device=device))
+    owner = [(b, q) for b in range(batch) for q in range(counts[b])][:tokens]
+    expected = np.zeros((4, batch * queries), np.int64)
+    for t, (b, q) in enumerate(owner):
+        expected[0, b * queries + q], expected[1, b * queries + q] = t, 1
+        expected[2, t], expected[3, t] = b * queries + q, 1
+    assert np.array_equal(tables.layout.cpu().numpy(), expected)
+    assert int(tables.starts[-1]) == len(owner) and int(tables.status) == (1 if sum(counts) > tokens else 0)
+    assert tables.requests.tolist() == [b for b, _ in owner] + [-1] * (tokens - len(owner))
