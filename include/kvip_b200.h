@@ -216,7 +216,7 @@ typedef struct KvipPackArgs {
   const uint8_t* weights_src;   /* [tokens, weights_row_bytes] or NULL */
   const float* scale_src;       /* [tokens, heads] or NULL */
   const int64_t* positions_src; /* [tokens] or NULL */
-  const int64_t* gather_indices;/* [rows] */
+  const int64_t* gather_indices;/* [rows]; a row of no token of 0 .. tokens - 1 gets query end 0 */
   const int64_t* query_valid;   /* [rows] 0/1 */
   uint8_t* query_dst;           /* [rows, query_row_bytes] */
   uint8_t* weights_dst;         /* [rows, weights_row_bytes] */
@@ -393,6 +393,16 @@ typedef struct KvipIngestArgs {
   uint32_t batch, queries, history, source_is_bf16;
 } KvipIngestArgs;
 uint32_t kvip_b200_ingest(const KvipIngestArgs* args, void* stream);
+
+/* The same with its bounds: a live row whose token, source row, owner or position is out of range (a token without a block
+ * has slot -1) is skipped and counted in *errors. kvip_b200_ingest knows no bounds and skips negative ones alone. */
+typedef struct KvipIngestCheckedArgs {
+  KvipIngestArgs rows;
+  int32_t* errors;               /* [1] in/out or NULL */
+  uint64_t source_rows;          /* rows of source_keys (and source_scales) */
+  uint32_t tokens, owners;       /* entries of slot_mapping; owners of keys and scales */
+} KvipIngestCheckedArgs;
+uint32_t kvip_b200_ingest_checked(const KvipIngestCheckedArgs* args, void* stream);
 
 /* Prefill-side import of Index rows: one launch for every request of a forward batch
  * (VllmIndexCacheStorage.ingest_prefill, python/kvip/adapters/vllm/index_import.py:17-36, does it with

@@ -101,6 +101,13 @@ IngestArgs = _struct("IngestArgs", (
     "source_keys", "source_scales", "slot_mapping", "gather_indices", "query_ends", "row_owners", "keys", "scales"),
     [(n, u32) for n in ("batch", "queries", "history", "source_is_bf16")])
 
+
+class IngestCheckedArgs(ctypes.Structure):
+    """KvipIngestCheckedArgs: the rows with the bounds of what their indices may name."""
+
+    _fields_ = [("rows", IngestArgs), ("errors", vp), ("source_rows", u64), ("tokens", u32), ("owners", u32)]
+
+
 IngestSpanArgs = _struct("IngestSpanArgs", (
     "source_keys", "source_scales", "block_table", "slot_mapping", "positions", "spans", "keys", "scales", "errors"),
     [("source_rows", u64)] + [(n, u32) for n in ("count", "max_tokens", "owners", "history", "block", "table_rows",
@@ -192,6 +199,7 @@ _STAGES = {
     "kvip_b200_topk_merge": MergeArgs, "kvip_b200_cold_predicate": ColdArgs,
     "kvip_b200_pack_inputs": PackArgs, "kvip_b200_resolve": ResolveArgs, "kvip_b200_fetch": FetchArgs,
     "kvip_b200_gather": GatherArgs, "kvip_b200_publish_residency": FetchArgs, "kvip_b200_exchange": ExchangeArgs, "kvip_b200_ingest": IngestArgs,
+    "kvip_b200_ingest_checked": IngestCheckedArgs,
     "kvip_b200_ingest_spans": IngestSpanArgs, "kvip_b200_peer_exchange": PeerExchangeArgs,
     "kvip_b200_lru_commit": LruArgs, "kvip_b200_lidu": LiduArgs, "kvip_b200_publish_pages": PagesArgs,
     "kvip_b200_window_bounds": WindowArgs, "kvip_b200_resident_threshold": ThresholdArgs,

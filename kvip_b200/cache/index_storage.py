@@ -103,7 +103,9 @@ class IndexCacheStorage:
 
     def ingest_decode(self, cache, metadata, inputs, row_owners):
         """Fixed-shape, graph-capturable write of the B*Q new rows: one launch. Padding rows of the graph write
-        distinct positions of reserved owner zero, so no live request is touched."""
+        distinct positions of reserved owner zero, so no live request is touched. Tokens without a slot (-1), or with an owner or a
+        position that the storage does not have, are skipped and counted in `ingest_errors`."""
         source_keys, source_scales = self._sources(cache)
         ops.ingest(self.keys.view(self.torch.uint8), self.scales, source_keys, source_scales, metadata.slot_mapping,
-                   inputs.gather_indices, inputs.query_ends, row_owners, queries=inputs.queries, history=self.history)
+                   inputs.gather_indices, inputs.query_ends, row_owners, queries=inputs.queries, history=self.history,
+                   errors=self.ingest_errors)

@@ -164,14 +164,29 @@ __global__ void __launch_bounds__(256) gather_rows(const KvipGatherArgs a) {
 }
 
 // ---- paged Index-cache ingest ----------------------------------------------------------------
-__global__ void __launch_bounds__(128) ingest_rows(const KvipIngestArgs a) {
+// What the indices of a step may name; every one of them may come from the device, where no host has seen it.
+struct IngestBounds {
+  uint64_t source_rows;
+  uint32_t tokens, owners;
+  int32_t* errors;
+};
+__global__ void __launch_bounds__(128) ingest_rows(const KvipIngestArgs a, const IngestBounds bounds) {
   const uint32_t row = blockIdx.x, d = threadIdx.x;
-  const bool live = a.query_ends[row] > 0;
+  const int32_t end = a.query_ends[row];
   int64_t source = 0;
   uint64_t target = row;  // padding rows land in owner 0 at distinct positions
-  if (live) {
-    source = a.slot_mapping[a.gather_indices[row]];
-    target = static_cast<uint64_t>(a.row_owners[row / a.queries]) * a.history + static_cast<uint32_t>(a.query_ends[row] - 1);
+  if (end > 0) {
+    const int64_t token = a.gather_indices[row];
+    const int32_t owner = a.row_owners[row / a.queries];
+    source = token >= 0 && token < static_cast<int64_t>(bounds.tokens) ? a.slot_mapping[token] : -1;   // -1: a token without a block, too
+    if (source < 0 || static_cast<uint64_t>(source) >= bounds.source_rows || static_cast<uint32_t>(end) > a.history ||
+        static_cast<uint32_t>(owner) >= bounds.owners) {
+      if (d == 0 && bounds.errors) atomicAdd(bounds.errors, 1);
+      return;
+    }
+    target = static_cast<uint64_t>(owner) * a.history + static_cast<uint32_t>(end - 1);
+  } else if (row >= a.history) {
+    return;               // owner 0 ends here
   }
   if (!a.source_is_bf16) {
     a.keys[target * 128u + d] = reinterpret_cast<const uint8_t*>(a.source_keys)[static_cast<uint64_t>(source) * 128u + d];
@@ -447,7 +462,8 @@ namespace {
 __global__ void __launch_bounds__(256) pack_rows(const KvipPackArgs a) {
   const uint32_t row = blockIdx.x, tid = threadIdx.x;
   int64_t token = a.gather_indices[row];
-  if (token < 0 || token >= static_cast<int64_t>(a.tokens)) token = 0;
+  const bool there = token >= 0 && token < static_cast<int64_t>(a.tokens);   // a slot of no token is not live
+  if (!there) token = 0;
   if (a.query_src) {
     const uint4* src = reinterpret_cast<const uint4*>(a.query_src + static_cast<uint64_t>(token) * a.query_row_bytes);
     uint4* dst = reinterpret_cast<uint4*>(a.query_dst + static_cast<uint64_t>(row) * a.query_row_bytes);
@@ -462,7 +478,7 @@ __global__ void __launch_bounds__(256) pack_rows(const KvipPackArgs a) {
     for (uint32_t i = tid; i < a.heads; i += 256u)
       a.scale_dst[static_cast<uint64_t>(row) * a.heads + i] = a.scale_src[static_cast<uint64_t>(token) * a.heads + i];
   if (a.positions_src && tid == 0) {
-    const int64_t end = (a.positions_src[token] + 1) * a.query_valid[row];
+    const int64_t end = there ? (a.positions_src[token] + 1) * a.query_valid[row] : 0;
     a.position_scratch[row] = end;
     a.query_ends[row] = static_cast<int32_t>(end);
   }
@@ -487,14 +503,29 @@ extern "C" uint32_t kvip_b200_pack_inputs(const KvipPackArgs* a, void* stream) {
   return kvip::check_launch("pack_rows");
 }
 
+namespace kvip {
+namespace {
+uint32_t launch_ingest(const KvipIngestArgs& a, const IngestBounds& bounds, void* stream) {
+  KVIP_REQUIRE(a.source_keys && a.slot_mapping && a.gather_indices && a.query_ends && a.row_owners && a.keys && a.scales, "ingest: null pointer");
+  KVIP_REQUIRE(a.source_is_bf16 || a.source_scales, "ingest: FP8 sources need their scales");
+  KVIP_REQUIRE(a.batch >= 1 && a.queries >= 1 && a.queries <= KVIP_MAX_QUERIES, "ingest: bad batch/queries");
+  ingest_rows<<<a.batch * a.queries, 128, 0, static_cast<cudaStream_t>(stream)>>>(a, bounds);
+  count_launch();
+  return check_launch("ingest_rows");
+}
+}  // namespace
+}  // namespace kvip
+
 extern "C" uint32_t kvip_b200_ingest(const KvipIngestArgs* a, void* stream) {
-  KVIP_REQUIRE(a && a->source_keys && a->slot_mapping && a->gather_indices && a->query_ends && a->row_owners &&
-                   a->keys && a->scales, "ingest: null pointer");
-  KVIP_REQUIRE(a->source_is_bf16 || a->source_scales, "ingest: FP8 sources need their scales");
-  KVIP_REQUIRE(a->batch >= 1 && a->queries >= 1 && a->queries <= KVIP_MAX_QUERIES, "ingest: bad batch/queries");
-  kvip::ingest_rows<<<a->batch * a->queries, 128, 0, static_cast<cudaStream_t>(stream)>>>(*a);
-  kvip::count_launch();
-  return kvip::check_launch("ingest_rows");
+  KVIP_REQUIRE(a, "ingest: null pointer");
+  return kvip::launch_ingest(*a, kvip::IngestBounds{~0ull, 0xffffffffu, 0x80000000u, nullptr}, stream);
+}
+
+extern "C" uint32_t kvip_b200_ingest_checked(const KvipIngestCheckedArgs* a, void* stream) {
+  KVIP_REQUIRE(a, "ingest_checked: null pointer");
+  KVIP_REQUIRE(!a->rows.source_keys || (a->source_rows >= 1 && a->owners >= 1 && a->owners <= 0x7fffffffu && a->rows.history >= 1),
+               "ingest_checked: at least one source row, one owner and one position");
+  return kvip::launch_ingest(a->rows, kvip::IngestBounds{a->source_rows, a->tokens, a->owners, a->errors}, stream);
 }
 
 extern "C" uint32_t kvip_b200_ingest_spans(const KvipIngestSpanArgs* a, void* stream) {

@@ -285,20 +285,28 @@ def gather(pool, slots, out=None, *, queries, output_stride, token_bytes, row_ow
 
 
 def ingest(keys, scales, source_keys, source_scales, slot_mapping, gather_indices, query_ends, row_owners, *,
-           queries, history):
-    """Scatter the new tokens' Index rows into persistent storage (quantising bf16 sources)."""
+           queries, history, errors=None):
+    """Scatter the new tokens' Index rows into persistent storage (quantising bf16 sources). Rows whose token, source row,
+    owner or position is out of range are skipped and counted in `errors`."""
     device = keys.device
     bf16 = source_keys.dtype == torch.bfloat16
     for name, t, dt in (("slot_mapping", slot_mapping, torch.int64), ("gather_indices", gather_indices, torch.int64),
                         ("query_ends", query_ends, torch.int32), ("row_owners", row_owners, torch.int32),
-                        ("scales", scales, torch.float32), ("source_scales", source_scales, torch.float32)):
+                        ("scales", scales, torch.float32), ("source_scales", source_scales, torch.float32),
+                        ("errors", errors, torch.int32)):
         _require(t, name, dt, device)
-    args = _lib.IngestArgs(
-        source_keys=_ptr(source_keys), source_scales=_ptr(source_scales), slot_mapping=_ptr(slot_mapping),
-        gather_indices=_ptr(gather_indices), query_ends=_ptr(query_ends), row_owners=_ptr(row_owners),
-        keys=_ptr(keys), scales=_ptr(scales), batch=row_owners.numel(), queries=queries, history=history,
-        source_is_bf16=int(bf16))
-    _lib.check(_lib.load_library().kvip_b200_ingest(ctypes.byref(args), _stream(device)), "ingest")
+    batch, rows, positions = row_owners.numel(), source_keys.numel() // 128, keys.numel() // 128
+    if min(gather_indices.numel(), query_ends.numel()) < batch * queries:
+        raise ValueError("ingest: gather_indices and query_ends hold an entry per query slot")
+    if positions % history or scales.numel() != positions or (source_scales is not None and source_scales.numel() < rows):
+        raise ValueError("ingest: keys and scales are [owners, history], with a scale per source row")
+    args = _lib.IngestCheckedArgs(
+        rows=_lib.IngestArgs(
+            source_keys=_ptr(source_keys), source_scales=_ptr(source_scales), slot_mapping=_ptr(slot_mapping),
+            gather_indices=_ptr(gather_indices), query_ends=_ptr(query_ends), row_owners=_ptr(row_owners),
+            keys=_ptr(keys), scales=_ptr(scales), batch=batch, queries=queries, history=history, source_is_bf16=int(bf16)),
+        errors=_ptr(errors), source_rows=rows, tokens=slot_mapping.numel(), owners=positions // history)
+    _lib.check(_lib.load_library().kvip_b200_ingest_checked(ctypes.byref(args), _stream(device)), "ingest")
 
 
 def ingest_spans(keys, scales, source_keys, source_scales, block_table, slot_mapping, positions, spans, *, history,

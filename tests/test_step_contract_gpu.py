@@ -85,3 +85,80 @@ def test_layout_ends_where_the_packed_tokens_end(device, counts, tokens):
     assert np.array_equal(tables.layout.cpu().numpy(), expected)
     assert int(tables.starts[-1]) == len(owner) and int(tables.status) == (1 if sum(counts) > tokens else 0)
     assert tables.requests.tolist() == [b for b, _ in owner] + [-1] * (tokens - len(owner))
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+def test_ingest_skips_and_counts_what_is_out_of_range(device, bf16):
+    """Slots, tokens, owners and positions out of range, one at a time among good rows: the good ones land, the storage keeps the rest."""
+    from kvip_b200 import ops
+    g = torch.Generator(device=device)
+    g.manual_seed(0)
+    owners, history, queries, batch, rows = 3, 256, 4, 5, 40
+    source = (torch.randn((rows, 128), generator=g, device=device).to(torch.bfloat16) if bf16 else
+              torch.randint(0, 120, (rows, 128), generator=g, device=device, dtype=torch.uint8))
+    source_scales = None if bf16 else torch.rand(rows, generator=g, device=device)
+    slots = torch.tensor([7, -1, 40, 3, 39, 1 << 40, 0], device=device)
+    gather = torch.tensor([0, 1, 2, 3, 4, 5, 6, 7, -1, 0, 3, 1 << 35, 0, 3, 4, 6, 0, 3, 4, 6], device=device)
+    ends = torch.tensor([10, 11, 12, 13, 256, 1, 257, 9, 9, 2, 3, 4, 20, 21, 0, 22, 30, 31, 32, 0], dtype=torch.int32, device=device)
+    row_owners = torch.tensor([1, 2, 1, 3, -1], dtype=torch.int32, device=device)
+    good = {0: 7, 3: 3, 4: 39, 9: 7, 10: 3}
+    padding = [14, 19]
+    keys = torch.randint(0, 120, (owners, history, 128), generator=g, device=device, dtype=torch.uint8)
+    scales, errors = torch.rand((owners, history), generator=g, device=device), torch.zeros(1, dtype=torch.int32, device=device)
+    want_keys, want_scales = keys.clone(), scales.clone()
+    one = torch.zeros(1, dtype=torch.int64, device=device)
+    for row, slot in [*good.items(), *((row, 0) for row in padding)]:
+        if bf16:
+            import kvip_b200 as kvip
+            code, scale = kvip.Rotary(torch, 2, device).quantise(one, source[slot].view(1, 1, 128))
+        else:
+            code, scale = source[slot], source_scales[slot]
+        at = (0, row) if row in padding else (int(row_owners[row // queries]), int(ends[row]) - 1)
+        want_keys[at], want_scales[at] = code.view(torch.uint8).view(128), scale.view(())
+    ops.ingest(keys, scales, source, source_scales, slots, gather, ends, row_owners, queries=queries, history=history, errors=errors)
+    assert torch.equal(keys, want_keys) and torch.equal(scales, want_scales)
+    assert int(errors) == 20 - len(good) - len(padding)
+    with pytest.raises(ValueError, match="query slot"):
+        ops.ingest(keys, scales, source, source_scales, slots, gather[:19], ends, row_owners, queries=queries, history=history)
+    with pytest.raises(ValueError, match="history"):
+        ops.ingest(keys, scales[:2], source, source_scales, slots, gather, ends, row_owners, queries=queries, history=history)
+
+
+def test_ingest_padding_rows_stay_in_the_first_owner(device):
+    """More query slots than owner 0 has positions: padding behind its last position is not written over the next owner's rows."""
+    from kvip_b200 import ops
+    keys = torch.full((2, 4, 128), 9, dtype=torch.uint8, device=device)
+    scales = torch.full((2, 4), 5.0, device=device)
+    source = torch.ones((1, 128), dtype=torch.uint8, device=device)
+    zeros = torch.zeros(6, dtype=torch.int64, device=device)
+    ops.ingest(keys, scales, source, torch.ones(1, device=device), zeros[:1], zeros, zeros.int(), zeros.int(), queries=1, history=4)
+    assert bool((keys[0] == 1).all()) and bool((keys[1] == 9).all()) and bool((scales[1] == 5).all())
+
+
+def test_packed_slots_of_no_token_are_not_live(device):
+    """A layout whose indices leave the packed tensors: those slots have query end 0, whatever their valid word says."""
+    import kvip_b200 as kvip
+    inputs = kvip.QueryInputs(torch, 3, device, history=256, queries=2)
+    layout = torch.tensor([[0, 2, 5, -1, 1, 1 << 40], [1] * 6, [0, 1, 2, 3, 4, 5], [1] * 6], device=device)
+    inputs.prepare_device(layout, torch.tensor([1, 2, 3], dtype=torch.int32, device=device))
+    assert inputs.bind_positions(torch.tensor([7, 8, 9], device=device)).tolist() == [[8, 10], [0, 0], [9, 0]]
+
+
+def test_tokens_without_a_block_leave_the_index_rows_alone(device):
+    """Tables with holes: the step's tokens have positions and slots of -1; their Index rows are not ingested, the others are."""
+    from types import SimpleNamespace
+
+    import kvip_b200 as kvip
+    tables = kvip.BlockTables(torch, device, batch=2, pages=4, blocks=4, tokens=8, block=4, queries=4)
+    tables.load(lengths=torch.tensor([3, 0]), held=torch.tensor([2, 0]), table=torch.tensor([[5, -1, -1, -1], [-1] * 4]), free=torch.tensor([6, -1, 8]))
+    tables.plan(torch.tensor([3, 4], dtype=torch.int32, device=device))
+    inputs = kvip.QueryInputs(torch, 2, device, history=128, queries=4)
+    inputs.prepare_device(tables.layout, torch.tensor([1, 2], dtype=torch.int32, device=device))
+    inputs.bind_positions(tables.positions)
+    storage = kvip.IndexCacheStorage(torch, 3, 128, 128, device)
+    cache = torch.arange(1, 9 * 4 + 1, device=device).to(torch.bfloat16)[:, None].expand(-1, 128).contiguous()
+    storage.ingest_decode((cache, None), SimpleNamespace(slot_mapping=tables.slot_mapping), inputs, inputs.row_owners)
+    assert tables.slot_mapping.tolist() == [23, -1, -1, 24, 25, 26, 27, -1]
+    assert int(storage.ingest_errors) == 2
+    expected = torch.tensor([[448.0, 448, 448, 24, 448], [25, 26, 27, 28, 448]]) / 448
+    assert torch.equal(storage.scales[1:, :5].cpu(), expected)
