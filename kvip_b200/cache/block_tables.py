@@ -16,9 +16,12 @@ class BlockTables:
         ...                       # the forward reads them
         tables.commit(kept)       # lengths += kept (the tokens that stay), the blocks of the plan become the request's
 
-    `plan` changes nothing but the table entries behind `held`, so a step that is planned again plans the same. Outputs are
+    `plan` changes nothing but the table entries behind `held`, so a step that is planned again plans the same. `commit`, `load` and
+    `release` end a plan: until the next one there is nothing to commit. Outputs are
     persistent buffers of this object, sized by `tokens` (packed tokens per step at most): the captured graph of a
     step finds them at the same place. `status` collects KVIP_ERR_* bits (include/kvip_b200.h: KvipSlotMapsArgs)."""
+
+    _planned = ()      # outputs of a plan that `commit` takes over, each with its value where nothing is planned
 
     def __init__(self, torch, device, *, batch, pages, blocks, tokens, block=_lib.BLOCK_TOKENS, queries=0):
         self.torch = torch
@@ -34,9 +37,10 @@ class BlockTables:
         self.batch, self.pages, self.blocks, self.tokens, self.block, self.queries = batch, pages, blocks, tokens, block, queries
         # one block of int32 and one of int64 words: a table is made in a few launches
         i32, i64 = dict(dtype=torch.int32, device=device), dict(dtype=torch.int64, device=device)
-        words = torch.zeros(5 * batch + 4 + tokens, **i32)
-        (self.lengths, self.held, self.ends, self.held_after, self.starts, self.head, self.taken, self.status, self.requests) = words.split(
-            (batch, batch, batch, batch, batch + 1, 1, 1, 1, tokens))
+        words = torch.zeros(5 * batch + 5 + tokens, **i32)
+        (self.lengths, self.held, self.ends, self.held_after, self.starts, self.head, self.taken, self.status, nothing, self.requests) = words.split(
+            (batch, batch, batch, batch, batch + 1, 1, 1, 1, 1, tokens))
+        self._planned = ((self.ends, self.lengths), (self.held_after, self.held), (self.taken, nothing))
         self.positions, self.slot_mapping = torch.full((2, tokens), -1, **i64).unbind(0)
         self.table = torch.full((batch, pages), -1, **i32)
         self.free = torch.arange(max(1, blocks), **i32)
@@ -69,6 +73,7 @@ class BlockTables:
         gap = self.blocks - free.numel()          # the list ends where the storage ends
         self.free[gap:self.blocks].copy_(free)
         self.head.fill_(gap + head)
+        self._end_plan()
 
     def plan(self, counts):
         """Maps of a step that adds counts[b] tokens to request b (int32 [batch] on the device): one launch, no host
@@ -81,15 +86,28 @@ class BlockTables:
 
     def commit(self, kept):
         """The planned blocks become the requests' own and `kept` [batch] int32 of the planned tokens stay (all of them, or
-        what a verification accepted). A request that keeps fewer holds its blocks for the tokens to come."""
-        self.lengths.add_(kept)
+        what a verification accepted). A request that keeps fewer holds its blocks for the tokens to come; one that the plan gave
+        no place (KVIP_ERR_*: `ends` is its length), or whose tokens were dropped behind the last output row, keeps none of those. A
+        plan is committed once: without another one a second call keeps nothing. `status` says KVIP_ERR_TOKEN_RANGE where more should
+        have been kept than was planned."""
+        if tuple(kept.shape) != (self.batch,):
+            raise ValueError("BlockTables kept counts must be [batch]")
+        torch = self.torch
+        room = torch.minimum(self.ends - self.lengths, self.starts[1:] - self.starts[:-1])
+        self.status.bitwise_or_((kept > room).any().to(torch.int32) * _lib.ERR_TOKEN_RANGE)
+        self.lengths.add_(torch.minimum(kept, room).clamp_(min=0))
         self.held.copy_(self.held_after)
         self.head.add_(self.taken)
+        self._end_plan()
+
+    def _end_plan(self):
+        for output, state in self._planned:
+            output.copy_(state)
 
     def release(self, rows):
         """Requests that have ended (host list of row numbers): their blocks return to the free list, their rows are
         empty. Fixed shapes, no device read on the host. Blocks that the list has no place for (rows of `load` that hold more than was
-        taken from it, or a block twice) are dropped, and `status` says KVIP_ERR_NO_SLOT."""
+        taken from it, or a block twice) are dropped, and `status` says KVIP_ERR_NO_SLOT. A plan that has not been committed ends here: its blocks are in the list still, and stay there."""
         rows = sorted(set(int(r) for r in rows))
         if not rows:
             return
@@ -115,3 +133,4 @@ class BlockTables:
         self.table[index] = -1
         self.held[index] = 0
         self.lengths[index] = 0
+        self._end_plan()

@@ -162,3 +162,34 @@ def test_tokens_without_a_block_leave_the_index_rows_alone(device):
     assert int(storage.ingest_errors) == 2
     expected = torch.tensor([[448.0, 448, 448, 24, 448], [25, 26, 27, 28, 448]]) / 448
     assert torch.equal(storage.scales[1:, :5].cpu(), expected)
+
+
+def test_block_tables_run_out_and_recover(device):
+    """More requests than blocks: those without keep their lengths whatever is committed, from a captured graph too, and go on when blocks
+    come back. Every block is in one place all the while."""
+    import kvip_b200 as kvip
+    batch, blocks = 4, 6
+    tables = kvip.BlockTables(torch, device, batch=batch, pages=4, blocks=blocks, tokens=32, block=4, queries=4)
+    counts, kept = (torch.full((batch,), n, dtype=torch.int32, device=device) for n in (4, 3))
+    stream = torch.cuda.Stream(device)
+    stream.wait_stream(torch.cuda.current_stream(device))
+    with torch.cuda.stream(stream):
+        tables.plan(torch.zeros_like(counts)).commit(torch.zeros_like(counts))
+        graph = torch.cuda.CUDAGraph()
+        stream.synchronize()
+        with torch.cuda.graph(graph, stream=stream):
+            tables.plan(counts).commit(kept)
+
+        def whole():
+            table, held = tables.table.cpu().numpy(), tables.held.cpu().numpy()
+            rows = [int(x) for b in range(batch) for x in table[b, :held[b]]]
+            return sorted(rows + tables.free[int(tables.head):].tolist()) == list(range(blocks))
+
+        graph.replay()
+        assert tables.lengths.tolist() == [3] * 4 and int(tables.status) == 0 and whole()
+        graph.replay()                           # two blocks for four requests
+        assert tables.lengths.tolist() == [6, 6, 3, 3] and int(tables.status) == 4 | 1 and whole()
+        tables.status.zero_()
+        tables.release([1])
+        graph.replay()
+        assert tables.lengths.tolist() == [9, 3, 3, 3] and tables.held.tolist() == [3, 1, 1, 1] and whole()
