@@ -107,7 +107,8 @@ class BlockTables:
     def release(self, rows):
         """Requests that have ended (host list of row numbers): their blocks return to the free list, their rows are
         empty. Fixed shapes, no device read on the host. Blocks that the list has no place for (rows of `load` that hold more than was
-        taken from it, or a block twice) are dropped, and `status` says KVIP_ERR_NO_SLOT. A plan that has not been committed ends here: its blocks are in the list still, and stay there."""
+        taken from it, or a block twice) are dropped, entries that are no block (a row with holes) are passed over, and `status` says
+        KVIP_ERR_NO_SLOT for either. A plan that has not been committed ends here: its blocks are in the list still, and stay there."""
         rows = sorted(set(int(r) for r in rows))
         if not rows:
             return
@@ -117,7 +118,8 @@ class BlockTables:
         index = torch.tensor(rows, dtype=torch.int64, device=self.device)
         table, held = self.table[index], self.held[index]
         page = torch.arange(self.pages, dtype=torch.int32, device=self.device)
-        mine = (page[None, :] < held[:, None]).reshape(-1)
+        listed = page[None, :] < held[:, None]
+        mine = (listed & (table >= 0)).reshape(-1)
         order = mine.cumsum(0)
         total = order[-1:]
         # the list grows downwards from head; entries that are no block, and blocks that the list has no place for (a state
@@ -128,7 +130,7 @@ class BlockTables:
         longer.scatter_(0, torch.where(fits, place, self.blocks), torch.where(fits, table.reshape(-1), longer[-1]))
         self.free[:self.blocks].copy_(longer[:-1])
         self.head.sub_(total.to(torch.int32)).clamp_(min=0)
-        lost = (mine & ~fits).any().to(torch.int32) * _lib.ERR_NO_SLOT
+        lost = ((mine & ~fits).any() | (listed & (table < 0)).any()).to(torch.int32) * _lib.ERR_NO_SLOT
         self.status.bitwise_or_(lost)
         self.table[index] = -1
         self.held[index] = 0

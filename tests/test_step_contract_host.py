@@ -1,5 +1,6 @@
 """Host-side halves of what the operators round the selection path owe one another: the state of the block tables between steps, with host
 tensors in the place of the device's."""
+import numpy as np
 import pytest
 import torch
 
@@ -98,3 +99,13 @@ def test_release_between_a_plan_and_its_commit_puts_no_block_into_two_rows(betwe
     t.plan([4, 8])
     t.commit(kept(4, 8))
     assert owned(t) == [0, 1, 2, 3, 4] and t.held.tolist() == [3 if not between else 2, 2]
+
+
+def test_release_passes_over_entries_that_are_no_block():
+    t = tables_on_the_host([9, 2], [3, 1], [[5, -1, 7], [8, -1, -1]], [0, 1, 2, 3], block=4, tokens=4, head=4)
+    t.release([0])
+    assert int(t.status) == 4 and int(t.head) == 2 and t.free.tolist() == [0, 1, 5, 7]
+    t.status.zero_()
+    t.release([1])
+    assert int(t.status) == 0 and int(t.head) == 1 and t.free.tolist() == [0, 8, 5, 7]
+    assert np.array_equal(t.held.numpy(), [0, 0]) and int(t.table.max()) == -1
