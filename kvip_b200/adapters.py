@@ -104,7 +104,8 @@ class IndexSelector:
     `LIFetch` and returns the logical TopK per query token; prefill rows of a mixed batch are selected by the
     model-side indexer over its own paged cache. `slots(n)` are the resident slots for the attention kernel.
 
-    The caller binds `inputs.bind_positions(positions)` before the call, as in the reference. With `rotary` (a
+    The caller binds `inputs.bind_positions(positions)` before the call, as in the reference. A step whose lengths the host
+    does not know is laid out by `prepare_device(tables, owners)` instead of `prepare`. With `rotary` (a
     `kvip.Rotary`), Index queries may come unrotated in the model's type and without scales: they are rotated by
     `positions`, one per query token, and quantised here. `attend` runs the attention of the decode rows over the slots."""
 
@@ -142,6 +143,17 @@ class IndexSelector:
             self.inputs.prepare([int(p.stop - p.begin) for p in self.decodes],
                                 query_starts=[int(p.begin) for p in self.decodes],
                                 query_owners=[int(p.owner) for p in self.decodes])
+        if self.row_owners.data_ptr() != self.inputs.row_owners.data_ptr():
+            self.row_owners.copy_(self.inputs.row_owners)
+
+    def prepare_device(self, tables, query_owners):
+        """`prepare` for a decode step whose request lengths are known on the device alone: `tables` the `BlockTables` that has
+        planned it, with as many query slots as the inputs, `query_owners` int32 [batch]. Device copies only, capturable. Plans
+        and slots of the step before are forgotten: every request of the step decodes."""
+        if tables.layout is None:
+            raise ValueError("LIFetch needs tables with query slots (BlockTables queries)")
+        self.inputs.prepare_device(tables.layout, query_owners)
+        self.plans, self.decodes, self.attention_indices = None, (), None
         if self.row_owners.data_ptr() != self.inputs.row_owners.data_ptr():
             self.row_owners.copy_(self.inputs.row_owners)
 

@@ -1,11 +1,13 @@
 """Host-side halves of what the operators round the selection path owe one another: the state of the block tables between steps, with host
 tensors in the place of the device's."""
+from types import SimpleNamespace
+
 import numpy as np
 import pytest
 import torch
 
 import step_reference as reference
-from kvip_b200 import BlockTables
+from kvip_b200 import BlockTables, IndexSelector, RequestPlan
 
 
 def tables_on_the_host(lengths, held, table, free, *, block, tokens, head=0):
@@ -109,3 +111,59 @@ def test_release_passes_over_entries_that_are_no_block():
     t.release([1])
     assert int(t.status) == 0 and int(t.head) == 1 and t.free.tolist() == [0, 8, 5, 7]
     assert np.array_equal(t.held.numpy(), [0, 0]) and int(t.table.max()) == -1
+
+
+class Inputs:
+    """What the selector asks of QueryInputs, on the host."""
+
+    batch, queries, index_heads = 2, 4, 64
+
+    def __init__(self):
+        self.query, self.weights, self.scale = torch.zeros(8, 64, 128), torch.zeros(8, 64), torch.zeros(8, 64)
+        self.row_owners = torch.zeros(2, dtype=torch.int32)
+        self.token_count, self.calls = 0, []
+
+    def prepare(self, counts, *, query_starts, query_owners):
+        self.row_owners[:len(query_owners)] = torch.tensor(query_owners, dtype=torch.int32)
+        self.token_count = sum(counts)
+
+    def prepare_device(self, layout, owners):
+        self.row_owners.copy_(owners)
+        self.token_count = 8
+
+    def pack(self, *_):
+        self.calls.append("pack")
+
+
+@pytest.mark.parametrize("plans", [[RequestPlan("a", 1, 0, 3, decode=False, key_end=3)],
+                                   [RequestPlan("a", 1, 0, 3, decode=True, key_end=9), RequestPlan("b", 2, 3, 5, decode=False, key_end=2)]])
+def test_a_step_prepared_on_the_device_forgets_the_plans_before_it(plans):
+    """A prefill or mixed forward, then a decode step whose layout the device has made: the step is packed and selected whole, its owners
+    reach a tensor of the selector's own, and slots of the step before are no longer there."""
+    inputs = Inputs()
+    storage = SimpleNamespace(prepare=lambda plans: None, ingest_prefill=lambda *_: inputs.calls.append("prefill"),
+                              ingest_decode=lambda cache, metadata, inputs, owners: inputs.calls.append(("decode", owners.tolist())))
+    rotating = SimpleNamespace(arguments=[inputs.query, None, inputs.weights, inputs.scale])
+    update = SimpleNamespace(logical_output=torch.arange(8 * 2048, dtype=torch.int32).view(8, 1, 2048), slot_output=torch.zeros(8, 1, 2048, dtype=torch.int32))
+    selector = IndexSelector(torch, inputs=inputs, rotating=rotating, update=update, logical_ids=torch.zeros(4, 8, dtype=torch.int64),
+                             row_owners=torch.zeros(2, dtype=torch.int32), storage=storage, forward=lambda: inputs.calls.append("forward"))
+    indexer = SimpleNamespace(k_cache=SimpleNamespace(kv_cache=None),
+                              select_topk_native=lambda query, *_: torch.zeros(query.shape[0], 1, 2048, dtype=torch.int32))
+    metadata = SimpleNamespace(block_table=torch.zeros(2, 4, dtype=torch.int32))
+
+    def step(tokens):
+        inputs.calls.clear()
+        return selector(torch.zeros(tokens, 64, 128), torch.zeros(tokens, 64), indexer, metadata, torch.ones(tokens, 64))
+
+    selector.prepare(plans)
+    step(plans[-1].stop)
+    assert "prefill" in inputs.calls
+    tables = SimpleNamespace(layout=torch.zeros(4, 8, dtype=torch.int64))
+    selector.prepare_device(tables, torch.tensor([3, 2], dtype=torch.int32))
+    with pytest.raises(RuntimeError, match="execute"):
+        selector.slots(1)
+    logical = step(6)
+    assert inputs.calls == [("decode", [3, 2]), "pack", "forward"]
+    assert torch.equal(logical, update.logical_output[:6]) and selector.slots(6).shape[0] == 6
+    with pytest.raises(ValueError, match="query slots"):
+        selector.prepare_device(SimpleNamespace(layout=None), torch.zeros(2, dtype=torch.int32))
