@@ -148,11 +148,16 @@ class IndexSelector:
 
     def prepare_device(self, tables, query_owners):
         """`prepare` for a decode step whose request lengths are known on the device alone: `tables` the `BlockTables` that has
-        planned it, with as many query slots as the inputs, `query_owners` int32 [batch]. Device copies only, capturable. Plans
-        and slots of the step before are forgotten: every request of the step decodes."""
+        planned it, with as many query slots as the inputs, `query_owners` int32 [batch]. Lays the query slots out, binds the
+        tokens' positions (`inputs.bind_positions`: the places where their Index keys go) and ends every list at `tables.lengths`: what a
+        token selects are cached tokens; those of its own step come to `attend` as `draft` rows, each once. Device copies only, capturable.
+        Plans and slots of the step before are forgotten: every request of the step decodes."""
         if tables.layout is None:
             raise ValueError("LIFetch needs tables with query slots (BlockTables queries)")
         self.inputs.prepare_device(tables.layout, query_owners)
+        self.inputs.bind_positions(tables.positions)
+        self.rotating.arguments[6].copy_(tables.lengths)      # the lengths that LI score and TopK read
+        self.positions = tables.positions
         self.plans, self.decodes, self.attention_indices = None, (), None
         if self.row_owners.data_ptr() != self.inputs.row_owners.data_ptr():
             self.row_owners.copy_(self.inputs.row_owners)
@@ -209,7 +214,8 @@ class IndexSelector:
         """Attention of the decode rows over the slots the selection has returned, straight from the resident pool:
         `attention` a `kvip.SlotAttention`, `query` [tokens, heads, 576] in packed order. `tables` (the `BlockTables` that
         planned the step) names the request of every token and where a request's tokens start; without it `requests` and,
-        for drafted rows, `starts` do, or the layout of the step is read."""
+        for drafted rows, `starts` do, or the layout of the step is read. Drafted rows are keys beside those of the lists: where the
+        lists may name the step's own tokens (lengths other than those that `prepare_device` sets), such a token would count twice."""
         if tables is not None:
             requests, starts = tables.requests, tables.starts
         elif requests is None:

@@ -131,6 +131,9 @@ class Inputs:
         self.row_owners.copy_(owners)
         self.token_count = 8
 
+    def bind_positions(self, positions):
+        self.positions = positions
+
     def pack(self, *_):
         self.calls.append("pack")
 
@@ -143,7 +146,7 @@ def test_a_step_prepared_on_the_device_forgets_the_plans_before_it(plans):
     inputs = Inputs()
     storage = SimpleNamespace(prepare=lambda plans: None, ingest_prefill=lambda *_: inputs.calls.append("prefill"),
                               ingest_decode=lambda cache, metadata, inputs, owners: inputs.calls.append(("decode", owners.tolist())))
-    rotating = SimpleNamespace(arguments=[inputs.query, None, inputs.weights, inputs.scale])
+    rotating = SimpleNamespace(arguments=[inputs.query, None, inputs.weights, inputs.scale, None, None, torch.full((2,), 99, dtype=torch.int32)])
     update = SimpleNamespace(logical_output=torch.arange(8 * 2048, dtype=torch.int32).view(8, 1, 2048), slot_output=torch.zeros(8, 1, 2048, dtype=torch.int32))
     selector = IndexSelector(torch, inputs=inputs, rotating=rotating, update=update, logical_ids=torch.zeros(4, 8, dtype=torch.int64),
                              row_owners=torch.zeros(2, dtype=torch.int32), storage=storage, forward=lambda: inputs.calls.append("forward"))
@@ -158,10 +161,12 @@ def test_a_step_prepared_on_the_device_forgets_the_plans_before_it(plans):
     selector.prepare(plans)
     step(plans[-1].stop)
     assert "prefill" in inputs.calls
-    tables = SimpleNamespace(layout=torch.zeros(4, 8, dtype=torch.int64))
+    tables = SimpleNamespace(layout=torch.zeros(4, 8, dtype=torch.int64), positions=torch.tensor([5, 6, 7, 8, 2, 3]),
+                             lengths=torch.tensor([5, 2], dtype=torch.int32))
     selector.prepare_device(tables, torch.tensor([3, 2], dtype=torch.int32))
     with pytest.raises(RuntimeError, match="execute"):
         selector.slots(1)
+    assert inputs.positions is tables.positions and selector.positions is tables.positions and rotating.arguments[6].tolist() == [5, 2]
     logical = step(6)
     assert inputs.calls == [("decode", [3, 2]), "pack", "forward"]
     assert torch.equal(logical, update.logical_output[:6]) and selector.slots(6).shape[0] == 6
