@@ -146,18 +146,19 @@ class IndexSelector:
         if self.row_owners.data_ptr() != self.inputs.row_owners.data_ptr():
             self.row_owners.copy_(self.inputs.row_owners)
 
-    def prepare_device(self, tables, query_owners):
+    def prepare_device(self, tables, query_owners, depths=None):
         """`prepare` for a decode step whose request lengths are known on the device alone: `tables` the `BlockTables` that has
         planned it, with as many query slots as the inputs, `query_owners` int32 [batch]. Lays the query slots out, binds the
         tokens' positions (`inputs.bind_positions`: the places where their Index keys go) and ends every list at `tables.lengths`: what a
-        token selects are cached tokens; those of its own step come to `attend` as `draft` rows, each once. Device copies only, capturable.
+        token selects are cached tokens; those of its own step come to `attend` as `draft` rows, each once. `depths` [tokens] int32, for trees: `self.positions`, by which
+        queries and keys turn, go by the depth of a token and not by its place. Device work only, capturable.
         Plans and slots of the step before are forgotten: every request of the step decodes."""
         if tables.layout is None:
             raise ValueError("LIFetch needs tables with query slots (BlockTables queries)")
         self.inputs.prepare_device(tables.layout, query_owners)
         self.inputs.bind_positions(tables.positions)
         self.rotating.arguments[6].copy_(tables.lengths)      # the lengths that LI score and TopK read
-        self.positions = tables.positions
+        self.positions = tables.positions if depths is None else tables.tree_positions(depths)
         self.plans, self.decodes, self.attention_indices = None, (), None
         if self.row_owners.data_ptr() != self.inputs.row_owners.data_ptr():
             self.row_owners.copy_(self.inputs.row_owners)

@@ -84,6 +84,21 @@ class BlockTables:
         self.launch(self.index, self._lengths, counts.data_ptr(), *self._rest)
         return self
 
+    def tree_positions(self, depths):
+        """Positions in the text of the planned tokens of trees: `lengths` + depth, where `positions` are the places of the tokens in
+        the caches, one for each. depths: int32 [tokens] (or longer), 0 for a request's first token and one more than its parent's
+        for the others. A depth that is negative or above the token's number in its request is taken as the nearest that is not
+        (KVIP_ERR_TOKEN_RANGE); -1 where a token has no position. int64 [tokens], new; between `plan` and `commit`, capturable."""
+        torch = self.torch
+        if depths.dtype != torch.int32 or depths.ndim != 1 or depths.numel() < self.tokens or depths.device != self.table.device:
+            raise ValueError("BlockTables depths must be flat int32 with an entry per packed token, on the tables' device")
+        live = self.positions >= 0
+        length = self.lengths[self.requests.clamp(min=0).long()]
+        number = self.positions - length
+        depth = depths[:self.tokens].long().clamp(min=0).minimum(number)
+        self.status.bitwise_or_((live & (depth != depths[:self.tokens])).any().to(torch.int32) * _lib.ERR_TOKEN_RANGE)
+        return torch.where(live, length + depth, -1)
+
     def commit(self, kept):
         """The planned blocks become the requests' own and `kept` [batch] int32 of the planned tokens stay (all of them, or
         what a verification accepted). A request that keeps fewer holds its blocks for the tokens to come; one that the plan gave

@@ -51,12 +51,12 @@ class Loop:
         row_owners = torch.zeros(BATCH, dtype=torch.int32, device=device) if own_owners else p.workspace.inputs.row_owners
         self.select = kvip.IndexSelector(torch, inputs=p.workspace.inputs, rotating=p.rotating, update=p.update, logical_ids=p.storage.logical_ids,
                                          row_owners=row_owners, storage=p.storage, forward=p.forward, rotary=self.rope)
-        self.model = {}
+        self.model, self.jumps = {}, 0
         self.new_inputs([4, 3, 4, 2, 4], tree=False)
 
     def new_inputs(self, counts, tree):
         """What the model computes for the step's tokens, in place, so that a captured graph reads it."""
-        device, g, tokens = self.device, self.g, self.tokens
+        device, g, tokens, self.tree = self.device, self.g, self.tokens, tree
         parents, depths, masks, drafted = (np.zeros(tokens, np.int64) for _ in range(4))
         t = 0
         for n in counts:
@@ -101,7 +101,7 @@ class Loop:
         t.commit(self.verify.counts)
 
     def prepare(self):
-        self.select.prepare_device(self.tables, self.owners)
+        self.select.prepare_device(self.tables, self.owners, self.model["depths"] if self.tree else None)
         return self.select.positions
 
     def keep(self):
@@ -149,6 +149,7 @@ class Loop:
             assert int(self.verify.counts[b]) == counts[0] and np.array_equal(self.verify.nodes[b].cpu().numpy(), nodes[0])
             path = a + nodes[0, :counts[0]]
             kept.append(int(counts[0]))
+            self.jumps += int((nodes[0, :counts[0]] != np.arange(counts[0])).any())
             self.rows[b] = np.concatenate([self.rows[b], rows[path]])
             x = host(m["index_key"])[path].astype(np.float32)
             scale = (np.abs(x).max(1) / np.float32(448)).astype(np.float32)
@@ -194,3 +195,12 @@ def run(loop, device, *, tree, captured, steps=5):
 @pytest.mark.parametrize("captured,own_owners", [(False, False), (True, False), (False, True)])
 def test_every_key_of_a_chain_is_seen_once(device, captured, own_owners):
     run(Loop(device, 3, own_owners), device, tree=False, captured=captured)
+
+
+@pytest.mark.parametrize("captured", [False, True])
+def test_nodes_of_a_tree_turn_by_their_depth_and_see_their_ancestors(device, captured):
+    """Trees of up to four nodes: siblings have one position and two places, a node selects none of the step's tokens, and the accepted path is
+    the continuation of the request whichever nodes it runs through."""
+    loop = Loop(device, 4)
+    run(loop, device, tree=True, captured=captured)
+    assert loop.jumps > 0                        # accepted paths that leave nodes out

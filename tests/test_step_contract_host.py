@@ -24,6 +24,7 @@ def tables_on_the_host(lengths, held, table, free, *, block, tokens, head=0):
         out = reference.slot_maps(t.lengths.numpy(), counts, t.held.numpy(), t.table.numpy(), t.free.numpy(), int(t.head), block=block, tokens=tokens)
         for name in ("table", "starts", "ends", "held_after", "taken"):
             getattr(t, name).copy_(torch.from_numpy(out[name]))
+        t.positions, t.requests = torch.from_numpy(out["positions"]), torch.from_numpy(out["requests"])
         t.status |= torch.from_numpy(out["status"])
         return out
 
@@ -111,6 +112,20 @@ def test_release_passes_over_entries_that_are_no_block():
     t.release([1])
     assert int(t.status) == 0 and int(t.head) == 1 and t.free.tolist() == [0, 8, 5, 7]
     assert np.array_equal(t.held.numpy(), [0, 0]) and int(t.table.max()) == -1
+
+
+def test_positions_of_trees_go_by_depth():
+    t = tables_on_the_host([5, 0, 9], [1, 0, 1], [[0, -1], [-1, -1], [1, -1]], [2, 3, 3, 3], block=16, tokens=9)
+    t.plan([4, 0, 3])
+    assert t.positions.tolist() == [5, 6, 7, 8, 9, 10, 11, -1, -1]
+    depths = torch.tensor([0, 1, 1, 2, 0, 1, 1, 5, -7], dtype=torch.int32)
+    assert t.tree_positions(depths).tolist() == [5, 6, 6, 7, 9, 10, 10, -1, -1] and int(t.status) == 0
+    depths[1:3] = torch.tensor([-1, 3])
+    assert t.tree_positions(depths).tolist() == [5, 5, 7, 7, 9, 10, 10, -1, -1] and int(t.status) == 1
+    with pytest.raises(ValueError, match="depths"):
+        t.tree_positions(depths[:8])
+    with pytest.raises(ValueError, match="depths"):
+        t.tree_positions(depths.long())
 
 
 class Inputs:
