@@ -686,7 +686,7 @@ uint32_t kvip_b200_rotary(const KvipRotaryArgs* args, void* stream);
  *                                            request with more drafted rows is a KVIP_ERR_TOKEN_RANGE).
  * A row has 576 elements, its first 512 are also the value:
  *   out[t,h] = sum p v, p = softmax(scale * query[t,h] . row); lse[t,h] = log of the sum of exp(scale * query . row).
- * A token that sees no row gets zeros and lse = -inf; a token with requests[t] < 0 is padding, its outputs are left as they are. */
+ * A token that sees no row (or none with a score above -inf) gets zeros and lse = -inf; a token with requests[t] < 0 is padding, its outputs are left as they are. */
 #define KVIP_ATTENTION_WIDTH 576u
 #define KVIP_ATTENTION_VALUE 512u
 typedef struct KvipAttentionArgs {

@@ -51,6 +51,7 @@ template <uint32_t kN> struct Warps {
 };
 constexpr uint32_t kOutRow = kValue * 2 + 16;           // bytes of an output row while it is laid out: four banks further than the last
 constexpr float kSlack = 8.f;                           // log2: p may reach 2^8 before the reference moves
+constexpr float kLowest = -3.402823466e38f;             // the reference before any row: finite, so that a score of -inf weighs 2^(-inf) = 0
 constexpr uint32_t kDefaultWaitKilocycles = 2000000u;   // about one second of SM clock
 
 // What token t may read.
@@ -423,7 +424,7 @@ attend_tiles(const __grid_constant__ CUtensorMap query_map, const __grid_constan
     const uint32_t side = warp >> 2, w = warp & 3u, head_at = side * kSideHeads;
     float ref[2 * kBlocks], sum[2 * kBlocks];
 #pragma unroll
-    for (uint32_t j = 0; j < 2 * kBlocks; ++j) { ref[j] = -INFINITY; sum[j] = 0.f; }
+    for (uint32_t j = 0; j < 2 * kBlocks; ++j) { ref[j] = kLowest; sum[j] = 0.f; }
     const float scale = a.scale * 1.4426950408889634f;
     const uint32_t quad = (w * 32u) << 16;
     const uint32_t row0 = w * 16u + (lane >> 2);
@@ -551,7 +552,7 @@ attend_tiles(const __grid_constant__ CUtensorMap query_map, const __grid_constan
     if (tid < heads) {
       const float total = (c.reduce[0][tid] + c.reduce[1][tid]) + (c.reduce[2][tid] + c.reduce[3][tid]);
       if (shares > 1) c.factor[tid] = written ? total : 0.f;   // no rows: no mass; scores of NaN have a mass of NaN
-      else c.factor[tid] = written ? 1.f / total : 0.f;
+      else c.factor[tid] = written && total != 0.f ? 1.f / total : 0.f;   // scores of -inf have no mass either
       if (shares == 1 && !idle && !dead)
         a.lse[static_cast<uint64_t>(t) * a.heads + head0 + tid] = written ? (c.top[tid] + log2f(total)) * 0.6931471805599453f : -INFINITY;
     }

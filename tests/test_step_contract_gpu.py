@@ -5,6 +5,9 @@ import numpy as np
 import pytest
 import torch
 
+import step_reference as reference
+from test_step_operators_gpu import HALF_STEP, attention_case, check_attention, host, visible_rows
+
 pytestmark = pytest.mark.gpu
 
 
@@ -193,3 +196,35 @@ def test_block_tables_run_out_and_recover(device):
         tables.release([1])
         graph.replay()
         assert tables.lengths.tolist() == [9, 3, 3, 3] and tables.held.tolist() == [3, 1, 1, 1] and whole()
+
+
+# ---- attention at the ends of its types ----------------------------------------------------------------------------------
+@pytest.mark.parametrize("splits", [1, 2, 8])
+@pytest.mark.parametrize("where", ["first tile", "middle", "all but one", "all"])
+def test_attention_scores_of_minus_infinity_weigh_nothing(device, where, splits):
+    """Finite queries and rows whose products leave fp32: scores of -inf in a head's first tile, in the middle of its list, in all of it. The
+    rows that are left make the head's answer; the other heads do not notice."""
+    import kvip_b200 as kvip
+    entries, hot = 640, [0, 9, 17]
+    case = attention_case(device, 51, counts=[1, 2], heads=24, entries=entries, stride=entries, context=[entries, entries], draft=False)
+    case["slots"][:] = torch.arange(entries, dtype=torch.int32, device=device)
+    low = torch.zeros(entries, dtype=torch.bool, device=device)
+    low[{"first tile": slice(0, 64), "middle": slice(100, 400), "all but one": slice(0, entries), "all": slice(0, entries)}[where]] = True
+    low[333] &= where != "all but one"
+    pool = case["pool"].view(-1, entries, 576)
+    pool[..., 0] = torch.where(low, -16.0, 0.0).to(torch.bfloat16)
+    case["query"][:, hot, 0] = 2.0 ** 126
+    attend = kvip.SlotAttention(torch, device, tokens=3, heads=24, entries=entries)
+    out, lse = attend(**case, splits=splits)
+    check_attention(dict(case, query=case["query"][:, [h for h in range(24) if h not in hot]]), out[:, [h for h in range(24) if h not in hot]],
+                    lse[:, [h for h in range(24) if h not in hot]])
+    for t in range(3):
+        rows = host(visible_rows(case, t))[~low.cpu().numpy()]
+        expected, log_sum, weight, size = reference.attention(host(case["query"][t, hot]), rows, case["scale"])
+        if where == "all":
+            assert bool((out[t, hot] == 0).all()) and bool((lse[t, hot] == float("-inf")).all())
+            continue
+        step, logit = HALF_STEP[torch.bfloat16], 577 * 2.0 ** -24 * size     # as in check_attention
+        assert (np.abs(host(out[t, hot]) - expected) <= weight * (2 * step + 2 * logit + 2.0 ** -18) + np.abs(expected) * step + 1e-7).all()
+        assert (np.abs(host(lse[t, hot]) - log_sum) <= logit + 2.0 ** -20 * (1 + np.abs(log_sum))).all()
+    assert int(attend.status) == 0
