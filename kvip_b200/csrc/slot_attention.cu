@@ -12,10 +12,10 @@
 // atom, K-major for the first product (elements along K) and M-major for the second (elements along M, rows along K).
 // So every row is fetched once, 512 accumulator columns of a [heads x 512] output become 4 x heads <= 256, and small head
 // counts cost small N. Rows as lanes also make the softmax cheap: p is scaled by a reference `ref` per head that only has
-// to be near the running maximum, so a tile needs no reduction over rows unless some score leaves ref + 8 (then the
+// to be near the running maximum, so a tile needs no reduction over rows unless some score leaves ref + 8 (fp16: 15; then the
 // maximum is taken, and the accumulators and sums are rescaled); sums of p stay per thread until the end.
 //
-// p is rounded to the rows' type for the second product (half a step, as the output is); its sum is taken before the
+// p is rounded to the rows' type for the second product (half a step, as the output is; fp16 ranges see Reference); its sum is taken before the
 // rounding, in fp32, because the log-sum is an output too.
 //
 // Bound, at 64 heads per CTA, by the loop of the two stages that shared memory holds beside the queries: a tile's rows need 3200
@@ -50,7 +50,11 @@ template <uint32_t kN> struct Warps {
   static constexpr uint32_t kThreads = 32 * (kValue + 1);
 };
 constexpr uint32_t kOutRow = kValue * 2 + 16;           // bytes of an output row while it is laid out: four banks further than the last
-constexpr float kSlack = 8.f;                           // log2: p may reach 2^8 before the reference moves
+// Weights lie at most 2^kSlack above the reference, and it moves to 2^kLift below the maximum. fp16 has 24 powers of two below 1 and 15
+// above: the largest weight of a head stays between 2^10 and 2^15, so weights keep all their bits down to 2^-24 of the largest, and what 2^20
+// rows beneath lose is 2^-15 of the result at most. With both as for bf16, whose exponents reach 2^-126, rows 2^-25 of the largest were lost.
+template <typename T> struct Reference { static constexpr float kSlack = 8.f, kLift = 0.f; };
+template <> struct Reference<__half> { static constexpr float kSlack = 15.f, kLift = 10.f; };
 constexpr float kLowest = -3.402823466e38f;             // the reference before any row: finite, so that a score of -inf weighs 2^(-inf) = 0
 constexpr uint32_t kDefaultWaitKilocycles = 2000000u;   // about one second of SM clock
 
@@ -447,14 +451,14 @@ attend_tiles(const __grid_constant__ CUtensorMap query_map, const __grid_constan
         __syncwarp();
         if (lane == 0) mbar_arrive(bar(c.taken[s]));
       }
-      // scores in units of log2; one more than 2^8 above its reference makes the whole side take the maximum
+      // scores in units of log2; one too far above its reference makes the whole side take the maximum
       float x[4 * kBlocks];
       bool above = false;
 #pragma unroll
       for (uint32_t j = 0; j < 4 * kBlocks; ++j) {
         const bool has = ok && ((j & 2u) ? has1 : has0);
         x[j] = has ? __uint_as_float(v[j]) * scale : -INFINITY;
-        above |= x[j] - ref[(j >> 2) * 2u + (j & 1u)] > kSlack;
+        above |= x[j] - ref[(j >> 2) * 2u + (j & 1u)] > Reference<T>::kSlack;
       }
       // Weights against the reference as it stands: on their way while the warps agree that it may stand.
       float e[4 * kBlocks];
@@ -478,7 +482,7 @@ attend_tiles(const __grid_constant__ CUtensorMap query_map, const __grid_constan
         for (uint32_t j = 0; j < 2 * kBlocks; ++j) {
           const uint32_t h = head_at + (j >> 1) * 8u + (lane & 3u) * 2u + (j & 1u);
           const float top = fmaxf(fmaxf(c.reduce[0][h], c.reduce[1][h]), fmaxf(c.reduce[2][h], c.reduce[3][h]));
-          const float next = fmaxf(ref[j], top);
+          const float next = fmaxf(ref[j], top - Reference<T>::kLift);
           const float factor = next == ref[j] ? 1.f : exp2_fast(ref[j] - next);   // 0 the first time
           ref[j] = next;
           sum[j] *= factor;

@@ -228,3 +228,32 @@ def test_attention_scores_of_minus_infinity_weigh_nothing(device, where, splits)
         assert (np.abs(host(out[t, hot]) - expected) <= weight * (2 * step + 2 * logit + 2.0 ** -18) + np.abs(expected) * step + 1e-7).all()
         assert (np.abs(host(lse[t, hot]) - log_sum) <= logit + 2.0 ** -20 * (1 + np.abs(log_sum))).all()
     assert int(attend.status) == 0
+
+
+@pytest.mark.parametrize("at", [0, 12345, -1])
+@pytest.mark.parametrize("kind,entries,below", [(torch.float16, 1 << 18, 25.4), (torch.float16, 1 << 20, 25.4), (torch.float16, 1 << 20, 31.0),
+                                                (torch.bfloat16, 1 << 18, 25.4), (torch.float16, 40000, 17.0)])
+def test_attention_of_one_large_row_among_very_many_small_ones(device, kind, entries, below, at):
+    """One row 2^below times as heavy as each of the others, whose values are 100 times its own: together they count. Closed form, with a
+    list that names two pool rows over and over."""
+    import kvip_b200 as kvip
+    attend = kvip.SlotAttention(torch, device, tokens=1, heads=16, entries=entries, dtype=kind)
+    pool = torch.zeros((128, 576), dtype=kind, device=device)
+    pool[1, 0] = 4.0                               # the heavy row, by the first element, which the value of the others lacks too
+    pool[0, 1:512], pool[1, 1:512] = 100.0, 1.0
+    query = torch.zeros((1, 16, 576), dtype=kind, device=device)
+    query[..., 0] = torch.linspace(0.5, 1, 16, device=device).to(kind)
+    slots = torch.zeros((1, entries), dtype=torch.int32, device=device)
+    slots[0, at] = 1
+    scale = below * np.log(2.0) / 4
+    logit = query[0, :, 0].double() * 4 * np.float64(np.float32(scale))
+    rest = (entries - 1) * torch.exp(-logit)
+    out, lse = attend(query, pool, slots, scale=scale, output_stride=128, requests=torch.zeros(1, dtype=torch.int32, device=device))
+    expected = (1 + 100 * rest) / (1 + rest)
+    # every weight half a step, the logit (two roundings in fp32, in the product and in units of log2) and exp2; sums in fp32: a thread adds an
+    # entry in 32, the accumulators take four products a tile, whose sums may be cut (a whole step); one rounding of the output
+    adds = entries / 32 * 2.0 ** -24 + entries / 16 * 2.0 ** -23
+    tolerance = 2 * HALF_STEP[kind] + 3 * 2.0 ** -24 * below + 2.0 ** -21 + adds + HALF_STEP[kind]
+    assert bool(((out[0, :, 1:].double() - expected[:, None]).abs() <= expected[:, None] * tolerance).all())
+    log_sum = logit + torch.log1p(rest)
+    assert bool(((lse[0].double() - log_sum).abs() <= 3 * 2.0 ** -24 * below + 2.0 ** -20 * (1 + log_sum) + adds).all())
