@@ -57,6 +57,7 @@ template <typename T> struct Reference { static constexpr float kSlack = 8.f, kL
 template <> struct Reference<__half> { static constexpr float kSlack = 15.f, kLift = 10.f; };
 constexpr float kLowest = -3.402823466e38f;             // the reference before any row: finite, so that a score of -inf weighs 2^(-inf) = 0
 constexpr uint32_t kDefaultWaitKilocycles = 2000000u;   // about one second of SM clock
+constexpr uint32_t kPromptKilocycles = 100000u;         // limits up to 50 ms
 
 // What token t may read.
 struct Rows {
@@ -89,29 +90,36 @@ __device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
 __device__ __forceinline__ void mbar_arrive(uint32_t bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
 }
+// A try sleeps until the phase ends or some time that the hardware sets is over, far more than a thousand clocks; a test does not.
 __device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
   uint32_t done;
   asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
                : "=r"(done) : "r"(bar), "r"(parity) : "memory");
   return done != 0u;
 }
+__device__ __forceinline__ bool mbar_test(uint32_t bar, uint32_t parity) {
+  uint32_t done;
+  asm volatile("{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+               : "=r"(done) : "r"(bar), "r"(parity) : "memory");
+  return done != 0u;
+}
 struct Waits {
   volatile uint32_t* abort_flag;   // set by the first wait of the CTA that gives up; read by all the others
   long long limit;                 // SM clock cycles a wait may take
+  bool prompt;                     // a limit near the length of a try's sleep: poll
 };
+__device__ __forceinline__ bool mbar_done(uint32_t bar, uint32_t parity, const Waits& w) { return w.prompt ? mbar_test(bar, parity) : mbar_try(bar, parity); }
 __device__ __forceinline__ bool mbar_wait_slow(uint32_t bar, uint32_t parity, const Waits& w) {
   const long long start = clock64();
-  for (;;) {
-    for (int i = 0; i < 32; ++i)
-      if (mbar_try(bar, parity)) return true;
+  do {                                 // the clock is read behind every try
+    if (mbar_done(bar, parity, w)) return true;
     if (*w.abort_flag) return false;
-    if (clock64() - start > w.limit) break;
-  }
+  } while (clock64() - start <= w.limit);
   *w.abort_flag = 1u;
   return false;
 }
 __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, const Waits& w) {
-  return mbar_try(bar, parity) || mbar_wait_slow(bar, parity, w);
+  return mbar_done(bar, parity, w) || mbar_wait_slow(bar, parity, w);
 }
 // Barrier of `kThreads` threads that also tells all of them whether any has `flag`.
 template <uint32_t kThreads = kRole> __device__ __forceinline__ bool role_any(uint32_t id, bool flag) {
@@ -300,7 +308,8 @@ attend_tiles(const __grid_constant__ CUtensorMap query_map, const __grid_constan
   const uint32_t shares_log = tiles <= 3u ? 0u : splits_log, shares = 1u << shares_log;
   const bool idle = rows.request < 0 || split >= shares;
   const uint32_t first = idle ? 0u : tiles * split >> shares_log, count = idle ? 0u : (tiles * (split + 1u) >> shares_log) - first;
-  const Waits waits{&c.abort_flag, static_cast<long long>(a.wait_kilocycles ? a.wait_kilocycles : kDefaultWaitKilocycles) << 10};
+  const Waits waits{&c.abort_flag, static_cast<long long>(a.wait_kilocycles ? a.wait_kilocycles : kDefaultWaitKilocycles) << 10,
+                    a.wait_kilocycles - 1u < kPromptKilocycles};
   constexpr uint32_t kScores = 0, kOut = 2 * kN;   // tensor-memory columns: two score tiles, four value blocks
   auto none = [&](uint32_t s) { return (c.valid[s][0] | c.valid[s][1] | c.valid[s][2] | c.valid[s][3]) == 0u; };
 

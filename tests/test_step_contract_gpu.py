@@ -257,3 +257,28 @@ def test_attention_of_one_large_row_among_very_many_small_ones(device, kind, ent
     assert bool(((out[0, :, 1:].double() - expected[:, None]).abs() <= expected[:, None] * tolerance).all())
     log_sum = logit + torch.log1p(rest)
     assert bool(((lse[0].double() - log_sum).abs() <= 3 * 2.0 ** -24 * below + 2.0 ** -20 * (1 + log_sum) + adds).all())
+
+
+@pytest.mark.parametrize("heads", [16, 64])
+def test_attention_waits_give_up(device, heads):
+    """Limits of one to a few kilocycles, which no tile's rows can meet everywhere: some call reports KVIP_ERR_PIPELINE, in one piece and in
+    shares, over full lists and over tiles without rows; each call ends by itself, and the next one without a limit is right."""
+    import kvip_b200 as kvip
+    case = attention_case(device, 60, counts=[40, 24], heads=heads, entries=2048, stride=4096, context=[2048, 2048], draft=False)
+    holes = dict(case, slots=case["slots"].clone())
+    for tile in (0, 5, 31):
+        holes["slots"][:, 64 * tile:64 * tile + 64] = -1
+    holes["slots"][::2, 1024:] = -1
+    attend = kvip.SlotAttention(torch, device, tokens=64, heads=heads)
+    for now in (case, holes):
+        for splits in (1, 4):
+            seen = set()
+            for limit in (1, 1, 2, 3):
+                attend(**now, splits=splits, wait_kilocycles=limit)
+                torch.cuda.synchronize()
+                seen.add(int(attend.status))
+                attend.status.zero_()
+            assert seen <= {0, 32} and 32 in seen, (splits, seen)
+            out, lse = attend(**now, splits=splits)
+            check_attention(now, out, lse, tokens=range(0, 64, 7))
+            assert int(attend.status) == 0
