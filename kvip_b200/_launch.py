@@ -33,7 +33,10 @@ class Launcher:
         self.what = name.replace("kvip_b200_", "")
 
     def __call__(self, index, *values):
-        record = self.pack(*values)
+        try:
+            record = self.pack(*values)
+        except struct.error as error:                  # a negative count, a number that its field does not hold
+            raise ValueError(f"{self.what}: {error}") from None
         if _current_device() == index:
             code = self.function(record, _raw_stream(index))
         else:

@@ -187,3 +187,17 @@ def test_a_step_prepared_on_the_device_forgets_the_plans_before_it(plans):
     assert torch.equal(logical, update.logical_output[:6]) and selector.slots(6).shape[0] == 6
     with pytest.raises(ValueError, match="query slots"):
         selector.prepare_device(SimpleNamespace(layout=None), torch.zeros(2, dtype=torch.int32))
+
+
+def test_numbers_that_a_record_does_not_hold_are_value_errors():
+    from kvip_b200 import _launch, _lib
+    from kvip_b200.build import build_library
+    build_library()
+    launch = _launch.Launcher("kvip_b200_slot_attention")
+    good = [0] * len(_lib.AttentionArgs._fields_)
+    names = [name for name, _ in _lib.AttentionArgs._fields_]
+    for name, value in (("splits", -1), ("wait_kilocycles", 1 << 32), ("output_stride", -5), ("scale", "x")):
+        values = list(good)
+        values[names.index(name)] = value
+        with pytest.raises(ValueError, match="slot_attention"):
+            launch(0, *values)
