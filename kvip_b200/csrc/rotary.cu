@@ -4,8 +4,8 @@
 // part (exact subtraction in fp64) goes to sincospi in fp32. A position of 2^21 keeps 32 bits behind the point that way,
 // where an fp32 angle would have none. The rotation is fp32, rounded once to the row's type.
 //
-// Bound by HBM: 8192 tokens x 129 rows of 64 inside rows of 576 take 50 us (5.4 TB/s), 16411 x 64 rows of 128 to FP8 87.6 us (4.65 TB/s); one
-// pair per thread instead of a unit of eight took 204 and 473.
+// Bound by HBM: 8192 tokens x 129 rows of 64 inside rows of 576 take 50 us (5.4 TB/s), 16411 x 64 rows of 128 to FP8 87.6 us (4.65 TB/s,
+// issue slots 68 % busy; 95 us where the power limit holds the clock down); one pair per thread instead of a unit of eight took 204 and 473.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>

@@ -20,9 +20,9 @@
 //
 // Bound, at 64 heads per CTA, by the loop of the two stages that shared memory holds beside the queries: a tile's rows need 3200
 // clocks to land while the other tile's products run (1253 for the copies alone), 1170 more until its scores are complete, 1140 for
-// the softmax and 760 until the value product lets go: 6270 clocks for two tiles. The tensor pipe is busy in about 53 % of a CTA's cycles. At
+// the softmax and 760 until the value product lets go: 6270 clocks for two tiles. The tensor pipe is busy in about 56 % of a CTA's cycles. At
 // 16 heads by HBM. Measured on one B200: 64 tokens x 128 heads x 2048 rows 64.5 us (36.5 GFLOP, 169 MB once), 128 tokens x 16 heads
-// 60.8 us (5.0 TB/s of rows), one token x 128 heads 13.8 us.
+// 60.8 us (5.0 TB/s of rows), one token x 128 heads 13.7 us.
 #include <atomic>
 #include <cuda.h>
 #include <cuda_bf16.h>

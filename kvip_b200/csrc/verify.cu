@@ -4,12 +4,13 @@
 // vocabulary only where a drafted token is rejected or the walk ends: the sum of what is left, and then the place where
 // the running sum passes sample * sum. A cluster of CTAs takes one request. Every CTA makes the whole walk from the same
 // numbers, so all of them take the same turns; a pass is split over the warps of the cluster in contiguous shares, whose sums
-// go to every CTA through distributed shared memory, and the warp whose share holds the border looks for it. Sums are fp64 and
-// their order is fixed. The rejections at one node need no pass of their own over each other's results: where r - Z q is not
-// cut off, r = max(target - C draft, 0) with C = 1 + Z_1 + .. + Z_(k-1), and what was cut off stays below. So a pass costs one fp64
-// fma, one add and two conversions (the slowest of them, 16 a clock and SM) per element, however many rejections. Bound by HBM: one
-// target row (and one draft row behind a rejection) per pass. Measured: 64 chains of 4 over 131072 tokens in fp32 18.8 us (67 MB, half of the
-// time in the pass), one request 9.7 us (latency), 48 trees of up to 16 nodes over 100003 bf16 tokens 31 us (five passes in one of them).
+// go to every CTA through distributed shared memory, and the warp whose share holds the border looks for it. Sums are fp64; how a row is
+// shared out goes by the batch, which moves a border by the roundings of fp64 and no more. The rejections at one node need no pass of their
+// own over each other's results: where r - Z q is not cut off, r = max(target - C draft, 0) with C = 1 + Z_1 + .. + Z_(k-1), and what was cut
+// off stays below. So a pass costs one fp64 fma, one add and two conversions per element, however many rejections, beside shifting rows of odd
+// length into place. Measured: 64 chains of 4 over 131072 tokens in fp32 18.9 us (67 MB; HBM 31 % of its peak, the rest is the latency before and
+// behind the pass), one request 9.7 us (latency), 48 trees of up to 16 nodes over 100003 bf16 tokens 31.7 us (ALU pipe of the busiest SM 94 %, its
+// conversions 54 %: the walk with the most rejections).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include "common.cuh"
