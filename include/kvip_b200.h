@@ -659,6 +659,24 @@ typedef struct KvipSlotMapsArgs {
 } KvipSlotMapsArgs;
 uint32_t kvip_b200_slot_maps(const KvipSlotMapsArgs* args, void* stream);
 
+/* Ends a planned step: request b keeps the first kept[b] of its planned tokens, at most those that got an output row and a block
+ * (KVIP_ERR_TOKEN_RANGE where more are asked for; negative counts keep nothing), and the planned blocks become its own:
+ *   lengths += min(kept, ends - lengths, starts[b + 1] - starts[b]), held = held_after, head += taken
+ * and nothing is planned any more: ends = lengths, taken = 0. The buffers are those of kvip_b200_slot_maps. */
+typedef struct KvipCommitTablesArgs {
+  const int32_t* kept;         /* [batch] */
+  const int32_t* starts;       /* [batch + 1] */
+  const int32_t* held_after;   /* [batch] */
+  int32_t* lengths;            /* [batch] */
+  int32_t* held;               /* [batch] */
+  int32_t* ends;               /* [batch] */
+  int32_t* head;               /* [1] */
+  int32_t* taken;              /* [1] */
+  int32_t* status;             /* [1] */
+  uint32_t batch, reserved0;
+} KvipCommitTablesArgs;
+uint32_t kvip_b200_commit_tables(const KvipCommitTablesArgs* args, void* stream);
+
 /* Rotary positions. Pair i of a rotated row (elements i and i + width/2 in the half layout, 2i and 2i + 1 in the
  * interleaved one) turns by the angle position * frequency_i; turns[i] = frequency_i / 2 pi. Rows of tokens with a
  * negative position are not written. `x[s]`: two sets of rows [tokens, heads[s], width] with their own strides (in

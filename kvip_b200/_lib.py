@@ -151,6 +151,9 @@ SlotMapsArgs = _struct("SlotMapsArgs", (
     "lengths", "counts", "held", "free_blocks", "head", "table", "positions", "slot_mapping", "requests", "starts", "ends",
     "held_after", "taken", "status", "layout"), [(n, u32) for n in ("batch", "pages", "blocks", "tokens", "block", "queries")])
 
+CommitTablesArgs = _struct("CommitTablesArgs", (
+    "kept", "starts", "held_after", "lengths", "held", "ends", "head", "taken", "status"), [("batch", u32), ("reserved0", u32)])
+
 
 class RotaryArgs(ctypes.Structure):
     """KvipRotaryArgs: up to two sets of rows (queries, keys) with strides of their own."""
@@ -203,7 +206,7 @@ _STAGES = {
     "kvip_b200_ingest_spans": IngestSpanArgs, "kvip_b200_peer_exchange": PeerExchangeArgs,
     "kvip_b200_lru_commit": LruArgs, "kvip_b200_lidu": LiduArgs, "kvip_b200_publish_pages": PagesArgs,
     "kvip_b200_window_bounds": WindowArgs, "kvip_b200_resident_threshold": ThresholdArgs,
-    "kvip_b200_speculate_window": SpeculateArgs, "kvip_b200_slot_maps": SlotMapsArgs, "kvip_b200_rotary": RotaryArgs,
+    "kvip_b200_speculate_window": SpeculateArgs, "kvip_b200_slot_maps": SlotMapsArgs, "kvip_b200_commit_tables": CommitTablesArgs, "kvip_b200_rotary": RotaryArgs,
     "kvip_b200_slot_attention": AttentionArgs, "kvip_b200_verify_drafts": VerifyArgs,
 }
 # every symbol include/kvip_b200.h declares

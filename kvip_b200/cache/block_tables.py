@@ -21,7 +21,7 @@ class BlockTables:
     persistent buffers of this object, sized by `tokens` (packed tokens per step at most): the captured graph of a
     step finds them at the same place. `status` collects KVIP_ERR_* bits (include/kvip_b200.h: KvipSlotMapsArgs)."""
 
-    _planned = ()      # outputs of a plan that `commit` takes over, each with its value where nothing is planned
+    _planned = ()      # outputs of a plan that `commit` takes over, each with its value where nothing is planned (then it keeps nothing)
 
     def __init__(self, torch, device, *, batch, pages, blocks, tokens, block=_lib.BLOCK_TOKENS, queries=0):
         self.torch = torch
@@ -46,7 +46,9 @@ class BlockTables:
         self.free = torch.arange(max(1, blocks), **i32)
         self.layout = torch.zeros((4, batch * queries), **i64) if queries else None
         self.device, self.index = self.table.device, self.table.get_device()
-        self.launch = _launch.Launcher("kvip_b200_slot_maps")
+        self.launch, self.launch_commit = _launch.Launcher("kvip_b200_slot_maps"), _launch.Launcher("kvip_b200_commit_tables")
+        self._commit = tuple(t.data_ptr() for t in (self.starts, self.held_after, self.lengths, self.held, self.ends, self.head, self.taken,
+                                                    self.status)) + (batch, 0)
         outputs = (self.table, self.positions, self.slot_mapping, self.requests, self.starts, self.ends, self.held_after, self.taken,
                    self.status)
         pointers = tuple(t.data_ptr() for t in outputs) + (self.layout.data_ptr() if queries else 0,)
@@ -101,19 +103,14 @@ class BlockTables:
 
     def commit(self, kept):
         """The planned blocks become the requests' own and `kept` [batch] int32 of the planned tokens stay (all of them, or
-        what a verification accepted). A request that keeps fewer holds its blocks for the tokens to come; one that the plan gave
-        no place (KVIP_ERR_*: `ends` is its length), or whose tokens were dropped behind the last output row, keeps none of those. A
-        plan is committed once: without another one a second call keeps nothing. `status` says KVIP_ERR_TOKEN_RANGE where more should
-        have been kept than was planned."""
-        if tuple(kept.shape) != (self.batch,):
-            raise ValueError("BlockTables kept counts must be [batch]")
-        torch = self.torch
-        room = torch.minimum(self.ends - self.lengths, self.starts[1:] - self.starts[:-1])
-        self.status.bitwise_or_((kept > room).any().to(torch.int32) * _lib.ERR_TOKEN_RANGE)
-        self.lengths.add_(torch.minimum(kept, room).clamp_(min=0))
-        self.held.copy_(self.held_after)
-        self.head.add_(self.taken)
-        self._end_plan()
+        what a verification accepted): one launch, capturable. A request that keeps fewer holds its blocks for the tokens to come; one
+        that the plan gave no place (KVIP_ERR_*: `ends` is its length), or whose tokens were dropped behind the last output row, keeps
+        none of those. A plan is committed once: without another one a second call keeps nothing. `status` says KVIP_ERR_TOKEN_RANGE
+        where more should have been kept than was planned."""
+        if tuple(kept.shape) != (self.batch,) or kept.get_device() != self.index:
+            raise ValueError("BlockTables kept counts must be [batch] on the tables' device")
+        kept = kept.to(self.torch.int32).contiguous()
+        self.launch_commit(self.index, kept.data_ptr(), *self._commit)
 
     def _end_plan(self):
         for output, state in self._planned:

@@ -181,6 +181,24 @@ __global__ void __launch_bounds__(kMapThreads) slot_map_rows(const __grid_consta
   }
 }
 
+// The end of a planned step, one CTA: as many loads as a plan, no scan (as single torch operations 16 launches).
+__global__ void __launch_bounds__(kMapThreads) commit_rows(const KvipCommitTablesArgs a) {
+  bool bad = false;
+  for (uint32_t b = threadIdx.x; b < a.batch; b += kMapThreads) {
+    const int32_t length = a.lengths[b], kept = a.kept[b], room = min(a.ends[b] - length, a.starts[b + 1] - a.starts[b]);
+    bad |= kept > room;
+    const int32_t after = length + max(0, min(kept, room));
+    a.lengths[b] = after;
+    a.ends[b] = after;
+    a.held[b] = a.held_after[b];
+  }
+  if (threadIdx.x == 0) {
+    a.head[0] += a.taken[0];
+    a.taken[0] = 0;
+  }
+  if (bad) atomicOr(a.status, static_cast<int32_t>(KVIP_ERR_TOKEN_RANGE));
+}
+
 }  // namespace
 }  // namespace kvip
 
@@ -203,4 +221,14 @@ extern "C" uint32_t kvip_b200_slot_maps(const KvipSlotMapsArgs* a, void* stream)
   slot_map_rows<<<grid, kMapThreads, 0, static_cast<cudaStream_t>(stream)>>>(*a);
   count_launch();
   return check_launch("slot_map_rows");
+}
+
+extern "C" uint32_t kvip_b200_commit_tables(const KvipCommitTablesArgs* a, void* stream) {
+  using namespace kvip;
+  KVIP_REQUIRE(a && a->kept && a->starts && a->held_after && a->lengths && a->held && a->ends && a->head && a->taken && a->status,
+               "commit_tables: null pointer");
+  KVIP_REQUIRE(a->batch >= 1 && a->batch <= kMapBatch, "commit_tables: batch must be in 1..1024");
+  commit_rows<<<1, kMapThreads, 0, static_cast<cudaStream_t>(stream)>>>(*a);
+  count_launch();
+  return check_launch("commit_rows");
 }

@@ -167,6 +167,90 @@ def test_tokens_without_a_block_leave_the_index_rows_alone(device):
     assert torch.equal(storage.scales[1:, :5].cpu(), expected)
 
 
+def owned(t):
+    """Blocks of all rows, then of the free list: each of them once, whatever happened."""
+    rows = [int(x) for b in range(t.batch) for x in t.table[b, :int(t.held[b])]]
+    return sorted(rows + t.free[int(t.head):].tolist())
+
+
+def counts_of(device, *counts):
+    return torch.tensor(counts, dtype=torch.int32, device=device)
+
+
+def tables_of(device, lengths, held, table, free, *, block, tokens, head=0):
+    """Tables in a given state; the free list has a place for every block."""
+    import kvip_b200 as kvip
+    tables = kvip.BlockTables(torch, device, batch=len(lengths), pages=len(table[0]), blocks=len(free), tokens=tokens, block=block)
+    tables.load(lengths=torch.tensor(lengths), held=torch.tensor(held), table=torch.tensor(table), free=torch.tensor(free), head=head)
+    return tables
+
+
+def test_commit_keeps_nothing_of_a_request_without_blocks(device):
+    """Three requests, blocks for one: the verifier returns a count for each of them all the same."""
+    t = tables_of(device, [4, 4, 4], [1, 1, 1], [[0, -1, -1], [1, -1, -1], [2, -1, -1]], [9, 9, 9, 3], block=4, tokens=12, head=3)
+    t.plan(counts_of(device, 2, 2, 2))
+    assert int(t.status) == 4
+    t.commit(counts_of(device, 2, 1, 2))
+    assert t.lengths.tolist() == [6, 4, 4] and t.held.tolist() == [2, 1, 1] and owned(t) == [0, 1, 2, 3]
+    assert int(t.status) == 4 | 1
+    t.status.zero_()
+    t.release([0])
+    t.plan(counts_of(device, 0, 2, 2))
+    assert int(t.status) == 0
+    t.commit(counts_of(device, 0, 2, 2))
+    assert t.lengths.tolist() == [0, 6, 6] and owned(t) == [0, 1, 2, 3] and int(t.status) == 0
+
+
+def test_commit_keeps_no_token_that_was_dropped(device):
+    t = tables_of(device, [0, 0], [0, 0], [[-1, -1], [-1, -1]], [0, 1, 2, 3], block=4, tokens=5)
+    t.plan(counts_of(device, 4, 4))
+    assert int(t.status) == 1
+    t.commit(counts_of(device, 4, 4))
+    assert t.lengths.tolist() == [4, 1]
+    assert owned(t) == [0, 1, 2, 3]
+
+
+def test_a_plan_is_committed_once(device):
+    t = tables_of(device, [3], [1], [[0, -1, -1]], [9, 1, 2], block=4, tokens=4, head=1)
+    t.plan(counts_of(device, 4))
+    t.commit(counts_of(device, 1))
+    assert t.lengths.tolist() == [4] and t.held.tolist() == [2] and int(t.status) == 0
+    t.commit(counts_of(device, 0))
+    assert int(t.status) == 0
+    t.commit(counts_of(device, 3))
+    assert t.lengths.tolist() == [4] and t.held.tolist() == [2] and int(t.head) == 2 and owned(t) == [0, 1, 2]
+    assert int(t.status) == 1
+    t.plan(counts_of(device, 2))
+    assert int(t.taken) == 0                        # the block of the rejected tokens is still the request's
+    t.commit(counts_of(device, -1))
+    assert t.lengths.tolist() == [4]
+    t.plan(counts_of(device, 2))
+    t.commit(torch.tensor([2], device=device))      # int64 counts are taken as well
+    assert t.lengths.tolist() == [6] and int(t.status) == 1
+    for bad in (counts_of(device, 1, 2), torch.ones(1, dtype=torch.int32)):
+        with pytest.raises(ValueError, match="batch"):
+            t.commit(bad)
+
+
+@pytest.mark.parametrize("between", [False, True])
+def test_release_between_a_plan_and_its_commit_puts_no_block_into_two_rows(device, between):
+    """`release` ends the open plan; committed or not, every block stays in one place, and what was to be kept is reported."""
+    t = tables_of(device, [4, 4], [1, 1], [[0, -1, -1], [1, -1, -1]], [9, 9, 2, 3, 4], block=4, tokens=8, head=2)
+    t.plan(counts_of(device, 2, 2))
+    if between:
+        t.release([1])
+        t.commit(counts_of(device, 2, 2))
+        assert t.lengths.tolist() == [4, 0] and int(t.status) == 1
+    else:
+        t.commit(counts_of(device, 2, 2))
+        t.release([1])
+        assert t.lengths.tolist() == [6, 0] and int(t.status) == 0
+    assert owned(t) == [0, 1, 2, 3, 4]
+    t.plan(counts_of(device, 4, 8))
+    t.commit(counts_of(device, 4, 8))
+    assert owned(t) == [0, 1, 2, 3, 4] and t.held.tolist() == [3 if not between else 2, 2]
+
+
 def test_block_tables_run_out_and_recover(device):
     """More requests than blocks: those without keep their lengths whatever is committed, from a captured graph too, and go on when blocks
     come back. Every block is in one place all the while."""

@@ -1,5 +1,5 @@
-"""Host-side halves of what the operators round the selection path owe one another: the state of the block tables between steps, with host
-tensors in the place of the device's."""
+"""Host-side halves of what the operators round the selection path owe one another, with host tensors in the place of the device's: what
+`release` returns, positions of trees, the selector's state between forwards."""
 from types import SimpleNamespace
 
 import numpy as np
@@ -30,78 +30,6 @@ def tables_on_the_host(lengths, held, table, free, *, block, tokens, head=0):
 
     t.plan = plan
     return t
-
-
-def owned(t):
-    """Blocks of all rows, then of the free list: each of them once, whatever happened."""
-    rows = [int(x) for b in range(t.batch) for x in t.table[b, :int(t.held[b])]]
-    return sorted(rows + t.free[int(t.head):].tolist())
-
-
-def kept(*counts):
-    return torch.tensor(counts, dtype=torch.int32)
-
-
-def test_commit_keeps_nothing_of_a_request_without_blocks():
-    """Three requests, blocks for one: the verifier returns a count for each of them all the same."""
-    t = tables_on_the_host([4, 4, 4], [1, 1, 1], [[0, -1, -1], [1, -1, -1], [2, -1, -1]], [9, 9, 9, 3], block=4, tokens=12, head=3)
-    t.plan([2, 2, 2])
-    assert int(t.status) == 4
-    t.commit(kept(2, 1, 2))
-    assert t.lengths.tolist() == [6, 4, 4] and t.held.tolist() == [2, 1, 1] and owned(t) == [0, 1, 2, 3]
-    assert int(t.status) == 4 | 1
-    t.status.zero_()
-    t.release([0])
-    t.plan([0, 2, 2])
-    assert int(t.status) == 0
-    t.commit(kept(0, 2, 2))
-    assert t.lengths.tolist() == [0, 6, 6] and owned(t) == [0, 1, 2, 3] and int(t.status) == 0
-
-
-def test_commit_keeps_no_token_that_was_dropped():
-    t = tables_on_the_host([0, 0], [0, 0], [[-1, -1], [-1, -1]], [0, 1, 2, 3], block=4, tokens=5)
-    t.plan([4, 4])
-    assert int(t.status) == 1
-    t.commit(kept(4, 4))
-    assert t.lengths.tolist() == [4, 1]
-    assert owned(t) == [0, 1, 2, 3]
-
-
-def test_a_plan_is_committed_once():
-    t = tables_on_the_host([3], [1], [[0, -1, -1]], [9, 1, 2], block=4, tokens=4, head=1)
-    t.plan([4])
-    t.commit(kept(1))
-    assert t.lengths.tolist() == [4] and t.held.tolist() == [2] and int(t.status) == 0
-    t.commit(kept(0))
-    assert int(t.status) == 0
-    t.commit(kept(3))
-    assert t.lengths.tolist() == [4] and t.held.tolist() == [2] and int(t.head) == 2 and owned(t) == [0, 1, 2]
-    assert int(t.status) == 1
-    t.plan([2])
-    assert int(t.taken) == 0                        # the block of the rejected tokens is still the request's
-    t.commit(kept(-1))
-    assert t.lengths.tolist() == [4]
-    with pytest.raises(ValueError, match="batch"):
-        t.commit(kept(1, 2))
-
-
-@pytest.mark.parametrize("between", [False, True])
-def test_release_between_a_plan_and_its_commit_puts_no_block_into_two_rows(between):
-    """`release` ends the open plan; committed or not, every block stays in one place, and what was to be kept is reported."""
-    t = tables_on_the_host([4, 4], [1, 1], [[0, -1, -1], [1, -1, -1]], [9, 9, 2, 3, 4], block=4, tokens=8, head=2)
-    t.plan([2, 2])
-    if between:
-        t.release([1])
-        t.commit(kept(2, 2))
-        assert t.lengths.tolist() == [4, 0] and int(t.status) == 1
-    else:
-        t.commit(kept(2, 2))
-        t.release([1])
-        assert t.lengths.tolist() == [6, 0] and int(t.status) == 0
-    assert owned(t) == [0, 1, 2, 3, 4]
-    t.plan([4, 8])
-    t.commit(kept(4, 8))
-    assert owned(t) == [0, 1, 2, 3, 4] and t.held.tolist() == [3 if not between else 2, 2]
 
 
 def test_release_passes_over_entries_that_are_no_block():
